@@ -37,7 +37,11 @@ typedef enum {
 enum { SABRE_BF16 = 0, SABRE_F16 = 1, SABRE_F32 = 2 /* sabre_chunk_vectors embeddings only */ };
 
 /* Device status flags (sabre_device_status). */
-enum { SABRE_DEV_TIMEOUT = 1u, SABRE_DEV_BAD_SMEM_ALIGN = 2u };
+enum {
+  SABRE_DEV_TIMEOUT = 1u,
+  SABRE_DEV_BAD_SMEM_ALIGN = 2u,
+  SABRE_DEV_BAD_PAGE = 4u /* a paged entry met a position or page outside the table or the pool */
+};
 
 int sabre_version(void);
 const char* sabre_status_string(int status);
@@ -363,6 +367,79 @@ int sabre_prefill_bsa_tokenmask(const void* q, const void* k, const void* v, voi
                                 int head_dim, int max_active, const int64_t* q_strides, const int64_t* k_strides,
                                 const int64_t* v_strides, const int64_t* o_strides, const int64_t* idx_strides,
                                 const int64_t* cnt_strides, float softmax_scale, int dtype, void* stream);
+
+/* ----------------------------------------------------------------------
+ * (4) Paged K/V cache.
+ *
+ * No counterpart in the reference (its cache is transformers' DynamicCache).
+ * Sequences of different lengths share one pool of pages:
+ *
+ * k_pages, v_pages : [num_pages, Hkv, page_size, D], element strides
+ *             kp_strides / vp_strides = {page, head, row} (d-stride 1,
+ *             positive multiples of 8; 16-byte aligned bases); page_size is a
+ *             power of two from 16 to 1024, head_dim 128, heads_kv <= 4096
+ * page_table : int32 [batch, max_pages], row stride table_stride: row t of
+ *             sequence b lies in page page_table[b][t / page_size]. -1 = the
+ *             page is absent: its rows are not stored and are not visible.
+ *             Any other value outside [0, num_pages) counts as absent and
+ *             records SABRE_DEV_BAD_PAGE. page_size * max_pages <= 2^30.
+ * seq_lens   : int32 [batch], rows of each sequence, the new ones included;
+ *             rows at or past page_size * max_pages are not stored and not
+ *             visible
+ * q_start    : int32 [batch + 1], ascending from 0: rows q_start[b] ..
+ *             q_start[b+1]-1 of the `rows` new rows are the last rows of
+ *             sequence b, so row r is at position seq_lens[b] -
+ *             (q_start[b+1] - r). Rows from q_start[batch] on (padding of a
+ *             captured batch) are neither read nor written.
+ *
+ * Visibility: the query at position i sees key j when j <= i,
+ * j < seq_lens[b], page j is present and (window < 0, or i - j <= window, or
+ * j < num_prefix_tokens). A query that sees nothing gives zeros. Rows that
+ * the sequence does not have, or whose page is absent, never reach a result,
+ * whatever they hold. heads_q / heads_kv must be an integer <= 8; query head
+ * h reads KV head h / (Hq / Hkv). softmax_scale <= 0 selects 1/sqrt(head_dim).
+ *
+ * sabre_paged_store: new rows k, v [rows, Hkv, D] (strides {row, head}) into
+ *   their pages. q_start NULL: one row per sequence (rows == batch). A row
+ *   whose position is negative or past the table is dropped and records
+ *   SABRE_DEV_BAD_PAGE. A page that two sequences share must not be the
+ *   target of both.
+ * sabre_paged_decode: one query row per sequence, q, o [batch, Hq, D]
+ *   (strides {b, h}), at position seq_lens[b] - 1.
+ * sabre_paged_prefill: q, o [rows, Hq, D] (strides {row, head}).
+ *   workspace: sabre_paged_*_workspace_size(...) bytes (may be 0, then NULL
+ *   is fine), 16-byte aligned; calls that may overlap on the GPU need their own.
+ * sabre_copy_pages: for each move m < moves, page dst[m] = page src[m] in
+ *   each of `buffers` pools (a cache's layers, K and V alike): pool u starts
+ *   at pages + u * buffer_stride, page i of it at i * page_stride and holds
+ *   page_bytes contiguous bytes (all in BYTES, multiples of 16). src and dst
+ *   are HOST arrays (they travel in the launch arguments: nothing is copied
+ *   to the device and the call can be captured). A page outside the pool,
+ *   written twice, or both read and written fails with
+ *   SABRE_ERR_INVALID_ARG and nothing is launched.
+ * ---------------------------------------------------------------------- */
+int sabre_paged_store(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* page_table,
+                      const int32_t* seq_lens, const int32_t* q_start, int rows, int batch, int heads_kv,
+                      int head_dim, int num_pages, int page_size, int max_pages, const int64_t* k_strides,
+                      const int64_t* v_strides, const int64_t* kp_strides, const int64_t* vp_strides,
+                      int64_t table_stride, int dtype, void* stream);
+size_t sabre_paged_decode_workspace_size(int batch, int heads_q, int heads_kv, int head_dim);
+int sabre_paged_decode(const void* q, const void* k_pages, const void* v_pages, void* o, const int32_t* page_table,
+                       const int32_t* seq_lens, int batch, int heads_q, int heads_kv, int head_dim, int num_pages,
+                       int page_size, int max_pages, int window, int num_prefix_tokens, const int64_t* q_strides,
+                       const int64_t* kp_strides, const int64_t* vp_strides, const int64_t* o_strides,
+                       int64_t table_stride, float softmax_scale, int dtype, void* workspace, size_t workspace_bytes,
+                       void* stream);
+size_t sabre_paged_prefill_workspace_size(int rows, int batch, int heads_q, int heads_kv, int head_dim, int page_size,
+                                          int max_pages, int window, int num_prefix_tokens);
+int sabre_paged_prefill(const void* q, const void* k_pages, const void* v_pages, void* o, const int32_t* page_table,
+                        const int32_t* seq_lens, const int32_t* q_start, int rows, int batch, int heads_q,
+                        int heads_kv, int head_dim, int num_pages, int page_size, int max_pages, int window,
+                        int num_prefix_tokens, const int64_t* q_strides, const int64_t* kp_strides,
+                        const int64_t* vp_strides, const int64_t* o_strides, int64_t table_stride,
+                        float softmax_scale, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+int sabre_copy_pages(void* pages, int buffers, int64_t buffer_stride, int num_pages, int64_t page_stride,
+                     int64_t page_bytes, const int32_t* src, const int32_t* dst, int moves, void* stream);
 
 #ifdef __cplusplus
 }

@@ -17,6 +17,7 @@ c_int, c_int64, c_float, c_size_t, c_void_p, c_uint = (ctypes.c_int, ctypes.c_in
                                                       ctypes.c_size_t, ctypes.c_void_p, ctypes.c_uint)
 P = ctypes.c_void_p
 I64P = ctypes.POINTER(ctypes.c_int64)
+I32P = ctypes.POINTER(ctypes.c_int32)
 
 # (name, restype, argtypes) for every symbol the header declares.
 SIGNATURES = {
@@ -53,6 +54,15 @@ SIGNATURES = {
     "sabre_token_tile_masks": (c_int, [P, P, P, P, c_int, c_int, c_int, P, c_int, P, P, P, P]),
     "sabre_prefill_bsa_tokenmask": (c_int, [P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int,
                                             I64P, I64P, I64P, I64P, I64P, I64P, c_float, c_int, P]),
+    "sabre_paged_store": (c_int, [P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                  I64P, I64P, I64P, I64P, c_int64, c_int, P]),
+    "sabre_paged_decode_workspace_size": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "sabre_paged_decode": (c_int, [P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                   I64P, I64P, I64P, I64P, c_int64, c_float, c_int, P, c_size_t, P]),
+    "sabre_paged_prefill_workspace_size": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "sabre_paged_prefill": (c_int, [P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                    c_int, c_int, I64P, I64P, I64P, I64P, c_int64, c_float, c_int, P, c_size_t, P]),
+    "sabre_copy_pages": (c_int, [P, c_int, c_int64, c_int, c_int64, c_int64, I32P, I32P, c_int, P]),
 }
 
 _lib: Optional[ctypes.CDLL] = None

@@ -5,6 +5,7 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <cstdlib>
 #include <cstring>
 #include <mutex>
 
@@ -17,6 +18,7 @@
 #include "topk.cu"
 #include "similarity.cu"
 #include "token_mask.cu"
+#include "paged_cache.cu"
 
 #define SABRE_VERSION 100
 
@@ -99,6 +101,7 @@ static int ensure_smem_attr(Kern kern, int bytes) {
 
 #include "decode_gqa.cu"
 #include "qkv_prefill.cu"
+#include "paged_attention.cu"
 
 using namespace sabre;
 

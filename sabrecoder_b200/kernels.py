@@ -8,8 +8,9 @@ allocates. There is no CPU path: non-CUDA tensors raise.
 
 from __future__ import annotations
 
+import ctypes
 import math
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -538,3 +539,205 @@ def token_tile_masks(tok_chunk: torch.Tensor, tok_group: torch.Tensor, tok_globa
     check(st, "sabre_token_tile_masks")
     LAUNCHES[0] += 1
     return masks, row_ptr
+
+
+# ---------------------------------------------------------------------------
+# (4) paged K/V cache
+# ---------------------------------------------------------------------------
+
+def _paged_check(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                 seq_lens: torch.Tensor, q_start: Optional[torch.Tensor], **rows: Optional[torch.Tensor]) -> int:
+    """Checks the arguments the paged calls share (``rows``: the ``[N, H, D]``
+    tensors of the new rows); returns the number of sequences."""
+    ts = dict(k_pages=k_pages, v_pages=v_pages, page_table=page_table, seq_lens=seq_lens, q_start=q_start, **rows)
+    if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
+        raise SabreError(f"{what}: k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} must both be "
+                         f"[num_pages, Hkv, page_size, D]")
+    if page_table.dim() != 2 or page_table.shape[1] < 1 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise SabreError(f"{what}: page_table {tuple(page_table.shape)} must be [B, max_pages >= 1] with unit column "
+                         f"stride")
+    B = page_table.shape[0]
+    for name, t, n in (("seq_lens", seq_lens, B), ("q_start", q_start, B + 1)):
+        if t is not None and (tuple(t.shape) != (n,) or not t.is_contiguous()):
+            raise SabreError(f"{what}: {name} {tuple(t.shape)} must be a contiguous [{n}]")
+    for name in ("page_table", "seq_lens", "q_start"):
+        if ts[name] is not None:
+            _i32(ts[name], name)
+    for name, t in rows.items():
+        if t is not None and (t.dim() != 3 or t.shape[-1] != k_pages.shape[-1] or t.stride(-1) != 1):
+            raise SabreError(f"{what}: {name} {tuple(t.shape)} must be [N, H, {k_pages.shape[-1]}] with unit last "
+                             f"stride")
+        if t is not None and t.dtype != k_pages.dtype:
+            raise SabreError(f"{what}: {name} is {t.dtype}, the pages are {k_pages.dtype}")
+    if k_pages.dtype not in DTYPE_CODE or v_pages.dtype != k_pages.dtype:
+        raise SabreError(f"{what}: pages must share dtype bf16 or f16 (got {k_pages.dtype}, {v_pages.dtype})")
+    if k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
+        raise SabreError(f"{what}: pages need unit head-dim stride")
+    _need_cuda(**ts)
+    for name, t in ts.items():
+        if t is not None and t.device != k_pages.device:
+            raise SabreError(f"{what}: {name} is on {t.device}, the pages are on {k_pages.device}")
+    return B
+
+
+def _paged_args(k_pages: torch.Tensor, page_table: torch.Tensor):
+    """(heads_kv, head_dim, num_pages, page_size, max_pages) for the C entry points."""
+    P, Hkv, ps, D = k_pages.shape
+    return Hkv, D, P, ps, page_table.shape[1]
+
+
+def _window_code(what: str, window_size: Optional[int], num_prefix_tokens: int) -> Tuple[int, int]:
+    """The C ABI's (window, prefix): -1 = no window; both held to int32."""
+    if num_prefix_tokens < 0 or (window_size is not None and window_size < 0):
+        raise SabreError(f"{what}: window_size {window_size} and num_prefix_tokens {num_prefix_tokens} must not be "
+                         f"negative (no window: None)")
+    w = -1 if window_size is None or window_size >= 2 ** 31 - 1 else int(window_size)
+    return w, min(int(num_prefix_tokens), 2 ** 31 - 1)
+
+
+def _workspace(what: str, workspace: Optional[torch.Tensor], need: int, device) -> Optional[torch.Tensor]:
+    if workspace is None:
+        return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+    if workspace.device != device or not workspace.is_contiguous():
+        raise SabreError(f"{what}: workspace must be contiguous on {device}")
+    if workspace.numel() * workspace.element_size() < need:
+        raise SabreError(f"{what}: workspace holds {workspace.numel() * workspace.element_size()} < {need} bytes")
+    return workspace
+
+
+def paged_store(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                page_table: torch.Tensor, seq_lens: torch.Tensor, q_start: Optional[torch.Tensor] = None) -> None:
+    """Writes new K/V rows into their pages.
+
+    k, v: ``[N, Hkv, D]`` (any row and head strides); k_pages, v_pages:
+    ``[num_pages, Hkv, page_size, D]``; page_table int32 ``[B, max_pages]``
+    (-1 = absent page, its rows are dropped); seq_lens int32 ``[B]``: lengths
+    with the new rows; q_start int32 ``[B + 1]``: rows ``q_start[b] ..
+    q_start[b+1]-1`` are the last rows of sequence b (default: one row each,
+    ``N == B``). Rows from ``q_start[B]`` on are padding."""
+    B = _paged_check("paged_store", k_pages, v_pages, page_table, seq_lens, q_start, k=k, v=v)
+    if k.shape != v.shape or k.shape[1] != k_pages.shape[1]:
+        raise SabreError(f"paged_store: k {tuple(k.shape)} and v {tuple(v.shape)} must both be [N, "
+                         f"{k_pages.shape[1]}, D]")
+    if q_start is None and k.shape[0] != B:
+        raise SabreError(f"paged_store: {k.shape[0]} rows for {B} sequences need q_start")
+    if k.shape[0] == 0 or B == 0:
+        return
+    with torch.cuda.device(k_pages.device):
+        st = lib().sabre_paged_store(
+            k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
+            seq_lens.data_ptr(), _ptr(q_start), k.shape[0], B, *_paged_args(k_pages, page_table),
+            i64(k.stride()[:2]), i64(v.stride()[:2]), i64(k_pages.stride()[:3]), i64(v_pages.stride()[:3]),
+            page_table.stride(0), DTYPE_CODE[k.dtype], _stream(k))
+    check(st, "sabre_paged_store")
+    LAUNCHES[0] += 1
+
+
+def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                 seq_lens: torch.Tensor, *, window_size: Optional[int] = None, num_prefix_tokens: int = 0,
+                 softmax_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                 workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention of one new token per sequence over a paged cache.
+
+    q: ``[B, Hq, D]``, the query at position ``seq_lens[b] - 1``; pages and
+    tables as in :func:`paged_store`. With a window the query at position i
+    sees key j <= i when ``i - j <= window_size`` or ``j < num_prefix_tokens``.
+    A sequence that sees nothing (length 0) gives zeros. Deterministic."""
+    window, prefix = _window_code("paged_decode", window_size, num_prefix_tokens)
+    B = _paged_check("paged_decode", k_pages, v_pages, page_table, seq_lens, None, q=q, out=out)
+    Hkv, Hq = k_pages.shape[1], q.shape[1]
+    if q.shape[0] != B or (out is not None and out.shape != q.shape):
+        raise SabreError(f"paged_decode: q {tuple(q.shape)} and out must be [B={B}, Hq, D]")
+    if out is None:
+        out = torch.empty_like(q)
+    if q.numel() == 0:
+        return out
+    ws = _workspace("paged_decode", workspace,
+                    int(lib().sabre_paged_decode_workspace_size(B, Hq, Hkv, q.shape[2])), q.device)
+    with torch.cuda.device(q.device):
+        st = lib().sabre_paged_decode(
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), page_table.data_ptr(),
+            seq_lens.data_ptr(), B, Hq, *_paged_args(k_pages, page_table), window, prefix, i64(q.stride()[:2]),
+            i64(k_pages.stride()[:3]), i64(v_pages.stride()[:3]), i64(out.stride()[:2]), page_table.stride(0),
+            float(softmax_scale or 0.0), DTYPE_CODE[q.dtype], _ptr(ws),
+            0 if ws is None else ws.numel() * ws.element_size(), _stream(q))
+    check(st, "sabre_paged_decode")
+    LAUNCHES[0] += 1
+    return out
+
+
+def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                  seq_lens: torch.Tensor, q_start: torch.Tensor, *, window_size: Optional[int] = None,
+                  num_prefix_tokens: int = 0, softmax_scale: Optional[float] = None,
+                  out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Causal attention of a ragged batch of new rows over a paged cache that
+    holds them already (:func:`paged_store` first).
+
+    q: ``[N, Hq, D]``; rows ``q_start[b] .. q_start[b+1]-1`` are the last
+    rows of sequence b, the rest as in :func:`paged_decode`. Rows of ``out``
+    from ``q_start[B]`` on are left as they are."""
+    window, prefix = _window_code("paged_prefill", window_size, num_prefix_tokens)
+    B = _paged_check("paged_prefill", k_pages, v_pages, page_table, seq_lens, q_start, q=q, out=out)
+    Hkv, Hq = k_pages.shape[1], q.shape[1]
+    if out is not None and out.shape != q.shape:
+        raise SabreError(f"paged_prefill: out {tuple(out.shape)} must have q's shape {tuple(q.shape)}")
+    if out is None:
+        out = torch.empty_like(q)
+    if q.numel() == 0 or B == 0:
+        return out
+    args = _paged_args(k_pages, page_table)
+    ws = _workspace("paged_prefill", workspace,
+                    int(lib().sabre_paged_prefill_workspace_size(q.shape[0], B, Hq, Hkv, q.shape[2], args[3], args[4],
+                                                                 window, prefix)), q.device)
+    with torch.cuda.device(q.device):
+        st = lib().sabre_paged_prefill(
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), page_table.data_ptr(),
+            seq_lens.data_ptr(), q_start.data_ptr(), q.shape[0], B, Hq, *args, window, prefix, i64(q.stride()[:2]),
+            i64(k_pages.stride()[:3]), i64(v_pages.stride()[:3]), i64(out.stride()[:2]), page_table.stride(0),
+            float(softmax_scale or 0.0), DTYPE_CODE[q.dtype], _ptr(ws),
+            0 if ws is None else ws.numel() * ws.element_size(), _stream(q))
+    check(st, "sabre_paged_prefill")
+    LAUNCHES[0] += 1
+    return out
+
+
+def copy_pages(pages: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -> None:
+    """Copies page ``src[m]`` to page ``dst[m]`` in every pool of ``pages``:
+    one pool ``[num_pages, Hkv, page_size, D]`` or several at one stride
+    ``[..., num_pages, Hkv, page_size, D]`` (e.g. a cache's layers, K and V),
+    each page contiguous, any dtype. ``src`` and ``dst`` are lists of ints (or
+    CPU integer tensors); they travel with the launch, so the call neither
+    synchronises nor copies to the device and can be captured. Pages are
+    copied in no order: a page outside the pool, written twice, or both read
+    and written raises and nothing is copied."""
+    for name, t in (("src", src), ("dst", dst)):
+        if isinstance(t, torch.Tensor) and (t.is_cuda or t.dim() != 1 or t.is_floating_point()):
+            raise SabreError(f"copy_pages: {name} must be a list of ints or a 1-D CPU integer tensor")
+    src = src.tolist() if isinstance(src, torch.Tensor) else list(src)
+    dst = dst.tolist() if isinstance(dst, torch.Tensor) else list(dst)
+    if len(src) != len(dst):
+        raise SabreError(f"copy_pages: {len(src)} sources for {len(dst)} destinations")
+    if pages.dim() < 4:
+        raise SabreError(f"copy_pages: pages {tuple(pages.shape)} must be [..., num_pages, Hkv, page_size, D]")
+    for m, (a, b) in enumerate(zip(src, dst)):
+        if not (0 <= a < pages.shape[-4] and 0 <= b < pages.shape[-4]):
+            raise SabreError(f"copy_pages: move {m} ({a} -> {b}) is outside the pool of {pages.shape[-4]} pages")
+    _need_cuda(pages=pages)
+    if pages.numel() == 0 or not src:
+        return
+    page = pages[(0,) * (pages.dim() - 3)]
+    if not page.is_contiguous():
+        raise SabreError("copy_pages: each page [Hkv, page_size, D] must be contiguous")
+    lead = pages.shape[:-4]
+    try:
+        flat = pages.view((-1,) + tuple(pages.shape[-4:]))
+    except RuntimeError as e:
+        raise SabreError(f"copy_pages: the pools {tuple(lead)} are not at one stride") from e
+    es = pages.element_size()
+    n = len(src)
+    with torch.cuda.device(pages.device):
+        st = lib().sabre_copy_pages(
+            flat.data_ptr(), flat.shape[0], flat.stride(0) * es, flat.shape[1], flat.stride(1) * es,
+            page.numel() * es, (ctypes.c_int32 * n)(*src), (ctypes.c_int32 * n)(*dst), n, _stream(pages))
+    check(st, "sabre_copy_pages")
+    LAUNCHES[0] += -(-n // 480)

@@ -1,0 +1,353 @@
+"""GPU tests of the paged K/V cache kernels against the 64-bit oracle. Every row
+of a pool that no sequence owns holds NaN, so a read of one shows."""
+
+import pytest
+import torch
+
+from oracle import paged_oracle as PO
+
+pytestmark = pytest.mark.gpu
+
+D = 128
+BF, FP = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module")
+def K():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from sabrecoder_b200 import kernels
+    return kernels
+
+
+def make(seed, lens, news, Hq, Hkv, ps, dtype, window=None, prefix=0, layout="phtd", extra_cols=1, drop=True,
+         spare=3):
+    """Pools, tables and queries of a ragged batch on the GPU. With a window,
+    pages that no new row can see are absent (drop)."""
+    gen = torch.Generator().manual_seed(seed)
+    cap = max(max((n + ps - 1) // ps for n in lens), 1) + extra_cols
+    table = torch.full((len(lens), cap), -1, dtype=torch.int32)
+    live = []
+    for b, (n, new) in enumerate(zip(lens, news)):
+        for p in range((n + ps - 1) // ps):
+            if drop and window is not None and p * ps >= prefix and (p + 1) * ps <= n - new - window:
+                continue
+            live.append((b, p))
+    P = len(live) + spare
+    ids = torch.randperm(P, generator=gen).tolist()
+    if layout == "phtd":
+        kp, vp = (torch.full((P, Hkv, ps, D), float("nan"), dtype=dtype) for _ in range(2))
+    else:  # K and V interleaved, heads inside a row: [P, ps, 2, Hkv, D]
+        both = torch.full((P, ps, 2, Hkv, D), float("nan"), dtype=dtype)
+        kp, vp = both[:, :, 0].transpose(1, 2), both[:, :, 1].transpose(1, 2)
+    for (b, p), page in zip(live, ids):
+        table[b, p] = page
+        m = min(ps, lens[b] - p * ps)
+        kp[page, :, :m] = torch.randn(Hkv, m, D, generator=gen).to(dtype)
+        vp[page, :, :m] = torch.randn(Hkv, m, D, generator=gen).to(dtype)
+    starts = torch.tensor([0] + torch.tensor(news).cumsum(0).tolist(), dtype=torch.int32)
+    q = torch.randn(int(starts[-1]), Hq, D, generator=gen).to(dtype)
+    if layout == "phtd":
+        kp, vp = kp.cuda(), vp.cuda()
+    else:
+        both = both.cuda()
+        kp, vp = both[:, :, 0].transpose(1, 2), both[:, :, 1].transpose(1, 2)
+    return (q.cuda(), kp, vp, table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), starts.cuda())
+
+
+def check(got, args, window=None, prefix=0, scale=None, starts=None):
+    """|got - exact| against the arithmetic of the kernels, each factor a bound:
+    a weight p is rounded to the type once (u = eps / 2 relative), the result
+    once; a score is a sum of 128 products (128 additions, up to 2^-23 each of
+    the sum of magnitudes ds, and 2^-23 for the scaling), and p moves by twice
+    that; ex2 and the joining of partial sums add 16 * 2^-23; the sums over n keys
+    n * 2^-23 of the magnitudes. f16 weights below its normal range are off by
+    half the smallest step, 2^-25, each."""
+    q, kp, vp, table, lens, _ = args
+    want, spread, ds = PO.attention(q, kp, vp, table, lens, starts, window=window, prefix=prefix, scale=scale)
+    u = torch.finfo(q.dtype).eps / 2
+    n = float(lens.max())
+    rel = u + 2 * (129 * ds + 16) * 2.0 ** -23 + n * 2.0 ** -23
+    tol = rel[..., None] * spread + u * want.abs() + 2.0 ** -25 * n * (q.dtype == FP) * 6.0 + 1e-7
+    err = (got.double() - want).abs()
+    assert torch.isfinite(got).all()
+    bad = err > tol * 1.01
+    assert not bad.any(), f"{int(bad.sum())} off, worst {(err / tol).max():.2f} of its bound, err {err.max():.3e}"
+
+
+DECODE = [
+    # lens, Hq, Hkv, page_size, dtype, window, prefix, layout
+    ([1], 1, 1, 16, BF, None, 0, "phtd"),
+    ([300], 16, 16, 16, BF, None, 0, "phtd"),
+    ([63, 64, 65, 0, 1], 4, 2, 64, BF, None, 0, "phtd"),
+    ([5000, 1, 777, 0, 0, 64, 2049], 7, 1, 32, FP, None, 0, "phtd"),
+    ([1500, 2600, 3, 129], 56, 8, 64, BF, None, 0, "ptkhd"),
+    ([4097, 15, 16, 17], 8, 1, 128, FP, None, 0, "phtd"),
+    ([900, 70, 1200, 200, 201, 66], 6, 2, 16, BF, 100, 0, "phtd"),
+    ([900, 70, 1200, 200, 201, 1100], 4, 4, 64, FP, 64, 33, "phtd"),
+    ([2000, 500, 129], 10, 2, 256, BF, 0, 5, "phtd"),
+    ([2000, 500, 129, 1], 5, 1, 1024, BF, 700, 200, "ptkhd"),
+    ([3000, 31, 400], 3, 1, 32, BF, 1000, 5000, "phtd"),
+    (list(range(0, 300)), 2, 2, 16, BF, None, 0, "phtd"),
+    ([40000], 32, 32, 128, BF, None, 0, "phtd"),
+    ([70001, 2], 7, 1, 64, FP, None, 0, "phtd"),
+]
+
+
+@pytest.mark.parametrize("case", range(len(DECODE)))
+def test_paged_decode_vs_oracle(K, case):
+    lens, Hq, Hkv, ps, dtype, window, prefix, layout = DECODE[case]
+    args = make(case, lens, [1] * len(lens), Hq, Hkv, ps, dtype, window, prefix, layout)
+    q, kp, vp, table, sl, _ = args
+    out = K.paged_decode(q, kp, vp, table, sl, window_size=window, num_prefix_tokens=prefix)
+    check(out, args, window, prefix)
+    again = K.paged_decode(q, kp, vp, table, sl, window_size=window, num_prefix_tokens=prefix)
+    assert torch.equal(out, again)
+    assert K.device_status(clear=True) == 0
+
+
+PREFILL = [
+    # lens, news, Hq, Hkv, page_size, dtype, window, prefix, layout
+    ([1], [1], 1, 1, 16, BF, None, 0, "phtd"),
+    ([64], [64], 2, 2, 64, BF, None, 0, "phtd"),
+    ([130, 128, 7], [130, 128, 7], 4, 4, 32, BF, None, 0, "phtd"),
+    ([700, 300, 1000], [130, 1, 257], 7, 1, 16, FP, None, 0, "phtd"),
+    ([200, 0, 333, 500], [5, 0, 333, 20], 56, 8, 64, BF, None, 0, "ptkhd"),
+    ([1100], [1000], 16, 16, 128, BF, None, 0, "phtd"),
+    ([900, 1300, 80], [900, 200, 80], 4, 2, 64, BF, 100, 0, "phtd"),
+    ([900, 1300, 80], [900, 200, 80], 3, 1, 16, FP, 64, 33, "phtd"),
+    ([900, 1300, 80], [300, 200, 80], 8, 1, 64, BF, 0, 0, "phtd"),
+    ([900, 1300, 80], [300, 200, 80], 5, 1, 1024, BF, 257, 128, "ptkhd"),
+    ([2100], [600], 6, 1, 32, BF, 500, 700, "phtd"),
+    ([9000], [20], 2, 2, 64, BF, None, 0, "phtd"),
+    ([9000, 31], [3, 2], 7, 1, 16, FP, None, 0, "phtd"),
+    (list(range(1, 120)), list(range(1, 120)), 2, 1, 16, BF, None, 0, "phtd"),
+]
+
+
+@pytest.mark.parametrize("case", range(len(PREFILL)))
+def test_paged_prefill_vs_oracle(K, case):
+    lens, news, Hq, Hkv, ps, dtype, window, prefix, layout = PREFILL[case]
+    args = make(100 + case, lens, news, Hq, Hkv, ps, dtype, window, prefix, layout)
+    q, kp, vp, table, sl, starts = args
+    pad = 5
+    qq = torch.cat([q, torch.full((pad,) + tuple(q.shape[1:]), float("nan"), dtype=dtype, device=q.device)])
+    out = torch.full_like(qq, 7.0)
+    K.paged_prefill(qq, kp, vp, table, sl, starts, window_size=window, num_prefix_tokens=prefix, out=out)
+    assert (out[q.shape[0]:] == 7.0).all(), "rows behind the last sequence were written"
+    check(out[:q.shape[0]], args, window, prefix, starts=starts)
+    again = K.paged_prefill(q, kp, vp, table, sl, starts, window_size=window, num_prefix_tokens=prefix)
+    assert torch.equal(out[:q.shape[0]], again)
+    assert K.device_status(clear=True) == 0
+
+
+def test_rows_that_see_nothing_give_zeros(K):
+    """Sequences shorter than their new rows, absent pages under every visible
+    key, lengths of zero."""
+    q, kp, vp, table, sl, starts = make(5, [40, 100, 64], [40, 100, 64], 4, 2, 16, BF)
+    table[1] = -1
+    sl[0] = 10  # 30 of the 40 rows lie before the sequence
+    out = K.paged_prefill(q, kp, vp, table, sl, starts)
+    assert (out[:30] == 0).all() and (out[40:140] == 0).all() and (out[140:] != 0).any()
+    check(out, (q, kp, vp, table, sl, starts), starts=starts)
+    sl[2] = 0
+    out = K.paged_decode(q[:3], kp, vp, table, sl)
+    assert (out[1:] == 0).all() and (out[0] != 0).any()
+
+
+@pytest.mark.parametrize("ps", [16, 64, 128])
+def test_absent_pages_inside_a_tile(K, ps):
+    """Pages missing at the start, inside and at the end are not visible."""
+    args = make(6, [1000, 900], [1, 1], 6, 2, ps, BF)
+    q, kp, vp, table, sl, _ = args
+    for b, p in ((0, 0), (0, 3), (0, 4), (1, 1), (1, 899 // ps)):
+        if table[b, p] >= 0:
+            kp[table[b, p]] = float("nan")
+            vp[table[b, p]] = float("nan")
+        table[b, p] = -1
+    check(K.paged_decode(q, kp, vp, table, sl), args)
+    starts = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    check(K.paged_prefill(q, kp, vp, table, sl, starts), args)
+    assert K.device_status(clear=True) == 0
+
+
+def test_pages_outside_the_pool_are_absent_and_recorded(K):
+    args = make(7, [200, 300], [1, 1], 4, 2, 32, BF)
+    q, kp, vp, table, sl, _ = args
+    table[0, 2] = kp.shape[0]
+    table[1, 1] = -5
+    check(K.paged_decode(q, kp, vp, table, sl), args)
+    assert K.device_status(clear=True) == 4
+    starts = torch.tensor([0, 1, 2], dtype=torch.int32, device="cuda")
+    check(K.paged_prefill(q, kp, vp, table, sl, starts), args)
+    assert K.device_status(clear=True) == 4
+    sl[0] = 96  # the new row would go to the bad page
+    before = kp.clone()
+    K.paged_store(q[:, :2], q[:, 2:], kp, vp, table, sl)
+    assert K.device_status(clear=True) == 4
+    changed = (kp != before) & ~(kp.isnan() & before.isnan())
+    assert changed.flatten(1).any(1).nonzero().flatten().tolist() == [int(table[1, 299 // 32])]
+
+
+def test_lengths_past_the_table_read_only_what_it_holds(K):
+    args = make(8, [128, 256], [1, 1], 2, 2, 64, BF, extra_cols=0)
+    q, kp, vp, table, sl, _ = args
+    sl[1] = 100000
+    check(K.paged_decode(q, kp, vp, table, sl), (q, kp, vp, table, sl, None))
+    K.paged_store(q, q, kp, vp, table, sl)  # the second row has no place
+    assert K.device_status(clear=True) == 4
+
+
+def test_strided_rows_scale_and_output(K):
+    """q a slice of a fused projection, out a view of a wider buffer, scores at
+    another scale."""
+    args = make(9, [500, 77, 130], [200, 77, 1], 4, 2, 32, BF)
+    q, kp, vp, table, sl, starts = args
+    fused = torch.randn(q.shape[0], 8, D, device="cuda").to(BF)
+    fused[:, 2:6] = q
+    wide = torch.full((q.shape[0], 8, D), 3.0, dtype=BF, device="cuda")
+    K.paged_prefill(fused[:, 2:6], kp, vp, table, sl, starts, softmax_scale=0.21, out=wide[:, 1:5])
+    check(wide[:, 1:5], args, scale=0.21, starts=starts)
+    assert (wide[:, 0] == 3.0).all() and (wide[:, 5:] == 3.0).all()
+    wide.fill_(3.0)
+    K.paged_decode(fused[:3, 2:6], kp, vp, table, sl, softmax_scale=0.21, out=wide[:3, 1:5])
+    check(wide[:3, 1:5], (q[:3],) + args[1:], scale=0.21)
+    assert (wide[:, 0] == 3.0).all() and (wide[:, 5:] == 3.0).all()
+
+
+def test_large_scores_stay_finite(K):
+    """Scores in the hundreds, rising along the sequence, in both types."""
+    for dtype in (BF, FP):
+        args = make(10, [700, 90], [150, 90], 4, 1, 16, dtype)
+        q, kp, vp, table, sl, starts = args
+        q *= 40
+        check(K.paged_prefill(q, kp, vp, table, sl, starts), args, starts=starts)
+        last = (q[starts[1:].long() - 1],) + args[1:]
+        check(K.paged_decode(*last[:5]), last)
+
+
+@pytest.mark.parametrize("dtype,ps,layout", [(BF, 16, "phtd"), (FP, 64, "ptkhd"), (BF, 1024, "phtd")])
+def test_paged_store_writes_its_rows_and_nothing_else(K, dtype, ps, layout):
+    lens, news = [1, 70, 300, 90, 64, 0], [1, 7, 290, 0, 64, 0]
+    args = make(11, lens, news, 1, 3, ps, dtype, layout=layout)
+    _, kp, vp, table, sl, starts = args
+    kp.fill_(0.5), vp.fill_(-0.5)
+    table[2, 1] = -1  # dropped silently
+    n = int(starts[-1])
+    k = torch.randn(n + 9, 6, D, device="cuda").to(dtype)[:, ::2]
+    v = torch.randn(n + 9, 3, D, device="cuda").to(dtype)
+    wk, wv = kp.clone(), vp.clone()
+    for r, page, off in PO.slots(table, sl, starts, ps, kp.shape[0]):
+        wk[page, :, off] = k[r]
+        wv[page, :, off] = v[r]
+    K.paged_store(k, v, kp, vp, table, sl, starts)
+    assert torch.equal(kp, wk) and torch.equal(vp, wv)
+    assert K.device_status(clear=True) == 0
+    # One row per sequence without starts.
+    B = len(lens)
+    sl2 = (sl + 1).clamp(max=table.shape[1] * ps)
+    for r, page, off in PO.slots(table, sl2, None, ps, kp.shape[0]):
+        wk[page, :, off] = k[r]
+        wv[page, :, off] = v[r]
+    K.paged_store(k[:B], v[:B], kp, vp, table, sl2)
+    assert torch.equal(kp, wk) and torch.equal(vp, wv)
+
+
+@pytest.mark.parametrize("shape,moves", [((5, 2, 9, 3, 16, D), 4), ((7, 1, 16, D), 2), ((2, 1300, 1, 16, D), 600),
+                                         ((3, 40, 8, 128, D), 17)])
+def test_copy_pages(K, shape, moves):
+    gen = torch.Generator().manual_seed(12)
+    pages = torch.randn(*shape, generator=gen).to(BF).cuda()
+    order = torch.randperm(shape[-4], generator=gen)
+    src, dst = order[:moves], order[moves:2 * moves]
+    want = pages.clone()
+    want[..., dst.cuda(), :, :, :] = want[..., src.cuda(), :, :, :]
+    K.copy_pages(pages, src, dst.tolist())
+    assert torch.equal(pages, want)
+
+
+def test_copy_pages_one_source_many_targets_strided_pool_other_type(K):
+    pool = torch.randint(-100, 100, (3, 12, 4, 2, 16, D), dtype=torch.int8, device="cuda")
+    pages = pool[:, :, 1]  # pages at a wider stride
+    want = pool.clone()
+    for d in (2, 5, 11):
+        want[:, d, 1] = want[:, 7, 1]
+    K.copy_pages(pages, [7, 7, 7], [2, 5, 11])
+    assert torch.equal(pool, want)
+    with pytest.raises(K.SabreError, match="written twice"):
+        K.copy_pages(pages, [1, 3], [4, 4])
+    with pytest.raises(K.SabreError, match="read and written"):
+        K.copy_pages(pages, [1, 4], [4, 6])
+    assert torch.equal(pool, want)
+
+
+def test_captured_step_replays_with_new_tables(K):
+    """Store and decode captured once; replays follow the tensors' contents, and
+    an eager call on another stream between them changes nothing."""
+    args = make(13, [200, 64, 900], [1, 1, 1], 4, 2, 32, BF)
+    q, kp, vp, table, sl, _ = args
+    k, v = (torch.randn(3, 2, D, device="cuda").to(BF) for _ in range(2))
+    out = torch.empty_like(q)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        K.paged_store(k, v, kp, vp, table, sl)
+        K.paged_decode(q, kp, vp, table, sl, out=out)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        K.paged_store(k, v, kp, vp, table, sl)
+        K.paged_decode(q, kp, vp, table, sl, out=out)
+    for step in range(3):
+        if step:
+            sl.sub_(1)
+            table.copy_(table.roll(1, 0))  # the sequences trade places
+            sl.copy_(sl.roll(1, 0))
+            q.copy_(torch.randn(q.shape, device="cuda").to(BF))
+        with torch.cuda.stream(side):
+            side.wait_stream(torch.cuda.current_stream())
+            K.paged_decode(q[:1], kp, vp, table[:1], sl[:1])
+        torch.cuda.current_stream().wait_stream(side)
+        graph.replay()
+        torch.cuda.synchronize()
+        check(out, (q, kp, vp, table, sl, None))
+    assert K.device_status(clear=True) == 0
+
+
+def test_pool_past_32_bit_offsets(K):
+    """Pages that start past 2^31 elements of the pool."""
+    Hkv, ps = 8, 128
+    P = 2 ** 31 // (Hkv * ps * D) + 40
+    kp = torch.empty(P, Hkv, ps, D, dtype=BF, device="cuda")
+    vp = torch.empty(P, Hkv, ps, D, dtype=BF, device="cuda")
+    kp[:40], vp[:40], kp[-40:], vp[-40:] = 9.0, 9.0, 0.0, 0.0
+    lens = [700, 129]
+    table = torch.full((2, 7), -1, dtype=torch.int32)
+    table[0, :6] = torch.arange(P - 1, P - 7, -1)
+    table[1, :2] = torch.tensor([P - 20, P - 10])
+    table = table.cuda()
+    sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    starts = torch.tensor([0, 700, 829], dtype=torch.int32, device="cuda")
+    k, v = (torch.randn(829, Hkv, D, device="cuda").to(BF) for _ in range(2))
+    K.paged_store(k, v, kp, vp, table, sl, starts)
+    assert torch.equal(PO.gather(kp, table[0], 700)[0], k[:700].double())
+    q = torch.randn(829, Hkv, D, device="cuda").to(BF)
+    args = (q, kp, vp, table, sl, starts)
+    check(K.paged_prefill(q, kp, vp, table, sl, starts), args, starts=starts)
+    last = (q[[699, 828]],) + args[1:]
+    check(K.paged_decode(*last[:5]), last)
+    K.copy_pages(kp, [P - 1, P - 20], [P - 30, 3])
+    assert torch.equal(kp[P - 30], kp[P - 1]) and torch.equal(kp[3], kp[P - 20])
+    assert (kp[:3] == 9.0).all() and (kp[4:40] == 9.0).all()
+
+
+def test_empty_calls(K):
+    q, kp, vp, table, sl, starts = make(14, [20], [20], 2, 1, 16, BF)
+    e = torch.empty(0, 2, D, dtype=BF, device="cuda")
+    none = torch.empty(0, 2, dtype=torch.int32, device="cuda")
+    zero = torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert K.paged_decode(e, kp, vp, none, zero[:0]).shape == (0, 2, D)
+    assert K.paged_prefill(e, kp, vp, none, zero[:0], zero).shape == (0, 2, D)
+    K.paged_store(e[:, :1], e[:, :1], kp, vp, none, zero[:0], zero)
+    K.copy_pages(kp, [], [])
