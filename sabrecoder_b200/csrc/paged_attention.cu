@@ -123,24 +123,6 @@ static int attend(const char* fn, const void* q, const void* k_pages, const void
 
 extern "C" {
 
-size_t sabre_paged_decode_workspace_size(int batch, int heads_q, int heads_kv, int head_dim) {
-  (void)batch, (void)heads_q, (void)heads_kv, (void)head_dim;
-  return 0;
-}
-
-int sabre_paged_decode(const void* q, const void* k_pages, const void* v_pages, void* o, const int32_t* page_table,
-                       const int32_t* seq_lens, int batch, int heads_q, int heads_kv, int head_dim, int num_pages,
-                       int page_size, int max_pages, int window, int num_prefix_tokens, const int64_t* q_strides,
-                       const int64_t* kp_strides, const int64_t* vp_strides, const int64_t* o_strides,
-                       int64_t table_stride, float softmax_scale, int dtype, void* workspace, size_t workspace_bytes,
-                       void* stream) {
-  (void)workspace, (void)workspace_bytes;
-  return sabre::paged::attend("sabre_paged_decode", q, k_pages, v_pages, o, page_table, seq_lens, nullptr, batch,
-                              batch, heads_q, heads_kv, head_dim, num_pages, page_size, max_pages, window,
-                              num_prefix_tokens, q_strides, kp_strides, vp_strides, o_strides, table_stride,
-                              softmax_scale, dtype, stream);
-}
-
 size_t sabre_paged_prefill_workspace_size(int rows, int batch, int heads_q, int heads_kv, int head_dim, int page_size,
                                           int max_pages, int window, int num_prefix_tokens) {
   (void)rows, (void)batch, (void)heads_q, (void)heads_kv, (void)head_dim, (void)page_size, (void)max_pages;

@@ -6,8 +6,7 @@
 // page page_table[b][t / page_size] at row t % page_size. A table entry of -1
 // means the page is absent: its rows are not stored and not visible. Any other
 // entry outside [0, num_pages) is treated the same way and recorded as
-// SABRE_DEV_BAD_PAGE.
-#include "common.cuh"
+// SABRE_DEV_BAD_PAGE. Included by sabre_capi.cu after its host helpers.
 
 namespace sabre {
 namespace paged {
@@ -151,8 +150,6 @@ __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_c
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
-static inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
-
 // Checks shared by the paged entry points; fills c. `kp` / `vp` strides are
 // {page, head, row} in elements.
 static int make_cache(Cache* c, const char* fn, const void* k_pages, const void* v_pages, const int32_t* page_table,

@@ -18,7 +18,6 @@
 #include "topk.cu"
 #include "similarity.cu"
 #include "token_mask.cu"
-#include "paged_cache.cu"
 
 #define SABRE_VERSION 100
 
@@ -101,6 +100,8 @@ static int ensure_smem_attr(Kern kern, int bytes) {
 
 #include "decode_gqa.cu"
 #include "qkv_prefill.cu"
+#include "paged_cache.cu"
+#include "paged_decode.cu"
 #include "paged_attention.cu"
 
 using namespace sabre;
