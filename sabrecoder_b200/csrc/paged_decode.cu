@@ -170,12 +170,12 @@ struct Segments {
   }
 };
 
-__device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* m, uint32_t bar, int row, int head,
-                                              int page) {
+__device__ __forceinline__ void tma_load_page(uint32_t dst, const CUtensorMap* m, uint32_t bar, int row, int half,
+                                              int head, int page) {
   asm volatile(
       "cp.async.bulk.tensor.5d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
       " [%0], [%1, {%3, %4, %5, %6, %7}], [%2];" ::"r"(dst),
-      "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(0), "r"(row), "r"(0), "r"(head), "r"(page)
+      "l"(reinterpret_cast<uint64_t>(m)), "r"(bar), "r"(0), "r"(row), "r"(half), "r"(head), "r"(page)
       : "memory");
 }
 
@@ -301,8 +301,8 @@ __global__ void __launch_bounds__(kDecThreads, 2)
           const int x = lane - (i - i0);
           if (x >= 0 && x < boxes && page >= 0) {
             const uint32_t dst = sbase + kRingOff + s * 2 * kTileBytes + x * box_bytes;
-            tma_load_page(dst, &tmK, full_bar(s), off, seg.hk, page);
-            tma_load_page(dst + kTileBytes, &tmV, full_bar(s), off, seg.hk, page);
+            tma_load_page(dst, &tmK, full_bar(s), off, 0, seg.hk, page);
+            tma_load_page(dst + kTileBytes, &tmV, full_bar(s), off, 0, seg.hk, page);
           }
           issued = it + 1;
         }

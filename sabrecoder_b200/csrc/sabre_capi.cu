@@ -102,7 +102,7 @@ static int ensure_smem_attr(Kern kern, int bytes) {
 #include "qkv_prefill.cu"
 #include "paged_cache.cu"
 #include "paged_decode.cu"
-#include "paged_attention.cu"
+#include "paged_prefill.cu"
 
 using namespace sabre;
 

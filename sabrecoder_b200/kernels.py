@@ -545,10 +545,36 @@ def token_tile_masks(tok_chunk: torch.Tensor, tok_group: torch.Tensor, tok_globa
 # (4) paged K/V cache
 # ---------------------------------------------------------------------------
 
-def _paged_check(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
-                 seq_lens: torch.Tensor, q_start: Optional[torch.Tensor], **rows: Optional[torch.Tensor]) -> int:
-    """Checks the arguments the paged calls share (``rows``: the ``[N, H, D]``
-    tensors of the new rows); returns the number of sequences."""
+_S2, _S3 = ctypes.c_int64 * 2, ctypes.c_int64 * 3
+
+
+def _paged_ok(k_pages, v_pages, page_table, seq_lens, q_start, rows) -> bool:
+    """The conditions of :func:`_paged_refuse` in one pass (a decode step is as
+    long as a few of these lookups)."""
+    dt, dev = k_pages.dtype, k_pages.get_device()
+    ks, vs, ts = k_pages.shape, v_pages.shape, page_table.shape
+    if dev < 0 or dt not in DTYPE_CODE or v_pages.dtype is not dt or len(ks) != 4 or vs != ks or len(ts) != 2:
+        return False
+    B, D = ts[0], ks[3]
+    if ts[1] < 1 or (ts[1] > 1 and page_table.stride(1) != 1) or k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
+        return False
+    if v_pages.get_device() != dev or page_table.dtype is not torch.int32 or page_table.get_device() != dev:
+        return False
+    if (seq_lens.shape != (B,) or seq_lens.dtype is not torch.int32 or not seq_lens.is_contiguous()
+            or seq_lens.get_device() != dev):
+        return False
+    if q_start is not None and (q_start.shape != (B + 1,) or q_start.dtype is not torch.int32
+                                or not q_start.is_contiguous() or q_start.get_device() != dev):
+        return False
+    for t in rows.values():
+        if t is not None and (t.dtype is not dt or t.dim() != 3 or t.shape[2] != D or t.stride(2) != 1
+                              or t.get_device() != dev):
+            return False
+    return True
+
+
+def _paged_refuse(what: str, k_pages, v_pages, page_table, seq_lens, q_start, rows) -> None:
+    """Raises with what is wrong about the arguments the paged calls share."""
     ts = dict(k_pages=k_pages, v_pages=v_pages, page_table=page_table, seq_lens=seq_lens, q_start=q_start, **rows)
     if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
         raise SabreError(f"{what}: k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} must both be "
@@ -577,13 +603,19 @@ def _paged_check(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor, page_t
     for name, t in ts.items():
         if t is not None and t.device != k_pages.device:
             raise SabreError(f"{what}: {name} is on {t.device}, the pages are on {k_pages.device}")
-    return B
+    raise SabreError(f"{what}: invalid arguments")
 
 
-def _paged_args(k_pages: torch.Tensor, page_table: torch.Tensor):
-    """(heads_kv, head_dim, num_pages, page_size, max_pages) for the C entry points."""
-    P, Hkv, ps, D = k_pages.shape
-    return Hkv, D, P, ps, page_table.shape[1]
+def _paged_call(what: str, dev: int, fn, *args) -> None:
+    """Calls a C entry point on the current stream of CUDA device `dev`, with
+    that device current."""
+    if torch.cuda.current_device() == dev:
+        st = fn(*args, torch.cuda.current_stream().cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            st = fn(*args, torch.cuda.current_stream().cuda_stream)
+    if st != 0:
+        check(st, what)
 
 
 def _window_code(what: str, window_size: Optional[int], num_prefix_tokens: int) -> Tuple[int, int]:
@@ -595,14 +627,19 @@ def _window_code(what: str, window_size: Optional[int], num_prefix_tokens: int) 
     return w, min(int(num_prefix_tokens), 2 ** 31 - 1)
 
 
-def _workspace(what: str, workspace: Optional[torch.Tensor], need: int, device) -> Optional[torch.Tensor]:
+def _workspace(what: str, workspace: Optional[torch.Tensor], need: int, device):
+    """(pointer, bytes, keep-alive) of the caller's workspace or of a new one."""
     if workspace is None:
-        return torch.empty(need, dtype=torch.uint8, device=device) if need else None
+        if not need:
+            return None, 0, None
+        workspace = torch.empty(need, dtype=torch.uint8, device=device)
+        return workspace.data_ptr(), need, workspace
+    nbytes = workspace.numel() * workspace.element_size()
     if workspace.device != device or not workspace.is_contiguous():
         raise SabreError(f"{what}: workspace must be contiguous on {device}")
-    if workspace.numel() * workspace.element_size() < need:
-        raise SabreError(f"{what}: workspace holds {workspace.numel() * workspace.element_size()} < {need} bytes")
-    return workspace
+    if nbytes < need:
+        raise SabreError(f"{what}: workspace holds {nbytes} < {need} bytes")
+    return workspace.data_ptr(), nbytes, workspace
 
 
 def paged_store(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -615,21 +652,21 @@ def paged_store(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages
     with the new rows; q_start int32 ``[B + 1]``: rows ``q_start[b] ..
     q_start[b+1]-1`` are the last rows of sequence b (default: one row each,
     ``N == B``). Rows from ``q_start[B]`` on are padding."""
-    B = _paged_check("paged_store", k_pages, v_pages, page_table, seq_lens, q_start, k=k, v=v)
-    if k.shape != v.shape or k.shape[1] != k_pages.shape[1]:
-        raise SabreError(f"paged_store: k {tuple(k.shape)} and v {tuple(v.shape)} must both be [N, "
-                         f"{k_pages.shape[1]}, D]")
-    if q_start is None and k.shape[0] != B:
-        raise SabreError(f"paged_store: {k.shape[0]} rows for {B} sequences need q_start")
-    if k.shape[0] == 0 or B == 0:
+    rows = dict(k=k, v=v)
+    if not _paged_ok(k_pages, v_pages, page_table, seq_lens, q_start, rows):
+        _paged_refuse("paged_store", k_pages, v_pages, page_table, seq_lens, q_start, rows)
+    (P, Hkv, ps, D), (B, cols), (N, heads, _) = k_pages.shape, page_table.shape, k.shape
+    if v.shape != k.shape or heads != Hkv:
+        raise SabreError(f"paged_store: k {tuple(k.shape)} and v {tuple(v.shape)} must both be [N, {Hkv}, {D}]")
+    if q_start is None and N != B:
+        raise SabreError(f"paged_store: {N} rows for {B} sequences need q_start")
+    if N == 0 or B == 0:
         return
-    with torch.cuda.device(k_pages.device):
-        st = lib().sabre_paged_store(
-            k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
-            seq_lens.data_ptr(), _ptr(q_start), k.shape[0], B, *_paged_args(k_pages, page_table),
-            i64(k.stride()[:2]), i64(v.stride()[:2]), i64(k_pages.stride()[:3]), i64(v_pages.stride()[:3]),
-            page_table.stride(0), DTYPE_CODE[k.dtype], _stream(k))
-    check(st, "sabre_paged_store")
+    _paged_call("sabre_paged_store", k.get_device(), lib().sabre_paged_store,
+                k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
+                seq_lens.data_ptr(), _ptr(q_start), N, B, Hkv, D, P, ps, cols, _S2(*k.stride()[:2]),
+                _S2(*v.stride()[:2]), _S3(*k_pages.stride()[:3]), _S3(*v_pages.stride()[:3]), page_table.stride(0),
+                DTYPE_CODE[k.dtype])
     LAUNCHES[0] += 1
 
 
@@ -644,25 +681,25 @@ def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     sees key j <= i when ``i - j <= window_size`` or ``j < num_prefix_tokens``.
     A sequence that sees nothing (length 0) gives zeros. Deterministic."""
     window, prefix = _window_code("paged_decode", window_size, num_prefix_tokens)
-    B = _paged_check("paged_decode", k_pages, v_pages, page_table, seq_lens, None, q=q, out=out)
-    Hkv, Hq = k_pages.shape[1], q.shape[1]
+    rows = dict(q=q, out=out)
+    if not _paged_ok(k_pages, v_pages, page_table, seq_lens, None, rows):
+        _paged_refuse("paged_decode", k_pages, v_pages, page_table, seq_lens, None, rows)
+    (P, Hkv, ps, D), (B, cols), Hq = k_pages.shape, page_table.shape, q.shape[1]
     if q.shape[0] != B or (out is not None and out.shape != q.shape):
         raise SabreError(f"paged_decode: q {tuple(q.shape)} and out must be [B={B}, Hq, D]")
     if out is None:
-        out = torch.empty_like(q)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if q.numel() == 0:
         return out
-    ws = _workspace("paged_decode", workspace,
-                    int(lib().sabre_paged_decode_workspace_size(B, Hq, Hkv, q.shape[2])), q.device)
-    with torch.cuda.device(q.device):
-        st = lib().sabre_paged_decode(
-            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), page_table.data_ptr(),
-            seq_lens.data_ptr(), B, Hq, *_paged_args(k_pages, page_table), window, prefix, i64(q.stride()[:2]),
-            i64(k_pages.stride()[:3]), i64(v_pages.stride()[:3]), i64(out.stride()[:2]), page_table.stride(0),
-            float(softmax_scale or 0.0), DTYPE_CODE[q.dtype], _ptr(ws),
-            0 if ws is None else ws.numel() * ws.element_size(), _stream(q))
-    check(st, "sabre_paged_decode")
-    LAUNCHES[0] += 1
+    L = lib()
+    ws, ws_bytes, _keep = _workspace("paged_decode", workspace,
+                                     L.sabre_paged_decode_workspace_size(B, Hq, Hkv, D), q.device)
+    _paged_call("sabre_paged_decode", q.get_device(), L.sabre_paged_decode,
+                q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), page_table.data_ptr(),
+                seq_lens.data_ptr(), B, Hq, Hkv, D, P, ps, cols, window, prefix, _S2(*q.stride()[:2]),
+                _S3(*k_pages.stride()[:3]), _S3(*v_pages.stride()[:3]), _S2(*out.stride()[:2]), page_table.stride(0),
+                softmax_scale or 0.0, DTYPE_CODE[q.dtype], ws, ws_bytes)
+    LAUNCHES[0] += 2
     return out
 
 
@@ -677,26 +714,24 @@ def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     rows of sequence b, the rest as in :func:`paged_decode`. Rows of ``out``
     from ``q_start[B]`` on are left as they are."""
     window, prefix = _window_code("paged_prefill", window_size, num_prefix_tokens)
-    B = _paged_check("paged_prefill", k_pages, v_pages, page_table, seq_lens, q_start, q=q, out=out)
-    Hkv, Hq = k_pages.shape[1], q.shape[1]
+    rows = dict(q=q, out=out)
+    if not _paged_ok(k_pages, v_pages, page_table, seq_lens, q_start, rows):
+        _paged_refuse("paged_prefill", k_pages, v_pages, page_table, seq_lens, q_start, rows)
+    (P, Hkv, ps, D), (B, cols), (N, Hq, _) = k_pages.shape, page_table.shape, q.shape
     if out is not None and out.shape != q.shape:
         raise SabreError(f"paged_prefill: out {tuple(out.shape)} must have q's shape {tuple(q.shape)}")
     if out is None:
-        out = torch.empty_like(q)
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if q.numel() == 0 or B == 0:
         return out
-    args = _paged_args(k_pages, page_table)
-    ws = _workspace("paged_prefill", workspace,
-                    int(lib().sabre_paged_prefill_workspace_size(q.shape[0], B, Hq, Hkv, q.shape[2], args[3], args[4],
-                                                                 window, prefix)), q.device)
-    with torch.cuda.device(q.device):
-        st = lib().sabre_paged_prefill(
-            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), page_table.data_ptr(),
-            seq_lens.data_ptr(), q_start.data_ptr(), q.shape[0], B, Hq, *args, window, prefix, i64(q.stride()[:2]),
-            i64(k_pages.stride()[:3]), i64(v_pages.stride()[:3]), i64(out.stride()[:2]), page_table.stride(0),
-            float(softmax_scale or 0.0), DTYPE_CODE[q.dtype], _ptr(ws),
-            0 if ws is None else ws.numel() * ws.element_size(), _stream(q))
-    check(st, "sabre_paged_prefill")
+    L = lib()
+    ws, ws_bytes, _keep = _workspace("paged_prefill", workspace, L.sabre_paged_prefill_workspace_size(
+        N, B, Hq, Hkv, D, ps, cols, window, prefix), q.device)
+    _paged_call("sabre_paged_prefill", q.get_device(), L.sabre_paged_prefill,
+                q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), page_table.data_ptr(),
+                seq_lens.data_ptr(), q_start.data_ptr(), N, B, Hq, Hkv, D, P, ps, cols, window, prefix,
+                _S2(*q.stride()[:2]), _S3(*k_pages.stride()[:3]), _S3(*v_pages.stride()[:3]), _S2(*out.stride()[:2]),
+                page_table.stride(0), softmax_scale or 0.0, DTYPE_CODE[q.dtype], ws, ws_bytes)
     LAUNCHES[0] += 1
     return out
 
@@ -710,34 +745,42 @@ def copy_pages(pages: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -> N
     synchronises nor copies to the device and can be captured. Pages are
     copied in no order: a page outside the pool, written twice, or both read
     and written raises and nothing is copied."""
+    moves = []
     for name, t in (("src", src), ("dst", dst)):
-        if isinstance(t, torch.Tensor) and (t.is_cuda or t.dim() != 1 or t.is_floating_point()):
-            raise SabreError(f"copy_pages: {name} must be a list of ints or a 1-D CPU integer tensor")
-    src = src.tolist() if isinstance(src, torch.Tensor) else list(src)
-    dst = dst.tolist() if isinstance(dst, torch.Tensor) else list(dst)
-    if len(src) != len(dst):
-        raise SabreError(f"copy_pages: {len(src)} sources for {len(dst)} destinations")
+        if isinstance(t, torch.Tensor):
+            if t.is_cuda or t.dim() != 1 or t.is_floating_point():
+                raise SabreError(f"copy_pages: {name} must be a list of ints or a 1-D CPU integer tensor")
+            t = t.tolist()
+        moves.append(t)
+    src, dst = moves
+    n = len(src)
+    if n != len(dst):
+        raise SabreError(f"copy_pages: {n} sources for {len(dst)} destinations")
     if pages.dim() < 4:
         raise SabreError(f"copy_pages: pages {tuple(pages.shape)} must be [..., num_pages, Hkv, page_size, D]")
-    for m, (a, b) in enumerate(zip(src, dst)):
-        if not (0 <= a < pages.shape[-4] and 0 <= b < pages.shape[-4]):
-            raise SabreError(f"copy_pages: move {m} ({a} -> {b}) is outside the pool of {pages.shape[-4]} pages")
+    shape, strides = pages.shape, pages.stride()
+    P = shape[-4]
+    for page in (*src, *dst):
+        if not 0 <= page < P:
+            raise SabreError(f"copy_pages: page {page} is outside the pool of {P} pages")
     _need_cuda(pages=pages)
-    if pages.numel() == 0 or not src:
+    if pages.numel() == 0 or n == 0:
         return
-    page = pages[(0,) * (pages.dim() - 3)]
-    if not page.is_contiguous():
-        raise SabreError("copy_pages: each page [Hkv, page_size, D] must be contiguous")
-    lead = pages.shape[:-4]
-    try:
-        flat = pages.view((-1,) + tuple(pages.shape[-4:]))
-    except RuntimeError as e:
-        raise SabreError(f"copy_pages: the pools {tuple(lead)} are not at one stride") from e
+    unit = 1
+    for size, stride in zip(shape[:-4:-1], strides[:-4:-1]):
+        if size > 1 and stride != unit:
+            raise SabreError("copy_pages: each page [Hkv, page_size, D] must be contiguous")
+        unit *= size
+    # The leading dimensions, flattened: buffers at one stride.
+    buffers, step = 1, 0
+    for size, stride in zip(shape[-5::-1], strides[-5::-1]):
+        if size > 1 and buffers > 1 and stride != buffers * step:
+            raise SabreError(f"copy_pages: the pools {tuple(shape[:-4])} are not at one stride")
+        if size > 1 and buffers == 1:
+            step = stride
+        buffers *= size
     es = pages.element_size()
-    n = len(src)
-    with torch.cuda.device(pages.device):
-        st = lib().sabre_copy_pages(
-            flat.data_ptr(), flat.shape[0], flat.stride(0) * es, flat.shape[1], flat.stride(1) * es,
-            page.numel() * es, (ctypes.c_int32 * n)(*src), (ctypes.c_int32 * n)(*dst), n, _stream(pages))
-    check(st, "sabre_copy_pages")
+    ids = ctypes.c_int32 * n
+    _paged_call("sabre_copy_pages", pages.get_device(), lib().sabre_copy_pages, pages.data_ptr(), buffers, step * es,
+                P, strides[-4] * es, unit * es, ids(*src), ids(*dst), n)
     LAUNCHES[0] += -(-n // 480)
