@@ -48,26 +48,18 @@ __device__ __forceinline__ int row_start(const int32_t* starts, int b, int rows)
   return starts ? min(max(starts[b], 0), rows) : min(b, rows);
 }
 
-// Sequence of a ragged row: the b with start(b) <= row < start(b + 1), or -1
-// behind the last one.
-__device__ __forceinline__ int sequence_of(const int32_t* starts, int batch, int rows, int row) {
-  if (!starts) return row < batch ? row : -1;
-  int lo = 0, hi = batch;  // start(lo) <= row < start(hi), once checked
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (row_start(starts, mid, rows) <= row)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  return row >= row_start(starts, lo, rows) && row < row_start(starts, lo + 1, rows) ? lo : -1;
-}
-
 // ---------------------------------------------------------------------------
 // store
+//
+// Moves 512 bytes per KV head and row, no arithmetic: bound by HBM, and by the
+// launch and three dependent loads (starts, length, page) for a few rows. A
+// warp finds the sequence of one row by counting the starts at or before it,
+// 32 at a time; a thread then moves the same 16 bytes of eight rows, all eight
+// loads in flight.
 // ---------------------------------------------------------------------------
 constexpr int kStoreThreads = 256;
-constexpr int kStoreRows = 8;  // rows of one CTA
+constexpr int kStoreBatch = 8;                                // rows of a thread at a time
+constexpr int kStoreMaxRows = kStoreBatch * kStoreThreads / 32;  // of a CTA, one KV head
 
 struct StoreParams {
   Cache c;
@@ -77,17 +69,30 @@ struct StoreParams {
   uint4* vp;
   const int32_t* starts;
   long long k_sr, k_sh, v_sr, v_sh;  // strides of the rows, in 16-byte units
-  int rows, heads;
+  int rows, heads, cta_rows;
 };
 
 __global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(const StoreParams p) {
-  __shared__ int s_page[kStoreRows], s_off[kStoreRows];
-  const int r0 = blockIdx.x * kStoreRows;
+  __shared__ int s_page[kStoreMaxRows], s_off[kStoreMaxRows];
+  const int r0 = blockIdx.x * p.cta_rows;
   const int tid = threadIdx.x;
-  if (tid < kStoreRows) {
-    const int row = r0 + tid;
+  const int lane = tid & 31;
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // a programmatic dependent launch: inputs are ready from here on
+  for (int r = tid >> 5; r < p.cta_rows; r += kStoreThreads / 32) {
+    const int row = r0 + r;
     int page = -1, off = 0;
-    const int b = row < p.rows ? sequence_of(p.starts, p.c.batch, p.rows, row) : -1;
+    // Sequence b: start(b) <= row < start(b + 1).
+    int b = -1;
+    if (row < p.rows) {
+      if (!p.starts) {
+        b = row;
+      } else {
+        int before = 0;  // starts at or before the row
+        for (int i = lane; i <= p.c.batch; i += 32) before += p.starts[i] <= row ? 1 : 0;
+        before = __reduce_add_sync(0xffffffffu, before);
+        b = before <= p.c.batch ? before - 1 : -1;
+      }
+    }
     if (b >= 0) {
       const int pos = p.c.seq_lens[b] - (row_start(p.starts, b + 1, p.rows) - row);
       if (pos >= 0 && pos < p.c.capacity()) {
@@ -97,24 +102,32 @@ __global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(const StoreP
         record_status(SABRE_DEV_BAD_PAGE);
       }
     }
-    s_page[tid] = page;
-    s_off[tid] = off;
+    if (lane == 0) {
+      s_page[r] = page;
+      s_off[r] = off;
+    }
   }
   __syncthreads();
   // 16 threads move one head's row of K or V (256 bytes).
-  const int per_row = p.heads * 32;
-  for (int i = tid; i < kStoreRows * per_row; i += kStoreThreads) {
-    const int r = i / per_row;
-    const int u = i - r * per_row;
+  const int units = p.heads * 32;
+  for (int i = tid; i < units * (p.cta_rows / kStoreBatch); i += kStoreThreads) {
+    const int rb = i / units * kStoreBatch;
+    const int u = i % units;
     const int h = u >> 5;
     const int ch = u & 15;
-    const int page = s_page[r];
-    if (page < 0) continue;
-    const long long row = r0 + r;
-    if (u & 16)
-      p.vp[page * p.c.v_sp + h * p.c.v_sh + s_off[r] * p.c.v_st + ch] = __ldg(p.v + row * p.v_sr + h * p.v_sh + ch);
-    else
-      p.kp[page * p.c.k_sp + h * p.c.k_sh + s_off[r] * p.c.k_st + ch] = __ldg(p.k + row * p.k_sr + h * p.k_sh + ch);
+    const bool is_v = (u & 16) != 0;
+    const uint4* src = (is_v ? p.v + h * p.v_sh : p.k + h * p.k_sh) + ch;
+    uint4* dst = (is_v ? p.vp + h * p.c.v_sh : p.kp + h * p.c.k_sh) + ch;
+    const long long sr = is_v ? p.v_sr : p.k_sr;
+    const long long sp = is_v ? p.c.v_sp : p.c.k_sp;
+    const long long st = is_v ? p.c.v_st : p.c.k_st;
+    uint4 x[kStoreBatch];
+#pragma unroll
+    for (int r = 0; r < kStoreBatch; ++r)
+      if (s_page[rb + r] >= 0) x[r] = src[(r0 + rb + r) * sr];
+#pragma unroll
+    for (int r = 0; r < kStoreBatch; ++r)
+      if (s_page[rb + r] >= 0) dst[s_page[rb + r] * sp + s_off[rb + r] * st] = x[r];
   }
 }
 
@@ -150,6 +163,24 @@ __global__ void __launch_bounds__(kCopyThreads) copy_pages_kernel(const __grid_c
 // ---------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------
+// Launches a programmatic dependent of the stream's previous kernel: its
+// set-up may overlap that kernel's tail; it must execute griddepcontrol.wait
+// before it touches memory.
+template <typename K, typename... A>
+static cudaError_t launch_dependent(dim3 grid, int threads, int smem, cudaStream_t s, K kernel, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // Checks shared by the paged entry points; fills c. `kp` / `vp` strides are
 // {page, head, row} in elements.
 static int make_cache(Cache* c, const char* fn, const void* k_pages, const void* v_pages, const int32_t* page_table,
@@ -229,8 +260,11 @@ int sabre_paged_store(const void* k, const void* v, void* k_pages, void* v_pages
   p.v_sh = v_strides[1] / 8;
   p.rows = rows;
   p.heads = heads_kv;
-  paged_store_kernel<<<(rows + kStoreRows - 1) / kStoreRows, kStoreThreads, 0, static_cast<cudaStream_t>(stream)>>>(p);
-  const cudaError_t e = cudaGetLastError();
+  // Eight rows of every head fill the threads from eight heads on; with fewer
+  // a CTA takes more rows.
+  p.cta_rows = kStoreBatch * (heads_kv < 8 ? 8 / heads_kv : 1);
+  const cudaError_t e = launch_dependent(dim3((rows + p.cta_rows - 1) / p.cta_rows), kStoreThreads, 0,
+                                         static_cast<cudaStream_t>(stream), paged_store_kernel, p);
   return e == cudaSuccess ? SABRE_OK : sabre_cuda_fail(e, "sabre_paged_store launch");
 }
 

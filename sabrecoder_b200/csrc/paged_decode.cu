@@ -54,6 +54,7 @@ struct DecodeParams {
   void* o;
   float* part_acc;  // [2 * kDecCtas][group][D]
   float* part_ml;   // [2 * kDecCtas][group][2]
+  int4* joins;      // [kDecCtas]: {parts, b, hk, slot of the first part} of the pair whose first part ends share x
   long long q_sb, q_sh, o_sb, o_sh;
   int heads_kv, group, ctas;
   int box_shift;  // a TMA box holds 1 << box_shift rows
@@ -259,7 +260,10 @@ __global__ void __launch_bounds__(kDecThreads, 2)
             *reinterpret_cast<uint4*>(out + b * p.o_sb + h * p.o_sh + d) = make_uint4(0u, 0u, 0u, 0u);
       });
   // locate()'s barriers order the mbarrier set-up above before its use.
-  if (!some) return;
+  if (!some) {
+    if (tid == 0) p.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
+    return;
+  }
   Segments seg(p, at, sh.first(blockIdx.x + 1) - sh.first(blockIdx.x));
   __syncthreads();  // the scratch of locate() is free
   bool ok = *abort_flag == 0;
@@ -451,7 +455,14 @@ __global__ void __launch_bounds__(kDecThreads, 2)
     named_bar_sync(1, kConsumers * 32);
     const bool whole_pair = seg.t0 == 0 && seg.t1 == seg.tiles.count;
     // A part is kept as the share's first (0) or last (1) segment.
-    const long long slot = (2ll * blockIdx.x + (seg.seen > 0 ? 1 : 0)) * p.group;
+    const int place = 2 * static_cast<int>(blockIdx.x) + (seg.seen > 0 ? 1 : 0);
+    const long long slot = static_cast<long long>(place) * p.group;
+    if (tid == 0 && seg.left == 0) {
+      // The share ends inside a pair that began in it: the pair is joined here.
+      const int more = seg.t0 == 0 ? seg.tiles.count - seg.t1 : 0;
+      const int parts = more > 0 ? sh.owner(sh.first(blockIdx.x + 1) + more - 1) - static_cast<int>(blockIdx.x) + 1 : 0;
+      p.joins[blockIdx.x] = make_int4(parts, seg.b, seg.hk, place);
+    }
     for (int g = 0; g < p.group; ++g) {
       float M = -INFINITY;
 #pragma unroll
@@ -482,47 +493,42 @@ __global__ void __launch_bounds__(kDecThreads, 2)
   }
 }
 
-// One CTA per (share, head of the group): when the share's last segment is the
-// first part of a pair, joins that pair's parts in share order.
+// One CTA per (share, head of the group): joins the parts of the pair whose
+// first part ends the share, if there is one, in share order.
 template <typename T>
 __global__ void __launch_bounds__(kD) paged_join_kernel(const DecodeParams p) {
   // The next call's kernel (a programmatic dependent too) may start its
   // set-up now; it waits for this grid before touching memory.
   if (threadIdx.x == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  __shared__ int scratch[kD / 32 + 8];
   __shared__ float sm_m[kDecCtas], sm_l[kDecCtas];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int x = blockIdx.x;
   const int g = blockIdx.y;
   const int d = threadIdx.x;
-  Shares sh;
-  Place at;
-  const bool some = locate<kD>(
-      p, p.ctas, scratch, sh, at,
-      [&](const Shares& s) { return x < s.ctas - 1 ? s.first(x + 1) - 1 : -1ll; }, [](int) {});
-  if (!some) return;
-  const long long last = sh.first(x + 1) - 1;  // the share's last tile, at `at`
-  const long long start = last - at.tile;      // the pair's tiles: [start, end)
-  const long long end = start + Tiles(p, at.b).count;
-  if (end <= last + 1 || start < sh.first(x)) return;  // finished here, or begun in an earlier share
-  const int parts = sh.owner(end - 1) - x + 1;
-  auto slot = [&](int i) -> long long {
-    return (2ll * (x + i) + (i == 0 && sh.first(x) < start ? 1 : 0)) * p.group + g;
-  };
+  const int4 job = p.joins[x];
+  const int parts = job.x;
+  if (parts == 0) return;
+  // The first part is the last segment of its share, the others open theirs.
+  auto slot = [&](int i) -> long long { return (i == 0 ? job.w : 2ll * (x + i)) * p.group + g; };
   for (int i = d; i < parts; i += kD) {
-    sm_m[i] = p.part_ml[slot(i) * 2];
-    sm_l[i] = p.part_ml[slot(i) * 2 + 1];
+    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot(i) * 2);
+    sm_m[i] = ml.x;
+    sm_l[i] = ml.y;
   }
+  constexpr int kBatch = 8;
+  float a[kBatch];
+#pragma unroll
+  for (int u = 0; u < kBatch; ++u) a[u] = u < parts ? p.part_acc[slot(u) * kD + d] : 0.f;
   __syncthreads();
   float M = -INFINITY;
   for (int i = 0; i < parts; ++i) M = fmaxf(M, sm_m[i]);
   float L = 0.f, A = 0.f;
   if (M != -INFINITY) {
-    constexpr int kBatch = 8;
     for (int i0 = 0; i0 < parts; i0 += kBatch) {
-      float a[kBatch];
+      if (i0 > 0) {
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) a[u] = i0 + u < parts ? p.part_acc[slot(i0 + u) * kD + d] : 0.f;
+        for (int u = 0; u < kBatch; ++u) a[u] = i0 + u < parts ? p.part_acc[slot(i0 + u) * kD + d] : 0.f;
+      }
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
         if (i0 + u >= parts) break;
@@ -532,7 +538,7 @@ __global__ void __launch_bounds__(kD) paged_join_kernel(const DecodeParams p) {
       }
     }
   }
-  static_cast<T*>(p.o)[at.b * p.o_sb + (at.hk * p.group + g) * p.o_sh + d] = DT<T>::from_f(L > 0.f ? A / L : 0.f);
+  static_cast<T*>(p.o)[job.y * p.o_sb + (job.z * p.group + g) * p.o_sh + d] = DT<T>::from_f(L > 0.f ? A / L : 0.f);
 }
 
 // Tensor map of a pool [num_pages, H, page_size, D]: dims (64 d, page rows, 2
@@ -556,21 +562,6 @@ static int make_map_pages(CUtensorMap* m, const void* base, int dtype, int pages
   return SABRE_OK;
 }
 
-template <typename K, typename... A>
-static cudaError_t launch_dependent(dim3 grid, int threads, int smem, cudaStream_t s, K kernel, A... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 // Checks of the query side, shared by the attention entry points.
 static int check_queries(const char* fn, const void* q, const void* o, int heads_q, int heads_kv, int prefix,
                          const int64_t* q_strides, const int64_t* o_strides) {
@@ -590,7 +581,10 @@ static float scale_log2(float softmax_scale) {
   return (softmax_scale > 0.f ? softmax_scale : 1.0f / sqrtf(static_cast<float>(kD))) * 1.4426950408889634f;
 }
 
-static size_t decode_workspace(int group) { return static_cast<size_t>(2) * kDecCtas * group * (kD + 2) * sizeof(float); }
+// Parts of two segments of every share, and the shares' joins.
+static size_t decode_workspace(int group) {
+  return kDecCtas * sizeof(int4) + static_cast<size_t>(2) * kDecCtas * group * (kD + 2) * sizeof(float);
+}
 
 template <typename T>
 static cudaError_t launch_paged_decode(const CUtensorMap& mk, const CUtensorMap& mv, const DecodeParams& p,
@@ -645,7 +639,8 @@ int sabre_paged_decode(const void* q, const void* k_pages, const void* v_pages, 
   const long long tiles = static_cast<long long>(batch) * heads_kv *
                           ((static_cast<long long>(page_size) * max_pages + kTile - 1) / kTile);
   p.ctas = tiles < kDecCtas ? static_cast<int>(tiles) : kDecCtas;
-  p.part_acc = static_cast<float*>(workspace);
+  p.joins = static_cast<int4*>(workspace);
+  p.part_acc = reinterpret_cast<float*>(p.joins + kDecCtas);
   p.part_ml = p.part_acc + static_cast<size_t>(2) * kDecCtas * p.group * kD;
   CUtensorMap mk, mv;
   if ((st = make_map_pages(&mk, k_pages, dtype, num_pages, heads_kv, page_size, p.c.k_sp, p.c.k_sh, p.c.k_st,

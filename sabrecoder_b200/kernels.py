@@ -547,6 +547,11 @@ def token_tile_masks(tok_chunk: torch.Tensor, tok_group: torch.Tensor, tok_globa
 
 _S2, _S3 = ctypes.c_int64 * 2, ctypes.c_int64 * 3
 
+# The current stream's handle without building a Stream object (3 us of a
+# decode step), where this torch has it.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
 
 def _paged_ok(k_pages, v_pages, page_table, seq_lens, q_start, rows) -> bool:
     """The conditions of :func:`_paged_refuse` in one pass (a decode step is as
@@ -610,10 +615,10 @@ def _paged_call(what: str, dev: int, fn, *args) -> None:
     """Calls a C entry point on the current stream of CUDA device `dev`, with
     that device current."""
     if torch.cuda.current_device() == dev:
-        st = fn(*args, torch.cuda.current_stream().cuda_stream)
+        st = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            st = fn(*args, torch.cuda.current_stream().cuda_stream)
+            st = fn(*args, _raw_stream(dev))
     if st != 0:
         check(st, what)
 
