@@ -30,6 +30,7 @@ import torch.nn as nn
 
 from . import kernels as K
 from .kv_cache import SabreKVCache
+from .paged_cache import SabrePagedKVCache
 from .sabrecoder_attention import StructureAwareSparseAttention
 
 _SPARSE_CALL_COUNT = 0
@@ -334,8 +335,21 @@ class StructureAwareAttentionWrapper(nn.Module):
                 _, qp, kp = K.rope_qkv(q, k, v, cos, sin, k_out, v_out, pos0=pos,
                                        pool_block=pool_block if pos == 0 else 0)
         # K and V rows go into [B, Hkv, T, D] storage: the cache's own buffers
-        # when it is a SabreKVCache, else new rows handed to the cache's update.
-        if isinstance(cache, SabreKVCache):
+        # when it is a SabreKVCache, else new rows handed to the cache's update
+        # or stored into the pages of a SabrePagedKVCache.
+        paged = isinstance(cache, SabrePagedKVCache)
+        fresh = True
+        if paged:
+            if self.use_sparse_for_generation:
+                raise ValueError("use_sparse_for_generation needs a contiguous cache: a SabrePagedKVCache decodes over "
+                                 "all rows or its window")
+            fresh = cache.get_seq_length(self.layer_idx) == 0
+            kn = torch.empty(B, L, Hkv, D, dtype=q.dtype, device=q.device)
+            vn = torch.empty_like(kn)
+            kh, vh = kn.transpose(1, 2), vn.transpose(1, 2)
+            store(kh, vh, 0)
+            cache.append(self.layer_idx, kn, vn)
+        elif isinstance(cache, SabreKVCache):
             kbuf, vbuf, pos0 = cache.slots(self.layer_idx, L)
             store(kbuf, vbuf, pos0)
             kh, vh = cache.advance(self.layer_idx, L)
@@ -353,7 +367,13 @@ class StructureAwareAttentionWrapper(nn.Module):
         if timing:
             torch.cuda.synchronize()
             t0 = time.perf_counter()
-        if L == 1:
+        if paged and (L == 1 or get_current_code() is None or not fresh):
+            # One new token, or prompt rows that continue cached ones (or have no
+            # structure): attention over the pages.
+            _DENSE_CALL_COUNT += 1
+            attn = (cache.decode(self.layer_idx, q.view(B, Hq, D), self.scaling) if L == 1 else
+                    cache.prefill(self.layer_idx, q, self.scaling)).view(B, L, Hq * D)
+        elif L == 1:
             _DENSE_CALL_COUNT += 0 if self.use_sparse_for_generation else 1
             _SPARSE_CALL_COUNT += 1 if self.use_sparse_for_generation else 0
             T = kh.shape[2]

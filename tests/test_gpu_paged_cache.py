@@ -1,0 +1,203 @@
+"""GPU tests of SabrePagedKVCache: the operators together, as a serving loop and
+as the patched model use them."""
+
+import pytest
+import torch
+
+from oracle import paged_oracle as PO
+from test_gpu_api import _tiny_llama
+from test_gpu_paged import check
+
+pytestmark = pytest.mark.gpu
+
+D = 128
+BF = torch.bfloat16
+
+
+@pytest.fixture(scope="module")
+def cuda():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    return torch.device("cuda")
+
+
+@pytest.mark.parametrize("Hq,Hkv,ps,window,prefix", [(4, 4, 16, None, 0), (7, 1, 64, None, 0), (8, 2, 32, 150, 40)])
+def test_serving_loop(cuda, Hq, Hkv, ps, window, prefix):
+    """Prompts of different lengths, a fork, continuations, decode steps, pages
+    given back and the pool compacted: every step's attention against the
+    64-bit oracle over the same rows held contiguously."""
+    from sabrecoder_b200 import kernels as K
+    from sabrecoder_b200.paged_cache import SabrePagedKVCache
+    gen = torch.Generator().manual_seed(ps)
+    c = SabrePagedKVCache(batch_size=4, max_seq_len=2048, num_pages=3 * 2048 // ps, page_size=ps, num_layers=2,
+                          num_kv_heads=Hkv, head_dim=D, window_size=window, num_prefix_tokens=prefix)
+    c.pool.fill_(float("nan"))
+    rows = [[torch.zeros(0, 2, Hkv, D, dtype=BF) for _ in range(4)] for _ in range(2)]
+
+    def step(new):
+        n = sum(new)
+        c.extend(new)
+        starts = torch.tensor([0] + torch.tensor(new).cumsum(0).tolist(), dtype=torch.int32, device=cuda)
+        for i, layer in enumerate(c.layers):
+            kv = torch.randn(n, 2, Hkv, D, generator=gen).to(BF)
+            for b in range(4):
+                rows[i][b] = torch.cat([rows[i][b], kv[starts[b]:starts[b + 1]]])
+            kv = kv.cuda()
+            q = torch.randn(n, Hq, D, generator=gen).to(BF).cuda()
+            K.paged_store(kv[:, 0], kv[:, 1], layer.k_pages, layer.v_pages, c.page_table, c.seq_lens, starts)
+            if all(m == 1 for m in new):
+                out = c.decode(i, q)
+            else:
+                out = K.paged_prefill(q, layer.k_pages, layer.v_pages, c.page_table, c.seq_lens, starts,
+                                      window_size=window, num_prefix_tokens=prefix)
+            # The oracle's cache: one page per sequence holding all its rows.
+            T = max(max(c.lengths), 1)
+            full = torch.zeros(4, 2, Hkv, T, D, dtype=BF)
+            for b in range(4):
+                full[b, :, :, :c.lengths[b]] = rows[i][b].permute(1, 2, 0, 3)
+            full = full.cuda()
+            check(out, (q, full[:, 0], full[:, 1], torch.arange(4, dtype=torch.int32, device=cuda)[:, None], c.seq_lens,
+                        None), window, prefix, starts=starts)
+
+    def copy(a, b):
+        for i in range(2):
+            rows[i][b] = rows[i][a]
+
+    step([300, 77, 0, 500])
+    step([1, 1, 1, 1])
+    c.fork(3, 1)
+    copy(3, 1)
+    step([5, 40, 130, 1])
+    for _ in range(ps + 3):
+        c.extend([1, 1, 1, 1])
+        c.truncate(0, c.lengths[0] - 1)
+        for b in (1, 2, 3):
+            c.truncate(b, c.lengths[b] - 1)
+    step([1, 1, 1, 1])
+    c.free(0)
+    for i in range(2):
+        rows[i][0] = rows[i][0][:0]
+    c.fork(1, 2)
+    copy(1, 2)
+    c.compact()
+    step([64, 1, 200, 3])
+    step([1, 1, 1, 1])
+    c.batch_select_indices([2, 2, 0, 1])
+    for i in range(2):
+        rows[i][:] = [rows[i][j] for j in (2, 2, 0, 1)]
+    step([1, 1, 1, 1])
+    step([2, 3, 0, 700])
+    assert K.device_status(clear=True) == 0
+
+
+def _model(cuda, H=4, Hkv=2):
+    from sabrecoder_b200 import sabrecoder_llama as SL
+    model = _tiny_llama(H, Hkv).to(cuda)
+    SL.patch_model_with_sabrecoder_attention(model, None, block_size=64, window_size=192, num_prefix_tokens=64,
+                                             num_suffix_tokens=128, global_last_k_chunks=0, max_chunk_tokens=128,
+                                             verbose=False)
+    return model
+
+
+def _close(a, b):
+    """bf16 models whose attention differs by rounding and order: within 3 % of the
+    largest logit, the bound the model tests use."""
+    assert (a.float() - b.float()).abs().max() <= 0.03 * b.float().abs().max()
+
+
+@pytest.mark.parametrize("H,Hkv", [(2, 2), (4, 2), (8, 1)])
+def test_patched_model_with_pages_matches_dynamic_cache(cuda, H, Hkv):
+    """Sparse prompt, then decode steps over the pages, in lockstep with
+    transformers' DynamicCache; a fork and a compaction on the way change nothing."""
+    from transformers import DynamicCache
+
+    from sabrecoder_b200 import sabrecoder_llama as SL
+    from sabrecoder_b200.paged_cache import SabrePagedKVCache
+    from sabrecoder_b200.sabrecoder_attention import StructureAwareMaskBuilder
+    from sabrecoder_b200.spans import make_spans
+    L = 500
+    model = _model(cuda, H, Hkv)
+    mb = StructureAwareMaskBuilder(None, block_size=64, window_size=192, num_prefix_tokens=64, num_suffix_tokens=128,
+                                   global_last_k_chunks=0, max_chunk_tokens=128)
+    bi, bc, _ = mb.build_block_indices_from_spans(make_spans(L, 8), cuda)
+    ids = torch.randint(0, 512, (1, L), generator=torch.Generator().manual_seed(1)).to(cuda)
+    ca = DynamicCache()
+    cb = SabrePagedKVCache(model.config, batch_size=1, max_seq_len=L + 40, page_size=32, device=cuda)
+    SL.set_current_code("<prompt>")
+    SL.set_precomputed_blocks(bi, bc)
+    try:
+        with torch.no_grad():
+            a = model(input_ids=ids, past_key_values=ca, use_cache=True, logits_to_keep=1).logits
+            b = model(input_ids=ids, past_key_values=cb, use_cache=True, logits_to_keep=1).logits
+            assert torch.equal(a, b)  # the same kernels on the same rows
+            for step in range(20):
+                tok = a[:, -1].argmax(-1, keepdim=True)
+                a = model(input_ids=tok, past_key_values=ca, use_cache=True).logits
+                b = model(input_ids=tok, past_key_values=cb, use_cache=True).logits
+                _close(b, a)
+                if step == 7:
+                    cb.compact()
+    finally:
+        SL.clear_current_code()
+        SL.clear_precomputed_blocks()
+    assert cb.get_seq_length() == ca.get_seq_length() == L + 20
+
+
+def test_prompt_in_chunks_and_a_forked_batch(cuda):
+    """A prompt without structure in uneven chunks gives the whole prompt's logits;
+    two forks of it continue apart, as two separate prompts would."""
+    from transformers import DynamicCache
+
+    from sabrecoder_b200.paged_cache import SabrePagedKVCache
+    model = _model(cuda)
+    ids = torch.randint(0, 512, (1, 413), generator=torch.Generator().manual_seed(2)).to(cuda)
+    tails = torch.randint(0, 512, (2, 30), generator=torch.Generator().manual_seed(3)).to(cuda)
+    cache = SabrePagedKVCache(model.config, batch_size=1, max_seq_len=600, num_pages=40, page_size=16, device=cuda)
+    with torch.no_grad():
+        want = model(input_ids=ids, past_key_values=DynamicCache(), use_cache=True).logits
+        got = [model(input_ids=part, past_key_values=cache, use_cache=True).logits for part in ids.split([200, 1, 212], 1)]
+        _close(torch.cat(got, 1), want)
+        cache.batch_repeat_interleave(2)
+        assert cache.pages_in_use == -(-413 // 16)  # shared
+        got = model(input_ids=tails, past_key_values=cache, use_cache=True).logits
+        both = torch.cat([ids.expand(2, -1), tails], 1)
+        want = model(input_ids=both, past_key_values=DynamicCache(), use_cache=True).logits[:, 413:]
+        _close(got, want)
+
+
+def test_generate_with_pages_and_a_window(cuda):
+    """model.generate over a windowed paged cache, against the same steps fed one by
+    one; the middle pages are given back."""
+    from sabrecoder_b200.paged_cache import SabrePagedKVCache
+    model = _model(cuda)
+    ids = torch.randint(0, 512, (1, 600), generator=torch.Generator().manual_seed(4)).to(cuda)
+
+    def new():
+        return SabrePagedKVCache(model.config, batch_size=1, max_seq_len=700, page_size=16, window_size=128,
+                                 num_prefix_tokens=32, device=cuda)
+
+    with torch.no_grad():
+        cache = new()
+        # The ids hold the pad id: without a mask generate would take those for padding.
+        out = model.generate(input_ids=ids, attention_mask=torch.ones_like(ids), past_key_values=cache,
+                             max_new_tokens=10, min_new_tokens=10, do_sample=False, pad_token_id=0)
+        assert out.shape == (1, 610) and cache.get_seq_length() == 609
+        assert cache.pages_in_use <= 2 + 10
+        again = new()
+        # The head over one row, as generate runs it: the steps are then the same
+        # kernels on the same values, and the tokens equal.
+        logits = model(input_ids=ids, past_key_values=again, use_cache=True, logits_to_keep=1).logits
+        for i in range(600, 609):
+            assert int(logits[0, -1].float().argmax()) == int(out[0, i])
+            logits = model(input_ids=out[:, i:i + 1], past_key_values=again, use_cache=True).logits
+
+
+def test_sparse_generation_refuses_pages(cuda):
+    from sabrecoder_b200 import sabrecoder_llama as SL
+    from sabrecoder_b200.paged_cache import SabrePagedKVCache
+    model = _tiny_llama(2, 2).to(cuda)
+    SL.patch_model_with_sabrecoder_attention(model, None, use_sparse_for_generation=True, verbose=False)
+    cache = SabrePagedKVCache(model.config, max_seq_len=64, device=cuda)
+    with pytest.raises(ValueError, match="contiguous cache"):
+        model(input_ids=torch.zeros(1, 8, dtype=torch.long, device=cuda), past_key_values=cache, use_cache=True)
+    assert cache.get_seq_length() == 0

@@ -1,0 +1,233 @@
+"""Host logic of SabrePagedKVCache on the CPU: the two kernels it calls are
+replaced by plain loops."""
+
+import random
+
+import pytest
+import torch
+
+from oracle import paged_oracle as PO
+from sabrecoder_b200 import paged_cache as PC
+
+H, D = 2, 8
+
+
+@pytest.fixture(autouse=True)
+def plain_kernels(monkeypatch):
+    def copy_pages(pages, src, dst):
+        assert len(set(dst)) == len(dst) and not set(src) & set(dst)
+        pages[..., dst, :, :, :] = pages[..., src, :, :, :]
+
+    def paged_store(k, v, kp, vp, table, lens, starts=None):
+        for r, page, off in PO.slots(table, lens, starts, kp.shape[2], kp.shape[0]):
+            kp[page, :, off], vp[page, :, off] = k[r], v[r]
+
+    monkeypatch.setattr(PC.K, "copy_pages", copy_pages)
+    monkeypatch.setattr(PC.K, "paged_store", paged_store)
+
+
+def cache(**kw):
+    a = dict(batch_size=3, max_seq_len=200, page_size=16, num_layers=2, num_kv_heads=H, head_dim=D, device="cpu",
+             dtype=torch.float32)
+    a.update(kw)
+    return PC.SabrePagedKVCache(**a)
+
+
+class Mirror:
+    """Every sequence's rows as plain lists; checks the cache against them."""
+
+    def __init__(self, c):
+        self.c, self.rows, self.next = c, [[] for _ in range(c.batch_size)], 0
+
+    def add(self, new):
+        c = self.c
+        c.extend(new)
+        fresh = []
+        for b, n in enumerate(new):
+            vals = [self.next + i for i in range(n)]
+            self.next += n
+            self.rows[b] += vals
+            fresh += vals
+        starts = torch.tensor([0] + torch.tensor(new).cumsum(0).tolist(), dtype=torch.int32)
+        rows = torch.tensor(fresh, dtype=torch.float32).view(-1, 1, 1).expand(-1, H, D)
+        for i, layer in enumerate(c.layers):
+            PC.K.paged_store(rows + 1000 * i, -rows - 1000 * i, layer.k_pages, layer.v_pages, c.page_table, c.seq_lens,
+                             starts)
+
+    def check(self):
+        c = self.c
+        assert c.lengths == [len(r) for r in self.rows] == c.seq_lens.tolist()
+        seen = {}
+        for b, table in enumerate(c.tables):
+            assert c.page_table[b].tolist() == table + [-1] * (c.max_pages - len(table))
+            for p in table:
+                if p >= 0:
+                    seen[p] = seen.get(p, 0) + 1
+        assert [seen.get(p, 0) for p in range(c.num_pages)] == c.refs
+        assert sorted(c.unused) == [p for p in range(c.num_pages) if p not in seen]
+        for i, layer in enumerate(c.layers):
+            for b, want in enumerate(self.rows):
+                k, there = PO.gather(layer.k_pages, c.page_table[b], len(want))
+                v, _ = PO.gather(layer.v_pages, c.page_table[b], len(want))
+                n = len(want)
+                must = torch.ones(n, dtype=torch.bool)
+                if c.window_size is not None and n:  # what the last query sees
+                    j = torch.arange(n)
+                    must = (n - 1 - j <= c.window_size) | (j < c.num_prefix_tokens)
+                assert there[must].all()
+                full = torch.tensor(want, dtype=torch.float64) + 1000 * i
+                assert torch.equal(k[there][:, 0, 0], full[there]) and torch.equal(v[there][:, 0, 0], -full[there])
+
+
+def test_extend_fork_copy_on_write_and_compact():
+    c = cache(num_pages=20)
+    m = Mirror(c)
+    m.add([40, 16, 0])
+    m.check()
+    assert c.pages_in_use == 4
+    c.fork(0, 2)
+    m.rows[2] = list(m.rows[0])
+    m.check()
+    assert c.pages_in_use == 4  # shared
+    m.add([1, 1, 2])  # both 0 and 2 write the shared page: one of them gets a copy
+    m.check()
+    assert c.pages_in_use == 6 and c.tables[0][:2] == c.tables[2][:2] and c.tables[0][2] != c.tables[2][2]
+    c.free(0)
+    m.rows[0] = []
+    m.check()
+    c.compact()
+    m.check()
+    assert all(c.refs[p] for p in range(c.pages_in_use))
+    c.truncate(2, 17)
+    m.rows[2] = m.rows[2][:17]
+    m.check()
+    m.add([200, 3, 4])
+    m.check()
+    c.reset()
+    m.rows = [[], [], []]
+    m.check()
+    assert c.pages_in_use == 0
+
+
+def test_full_pool_and_full_sequence_change_nothing():
+    c = cache(num_pages=5)
+    m = Mirror(c)
+    m.add([30, 30, 0])
+    with pytest.raises(ValueError, match="out of pages"):
+        c.extend([0, 3, 17])
+    m.check()
+    with pytest.raises(ValueError, match="full"):
+        c.extend([171, 0, 0])
+    m.check()
+    c.fork(0, 2)
+    m.rows[2] = list(m.rows[0])
+    m.add([0, 2, 1])  # the copy on write takes the last page
+    m.check()
+    with pytest.raises(ValueError, match="out of pages"):
+        c.extend([3, 0, 0])
+    m.check()
+    with pytest.raises(ValueError, match="counts"):
+        c.extend([1, 1])
+    with pytest.raises(ValueError, match="counts"):
+        c.extend([1, -1, 0])
+
+
+@pytest.mark.parametrize("window,prefix", [(20, 0), (0, 0), (33, 5), (16, 32), (15, 16)])
+def test_window_drops_pages_nobody_will_see(window, prefix):
+    c = cache(window_size=window, num_prefix_tokens=prefix, max_seq_len=2000, num_pages=30)
+    m = Mirror(c)
+    for n in [7, 30, 1, 1, 1, 16, 50] + [1] * 40:
+        m.add([n, n // 2, 0])
+        m.check()
+    keep = -(-prefix // 16) + (window + 1 + 15) // 16 + 1
+    assert sum(p >= 0 for p in c.tables[0]) <= keep
+    with pytest.raises(ValueError, match="dropped already"):
+        c.truncate(0, 60)
+    m.check()
+    c.fork(0, 2)
+    m.rows[2] = list(m.rows[0])
+    m.add([1, 0, 20])
+    m.check()
+
+
+@pytest.mark.parametrize("seed,window", [(0, None), (1, None), (2, 25), (3, 70)])
+def test_random_use(seed, window):
+    rng = random.Random(seed)
+    c = cache(batch_size=4, max_seq_len=600, num_pages=40, window_size=window, num_prefix_tokens=10 if window else 0)
+    m = Mirror(c)
+    full = 0
+    for _ in range(150):
+        op = rng.choice(("add", "add", "add", "fork", "truncate", "free", "compact", "select"))
+        try:
+            if op == "add":
+                m.add([rng.choice((0, 1, 1, 5, 40)) for _ in range(4)])
+            elif op == "fork":
+                a, b = rng.randrange(4), rng.randrange(4)
+                c.fork(a, b)
+                m.rows[b] = list(m.rows[a])
+            elif op == "truncate":
+                b = rng.randrange(4)
+                n = rng.randint(0, len(m.rows[b]))
+                c.truncate(b, n)
+                m.rows[b] = m.rows[b][:n]
+            elif op == "free" and rng.random() < 0.5:
+                b = rng.randrange(4)
+                c.free(b)
+                m.rows[b] = []
+            elif op == "compact":
+                c.compact()
+                assert all(c.refs[p] for p in range(c.pages_in_use))
+            elif op == "select":
+                idx = [rng.randrange(4) for _ in range(4)]
+                c.reorder_cache(torch.tensor(idx))
+                m.rows = [list(m.rows[i]) for i in idx]
+        except ValueError:
+            full += 1
+        m.check()
+    assert full < 100
+
+
+def test_transformers_protocol():
+    c = cache(batch_size=2)
+    assert c.get_seq_length() == 0 and c.get_mask_sizes(5, 0) == (5, 0) and c.max_cache_len == 200
+    assert c.max_batch_size == 2 and not any(c.is_sliding)
+    k = torch.randn(2, H, 20, D)
+    kk, vv = c.update(k, k + 1, 0)
+    assert torch.equal(kk, k) and torch.equal(vv, k + 1)
+    assert c.get_seq_length(0) == 20 and c.get_seq_length(1) == 0
+    with pytest.raises(ValueError, match="out of step"):
+        c.update(k[:, :, :3], k[:, :, :3], 1)
+    c.update(k, k, 1)
+    assert c.get_seq_length(1) == 20
+    c.update(k[:, :, :1], k[:, :, :1], 0)
+    kk, _ = c.update(k[:, :, :1], k[:, :, :1], 1)
+    assert kk.shape == (2, H, 21, D) and torch.equal(kk[:, :, 20:], k[:, :, :1])
+    c.batch_repeat_interleave(2)
+    assert c.batch_size == 4 and c.page_table.shape[0] == 4 and c.tables[0] == c.tables[1]
+    c.crop(-1)
+    assert c.lengths == [20] * 4
+    with pytest.raises(ValueError, match="sequences"):
+        c.update(k, k, 0)
+    with pytest.raises(ValueError, match="patched attention"):
+        cache(window_size=4).update(k, k, 0)
+
+
+@pytest.mark.parametrize("kw", [dict(page_size=24), dict(page_size=8), dict(batch_size=0), dict(max_seq_len=0),
+                                dict(num_pages=0), dict(window_size=-1), dict(num_prefix_tokens=-1),
+                                dict(num_layers=None)])
+def test_constructor_refusals(kw):
+    with pytest.raises(ValueError):
+        cache(**kw)
+
+
+def test_the_pool_goes_with_the_cache():
+    import gc
+    import weakref
+    gc.disable()
+    try:
+        c = cache()
+        ref = weakref.ref(c)
+        del c
+        assert ref() is None
+    finally:
+        gc.enable()
