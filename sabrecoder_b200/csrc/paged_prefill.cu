@@ -156,13 +156,6 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int hk = hs / p.splits;
   const int split = hs - hk * p.splits;
   const int slot = p.slots - 1 - static_cast<int>(p.head_major ? blockIdx.x : blockIdx.y);
-  Job job;
-  if (!find_job(p, slot, reinterpret_cast<int*>(smem + kMiscOff + 8), job)) return;
-  // This part's key tiles.
-  const int j0 = static_cast<int>(static_cast<long long>(job.tiles) * split / p.splits);
-  const int nt = static_cast<int>(static_cast<long long>(job.tiles) * (split + 1) / p.splits) - j0;
-
-  const uint32_t q_bytes = static_cast<uint32_t>(p.group * p.tokens) * 128u;  // of one d-half
   if (tid == 0) {
     const bool bad = (sbase & 1023u) != 0u;
     *abort_flag = bad ? 1 : 0;
@@ -180,32 +173,31 @@ __global__ void __launch_bounds__(kThreads, 2)
     mbar_init(bar(V_RAW), 1);
     mbar_init(bar(MMA_DONE), 1);
     fence_mbar_init();
+    tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
-    if ((sbase & 1023u) == 0u) {
-      mbar_arrive_expect_tx(bar(Q_FULL), 2 * q_bytes);
-      const uint64_t pol = l2_policy_evict_first();
-      tma_load_4d_hint(sbase + kQOff, &tmQ, bar(Q_FULL), 0, 0, job.row0, hk, pol);
-      tma_load_4d_hint(sbase + kQOff + kQBytes / 2, &tmQ, bar(Q_FULL), 64, 0, job.row0, hk, pol);
-    }
   }
   if (warp == 5) {
     tmem_alloc(smem_u32(tmem_slot), kTmemCols);
     tmem_relinquish();
+    tc_fence_before();
   }
-  // Does any page of this part's tiles miss? Rarely: then the softmax looks
-  // each tile's pages up.
-  int hole = 0;
-  const int boxes = kTile >> p.box_shift;
-  const int box_rows = 1 << p.box_shift;
-  for (int i = tid; i < nt * boxes; i += kThreads) {
-    const int t = job.pos(j0 + i / boxes) + ((i % boxes) << p.box_shift);
-    if (job.any(p.w, t, box_rows) && p.c.page_of(job.b, t) < 0) hole = 1;
-  }
-  const bool holes = __syncthreads_or(hole) != 0;
+  // The set-up above overlaps the loads of find_job, whose barriers order it
+  // before its use.
+  Job job;
+  const bool any_job = find_job(p, slot, reinterpret_cast<int*>(smem + kMiscOff + 8), job);
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  if (!any_job) {
+    if (warp == 5) tmem_dealloc(tmem, kTmemCols);
+    return;
+  }
+  // This part's key tiles.
+  const int j0 = static_cast<int>(static_cast<long long>(job.tiles) * split / p.splits);
+  const int nt = static_cast<int>(static_cast<long long>(job.tiles) * (split + 1) / p.splits) - j0;
   const bool start_ok = (*abort_flag == 0);
+  const int boxes = kTile >> p.box_shift;
+  const int box_rows = 1 << p.box_shift;
 
   constexpr uint32_t kIdescQK = idesc_f16(128, 64, DT<T>::kBf16, false);
   constexpr uint32_t kIdescPV = idesc_f16(128, 128, DT<T>::kBf16, true);
@@ -216,6 +208,12 @@ __global__ void __launch_bounds__(kThreads, 2)
     const int full0 = is_k ? K_FULL : V_FULL;
     const uint32_t ring = sbase + (is_k ? kKOff : kVOff);
     const CUtensorMap* map = is_k ? &tmK : &tmV;
+    if (is_k && lane == 0 && start_ok) {
+      mbar_arrive_expect_tx(bar(Q_FULL), static_cast<uint32_t>(p.group * p.tokens) * 256u);
+      const uint64_t pol = l2_policy_evict_first();
+      tma_load_4d_hint(sbase + kQOff, &tmQ, bar(Q_FULL), 0, 0, job.row0, hk, pol);
+      tma_load_4d_hint(sbase + kQOff + kQBytes / 2, &tmQ, bar(Q_FULL), 64, 0, job.row0, hk, pol);
+    }
     int issued = 0;    // tiles
     bool raw = false;  // the last one went through V_RAW
     bool ok = start_ok;
@@ -343,6 +341,14 @@ __global__ void __launch_bounds__(kThreads, 2)
     float m_run = -INFINITY;
     float l_run = 0.f;
     bool ok = start_ok;
+    // Does any page of this part's tiles miss? Rarely: then each tile's pages
+    // are looked up. (Each warp finds out for itself while S(0) is on its way.)
+    bool hole = false;
+    for (int i = lane; i < nt * boxes; i += 32) {
+      const int t = job.pos(j0 + i / boxes) + ((i % boxes) << p.box_shift);
+      hole |= job.any(p.w, t, box_rows) && p.c.page_of(job.b, t) < 0;
+    }
+    const bool holes = __any_sync(0xffffffffu, hole);
     for (int j = 0; ok && j < nt; ++j) {
       const int t = job.pos(j0 + j);
       unsigned long long see = low_bits(seen - t) & (~low_bits(wlo - t) | low_bits(p.w.prefix - t));
@@ -518,25 +524,28 @@ static inline long long row_slots(int rows, int batch, int tokens) {
   return static_cast<long long>(rows) / tokens + (rows < batch ? rows : batch);
 }
 
-// CTAs per row tile: enough that the card's 296 places are filled, with at
-// least four key tiles each.
-static inline int choose_splits(long long ctas, long long span) {
-  long long s = kDecCtas / ctas;
-  const long long most = (span + 4 * kTile - 1) / (4 * kTile);
-  if (s > most) s = most;
-  if (s > kMaxSplits) s = kMaxSplits;
-  return s < 1 ? 1 : static_cast<int>(s);
-}
-
+// CTAs per row tile, as far as the host can tell: enough that the card's 296
+// places are filled, with at least eight key tiles each, counted for a row
+// tile in the middle of its sequence's new rows. A part costs a CTA's start
+// and read-out and 516 bytes per row and head through the workspace: 512 rows
+// of a single sequence at 56/8 heads on 15872 rows run 297 us whole and 307 in
+// two parts (232 row tiles), 64 rows at 16 heads on 16000 rows 234 us whole
+// and 37 in 16 parts; 1000 rows on none run 22 us whole and 25 in two.
 static int plan_splits(int rows, int batch, int heads_q, int heads_kv, int page_size, int max_pages, int window,
                        int prefix) {
   const int tokens = kRows / (heads_q / heads_kv);
   long long span = static_cast<long long>(page_size) * max_pages;
+  span -= (rows / batch < span ? rows / batch : span) / 2;
   if (window >= 0) {
     const long long seen = static_cast<long long>(window) + tokens + prefix;
     if (seen < span) span = seen;
   }
-  return choose_splits(row_slots(rows, batch, tokens) * heads_kv, span);
+  const long long tiles = span / kTile;
+  if (tiles < 32) return 1;
+  long long s = kDecCtas / (row_slots(rows, batch, tokens) * heads_kv);
+  if (s > tiles / 8) s = tiles / 8;
+  if (s > kMaxSplits) s = kMaxSplits;
+  return s < 1 ? 1 : static_cast<int>(s);
 }
 
 static size_t workspace_bytes(int rows, int heads_q, int splits) {
