@@ -9,6 +9,7 @@ allocates. There is no CPU path: non-CUDA tensors raise.
 from __future__ import annotations
 
 import ctypes
+import functools
 import math
 from typing import Optional, Sequence, Tuple
 
@@ -547,6 +548,13 @@ def token_tile_masks(tok_chunk: torch.Tensor, tok_group: torch.Tensor, tok_globa
 
 _S2, _S3 = ctypes.c_int64 * 2, ctypes.c_int64 * 3
 
+
+@functools.lru_cache(maxsize=1024)
+def _paged_workspace(what: str, *sizes: int) -> int:
+    """Workspace bytes of a paged call: a function of these sizes alone."""
+    return int(getattr(lib(), f"sabre_{what}_workspace_size")(*sizes))
+
+
 # The current stream's handle without building a Stream object (3 us of a
 # decode step), where this torch has it.
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
@@ -554,25 +562,26 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
 
 
 def _paged_ok(k_pages, v_pages, page_table, seq_lens, q_start, rows) -> bool:
-    """The conditions of :func:`_paged_refuse` in one pass (a decode step is as
-    long as a few of these lookups)."""
+    """The conditions of :func:`_paged_refuse` in one pass (a decode step on the
+    device is as short as a few of these lookups). ``rows``: the ``[N, H, D]``
+    tensors of the new rows, some of them None."""
     dt, dev = k_pages.dtype, k_pages.get_device()
-    ks, vs, ts = k_pages.shape, v_pages.shape, page_table.shape
-    if dev < 0 or dt not in DTYPE_CODE or v_pages.dtype is not dt or len(ks) != 4 or vs != ks or len(ts) != 2:
+    ks, ts = k_pages.shape, page_table.shape
+    if dev < 0 or dt not in DTYPE_CODE or v_pages.dtype is not dt or len(ks) != 4 or v_pages.shape != ks or len(ts) != 2:
         return False
-    B, D = ts[0], ks[3]
-    if ts[1] < 1 or (ts[1] > 1 and page_table.stride(1) != 1) or k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
+    B, cols = ts
+    if cols < 1 or (cols > 1 and page_table.stride(1) != 1) or k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
         return False
-    if v_pages.get_device() != dev or page_table.dtype is not torch.int32 or page_table.get_device() != dev:
+    if (page_table.dtype is not torch.int32 or seq_lens.dtype is not torch.int32 or seq_lens.shape != (B,)
+            or not seq_lens.is_contiguous()):
         return False
-    if (seq_lens.shape != (B,) or seq_lens.dtype is not torch.int32 or not seq_lens.is_contiguous()
-            or seq_lens.get_device() != dev):
+    if not dev == v_pages.get_device() == page_table.get_device() == seq_lens.get_device():
         return False
     if q_start is not None and (q_start.shape != (B + 1,) or q_start.dtype is not torch.int32
                                 or not q_start.is_contiguous() or q_start.get_device() != dev):
         return False
-    for t in rows.values():
-        if t is not None and (t.dtype is not dt or t.dim() != 3 or t.shape[2] != D or t.stride(2) != 1
+    for t in rows:
+        if t is not None and (t.dtype is not dt or t.dim() != 3 or t.shape[2] != ks[3] or t.stride(2) != 1
                               or t.get_device() != dev):
             return False
     return True
@@ -657,9 +666,8 @@ def paged_store(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages
     with the new rows; q_start int32 ``[B + 1]``: rows ``q_start[b] ..
     q_start[b+1]-1`` are the last rows of sequence b (default: one row each,
     ``N == B``). Rows from ``q_start[B]`` on are padding."""
-    rows = dict(k=k, v=v)
-    if not _paged_ok(k_pages, v_pages, page_table, seq_lens, q_start, rows):
-        _paged_refuse("paged_store", k_pages, v_pages, page_table, seq_lens, q_start, rows)
+    if not _paged_ok(k_pages, v_pages, page_table, seq_lens, q_start, (k, v)):
+        _paged_refuse("paged_store", k_pages, v_pages, page_table, seq_lens, q_start, dict(k=k, v=v))
     (P, Hkv, ps, D), (B, cols), (N, heads, _) = k_pages.shape, page_table.shape, k.shape
     if v.shape != k.shape or heads != Hkv:
         raise SabreError(f"paged_store: k {tuple(k.shape)} and v {tuple(v.shape)} must both be [N, {Hkv}, {D}]")
@@ -686,9 +694,8 @@ def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     sees key j <= i when ``i - j <= window_size`` or ``j < num_prefix_tokens``.
     A sequence that sees nothing (length 0) gives zeros. Deterministic."""
     window, prefix = _window_code("paged_decode", window_size, num_prefix_tokens)
-    rows = dict(q=q, out=out)
-    if not _paged_ok(k_pages, v_pages, page_table, seq_lens, None, rows):
-        _paged_refuse("paged_decode", k_pages, v_pages, page_table, seq_lens, None, rows)
+    if not _paged_ok(k_pages, v_pages, page_table, seq_lens, None, (q, out)):
+        _paged_refuse("paged_decode", k_pages, v_pages, page_table, seq_lens, None, dict(q=q, out=out))
     (P, Hkv, ps, D), (B, cols), Hq = k_pages.shape, page_table.shape, q.shape[1]
     if q.shape[0] != B or (out is not None and out.shape != q.shape):
         raise SabreError(f"paged_decode: q {tuple(q.shape)} and out must be [B={B}, Hq, D]")
@@ -696,10 +703,9 @@ def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if q.numel() == 0:
         return out
-    L = lib()
-    ws, ws_bytes, _keep = _workspace("paged_decode", workspace,
-                                     L.sabre_paged_decode_workspace_size(B, Hq, Hkv, D), q.device)
-    _paged_call("sabre_paged_decode", q.get_device(), L.sabre_paged_decode,
+    ws, ws_bytes, _keep = _workspace("paged_decode", workspace, _paged_workspace("paged_decode", B, Hq, Hkv, D),
+                                     q.device)
+    _paged_call("sabre_paged_decode", q.get_device(), lib().sabre_paged_decode,
                 q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), page_table.data_ptr(),
                 seq_lens.data_ptr(), B, Hq, Hkv, D, P, ps, cols, window, prefix, _S2(*q.stride()[:2]),
                 _S3(*k_pages.stride()[:3]), _S3(*v_pages.stride()[:3]), _S2(*out.stride()[:2]), page_table.stride(0),
@@ -719,9 +725,8 @@ def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     rows of sequence b, the rest as in :func:`paged_decode`. Rows of ``out``
     from ``q_start[B]`` on are left as they are."""
     window, prefix = _window_code("paged_prefill", window_size, num_prefix_tokens)
-    rows = dict(q=q, out=out)
-    if not _paged_ok(k_pages, v_pages, page_table, seq_lens, q_start, rows):
-        _paged_refuse("paged_prefill", k_pages, v_pages, page_table, seq_lens, q_start, rows)
+    if not _paged_ok(k_pages, v_pages, page_table, seq_lens, q_start, (q, out)):
+        _paged_refuse("paged_prefill", k_pages, v_pages, page_table, seq_lens, q_start, dict(q=q, out=out))
     (P, Hkv, ps, D), (B, cols), (N, Hq, _) = k_pages.shape, page_table.shape, q.shape
     if out is not None and out.shape != q.shape:
         raise SabreError(f"paged_prefill: out {tuple(out.shape)} must have q's shape {tuple(q.shape)}")
@@ -729,10 +734,9 @@ def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     if q.numel() == 0 or B == 0:
         return out
-    L = lib()
-    ws, ws_bytes, _keep = _workspace("paged_prefill", workspace, L.sabre_paged_prefill_workspace_size(
-        N, B, Hq, Hkv, D, ps, cols, window, prefix), q.device)
-    _paged_call("sabre_paged_prefill", q.get_device(), L.sabre_paged_prefill,
+    ws, ws_bytes, _keep = _workspace("paged_prefill", workspace, _paged_workspace(
+        "paged_prefill", N, B, Hq, Hkv, D, ps, cols, window, prefix), q.device)
+    _paged_call("sabre_paged_prefill", q.get_device(), lib().sabre_paged_prefill,
                 q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), page_table.data_ptr(),
                 seq_lens.data_ptr(), q_start.data_ptr(), N, B, Hq, Hkv, D, P, ps, cols, window, prefix,
                 _S2(*q.stride()[:2]), _S3(*k_pages.stride()[:3]), _S3(*v_pages.stride()[:3]), _S2(*out.stride()[:2]),
