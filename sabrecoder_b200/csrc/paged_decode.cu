@@ -214,6 +214,13 @@ __device__ __forceinline__ void mma_16x8x16(float (&c)[4], const uint32_t (&a)[4
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// out[4 lane ..] = a / l, zeros where nothing was visible.
+template <typename T>
+__device__ __forceinline__ void store_row(T* out, int lane, const float4& a, float l) {
+  const float inv = l > 0.f ? 1.0f / l : 0.f;
+  *reinterpret_cast<uint2*>(out + lane * 4) = make_uint2(DT<T>::pack(a.x * inv, a.y * inv), DT<T>::pack(a.z * inv, a.w * inv));
+}
+
 template <typename T>
 __global__ void __launch_bounds__(kDecThreads, 2)
     paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
@@ -433,8 +440,8 @@ __global__ void __launch_bounds__(kDecThreads, 2)
       if (lane == 0) mbar_arrive(empty_bar(s));
     }
 
-    // Join the four warps: (m, l, acc) through shared memory, then thread d
-    // sums column d of each head.
+    // Join the four warps: (m, l, acc) through shared memory, then a warp sums
+    // two heads, a lane four columns of each.
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) {
       l[0] += __shfl_xor_sync(0xffffffffu, l[0], o);
@@ -463,82 +470,120 @@ __global__ void __launch_bounds__(kDecThreads, 2)
       const int parts = more > 0 ? sh.owner(sh.first(blockIdx.x + 1) + more - 1) - static_cast<int>(blockIdx.x) + 1 : 0;
       p.joins[blockIdx.x] = make_int4(parts, seg.b, seg.hk, place);
     }
-    for (int g = 0; g < p.group; ++g) {
-      float M = -INFINITY;
+    // After a timeout anywhere in the CTA the segment is incomplete: store nothing.
+    if (ok && *abort_flag == 0) {
 #pragma unroll
-      for (int w = 0; w < kConsumers; ++w) M = fmaxf(M, ml_sm[(w * kGroup + g) * 2]);
-      float L = 0.f, A = 0.f;
-      if (M != -INFINITY) {
+      for (int u = 0; u < kGroup / kConsumers; ++u) {
+        const int g = warp + u * kConsumers;
+        if (g >= p.group) break;
+        float mw[kConsumers], M = -INFINITY, L = 0.f;
+        float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < kConsumers; ++w) {
-          const float a = ex2(ml_sm[(w * kGroup + g) * 2] - M);
+          mw[w] = ml_sm[(w * kGroup + g) * 2];
+          M = fmaxf(M, mw[w]);
+        }
+#pragma unroll
+        for (int w = 0; w < kConsumers; ++w) {
+          const float a = M == -INFINITY ? 0.f : ex2(mw[w] - M);
+          const float4 x = *reinterpret_cast<const float4*>(acc_sm + (w * kGroup + g) * kAccRow + lane * 4);
           L += a * ml_sm[(w * kGroup + g) * 2 + 1];
-          A += a * acc_sm[(w * kGroup + g) * kAccRow + tid];
+          A.x += a * x.x;
+          A.y += a * x.y;
+          A.z += a * x.z;
+          A.w += a * x.w;
         }
-      }
-      // After a timeout anywhere in the CTA the segment is incomplete: store nothing.
-      if (ok && *abort_flag == 0) {
-        if (whole_pair) {
-          out[seg.b * p.o_sb + (seg.hk * p.group + g) * p.o_sh + tid] = DT<T>::from_f(L > 0.f ? A / L : 0.f);
-        } else {
-          p.part_acc[(slot + g) * kD + tid] = A;
-          if (tid == 0) {
-            p.part_ml[(slot + g) * 2] = M;
-            p.part_ml[(slot + g) * 2 + 1] = L;
-          }
-        }
+        if (whole_pair)
+          store_row<T>(out + seg.b * p.o_sb + (seg.hk * p.group + g) * p.o_sh, lane, A, L);
+        else
+          *reinterpret_cast<float4*>(p.part_acc + (slot + g) * kD + lane * 4) = A;
+        if (!whole_pair && lane == 0) *reinterpret_cast<float2*>(p.part_ml + (slot + g) * 2) = make_float2(M, L);
       }
     }
     named_bar_sync(1, kConsumers * 32);  // the joining buffers are free again
   }
 }
 
-// One CTA per (share, head of the group): joins the parts of the pair whose
-// first part ends the share, if there is one, in share order.
+// One CTA per share: joins the parts of the pair whose first part ends the
+// share, if there is one. kJoinWarps / group warps take a head's parts in turn
+// (four columns a lane, eight parts in flight), then the warps' sums are added
+// in order: the result is the same every time.
+constexpr int kJoinWarps = 8;
 template <typename T>
-__global__ void __launch_bounds__(kD) paged_join_kernel(const DecodeParams p) {
+__global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const DecodeParams p) {
   // The next call's kernel (a programmatic dependent too) may start its
   // set-up now; it waits for this grid before touching memory.
   if (threadIdx.x == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  __shared__ float sm_m[kDecCtas], sm_l[kDecCtas];
+  __shared__ float sm_m[kJoinWarps], sm_l[kJoinWarps];
+  __shared__ float4 sm_a[kJoinWarps][32];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int x = blockIdx.x;
-  const int g = blockIdx.y;
-  const int d = threadIdx.x;
+  const int warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31;
   const int4 job = p.joins[x];
   const int parts = job.x;
   if (parts == 0) return;
+  const int per = kJoinWarps / p.group;  // warps of a head
+  const int g = warp / per;
   // The first part is the last segment of its share, the others open theirs.
   auto slot = [&](int i) -> long long { return (i == 0 ? job.w : 2ll * (x + i)) * p.group + g; };
-  for (int i = d; i < parts; i += kD) {
-    const float2 ml = *reinterpret_cast<const float2*>(p.part_ml + slot(i) * 2);
-    sm_m[i] = ml.x;
-    sm_l[i] = ml.y;
-  }
-  constexpr int kBatch = 8;
-  float a[kBatch];
-#pragma unroll
-  for (int u = 0; u < kBatch; ++u) a[u] = u < parts ? p.part_acc[slot(u) * kD + d] : 0.f;
-  __syncthreads();
-  float M = -INFINITY;
-  for (int i = 0; i < parts; ++i) M = fmaxf(M, sm_m[i]);
-  float L = 0.f, A = 0.f;
-  if (M != -INFINITY) {
-    for (int i0 = 0; i0 < parts; i0 += kBatch) {
-      if (i0 > 0) {
-#pragma unroll
-        for (int u = 0; u < kBatch; ++u) a[u] = i0 + u < parts ? p.part_acc[slot(i0 + u) * kD + d] : 0.f;
-      }
+  float M = -INFINITY, L = 0.f;
+  float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (g < p.group) {
+    constexpr int kBatch = 8;
+    for (int i0 = warp - g * per; i0 < parts; i0 += per * kBatch) {
+      float2 ml[kBatch];
+      float4 a[kBatch];
 #pragma unroll
       for (int u = 0; u < kBatch; ++u) {
-        if (i0 + u >= parts) break;
-        const float w = ex2(sm_m[i0 + u] - M);
-        L += w * sm_l[i0 + u];
-        A += w * a[u];
+        const int i = i0 + u * per;
+        ml[u] = i < parts ? *reinterpret_cast<const float2*>(p.part_ml + slot(i) * 2) : make_float2(-INFINITY, 0.f);
+        a[u] = i < parts ? *reinterpret_cast<const float4*>(p.part_acc + slot(i) * kD + lane * 4)
+                         : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float mn = M;
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) mn = fmaxf(mn, ml[u].x);
+      if (mn == -INFINITY) continue;
+      const float r = ex2(M - mn);
+      M = mn;
+      L *= r;
+      A = make_float4(A.x * r, A.y * r, A.z * r, A.w * r);
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const float w = ex2(ml[u].x - mn);
+        L += w * ml[u].y;
+        A.x += w * a[u].x;
+        A.y += w * a[u].y;
+        A.z += w * a[u].z;
+        A.w += w * a[u].w;
       }
     }
   }
-  static_cast<T*>(p.o)[job.y * p.o_sb + (job.z * p.group + g) * p.o_sh + d] = DT<T>::from_f(L > 0.f ? A / L : 0.f);
+  if (per > 1) {
+    if (lane == 0) {
+      sm_m[warp] = M;
+      sm_l[warp] = L;
+    }
+    sm_a[warp][lane] = A;
+    __syncthreads();
+    if (warp % per != 0) return;
+    float mn = -INFINITY;
+    for (int w = 0; w < per; ++w) mn = fmaxf(mn, sm_m[(warp + w) % kJoinWarps]);
+    L = 0.f;
+    A = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int w = 0; w < per && mn != -INFINITY; ++w) {
+      const int s = (warp + w) % kJoinWarps;
+      const float r = ex2(sm_m[s] - mn);
+      L += r * sm_l[s];
+      A.x += r * sm_a[s][lane].x;
+      A.y += r * sm_a[s][lane].y;
+      A.z += r * sm_a[s][lane].z;
+      A.w += r * sm_a[s][lane].w;
+    }
+  }
+  if (g < p.group)
+    store_row<T>(static_cast<T*>(p.o) + job.y * p.o_sb + (job.z * p.group + g) * p.o_sh, lane, A, L);
 }
 
 // Tensor map of a pool [num_pages, H, page_size, D]: dims (64 d, page rows, 2
@@ -593,7 +638,7 @@ static cudaError_t launch_paged_decode(const CUtensorMap& mk, const CUtensorMap&
   if (e != cudaSuccess) return e;
   e = launch_dependent(dim3(p.ctas), kDecThreads, kDecSmem, s, paged_decode_kernel<T>, mk, mv, p);
   if (e != cudaSuccess || p.ctas == 1) return e;  // a single share is finished where it is
-  return launch_dependent(dim3(p.ctas - 1, p.group), kD, 0, s, paged_join_kernel<T>, p);
+  return launch_dependent(dim3(p.ctas - 1), kJoinWarps * 32, 0, s, paged_join_kernel<T>, p);
 }
 
 }  // namespace paged
