@@ -37,8 +37,9 @@ constexpr int kTileBytes = kTile * kD * 2;  // 16384: per box [d-half][rows][128
 constexpr int kConsumers = 4;
 constexpr int kDecThreads = (kConsumers + 1) * 32;
 constexpr int kDecCtas = 2 * 148;
-constexpr int kGroup = 8;     // query heads per KV head, at most
-constexpr int kAccRow = 132;  // padded head row: the 32 lanes of a store hit 32 banks
+constexpr int kMaxParts = 128;  // parts of one pair, were all sequences alike
+constexpr int kGroup = 8;       // query heads per KV head, at most
+constexpr int kAccRow = 132;    // padded head row: the 32 lanes of a store hit 32 banks
 constexpr int kRingOff = 0;
 constexpr int kAccOff = kRingOff + kStages * 2 * kTileBytes;
 constexpr int kMlOff = kAccOff + kConsumers * kGroup * kAccRow * 4;
@@ -90,13 +91,12 @@ struct Place {
   int b, hk, tile;
 };
 
-// Finds the shares and the place of unit `unit(shares)` with the whole CTA
-// (kThreads threads); scratch: kThreads / 32 + 8 ints of shared memory.
-// Returns false when there is no such unit. Calls on_empty(b) for
-// sequences without a tile.
-template <int kThreads, typename U, typename E>
-__device__ __forceinline__ bool locate(const DecodeParams& p, int ctas, int* scratch, Shares& sh, Place& at, U unit,
-                                       E on_empty) {
+// Finds the shares and the place of this CTA's first unit with the whole CTA
+// (kDecThreads threads); scratch: 16 ints of shared memory. False for a CTA
+// without a share. Calls on_empty(b) for sequences without a tile.
+template <typename E>
+__device__ __forceinline__ bool locate(const DecodeParams& p, int* scratch, Shares& sh, Place& at, E on_empty) {
+  constexpr int kThreads = kDecThreads;
   const int tid = threadIdx.x;
   const int per = (p.c.batch + kThreads - 1) / kThreads;
   const int b0 = min(tid * per, p.c.batch), b1 = min(b0 + per, p.c.batch);
@@ -122,10 +122,9 @@ __device__ __forceinline__ bool locate(const DecodeParams& p, int ctas, int* scr
   }
   sh.total = static_cast<long long>(all) * p.heads_kv;
   if (all == 0) return false;
-  sh.ctas = static_cast<int>(min(static_cast<long long>(ctas), sh.total));
-  const long long u = unit(sh);
-  if (u < 0 || u >= sh.total) return false;
-  long long left = u - static_cast<long long>(before + incl - mine) * p.heads_kv;
+  sh.ctas = static_cast<int>(min(static_cast<long long>(p.ctas), sh.total));
+  if (static_cast<int>(blockIdx.x) >= sh.ctas) return false;
+  long long left = sh.first(blockIdx.x) - static_cast<long long>(before + incl - mine) * p.heads_kv;
   int* found = scratch + kThreads / 32;
   if (left >= 0 && left < static_cast<long long>(mine) * p.heads_kv) {
     for (int b = b0; b < b1; ++b) {
@@ -256,16 +255,13 @@ __global__ void __launch_bounds__(kDecThreads, 2)
   Shares sh;
   Place at;
   T* const out = static_cast<T*>(p.o);
-  const bool some = locate<kDecThreads>(
-      p, gridDim.x, reinterpret_cast<int*>(smem + kAccOff), sh, at,
-      [&](const Shares& s) { return static_cast<int>(blockIdx.x) < s.ctas ? s.first(blockIdx.x) : -1ll; },
-      [&](int b) {
-        // No visible tile: the sequence's rows are zero.
-        if (b % static_cast<int>(gridDim.x) != static_cast<int>(blockIdx.x)) return;
-        for (int h = 0; h < p.heads_kv * p.group; ++h)
-          for (int d = 0; d < kD; d += 8)
-            *reinterpret_cast<uint4*>(out + b * p.o_sb + h * p.o_sh + d) = make_uint4(0u, 0u, 0u, 0u);
-      });
+  const bool some = locate(p, reinterpret_cast<int*>(smem + kAccOff), sh, at, [&](int b) {
+    // No visible tile: the sequence's rows are zero.
+    if (b % p.ctas != static_cast<int>(blockIdx.x)) return;
+    for (int h = 0; h < p.heads_kv * p.group; ++h)
+      for (int d = 0; d < kD; d += 8)
+        *reinterpret_cast<uint4*>(out + b * p.o_sb + h * p.o_sh + d) = make_uint4(0u, 0u, 0u, 0u);
+  });
   // locate()'s barriers order the mbarrier set-up above before its use.
   if (!some) {
     if (tid == 0) p.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
@@ -340,17 +336,19 @@ __global__ void __launch_bounds__(kDecThreads, 2)
   float* acc_sm = reinterpret_cast<float*>(smem + kAccOff);
   float* ml_sm = reinterpret_cast<float*>(smem + kMlOff);
   int it = 0;
-  while (seg.next()) {
-    // Q as the B operand: b0 = Q[head r4][16 kk + c2, +1], b1 the same 8 further.
-    uint32_t qf[8][2];
-    {
-      const T* qp = static_cast<const T*>(p.q) + seg.b * p.q_sb + (seg.hk * p.group + r4) * p.q_sh + c2;
+  // Q as the B operand: b0 = Q[head r4][16 kk + c2, +1], b1 the same 8 further.
+  uint32_t qf[8][2];
+  auto load_q = [&]() {
+    const T* qp = static_cast<const T*>(p.q) + seg.b * p.q_sb + (seg.hk * p.group + r4) * p.q_sh + c2;
 #pragma unroll
-      for (int kk = 0; kk < 8; ++kk) {
-        qf[kk][0] = r4 < p.group ? *reinterpret_cast<const uint32_t*>(qp + kk * 16) : 0u;
-        qf[kk][1] = r4 < p.group ? *reinterpret_cast<const uint32_t*>(qp + kk * 16 + 8) : 0u;
-      }
+    for (int kk = 0; kk < 8; ++kk) {
+      qf[kk][0] = r4 < p.group ? *reinterpret_cast<const uint32_t*>(qp + kk * 16) : 0u;
+      qf[kk][1] = r4 < p.group ? *reinterpret_cast<const uint32_t*>(qp + kk * 16 + 8) : 0u;
     }
+  };
+  bool more = seg.next();
+  if (more) load_q();
+  while (more) {
     float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
     float acc[8][4];
 #pragma unroll
@@ -440,6 +438,20 @@ __global__ void __launch_bounds__(kDecThreads, 2)
       if (lane == 0) mbar_arrive(empty_bar(s));
     }
 
+    const int b = seg.b, hk = seg.hk;
+    const bool whole_pair = seg.t0 == 0 && seg.t1 == seg.tiles.count;
+    // A part is kept as the share's first (0) or last (1) segment.
+    const int place = 2 * static_cast<int>(blockIdx.x) + (seg.seen > 0 ? 1 : 0);
+    if (tid == 0 && seg.left == 0) {
+      // When the share ends inside a pair that began in it, the pair is joined for it.
+      const int rest = seg.t0 == 0 ? seg.tiles.count - seg.t1 : 0;
+      const int parts = rest > 0 ? sh.owner(sh.first(blockIdx.x + 1) + rest - 1) - static_cast<int>(blockIdx.x) + 1 : 0;
+      p.joins[blockIdx.x] = make_int4(parts, b, hk, place);
+    }
+    // The next segment's Q is on its way while this one is joined.
+    more = seg.next();
+    if (more) load_q();
+
     // Join the four warps: (m, l, acc) through shared memory, then a warp sums
     // two heads, a lane four columns of each.
 #pragma unroll
@@ -460,16 +472,7 @@ __global__ void __launch_bounds__(kDecThreads, 2)
       for (int e = 0; e < 4; ++e)
         acc_sm[(warp * kGroup + c2 + (e & 1)) * kAccRow + i * 16 + r4 + (e >> 1) * 8] = acc[i][e];
     named_bar_sync(1, kConsumers * 32);
-    const bool whole_pair = seg.t0 == 0 && seg.t1 == seg.tiles.count;
-    // A part is kept as the share's first (0) or last (1) segment.
-    const int place = 2 * static_cast<int>(blockIdx.x) + (seg.seen > 0 ? 1 : 0);
     const long long slot = static_cast<long long>(place) * p.group;
-    if (tid == 0 && seg.left == 0) {
-      // The share ends inside a pair that began in it: the pair is joined here.
-      const int more = seg.t0 == 0 ? seg.tiles.count - seg.t1 : 0;
-      const int parts = more > 0 ? sh.owner(sh.first(blockIdx.x + 1) + more - 1) - static_cast<int>(blockIdx.x) + 1 : 0;
-      p.joins[blockIdx.x] = make_int4(parts, seg.b, seg.hk, place);
-    }
     // After a timeout anywhere in the CTA the segment is incomplete: store nothing.
     if (ok && *abort_flag == 0) {
 #pragma unroll
@@ -494,7 +497,7 @@ __global__ void __launch_bounds__(kDecThreads, 2)
           A.w += a * x.w;
         }
         if (whole_pair)
-          store_row<T>(out + seg.b * p.o_sb + (seg.hk * p.group + g) * p.o_sh, lane, A, L);
+          store_row<T>(out + b * p.o_sb + (hk * p.group + g) * p.o_sh, lane, A, L);
         else
           *reinterpret_cast<float4*>(p.part_acc + (slot + g) * kD + lane * 4) = A;
         if (!whole_pair && lane == 0) *reinterpret_cast<float2*>(p.part_ml + (slot + g) * 2) = make_float2(M, L);
@@ -504,11 +507,14 @@ __global__ void __launch_bounds__(kDecThreads, 2)
   }
 }
 
-// One CTA per share: joins the parts of the pair whose first part ends the
-// share, if there is one. kJoinWarps / group warps take a head's parts in turn
-// (four columns a lane, eight parts in flight), then the warps' sums are added
-// in order: the result is the same every time.
-constexpr int kJoinWarps = 8;
+// One CTA per (share, head of the group): joins the parts of the pair whose
+// first part ends the share, if there is one. Its warps (one for every eight
+// parts, up to four) take the parts in turn, four columns a lane and eight
+// parts in flight; the warps' sums are then added in order, so the result is
+// the same every time. A CTA for each head rather than a warp of one CTA: 12289
+// rows at 56/8 heads (37 parts a pair) take 13.2 us a call instead of 16.5,
+// 300 rows at 16/16 heads 6.6 instead of 7.0; the batches run alike.
+constexpr int kJoinWarps = 4;
 template <typename T>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const DecodeParams p) {
   // The next call's kernel (a programmatic dependent too) may start its
@@ -518,72 +524,67 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Decod
   __shared__ float4 sm_a[kJoinWarps][32];
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int x = blockIdx.x;
+  const int g = blockIdx.y;
   const int warp = threadIdx.x >> 5;
   const int lane = threadIdx.x & 31;
   const int4 job = p.joins[x];
   const int parts = job.x;
   if (parts == 0) return;
-  const int per = kJoinWarps / p.group;  // warps of a head
-  const int g = warp / per;
+  constexpr int kBatch = 8;
+  const int warps = min(kJoinWarps, (parts + kBatch - 1) / kBatch);
   // The first part is the last segment of its share, the others open theirs.
   auto slot = [&](int i) -> long long { return (i == 0 ? job.w : 2ll * (x + i)) * p.group + g; };
   float M = -INFINITY, L = 0.f;
   float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (g < p.group) {
-    constexpr int kBatch = 8;
-    for (int i0 = warp - g * per; i0 < parts; i0 += per * kBatch) {
-      float2 ml[kBatch];
-      float4 a[kBatch];
+  for (int i0 = warp; warp < warps && i0 < parts; i0 += warps * kBatch) {
+    float2 ml[kBatch];
+    float4 a[kBatch];
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        const int i = i0 + u * per;
-        ml[u] = i < parts ? *reinterpret_cast<const float2*>(p.part_ml + slot(i) * 2) : make_float2(-INFINITY, 0.f);
-        a[u] = i < parts ? *reinterpret_cast<const float4*>(p.part_acc + slot(i) * kD + lane * 4)
-                         : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
-      float mn = M;
+    for (int u = 0; u < kBatch; ++u) {
+      const int i = i0 + u * warps;
+      ml[u] = i < parts ? *reinterpret_cast<const float2*>(p.part_ml + slot(i) * 2) : make_float2(-INFINITY, 0.f);
+      a[u] = i < parts ? *reinterpret_cast<const float4*>(p.part_acc + slot(i) * kD + lane * 4)
+                       : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float mn = M;
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) mn = fmaxf(mn, ml[u].x);
-      if (mn == -INFINITY) continue;
-      const float r = ex2(M - mn);
-      M = mn;
-      L *= r;
-      A = make_float4(A.x * r, A.y * r, A.z * r, A.w * r);
+    for (int u = 0; u < kBatch; ++u) mn = fmaxf(mn, ml[u].x);
+    if (mn == -INFINITY) continue;
+    const float r = ex2(M - mn);
+    M = mn;
+    L *= r;
+    A = make_float4(A.x * r, A.y * r, A.z * r, A.w * r);
 #pragma unroll
-      for (int u = 0; u < kBatch; ++u) {
-        const float w = ex2(ml[u].x - mn);
-        L += w * ml[u].y;
-        A.x += w * a[u].x;
-        A.y += w * a[u].y;
-        A.z += w * a[u].z;
-        A.w += w * a[u].w;
-      }
+    for (int u = 0; u < kBatch; ++u) {
+      const float w = ex2(ml[u].x - mn);
+      L += w * ml[u].y;
+      A.x += w * a[u].x;
+      A.y += w * a[u].y;
+      A.z += w * a[u].z;
+      A.w += w * a[u].w;
     }
   }
-  if (per > 1) {
+  if (warps > 1) {
     if (lane == 0) {
       sm_m[warp] = M;
       sm_l[warp] = L;
     }
     sm_a[warp][lane] = A;
     __syncthreads();
-    if (warp % per != 0) return;
     float mn = -INFINITY;
-    for (int w = 0; w < per; ++w) mn = fmaxf(mn, sm_m[(warp + w) % kJoinWarps]);
+    for (int w = 0; w < warps; ++w) mn = fmaxf(mn, sm_m[w]);
     L = 0.f;
     A = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int w = 0; w < per && mn != -INFINITY; ++w) {
-      const int s = (warp + w) % kJoinWarps;
-      const float r = ex2(sm_m[s] - mn);
-      L += r * sm_l[s];
-      A.x += r * sm_a[s][lane].x;
-      A.y += r * sm_a[s][lane].y;
-      A.z += r * sm_a[s][lane].z;
-      A.w += r * sm_a[s][lane].w;
+    for (int w = 0; w < warps && mn != -INFINITY; ++w) {
+      const float r = ex2(sm_m[w] - mn);
+      L += r * sm_l[w];
+      A.x += r * sm_a[w][lane].x;
+      A.y += r * sm_a[w][lane].y;
+      A.z += r * sm_a[w][lane].z;
+      A.w += r * sm_a[w][lane].w;
     }
   }
-  if (g < p.group)
-    store_row<T>(static_cast<T*>(p.o) + job.y * p.o_sb + (job.z * p.group + g) * p.o_sh, lane, A, L);
+  if (warp == 0) store_row<T>(static_cast<T*>(p.o) + job.y * p.o_sb + (job.z * p.group + g) * p.o_sh, lane, A, L);
 }
 
 // Tensor map of a pool [num_pages, H, page_size, D]: dims (64 d, page rows, 2
@@ -638,7 +639,7 @@ static cudaError_t launch_paged_decode(const CUtensorMap& mk, const CUtensorMap&
   if (e != cudaSuccess) return e;
   e = launch_dependent(dim3(p.ctas), kDecThreads, kDecSmem, s, paged_decode_kernel<T>, mk, mv, p);
   if (e != cudaSuccess || p.ctas == 1) return e;  // a single share is finished where it is
-  return launch_dependent(dim3(p.ctas - 1), kJoinWarps * 32, 0, s, paged_join_kernel<T>, p);
+  return launch_dependent(dim3(p.ctas - 1, p.group), kJoinWarps * 32, 0, s, paged_join_kernel<T>, p);
 }
 
 }  // namespace paged
@@ -680,10 +681,14 @@ int sabre_paged_decode(const void* q, const void* k_pages, const void* v_pages, 
     return sabre_fail(SABRE_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", fn, workspace_bytes,
                       decode_workspace(p.group));
   if (!aligned16(workspace)) return sabre_fail(SABRE_ERR_ALIGNMENT, "%s: workspace must be 16-byte aligned", fn);
-  // No more CTAs than the table has tiles.
+  // No more CTAs than the table has tiles, nor parts of a pair than pay for
+  // their joining (12000 rows of one KV head, 188 tiles: 11.2 us a call in 188
+  // parts, 9.3 in 94; below that a tile a CTA is the fastest).
   const long long tiles = static_cast<long long>(batch) * heads_kv *
                           ((static_cast<long long>(page_size) * max_pages + kTile - 1) / kTile);
-  p.ctas = tiles < kDecCtas ? static_cast<int>(tiles) : kDecCtas;
+  long long ctas = static_cast<long long>(batch) * heads_kv * kMaxParts;
+  if (ctas > tiles) ctas = tiles;
+  p.ctas = static_cast<int>(ctas < kDecCtas ? ctas : kDecCtas);
   p.joins = static_cast<int4*>(workspace);
   p.part_acc = reinterpret_cast<float*>(p.joins + kDecCtas);
   p.part_ml = p.part_acc + static_cast<size_t>(2) * kDecCtas * p.group * kD;

@@ -519,9 +519,11 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const Params p) {
       make_uint2(DT<T>::pack(acc.x * inv, acc.y * inv), DT<T>::pack(acc.z * inv, acc.w * inv));
 }
 
-// Row tiles that `rows` rows of `batch` sequences need at most.
+// Row tiles that `rows` rows of `batch` sequences need at most: a sequence of
+// l > 0 rows takes (l - 1) / tokens + 1.
 static inline long long row_slots(int rows, int batch, int tokens) {
-  return static_cast<long long>(rows) / tokens + (rows < batch ? rows : batch);
+  const int k = rows < batch ? rows : batch;
+  return static_cast<long long>(rows - k) / tokens + k;
 }
 
 // CTAs per row tile, as far as the host can tell: enough that the card's 296
