@@ -26,12 +26,14 @@ struct Cache {
 
   __device__ __forceinline__ int capacity() const { return max_pages << page_shift; }
   __device__ __forceinline__ int length(int b) const { return min(max(seq_lens[b], 0), capacity()); }
-  // Page of a position below capacity(), or -1 when it is absent.
-  __device__ __forceinline__ int page_of(int b, int pos) const {
-    const int page = table[b * table_sb + (pos >> page_shift)];
+  // Table entry of a position below capacity().
+  __device__ __forceinline__ int entry(int b, int pos) const { return table[b * table_sb + (pos >> page_shift)]; }
+  // The entry as a page of the pool, or -1: absent.
+  __device__ __forceinline__ int checked(int page) const {
     if (page < -1 || page >= num_pages) record_status(SABRE_DEV_BAD_PAGE);
     return page >= 0 && page < num_pages ? page : -1;
   }
+  __device__ __forceinline__ int page_of(int b, int pos) const { return checked(entry(b, pos)); }
 };
 
 // Key j < n is visible to the query at position i when j <= i and (no window,

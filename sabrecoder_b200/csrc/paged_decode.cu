@@ -680,8 +680,10 @@ int sabre_paged_decode(const void* q, const void* k_pages, const void* v_pages, 
   // No more CTAs than the table has tiles, nor parts of a pair than pay for
   // their joining (12000 rows of one KV head, 188 tiles: 11.2 us a call in 188
   // parts, 9.3 in 94; below that a tile a CTA is the fastest).
-  const long long tiles = static_cast<long long>(batch) * heads_kv *
-                          ((static_cast<long long>(page_size) * max_pages + kTile - 1) / kTile);
+  const long long per_head = static_cast<long long>(batch) * ((page_size * max_pages + kTile - 1) / kTile);
+  if (per_head > 0x7fffffffll)
+    return sabre_fail(SABRE_ERR_UNSUPPORTED, "%s: batch * page_size * max_pages exceeds 2^37 rows", fn);
+  const long long tiles = per_head * heads_kv;
   long long ctas = static_cast<long long>(batch) * heads_kv * kMaxParts;
   if (ctas > tiles) ctas = tiles;
   p.ctas = static_cast<int>(ctas < kDecCtas ? ctas : kDecCtas);

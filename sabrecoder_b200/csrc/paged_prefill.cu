@@ -341,24 +341,27 @@ __global__ void __launch_bounds__(kThreads, 2)
     float m_run = -INFINITY;
     float l_run = 0.f;
     bool ok = start_ok;
-    // Does any page of this part's tiles miss? Rarely: then each tile's pages
-    // are looked up. (Each warp finds out for itself while S(0) is on its way.)
-    bool hole = false;
-    for (int i = lane; i < nt * boxes; i += 32) {
+    // Absent pages are not visible: the boxes of the next 32 / boxes tiles are
+    // looked up by the lanes, a batch ahead.
+    auto lookup = [&](int i) -> int {
       const int t = job.pos(j0 + i / boxes) + ((i % boxes) << p.box_shift);
-      hole |= job.any(p.w, t, box_rows) && p.c.page_of(job.b, t) < 0;
-    }
-    const bool holes = __any_sync(0xffffffffu, hole);
+      return i < nt * boxes && job.any(p.w, t, box_rows) ? p.c.entry(job.b, t) : 0;
+    };
+    int entry_ahead = lookup(lane);
+    uint32_t absent = 0;
     for (int j = 0; ok && j < nt; ++j) {
       const int t = job.pos(j0 + j);
+      const int i = j * boxes;
+      if ((i & 31) == 0) {
+        absent = __ballot_sync(0xffffffffu, p.c.checked(entry_ahead) < 0);
+        entry_ahead = lookup(i + 32 + lane);
+      }
       unsigned long long see = low_bits(seen - t) & (~low_bits(wlo - t) | low_bits(p.w.prefix - t));
-      if (holes) {
+      const uint32_t missing = (absent >> (i & 31)) & ((1u << boxes) - 1u);
+      if (missing != 0u) {
 #pragma unroll 1
-        for (int x = 0; x < boxes; ++x) {
-          const int tb = t + (x << p.box_shift);
-          if (job.any(p.w, tb, box_rows) && p.c.page_of(job.b, tb) < 0)
-            see &= ~(low_bits(box_rows) << (x << p.box_shift));
-        }
+        for (int x = 0; x < boxes; ++x)
+          if ((missing >> x) & 1u) see &= ~(low_bits(box_rows) << (x << p.box_shift));
       }
       // A warp whose rows see no key of this tile stores P = 0 and leaves the
       // exponential unit to the others.

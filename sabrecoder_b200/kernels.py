@@ -725,6 +725,8 @@ def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     rows of sequence b, the rest as in :func:`paged_decode`. Rows of ``out``
     from ``q_start[B]`` on are left as they are."""
     window, prefix = _window_code("paged_prefill", window_size, num_prefix_tokens)
+    if q_start is None:
+        raise SabreError("paged_prefill needs q_start")
     if not _paged_ok(k_pages, v_pages, page_table, seq_lens, q_start, (q, out)):
         _paged_refuse("paged_prefill", k_pages, v_pages, page_table, seq_lens, q_start, dict(q=q, out=out))
     (P, Hkv, ps, D), (B, cols), (N, Hq, _) = k_pages.shape, page_table.shape, q.shape

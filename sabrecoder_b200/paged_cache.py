@@ -349,6 +349,25 @@ class SabrePagedKVCache(Cache):
 
     def reset(self) -> None:
         self._truncate({b: 0 for b in range(self.batch_size)})
+        for layer in self.layers:  # a step that an error cut off is over
+            layer.step = self.step
+
+    def __deepcopy__(self, memo) -> "SabrePagedKVCache":
+        """A cache of its own with the same contents, as prompts are reused."""
+        _, _, n, heads, _, dim = self.pool.shape
+        new = SabrePagedKVCache(batch_size=self.batch_size, max_seq_len=self.max_seq_len, num_pages=n,
+                                page_size=self.page_size, window_size=self.window_size,
+                                num_prefix_tokens=self.num_prefix_tokens, device=self.pool.device,
+                                dtype=self.pool.dtype, num_layers=self.pool.shape[0], num_kv_heads=heads,
+                                head_dim=dim)
+        memo[id(self)] = new
+        new.pool.copy_(self.pool)
+        new.refs, new.unused = list(self.refs), list(self.unused)
+        new.step, new.step_rows = self.step, self.step_rows
+        for a, b in zip(new.layers, self.layers):
+            a.step = b.step
+        new._batch([list(t) for t in self.tables], list(self.lengths), list(self.tops))
+        return new
 
     def crop(self, max_length: int) -> None:
         top = max(self.lengths, default=0)

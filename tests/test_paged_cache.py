@@ -212,6 +212,34 @@ def test_transformers_protocol():
         cache(window_size=4).update(k, k, 0)
 
 
+def test_a_step_cut_off_by_an_error_and_a_reset():
+    c = cache(batch_size=1)
+    k = torch.randn(1, H, 5, D)
+    c.update(k, k, 0)  # layer 1 never gets there
+    c.reset()
+    for i in (0, 1):
+        kk, _ = c.update(k, k, i)
+        assert torch.equal(kk, k)
+
+
+def test_deepcopy_is_a_cache_of_its_own():
+    import copy
+    c = cache(num_pages=20)
+    m = Mirror(c)
+    m.add([40, 16, 0])
+    c.fork(0, 2)
+    m.rows[2] = list(m.rows[0])
+    d = copy.deepcopy(c)
+    n = Mirror(d)
+    n.rows, n.next = [list(r) for r in m.rows], m.next
+    m.add([1, 2, 3])
+    n.check()
+    n.add([7, 0, 7])
+    m.check()
+    n.check()
+    assert d.layers[0]._cache is d and d.layers[0].k_pages.data_ptr() != c.layers[0].k_pages.data_ptr()
+
+
 @pytest.mark.parametrize("kw", [dict(page_size=24), dict(page_size=8), dict(batch_size=0), dict(max_seq_len=0),
                                 dict(num_pages=0), dict(window_size=-1), dict(num_prefix_tokens=-1),
                                 dict(num_layers=None)])

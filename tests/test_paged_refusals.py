@@ -64,6 +64,11 @@ def test_row_starts_are_checked(call):
         call(args(q_start=torch.zeros(4, dtype=torch.int64)))
 
 
+def test_prefill_needs_row_starts():
+    with pytest.raises(_lib.SabreError, match="needs q_start"):
+        prefill(args(q_start=None))
+
+
 def test_rows_are_checked():
     half = torch.zeros(3, 4, 64, dtype=torch.bfloat16)
     with pytest.raises(_lib.SabreError, match="unit last"):
@@ -138,6 +143,15 @@ def test_c_attention_checks(call):
     assert call(prefix=-1) == -1 and b"num_prefix_tokens" in err()
     assert call(q=20) == -3 and call(o=20) == -3
     assert call(qs=i64(1024, 100)) == -3 and call(os=i64(100, 128)) == -3
+
+
+def test_c_decode_workspace_and_size():
+    err = _lib.lib().sabre_last_error
+    need = _lib.lib().sabre_paged_decode_workspace_size(2, 8, 2, 128)
+    assert need > 0
+    assert c_decode(ws=None) == -5 and c_decode(ws=16, wsb=need - 1) == -5 and b"workspace" in err()
+    assert c_decode(ws=24, wsb=need) == -3
+    assert c_decode(batch=1 << 24, cols=1 << 20, ts=1 << 20, ws=16, wsb=1 << 40) == -2 and b"2^37" in err()
 
 
 def test_c_store_and_prefill_rows():
