@@ -90,6 +90,9 @@ __device__ __forceinline__ bool find_job(const Params& p, int slot, int* scratch
   const int tid = threadIdx.x;
   const int per = (p.c.batch + kThreads - 1) / kThreads;
   const int b0 = min(tid * per, p.c.batch), b1 = min(b0 + per, p.c.batch);
+  // The first length comes with the starts, not after them: one round trip
+  // for as many sequences as threads.
+  const int len0 = b0 < b1 ? p.c.seq_lens[b0] : 0;
   int mine = 0;
   for (int b = b0; b < b1; ++b) {
     const int len = row_start(p.starts, b + 1, p.rows) - row_start(p.starts, b, p.rows);
@@ -108,11 +111,15 @@ __device__ __forceinline__ bool find_job(const Params& p, int slot, int* scratch
   for (int w = 0; w < (tid >> 5); ++w) left -= scratch[w];
   if (left >= 0 && left < mine) {
     for (int b = b0; b < b1; ++b) {
-      const int len = row_start(p.starts, b + 1, p.rows) - row_start(p.starts, b, p.rows);
+      const int first = row_start(p.starts, b, p.rows);
+      const int len = row_start(p.starts, b + 1, p.rows) - first;
       const int nt = (max(len, 0) + p.tokens - 1) / p.tokens;
       if (left < nt) {
         scratch[8] = b;
-        scratch[9] = left;
+        scratch[9] = left * p.tokens;
+        scratch[10] = first;
+        scratch[11] = len;
+        scratch[12] = b == b0 ? len0 : p.c.seq_lens[b];
         break;
       }
       left -= nt;
@@ -121,13 +128,11 @@ __device__ __forceinline__ bool find_job(const Params& p, int slot, int* scratch
   __syncthreads();
   job.b = scratch[8];
   if (job.b < 0) return false;
-  const int first = row_start(p.starts, job.b, p.rows);
-  const int len = row_start(p.starts, job.b + 1, p.rows) - first;
-  const int r = scratch[9] * p.tokens;
-  job.row0 = first + r;
+  const int r = scratch[9], len = scratch[11], length = scratch[12];
+  job.row0 = scratch[10] + r;
   job.count = min(p.tokens, len - r);
-  job.pos0 = p.c.seq_lens[job.b] - len + r;
-  job.n = min(p.c.length(job.b), max(job.pos0 + job.count, 0));  // keys that some row may see
+  job.pos0 = length - len + r;
+  job.n = min(min(max(length, 0), p.c.capacity()), max(job.pos0 + job.count, 0));  // keys that some row may see
   job.lo = p.w.first(job.pos0);
   job.from = job.lo / kTile;
   job.head = min((min(p.w.prefix, job.lo) + kTile - 1) / kTile, job.from);
@@ -182,8 +187,10 @@ __global__ void __launch_bounds__(kThreads, 2)
     tmem_relinquish();
     tc_fence_before();
   }
-  // The set-up above overlaps the loads of find_job, whose barriers order it
-  // before its use.
+  // The set-up above overlaps the tail of the stream's previous kernel (this is
+  // a programmatic dependent launch) and the loads of find_job, whose barriers
+  // order it before its use. Nothing before this line reads what that kernel wrote.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   Job job;
   const bool any_job = find_job(p, slot, reinterpret_cast<int*>(smem + kMiscOff + 8), job);
   tc_fence_after();
@@ -488,6 +495,7 @@ __global__ void __launch_bounds__(kThreads, 2)
 // One warp per (row, head): joins the parts of a split call in order.
 template <typename T>
 __global__ void __launch_bounds__(256) paged_combine_kernel(const Params p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int heads = p.heads_kv * p.group;
   const long long i = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) >> 5;
   const int lane = threadIdx.x & 31;
@@ -586,12 +594,10 @@ static cudaError_t launch(const CUtensorMap& mq, const CUtensorMap& mk, const CU
   if (e != cudaSuccess) return e;
   const unsigned hs = static_cast<unsigned>(p.heads_kv * p.splits);
   const dim3 grid = p.head_major ? dim3(p.slots, hs) : dim3(hs, p.slots);
-  paged_prefill_kernel<T><<<grid, kThreads, kSmemBytes, s>>>(mq, mk, mv, p);
-  if (p.splits > 1) {
-    const long long warps = static_cast<long long>(p.rows) * p.heads_kv * p.group;
-    paged_combine_kernel<T><<<static_cast<unsigned>((warps + 7) / 8), 256, 0, s>>>(p);
-  }
-  return cudaGetLastError();
+  e = launch_dependent(grid, kThreads, kSmemBytes, s, paged_prefill_kernel<T>, mq, mk, mv, p);
+  if (e != cudaSuccess || p.splits == 1) return e;
+  const long long warps = static_cast<long long>(p.rows) * p.heads_kv * p.group;
+  return launch_dependent(dim3(static_cast<unsigned>((warps + 7) / 8)), 256, 0, s, paged_combine_kernel<T>, p);
 }
 
 }  // namespace pre
