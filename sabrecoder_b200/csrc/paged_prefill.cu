@@ -9,11 +9,14 @@
 // consecutive tokens times the g query heads of the group, token by token, so
 // that a group's heads share each K/V tile, a short continuation fills its
 // rows, and a window's span grows by fewer tokens. Its key tiles (64 keys) are
-// the prefix tiles, then those of the window: nothing else is visited. When
-// the tiles of rows alone would leave SMs idle, the key tiles of a row tile
-// are dealt out to `splits` CTAs whose parts paged_combine_kernel joins.
-// Sequences, lengths and pages are only read on the device, so a captured
-// call follows them; the grid is the most row tiles that the rows could need.
+// the prefix tiles, then those of the window: nothing else is visited. Many
+// (row tile, KV head) pairs run as one CTA each, heaviest first. When there are
+// too few of them to fill the card evenly, and they are long, their key tiles
+// are dealt out in equal contiguous shares to two CTAs per SM instead
+// (kShares): a CTA walks its share as segments, a pair inside one share is
+// finished there, the others leave (m, l, O) per row and paged_combine_kernel
+// adds them in share order. Sequences, lengths and pages are only read on the
+// device, so a captured call follows them.
 //
 // Roles, tensor-memory layout and barrier protocol are those of
 // prefill_bsa.cu (224 threads, two CTAs per SM: warps 0-3 softmax, 4 Q and K
@@ -34,7 +37,8 @@ using prefill::row_max64;
 
 constexpr int kThreads = 224;
 constexpr int kRows = 128;
-constexpr int kMaxSplits = 32;
+constexpr int kShareBatch = 128;  // sequences of a call that runs in shares, at most
+constexpr int kMinShare = 8;      // key tiles of a share, at least
 constexpr int kQBytes = kRows * kD * 2;  // [d-half][128 rows][128 B], 128-byte swizzle
 constexpr int kQOff = 0;
 constexpr int kKOff = kQOff + kQBytes;
@@ -53,6 +57,9 @@ enum Bar {
 };
 constexpr int kMiscOff = kBarOff + NUM_BARS * 8;
 constexpr int kSmemBytes = kMiscOff + 72;
+// kShares also keeps, per sequence: first row, rows, length, row tiles before it.
+constexpr int kSeqOff = kSmemBytes;
+constexpr int kShareSmemBytes = kSeqOff + 4 * kShareBatch * 4;
 constexpr uint32_t kTmemCols = 256;
 constexpr uint32_t kTmemS = 128;  // + 64 * buffer
 
@@ -61,12 +68,16 @@ struct Params {
   Window w;
   const int32_t* starts;
   void* o;
-  float* part_acc;  // [splits][rows][Hq][D]
-  float* part_ml;   // [splits][rows][Hq][2]
+  // kShares: the parts of two segments of every share, and the pair whose first
+  // part ends the share: {parts (0: none), KV head, place of the first part, -},
+  // {first row, tokens, -, -}.
+  float* part_acc;  // [2 * kDecCtas][kRows][D]
+  float* part_ml;   // [2 * kDecCtas][kRows][2]
+  int4* joins;      // [kDecCtas][2]
   long long o_sr, o_sh;
   int rows, heads_kv, group, tokens;  // tokens of a row tile: 128 / group
-  int box_shift, splits, slots;       // slots: row tiles of the grid
-  int head_major;
+  int box_shift, slots;               // slots: row tiles of the grid
+  int head_major, ctas;               // ctas: of a call in shares, else 0
   float scale_log2;
 };
 
@@ -85,6 +96,45 @@ struct Job {
   }
 };
 
+// The row tile at row r of sequence b, whose `len` new rows begin at row
+// `first` and end its `length` rows.
+__device__ __forceinline__ Job make_job(const Params& p, int b, int r, int first, int len, int length) {
+  Job job;
+  job.b = b;
+  job.row0 = first + r;
+  job.count = min(p.tokens, len - r);
+  job.pos0 = length - len + r;
+  job.n = min(min(max(length, 0), p.c.capacity()), max(job.pos0 + job.count, 0));  // keys that some row may see
+  job.lo = p.w.first(job.pos0);
+  job.from = job.lo / kTile;
+  const int whole = (job.n + kTile - 1) / kTile;
+  job.head = min(min((min(p.w.prefix, job.lo) + kTile - 1) / kTile, job.from), whole);
+  job.tiles = job.head + max(0, whole - job.from);
+  return job;
+}
+
+// Exclusive prefix sum over the CTA's threads; scratch: 8 ints. `all`: the total.
+__device__ __forceinline__ int prefix_sum(int mine, int* scratch, int& all) {
+  const int tid = threadIdx.x;
+  int incl = mine;
+#pragma unroll
+  for (int s = 1; s < 32; s <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, incl, s);
+    if ((tid & 31) >= s) incl += up;
+  }
+  __syncthreads();  // scratch is free
+  if ((tid & 31) == 31) scratch[tid >> 5] = incl;
+  __syncthreads();
+  int before = 0;
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    before += w < (tid >> 5) ? scratch[w] : 0;
+    all += scratch[w];
+  }
+  return before + incl - mine;
+}
+
 // Row tile `slot` of the batch, found by the whole CTA; scratch: 16 ints.
 __device__ __forceinline__ bool find_job(const Params& p, int slot, int* scratch, Job& job) {
   const int tid = threadIdx.x;
@@ -98,17 +148,9 @@ __device__ __forceinline__ bool find_job(const Params& p, int slot, int* scratch
     const int len = row_start(p.starts, b + 1, p.rows) - row_start(p.starts, b, p.rows);
     mine += (max(len, 0) + p.tokens - 1) / p.tokens;
   }
-  int incl = mine;
-#pragma unroll
-  for (int s = 1; s < 32; s <<= 1) {
-    const int up = __shfl_up_sync(0xffffffffu, incl, s);
-    if ((tid & 31) >= s) incl += up;
-  }
-  if ((tid & 31) == 31) scratch[tid >> 5] = incl;
   if (tid == 0) scratch[8] = -1;
-  __syncthreads();
-  int left = slot - (incl - mine);
-  for (int w = 0; w < (tid >> 5); ++w) left -= scratch[w];
+  int all = 0;
+  int left = slot - prefix_sum(mine, scratch, all);
   if (left >= 0 && left < mine) {
     for (int b = b0; b < b1; ++b) {
       const int first = row_start(p.starts, b, p.rows);
@@ -126,23 +168,90 @@ __device__ __forceinline__ bool find_job(const Params& p, int slot, int* scratch
     }
   }
   __syncthreads();
-  job.b = scratch[8];
-  if (job.b < 0) return false;
-  const int r = scratch[9], len = scratch[11], length = scratch[12];
-  job.row0 = scratch[10] + r;
-  job.count = min(p.tokens, len - r);
-  job.pos0 = length - len + r;
-  job.n = min(min(max(length, 0), p.c.capacity()), max(job.pos0 + job.count, 0));  // keys that some row may see
-  job.lo = p.w.first(job.pos0);
-  job.from = job.lo / kTile;
-  job.head = min((min(p.w.prefix, job.lo) + kTile - 1) / kTile, job.from);
-  const int whole = (job.n + kTile - 1) / kTile;
-  job.head = min(job.head, whole);
-  job.tiles = job.head + max(0, whole - job.from);
+  if (scratch[8] < 0) return false;
+  job = make_job(p, scratch[8], scratch[9], scratch[10], scratch[11], scratch[12]);
   return true;
 }
 
+// A place in a call's order of work: key tile `tile` of KV head hk and the row
+// tile that begins at row r of sequence b.
+struct RowPlace {
+  int b, r, hk, tile;
+};
+
+// kShares: lists the sequences in seq, then finds the shares and the place of
+// this CTA's first tile; scratch: 16 ints. Rows of row tiles that see no key
+// are zeroed on the way. False without a share.
 template <typename T>
+__device__ __forceinline__ bool find_share(const Params& p, int* seq, int* scratch, Shares& sh, RowPlace& at) {
+  const int tid = threadIdx.x;
+  int* const first_slot = seq + 3 * kShareBatch;
+  int slots = 0;
+  if (tid < p.c.batch) {
+    const int first = row_start(p.starts, tid, p.rows);
+    const int len = max(row_start(p.starts, tid + 1, p.rows) - first, 0);
+    slots = (len + p.tokens - 1) / p.tokens;
+    seq[tid] = first;
+    seq[kShareBatch + tid] = len;
+    seq[2 * kShareBatch + tid] = p.c.seq_lens[tid];
+  }
+  int nslots = 0;
+  const int before = prefix_sum(slots, scratch, nslots);
+  if (tid < p.c.batch) first_slot[tid] = before;
+  __syncthreads();
+  auto sequence = [&](int slot) -> int {  // the last b with first_slot[b] <= slot
+    int lo = 0, hi = p.c.batch;
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      (first_slot[mid] <= slot ? lo : hi) = mid;
+    }
+    return lo;
+  };
+  auto job_of = [&](int slot) -> Job {
+    const int b = sequence(slot);
+    return make_job(p, b, (slot - first_slot[b]) * p.tokens, seq[b], seq[kShareBatch + b], seq[2 * kShareBatch + b]);
+  };
+  const int per = (nslots + kThreads - 1) / kThreads;
+  const int s0 = min(tid * per, nslots), s1 = min(s0 + per, nslots);
+  int mine = 0;
+  for (int s = s0; s < s1; ++s) mine += job_of(s).tiles;
+  int all = 0;
+  const int ahead = prefix_sum(mine, scratch, all);
+  const int units = p.heads_kv * p.group * (kD / 8);  // 16-byte stores of a row
+  for (int s = blockIdx.x; s < nslots; s += p.ctas) {
+    const Job job = job_of(s);
+    if (job.tiles > 0) continue;
+    for (int i = tid; i < job.count * units; i += kThreads) {
+      const int u = i % units;
+      *reinterpret_cast<uint4*>(static_cast<T*>(p.o) + static_cast<long long>(job.row0 + i / units) * p.o_sr +
+                                u / (kD / 8) * p.o_sh + u % (kD / 8) * 8) = make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
+  sh.total = static_cast<long long>(all) * p.heads_kv;
+  sh.ctas = static_cast<int>(max(1ll, min(static_cast<long long>(p.ctas), sh.total / kMinShare)));
+  if (all == 0 || static_cast<int>(blockIdx.x) >= sh.ctas) return false;
+  long long left = sh.first(blockIdx.x) - static_cast<long long>(ahead) * p.heads_kv;
+  if (left >= 0 && left < static_cast<long long>(mine) * p.heads_kv) {
+    for (int s = s0; s < s1; ++s) {
+      const Job job = job_of(s);
+      const long long here = static_cast<long long>(job.tiles) * p.heads_kv;
+      if (left < here) {
+        scratch[8] = job.b;
+        scratch[9] = (s - first_slot[job.b]) * p.tokens;
+        scratch[10] = static_cast<int>(left / job.tiles);
+        scratch[11] = static_cast<int>(left % job.tiles);
+        break;
+      }
+      left -= here;
+    }
+  }
+  __syncthreads();
+  at = RowPlace{scratch[8], scratch[9], scratch[10], scratch[11]};
+  return true;
+}
+
+// kShares: the CTA walks a share of all key tiles; else it owns a whole pair.
+template <typename T, bool kShares>
 __global__ void __launch_bounds__(kThreads, 2)
     paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                          const __grid_constant__ CUtensorMap tmV, const Params p) {
@@ -155,28 +264,13 @@ __global__ void __launch_bounds__(kThreads, 2)
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kMiscOff + 4);
   auto bar = [&](int i) -> uint32_t { return sbase + kBarOff + 8u * i; };
 
-  // Later row tiles of a sequence see more keys: heaviest first. Row-major
-  // (grid x = head) or head-major (grid x = row tile), as in prefill_bsa.cu.
-  const int hs = p.head_major ? static_cast<int>(blockIdx.y) : static_cast<int>(blockIdx.x);
-  const int hk = hs / p.splits;
-  const int split = hs - hk * p.splits;
-  const int slot = p.slots - 1 - static_cast<int>(p.head_major ? blockIdx.x : blockIdx.y);
   if (tid == 0) {
     const bool bad = (sbase & 1023u) != 0u;
     *abort_flag = bad ? 1 : 0;
     if (bad) record_status(SABRE_DEV_BAD_SMEM_ALIGN);
   }
   if (warp == 4 && lane == 0) {
-    mbar_init(bar(Q_FULL), 1);
-    for (int s = 0; s < 2; ++s) {
-      mbar_init(bar(K_FULL + s), 1);
-      mbar_init(bar(V_FULL + s), 1);
-      mbar_init(bar(PRO + s), 1);
-      mbar_init(bar(DONE + s), 1);
-      mbar_init(bar(P_FULL + s), 4);
-    }
-    mbar_init(bar(V_RAW), 1);
-    mbar_init(bar(MMA_DONE), 1);
+    for (int i = 0; i < NUM_BARS; ++i) mbar_init(bar(i), i == P_FULL || i == P_FULL + 1 ? 4 : 1);
     fence_mbar_init();
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmK);
@@ -188,23 +282,81 @@ __global__ void __launch_bounds__(kThreads, 2)
     tc_fence_before();
   }
   // The set-up above overlaps the tail of the stream's previous kernel (this is
-  // a programmatic dependent launch) and the loads of find_job, whose barriers
-  // order it before its use. Nothing before this line reads what that kernel wrote.
+  // a programmatic dependent launch) and the loads below, whose barriers order
+  // it before its use. Nothing before this line reads what that kernel wrote.
   asm volatile("griddepcontrol.wait;" ::: "memory");
+  int* const scratch = reinterpret_cast<int*>(smem + kMiscOff + 8);
+  int* const seq = reinterpret_cast<int*>(smem + kSeqOff);
   Job job;
-  const bool any_job = find_job(p, slot, reinterpret_cast<int*>(smem + kMiscOff + 8), job);
+  Shares sh;
+  RowPlace at;
+  long long units = 0;  // key tiles of the share still to be done
+  int hk = 0;
+  bool some;
+  if constexpr (kShares) {
+    // Nothing to join, unless the last segment says so.
+    if (tid == 0) p.joins[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
+    some = find_share<T>(p, seq, scratch, sh, at);
+    if (some) units = sh.first(blockIdx.x + 1) - sh.first(blockIdx.x);
+  } else {
+    // Later row tiles of a sequence see more keys: heaviest first. Row-major
+    // (grid x = head) or head-major (grid x = row tile), as in prefill_bsa.cu.
+    hk = p.head_major ? static_cast<int>(blockIdx.y) : static_cast<int>(blockIdx.x);
+    some = find_job(p, p.slots - 1 - static_cast<int>(p.head_major ? blockIdx.x : blockIdx.y), scratch, job);
+  }
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  if (!any_job) {
-    if (warp == 5) tmem_dealloc(tmem, kTmemCols);
-    return;
-  }
-  // This part's key tiles.
-  const int j0 = static_cast<int>(static_cast<long long>(job.tiles) * split / p.splits);
-  const int nt = static_cast<int>(static_cast<long long>(job.tiles) * (split + 1) / p.splits) - j0;
-  const bool start_ok = (*abort_flag == 0);
   const int boxes = kTile >> p.box_shift;
   const int box_rows = 1 << p.box_shift;
+  const bool start_ok = (*abort_flag == 0);
+
+  // The barriers' phases run on over the segments: every completion of a segment
+  // has been waited for when it ends, so a wait's parity is that of a first
+  // segment plus what the earlier ones completed: one phase a segment (Q_FULL,
+  // PRO[0], MMA_DONE), one for each with a second tile (PRO[1]: twos), one for
+  // each even (d0) or odd (d1) tile (K_FULL, V_FULL, P_FULL, DONE), one for
+  // each tile that was zeroed (V_RAW: raws).
+  int d0 = 0, d1 = 0, twos = 0, raws = 0;
+  for (int segment = 0; some; ++segment) {
+  const int seg_par = segment & 1, two_par = twos & 1;
+  // Parity of the completion for the k-th tile of stage s (0 or 1).
+  auto par = [&](int s, int k) -> uint32_t { return static_cast<uint32_t>(k + (s ? d1 : d0)) & 1u; };
+  // This segment: key tiles [j0, j0 + nt) of the pair.
+  int j0 = 0, nt = job.tiles, place = 0;
+  bool part = false;
+  if constexpr (kShares) {
+    if (segment > 0) {
+      at.tile = 0;
+      if (++at.hk == p.heads_kv) {
+        at.hk = 0;
+        at.r += p.tokens;
+      }
+    }
+    for (;;) {  // the next row tile that sees a key; units > 0: there is one
+      while (at.b < p.c.batch - 1 && at.r >= seq[kShareBatch + at.b]) {
+        ++at.b;
+        at.r = 0;
+      }
+      job = make_job(p, at.b, at.r, seq[at.b], seq[kShareBatch + at.b], seq[2 * kShareBatch + at.b]);
+      if (job.tiles > 0 || job.count <= 0) break;
+      at.r += p.tokens;
+    }
+    hk = at.hk;
+    j0 = at.tile;
+    nt = static_cast<int>(min(static_cast<long long>(job.tiles - j0), units));
+    units -= nt;
+    part = nt < job.tiles;
+    // A part is kept as the share's first (0) or last (1) segment.
+    place = 2 * static_cast<int>(blockIdx.x) + (segment > 0 ? 1 : 0);
+    if (units == 0 && tid == 0) {
+      // When the share ends inside a pair that began in it, the pair is joined for it.
+      const int rest = j0 == 0 ? job.tiles - nt : 0;
+      const int parts = rest > 0 ? sh.owner(sh.first(blockIdx.x + 1) + rest - 1) - static_cast<int>(blockIdx.x) + 1 : 0;
+      p.joins[2 * blockIdx.x] = make_int4(parts, hk, place, 0);
+      p.joins[2 * blockIdx.x + 1] = make_int4(job.row0, job.count, 0, 0);
+    }
+    __syncthreads();
+  }
 
   constexpr uint32_t kIdescQK = idesc_f16(128, 64, DT<T>::kBf16, false);
   constexpr uint32_t kIdescPV = idesc_f16(128, 128, DT<T>::kBf16, true);
@@ -241,9 +393,10 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (j >= 2) {
           // As in prefill_bsa.cu: K(j) may overwrite its stage after S(j-2)
           // (PRO[j-2] for j < 4, else in C(j-4)), V(j) after P.V(j-2) (C(j-2)).
-          const int wb = is_k && j < 4 ? PRO + (j - 2) : DONE + s;
-          const int par = is_k ? (j < 4 ? 0 : (j >> 1) & 1) : ((j >> 1) - 1) & 1;
-          ok = mbar_wait_warp(bar(wb), par, abort_flag);
+          if (is_k && j < 4)
+            ok = mbar_wait_warp(bar(PRO + (j - 2)), j == 2 ? seg_par : two_par, abort_flag);
+          else
+            ok = mbar_wait_warp(bar(DONE + s), par(s, (j >> 1) - (is_k ? 2 : 1)), abort_flag);
           if (!ok) break;
         }
         // Rows of V at and past the sequence's end inside a box are zeroed.
@@ -262,9 +415,10 @@ __global__ void __launch_bounds__(kThreads, 2)
         issued = j + 1;
         if (clean) {
           raw = true;
-          ok = mbar_wait_warp(bar(V_RAW), 0, abort_flag);
+          const int raw_par = raws++ & 1;
+          ok = mbar_wait_warp(bar(V_RAW), raw_par, abort_flag);
           if (!ok) break;
-          (void)mbar_test_wait(bar(V_RAW), 0);  // each lane's own acquire of the copied bytes
+          (void)mbar_test_wait(bar(V_RAW), raw_par);  // each lane's own acquire of the copied bytes
           const int end = (over + box_rows) & ~(box_rows - 1);
           for (int c = lane; c < (end - over) * 16; c += 32) {
             const int row = over + (c >> 4);
@@ -280,12 +434,12 @@ __global__ void __launch_bounds__(kThreads, 2)
     // Every issued copy must land before the CTA may exit. (The tile that ends
     // the sequence is the last one: only it can have gone through V_RAW.)
     if (lane == 0 && start_ok) {
-      if (is_k) mbar_wait_drain(bar(Q_FULL), 0);
+      if (is_k) mbar_wait_drain(bar(Q_FULL), seg_par);
       for (int j = max(0, issued - 2); j < issued; ++j) {
         if (raw && j == issued - 1)
-          mbar_wait_drain(bar(V_RAW), 0);
+          mbar_wait_drain(bar(V_RAW), (raws - 1) & 1);
         else
-          mbar_wait_drain(bar(full0 + (j & 1)), (j >> 1) & 1);
+          mbar_wait_drain(bar(full0 + (j & 1)), par(j & 1, j >> 1));
       }
     }
   } else if (warp == 5) {
@@ -295,10 +449,10 @@ __global__ void __launch_bounds__(kThreads, 2)
       const uint64_t kd0 = smem_desc_sw128(sbase + kKOff, 16, 1024);
       const uint64_t vd0 = smem_desc_sw128(sbase + kVOff, kTileBytes / 2, 1024);
       const uint32_t s_tmem = tmem + kTmemS;
-      bool ok = mbar_wait(bar(Q_FULL), 0, abort_flag);
+      bool ok = mbar_wait(bar(Q_FULL), seg_par, abort_flag);
       auto issue_s = [&](int j) -> bool {
         const int ks = j & 1;
-        if (!mbar_wait(bar(K_FULL + ks), (j >> 1) & 1, abort_flag)) return false;
+        if (!mbar_wait(bar(K_FULL + ks), par(ks, j >> 1), abort_flag)) return false;
         tc_fence_after();
         const uint64_t kd = kd0 + static_cast<uint64_t>(ks * (kTileBytes >> 4));
         const uint32_t dst = s_tmem + 64 * ks;
@@ -312,8 +466,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       };
       auto issue_pv = [&](int i) -> bool {
         const int pb = i & 1;
-        if (!mbar_wait(bar(P_FULL + pb), (i >> 1) & 1, abort_flag)) return false;
-        if (!mbar_wait(bar(V_FULL + pb), (i >> 1) & 1, abort_flag)) return false;
+        if (!mbar_wait(bar(P_FULL + pb), par(pb, i >> 1), abort_flag)) return false;
+        if (!mbar_wait(bar(V_FULL + pb), par(pb, i >> 1), abort_flag)) return false;
         tc_fence_after();
         const uint64_t vd = vd0 + static_cast<uint64_t>(pb * (kTileBytes >> 4));
         const uint32_t pa = s_tmem + 64 * pb;
@@ -333,7 +487,12 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       // Whatever was issued must finish before tensor memory is released.
       mma_commit(bar(MMA_DONE));
-      mbar_wait_drain(bar(MMA_DONE), 0);
+      mbar_wait_drain(bar(MMA_DONE), seg_par);
+      if constexpr (kShares) {
+        // C(nt-2), which nobody else may wait for, has arrived too.
+        for (int x = 0; ok && x < 2; ++x)
+          if (nt > x) mbar_wait_drain(bar(DONE + x), par(x, (nt - x - 1) >> 1));
+      }
     }
   } else {
     // ---------------- softmax + epilogue (warps 0-3) ----------------
@@ -376,8 +535,8 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int sb = j & 1;
       const uint32_t ts = tl + kTmemS + 64 * sb;
       // S(j): PRO[j] for j < 2, else in C(j-2)
-      ok = j < 2 ? mbar_wait_warp(bar(PRO + j), 0, abort_flag)
-                 : mbar_wait_warp(bar(DONE + sb), ((j >> 1) - 1) & 1, abort_flag);
+      ok = j < 2 ? mbar_wait_warp(bar(PRO + j), j == 0 ? seg_par : two_par, abort_flag)
+                 : mbar_wait_warp(bar(DONE + sb), par(sb, (j >> 1) - 1), abort_flag);
       if (!ok) break;
       tc_fence_after();
       uint32_t pk[32];
@@ -415,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, 2)
       }
       // O must not change under a running P.V: rescale only after P.V(j-1).
       if (j >= 1 && __any_sync(0xffffffffu, rescale)) {
-        ok = mbar_wait_warp(bar(DONE + ((j - 1) & 1)), ((j - 1) >> 1) & 1, abort_flag);
+        ok = mbar_wait_warp(bar(DONE + ((j - 1) & 1)), par((j - 1) & 1, (j - 1) >> 1), abort_flag);
         if (!ok) break;
         tc_fence_after();
 #pragma unroll 1
@@ -436,16 +595,15 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (lane == 0) mbar_arrive(bar(P_FULL + sb));
     }
     if (ok && nt >= 1) {
-      ok = mbar_wait(bar(DONE + ((nt - 1) & 1)), ((nt - 1) >> 1) & 1, abort_flag);
+      ok = mbar_wait(bar(DONE + ((nt - 1) & 1)), par((nt - 1) & 1, (nt - 1) >> 1), abort_flag);
       ok = __all_sync(0xffffffffu, ok);
       tc_fence_after();
     }
     ok = __all_sync(0xffffffffu, ok);
     // After a timeout anywhere in the CTA the tile is incomplete: store nothing.
     if (ok && *abort_flag == 0) {
-      const long long row = job.row0 + tok;
-      const long long part = (split * static_cast<long long>(p.rows) + row) * (p.heads_kv * p.group) + head;
-      T* orow = static_cast<T*>(p.o) + row * p.o_sr + head * p.o_sh;
+      T* orow = static_cast<T*>(p.o) + static_cast<long long>(job.row0 + tok) * p.o_sr + head * p.o_sh;
+      const long long prow = static_cast<long long>(place) * kRows + tid;
       const float inv = 1.0f / l_run;  // unused where the row saw nothing: it is zero
       const uint64_t opol = l2_policy_evict_first();
 #pragma unroll 1
@@ -459,8 +617,8 @@ __global__ void __launch_bounds__(kThreads, 2)
           for (int c = 0; c < 32; ++c) ov[c] = 0u;
         }
         if (!real) continue;
-        if (p.splits > 1) {
-          uint4* dst = reinterpret_cast<uint4*>(p.part_acc + part * kD + ch * 32);
+        if (part) {
+          uint4* dst = reinterpret_cast<uint4*>(p.part_acc + prow * kD + ch * 32);
 #pragma unroll
           for (int q4 = 0; q4 < 8; ++q4)
             dst[q4] = make_uint4(ov[4 * q4], ov[4 * q4 + 1], ov[4 * q4 + 2], ov[4 * q4 + 3]);
@@ -478,56 +636,73 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
         }
       }
-      if (real && p.splits > 1) {
-        p.part_ml[part * 2] = m_run;
-        p.part_ml[part * 2 + 1] = l_run;
-      }
+      if (real && part) *reinterpret_cast<float2*>(p.part_ml + prow * 2) = make_float2(m_run, l_run);
     }
   }
 
+  tc_fence_before();
   __syncthreads();
-  if (warp == 5) {
-    tc_fence_after();
-    tmem_dealloc(tmem, kTmemCols);
-  }
+  tc_fence_after();
+  if (!kShares || units == 0 || *abort_flag != 0) break;
+  d0 += (nt + 1) >> 1;
+  d1 += nt >> 1;
+  twos += nt >= 2 ? 1 : 0;
+  }  // segments
+
+  if (warp == 5) tmem_dealloc(tmem, kTmemCols);
 }
 
-// One warp per (row, head): joins the parts of a split call in order.
+// Joins the parts of the pair whose first part ends share blockIdx.x, if there
+// is one, in share order: a warp per row, four columns a lane, eight parts in
+// flight.
 template <typename T>
 __global__ void __launch_bounds__(256) paged_combine_kernel(const Params p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int heads = p.heads_kv * p.group;
-  const long long i = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) >> 5;
+  const int x = blockIdx.x;
   const int lane = threadIdx.x & 31;
-  const long long row = i / heads;
-  const int head = static_cast<int>(i - row * heads);
-  // No sequence's row: padding behind the last one.
-  if (row < row_start(p.starts, 0, p.rows) || row >= row_start(p.starts, p.c.batch, p.rows)) return;
-  const long long step = static_cast<long long>(p.rows) * heads;
-  float m = -INFINITY, l = 0.f;
-  if (lane < p.splits) {
-    m = p.part_ml[(i + lane * step) * 2];
-    l = p.part_ml[(i + lane * step) * 2 + 1];
-  }
-  float M = m;
+  const int row = blockIdx.y * 8 + (threadIdx.x >> 5);
+  const int4 pair = p.joins[2 * x];
+  const int parts = pair.x;
+  if (parts == 0) return;
+  const int4 rows = p.joins[2 * x + 1];
+  const int tok = row / p.group;
+  if (tok >= rows.y) return;
+  // The first part is the last segment of its share, the others open theirs.
+  auto slot = [&](int i) -> long long { return static_cast<long long>(i == 0 ? pair.z : 2 * (x + i)) * kRows + row; };
+  constexpr int kBatch = 8;
+  float M = -INFINITY, L = 0.f;
+  float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < parts; i0 += kBatch) {
+    float2 ml[kBatch];
+    float4 a[kBatch];
 #pragma unroll
-  for (int o = 16; o; o >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, o));
-  const float w = M == -INFINITY ? 0.f : ex2(m - M);
-  float L = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int s = 0; s < p.splits; ++s) {
-    const float ws = __shfl_sync(0xffffffffu, w, s);
-    L += ws * __shfl_sync(0xffffffffu, l, s);
-    if (ws == 0.f) continue;  // a part that saw nothing
-    const float4 a = *reinterpret_cast<const float4*>(p.part_acc + (i + s * step) * kD + lane * 4);
-    acc.x += ws * a.x;
-    acc.y += ws * a.y;
-    acc.z += ws * a.z;
-    acc.w += ws * a.w;
+    for (int u = 0; u < kBatch; ++u) {
+      const int i = i0 + u;
+      ml[u] = i < parts ? *reinterpret_cast<const float2*>(p.part_ml + slot(i) * 2) : make_float2(-INFINITY, 0.f);
+      a[u] = i < parts ? *reinterpret_cast<const float4*>(p.part_acc + slot(i) * kD + lane * 4)
+                       : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+    float mn = M;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) mn = fmaxf(mn, ml[u].x);
+    if (mn == -INFINITY) continue;
+    const float r = ex2(M - mn);
+    M = mn;
+    L *= r;
+    A = make_float4(A.x * r, A.y * r, A.z * r, A.w * r);
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u) {
+      const float w = ex2(ml[u].x - mn);
+      L += w * ml[u].y;
+      A.x += w * a[u].x;
+      A.y += w * a[u].y;
+      A.z += w * a[u].z;
+      A.w += w * a[u].w;
+    }
   }
-  const float inv = L > 0.f ? 1.0f / L : 0.f;
-  *reinterpret_cast<uint2*>(static_cast<T*>(p.o) + row * p.o_sr + head * p.o_sh + lane * 4) =
-      make_uint2(DT<T>::pack(acc.x * inv, acc.y * inv), DT<T>::pack(acc.z * inv, acc.w * inv));
+  store_row<T>(static_cast<T*>(p.o) + static_cast<long long>(rows.x + tok) * p.o_sr +
+                   (pair.y * p.group + row - tok * p.group) * p.o_sh,
+               lane, A, L);
 }
 
 // Row tiles that `rows` rows of `batch` sequences need at most: a sequence of
@@ -537,15 +712,11 @@ static inline long long row_slots(int rows, int batch, int tokens) {
   return static_cast<long long>(rows - k) / tokens + k;
 }
 
-// CTAs per row tile, as far as the host can tell: enough that the card's 296
-// places are filled, with at least eight key tiles each, counted for a row
-// tile in the middle of its sequence's new rows. A part costs a CTA's start
-// and read-out and 516 bytes per row and head through the workspace: 512 rows
-// of a single sequence at 56/8 heads on 15872 rows run 297 us whole and 307 in
-// two parts (232 row tiles), 64 rows at 16 heads on 16000 rows 234 us whole
-// and 37 in 16 parts; 1000 rows on none run 22 us whole and 25 in two.
-static int plan_splits(int rows, int batch, int heads_q, int heads_kv, int page_size, int max_pages, int window,
-                       int prefix) {
+// Whether a call runs in shares, as far as the host can tell: few pairs (row
+// tile, KV head) that are long, 32 key tiles or more, counted for a row tile in
+// the middle of its sequence's new rows.
+static bool in_shares(int rows, int batch, int heads_q, int heads_kv, int page_size, int max_pages, int window,
+                      int prefix) {
   const int tokens = kRows / (heads_q / heads_kv);
   long long span = static_cast<long long>(page_size) * max_pages;
   span -= (rows / batch < span ? rows / batch : span) / 2;
@@ -553,17 +724,12 @@ static int plan_splits(int rows, int batch, int heads_q, int heads_kv, int page_
     const long long seen = static_cast<long long>(window) + tokens + prefix;
     if (seen < span) span = seen;
   }
-  const long long tiles = span / kTile;
-  if (tiles < 32) return 1;
-  long long s = kDecCtas / (row_slots(rows, batch, tokens) * heads_kv);
-  if (s > tiles / 8) s = tiles / 8;
-  if (s > kMaxSplits) s = kMaxSplits;
-  return s < 1 ? 1 : static_cast<int>(s);
+  return batch <= kShareBatch && row_slots(rows, batch, tokens) * heads_kv <= 2 * kDecCtas && span >= 32 * kTile;
 }
 
-static size_t workspace_bytes(int rows, int heads_q, int splits) {
-  return splits == 1 ? 0 : static_cast<size_t>(splits) * rows * heads_q * (kD + 2) * sizeof(float);
-}
+// Joins, then the parts of two segments of every share.
+static constexpr size_t kShareWorkspace =
+    kDecCtas * 2 * sizeof(int4) + static_cast<size_t>(2) * kDecCtas * kRows * (kD + 2) * sizeof(float);
 
 // Tensor map of q [rows, Hq, D]: dims (128 d, g heads of a group, rows, KV
 // heads); box = (64 d, g, tokens, 1): one d-half of a row tile, token by token.
@@ -590,14 +756,15 @@ static int make_map_q(CUtensorMap* m, const void* q, int dtype, int rows, int he
 template <typename T>
 static cudaError_t launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Params& p,
                           cudaStream_t s) {
-  cudaError_t e = cudaFuncSetAttribute(paged_prefill_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  const int smem = p.ctas > 0 ? kShareSmemBytes : kSmemBytes;
+  auto kernel = p.ctas > 0 ? paged_prefill_kernel<T, true> : paged_prefill_kernel<T, false>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
-  const unsigned hs = static_cast<unsigned>(p.heads_kv * p.splits);
-  const dim3 grid = p.head_major ? dim3(p.slots, hs) : dim3(hs, p.slots);
-  e = launch_dependent(grid, kThreads, kSmemBytes, s, paged_prefill_kernel<T>, mq, mk, mv, p);
-  if (e != cudaSuccess || p.splits == 1) return e;
-  const long long warps = static_cast<long long>(p.rows) * p.heads_kv * p.group;
-  return launch_dependent(dim3(static_cast<unsigned>((warps + 7) / 8)), 256, 0, s, paged_combine_kernel<T>, p);
+  const dim3 grid = p.ctas > 0 ? dim3(p.ctas) : p.head_major ? dim3(p.slots, p.heads_kv) : dim3(p.heads_kv, p.slots);
+  e = launch_dependent(grid, kThreads, smem, s, kernel, mq, mk, mv, p);
+  if (e != cudaSuccess || p.ctas == 0) return e;
+  const int tile_rows = (p.rows < p.tokens ? p.rows : p.tokens) * p.group;
+  return launch_dependent(dim3(p.ctas, (tile_rows + 7) / 8), 256, 0, s, paged_combine_kernel<T>, p);
 }
 
 }  // namespace pre
@@ -612,8 +779,9 @@ size_t sabre_paged_prefill_workspace_size(int rows, int batch, int heads_q, int 
   if (rows <= 0 || batch <= 0 || heads_q <= 0 || heads_kv <= 0 || head_dim != kD || heads_q % heads_kv != 0 ||
       heads_q / heads_kv > kGroup || page_size <= 0 || max_pages <= 0)
     return 0;
-  return pre::workspace_bytes(rows, heads_q, pre::plan_splits(rows, batch, heads_q, heads_kv, page_size, max_pages,
-                                                              window, num_prefix_tokens));
+  return pre::in_shares(rows, batch, heads_q, heads_kv, page_size, max_pages, window, num_prefix_tokens)
+             ? pre::kShareWorkspace
+             : 0;
 }
 
 int sabre_paged_prefill(const void* q, const void* k_pages, const void* v_pages, void* o, const int32_t* page_table,
@@ -641,25 +809,21 @@ int sabre_paged_prefill(const void* q, const void* k_pages, const void* v_pages,
   p.group = heads_q / heads_kv;
   p.tokens = pre::kRows / p.group;
   p.box_shift = p.c.page_shift < 6 ? p.c.page_shift : 6;
-  p.splits = pre::plan_splits(rows, batch, heads_q, heads_kv, page_size, max_pages, window, num_prefix_tokens);
   p.scale_log2 = scale_log2(softmax_scale);
-  const size_t need = pre::workspace_bytes(rows, heads_q, p.splits);
-  if (need > 0 && (!workspace || workspace_bytes < need))
-    return sabre_fail(SABRE_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", fn, workspace_bytes, need);
-  if (need > 0 && !aligned16(workspace))
+  const bool shares =
+      pre::in_shares(rows, batch, heads_q, heads_kv, page_size, max_pages, window, num_prefix_tokens);
+  p.ctas = shares ? kDecCtas : 0;
+  if (shares && (!workspace || workspace_bytes < pre::kShareWorkspace))
+    return sabre_fail(SABRE_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", fn, workspace_bytes, pre::kShareWorkspace);
+  if (shares && !aligned16(workspace))
     return sabre_fail(SABRE_ERR_ALIGNMENT, "%s: workspace must be 16-byte aligned", fn);
-  p.part_acc = static_cast<float*>(workspace);
-  p.part_ml = need > 0 ? p.part_acc + static_cast<size_t>(p.splits) * rows * heads_q * kD : nullptr;
+  p.joins = static_cast<int4*>(workspace);
+  p.part_acc = shares ? reinterpret_cast<float*>(p.joins + 2 * kDecCtas) : nullptr;
+  p.part_ml = shares ? p.part_acc + static_cast<size_t>(2) * kDecCtas * pre::kRows * kD : nullptr;
   const long long slots = pre::row_slots(rows, batch, p.tokens);
   // The rule of prefill_bsa.cu: K/V larger than this -> head-major order.
   const long long kv_bytes = 4ll * heads_kv * kD * batch * page_size * max_pages;
-  p.head_major = kv_bytes > (112ll << 20) ? 1 : 0;
-  const long long hs = static_cast<long long>(heads_kv) * p.splits;
-  if ((p.head_major ? hs : slots) > 65535) p.head_major ^= 1;
-  if ((p.head_major ? hs : slots) > 65535)
-    return sabre_fail(SABRE_ERR_UNSUPPORTED, "%s: %lld row tiles of %lld head parts exceed the grid", fn, slots, hs);
-  if ((static_cast<long long>(rows) * heads_q + 7) / 8 > 0x7fffffffll)
-    return sabre_fail(SABRE_ERR_UNSUPPORTED, "%s: rows * heads_q too large", fn);
+  p.head_major = kv_bytes > (112ll << 20) || slots > 65535 ? 1 : 0;
   p.slots = static_cast<int>(slots);
   CUtensorMap mq, mk, mv;
   if ((st = pre::make_map_q(&mq, q, dtype, rows, heads_kv, p.group, p.tokens, q_strides[0], q_strides[1])) != SABRE_OK)

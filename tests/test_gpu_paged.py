@@ -122,6 +122,14 @@ PREFILL = [
     ([9000], [20], 2, 2, 64, BF, None, 0, "phtd"),
     ([9000, 31], [3, 2], 7, 1, 16, FP, None, 0, "phtd"),
     (list(range(1, 120)), list(range(1, 120)), 2, 1, 16, BF, None, 0, "phtd"),
+    # Few row tiles over a long table: the call runs in shares of the key tiles.
+    ([3000, 5000, 100], [300, 129, 100], 4, 2, 64, BF, None, 0, "phtd"),
+    ([2500, 0, 6000, 4096], [1, 0, 700, 64], 7, 1, 16, FP, None, 0, "ptkhd"),
+    ([8000, 3000], [200, 3000], 2, 2, 128, BF, 2500, 100, "phtd"),
+    ([20000], [130], 56, 8, 64, BF, None, 0, "phtd"),
+    ([4000, 30, 2100, 2], [40, 30, 1, 2], 8, 1, 1024, BF, 2050, 0, "phtd"),
+    ([17 * i % 400 + 2100 for i in range(128)], [i % 3 for i in range(128)], 3, 1, 16, BF, None, 0, "phtd"),
+    ([17 * i % 400 + 2100 for i in range(129)], [i % 3 for i in range(129)], 3, 1, 16, FP, None, 0, "phtd"),
 ]
 
 
@@ -141,24 +149,29 @@ def test_paged_prefill_vs_oracle(K, case):
     assert K.device_status(clear=True) == 0
 
 
-def test_rows_that_see_nothing_give_zeros(K):
+@pytest.mark.parametrize("extra_cols", [1, 300])  # 300: the call runs in shares
+def test_rows_that_see_nothing_give_zeros(K, extra_cols):
     """Sequences shorter than their new rows, absent pages under every visible
     key, lengths of zero."""
-    q, kp, vp, table, sl, starts = make(5, [40, 100, 64], [40, 100, 64], 4, 2, 16, BF)
+    q, kp, vp, table, sl, starts = make(5, [40, 100, 64], [40, 100, 64], 4, 2, 16, BF, extra_cols=extra_cols)
     table[1] = -1
     sl[0] = 10  # 30 of the 40 rows lie before the sequence
     out = K.paged_prefill(q, kp, vp, table, sl, starts)
     assert (out[:30] == 0).all() and (out[40:140] == 0).all() and (out[140:] != 0).any()
     check(out, (q, kp, vp, table, sl, starts), starts=starts)
-    sl[2] = 0
+    sl[1] = 0  # a whole row tile before the sequence
+    out = K.paged_prefill(q, kp, vp, table, sl, starts)
+    assert (out[:30] == 0).all() and (out[40:140] == 0).all() and (out[140:] != 0).any()
+    check(out, (q, kp, vp, table, sl, starts), starts=starts)
+    sl[1], sl[2] = 100, 0
     out = K.paged_decode(q[:3], kp, vp, table, sl)
     assert (out[1:] == 0).all() and (out[0] != 0).any()
 
 
-@pytest.mark.parametrize("ps", [16, 64, 128])
-def test_absent_pages_inside_a_tile(K, ps):
+@pytest.mark.parametrize("ps,extra_cols", [(16, 1), (64, 1), (128, 1), (16, 300), (64, 50)])
+def test_absent_pages_inside_a_tile(K, ps, extra_cols):
     """Pages missing at the start, inside and at the end are not visible."""
-    args = make(6, [1000, 900], [1, 1], 6, 2, ps, BF)
+    args = make(6, [1000, 900], [1, 1], 6, 2, ps, BF, extra_cols=extra_cols)
     q, kp, vp, table, sl, _ = args
     for b, p in ((0, 0), (0, 3), (0, 4), (1, 1), (1, 899 // ps)):
         if table[b, p] >= 0:
