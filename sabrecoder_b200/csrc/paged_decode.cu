@@ -224,7 +224,8 @@ __device__ __forceinline__ void mma_16x8x16(float (&c)[4], const uint32_t (&a)[4
 template <typename T>
 __device__ __forceinline__ void store_row(T* out, int lane, const float4& a, float l) {
   const float inv = l > 0.f ? 1.0f / l : 0.f;
-  *reinterpret_cast<uint2*>(out + lane * 4) = make_uint2(DT<T>::pack(a.x * inv, a.y * inv), DT<T>::pack(a.z * inv, a.w * inv));
+  *reinterpret_cast<uint2*>(out + lane * 4) =
+      make_uint2(DT<T>::pack(a.x * inv, a.y * inv), DT<T>::pack(a.z * inv, a.w * inv));
 }
 
 template <typename T>

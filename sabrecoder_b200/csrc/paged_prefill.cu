@@ -12,17 +12,18 @@
 // the prefix tiles, then those of the window: nothing else is visited. Many
 // (row tile, KV head) pairs run as one CTA each, heaviest first. When there are
 // too few of them to fill the card evenly, and they are long, their key tiles
-// are dealt out in equal contiguous shares to two CTAs per SM instead
-// (kShares): a CTA walks its share as segments, a pair inside one share is
-// finished there, the others leave (m, l, O) per row and paged_combine_kernel
-// adds them in share order. Sequences, lengths and pages are only read on the
+// are dealt out to two CTAs per SM instead (kShares, see RowShares): a CTA
+// walks its share as segments, a pair inside one share is finished there, the
+// others leave (m, l, O) per row and paged_combine_kernel adds them in share
+// order. Sequences, lengths and pages are only read on the
 // device, so a captured call follows them.
 //
 // Roles, tensor-memory layout and barrier protocol are those of
 // prefill_bsa.cu (224 threads, two CTAs per SM: warps 0-3 softmax, 4 Q and K
 // producer, 5 MMA issuer, 6 V producer; S = Q K^T of M=128 N=64 into two
-// buffers, P over its S, O += P V with P from tensor memory), whose model
-// check covers them. Different here: tiles come box by box from pages (a TMA
+// buffers, P over its S, O += P V with P from tensor memory); from one segment
+// of a share to the next each role goes on by itself (model-checked:
+// tests/test_paged_prefill_protocol.py). Different here: tiles come box by box from pages (a TMA
 // box is min(page_size, 64) rows; absent pages and boxes that no row sees are
 // read outside the pool and give zeros), and rows past the sequence's end
 // inside a page are zeroed in V before its tile is handed to the MMA, since
@@ -39,6 +40,7 @@ constexpr int kThreads = 224;
 constexpr int kRows = 128;
 constexpr int kShareBatch = 128;  // sequences of a call that runs in shares, at most
 constexpr int kMinShare = 8;      // key tiles of a share, at least
+constexpr int kMaxPairs = 2 * kDecCtas;
 constexpr int kQBytes = kRows * kD * 2;  // [d-half][128 rows][128 B], 128-byte swizzle
 constexpr int kQOff = 0;
 constexpr int kKOff = kQOff + kQBytes;
@@ -57,9 +59,9 @@ enum Bar {
 };
 constexpr int kMiscOff = kBarOff + NUM_BARS * 8;
 constexpr int kSmemBytes = kMiscOff + 72;
-// kShares also keeps, per sequence: first row, rows, length, row tiles before it.
+// kShares also keeps, per sequence: first row, rows, length, row tiles before it; and 64 counts.
 constexpr int kSeqOff = kSmemBytes;
-constexpr int kShareSmemBytes = kSeqOff + 4 * kShareBatch * 4;
+constexpr int kShareSmemBytes = kSeqOff + (4 * kShareBatch + 64) * 4;
 constexpr uint32_t kTmemCols = 256;
 constexpr uint32_t kTmemS = 128;  // + 64 * buffer
 
@@ -68,12 +70,12 @@ struct Params {
   Window w;
   const int32_t* starts;
   void* o;
-  // kShares: the parts of two segments of every share, and the pair whose first
-  // part ends the share: {parts (0: none), KV head, place of the first part, -},
-  // {first row, tokens, -, -}.
+  // kShares: the parts of two segments of every share, and for every pair (row
+  // tile times KV heads plus head) {parts (0: finished), share and place of the
+  // first, -}, {first row, tokens, -, -}.
   float* part_acc;  // [2 * kDecCtas][kRows][D]
   float* part_ml;   // [2 * kDecCtas][kRows][2]
-  int4* joins;      // [kDecCtas][2]
+  int4* joins;      // [kMaxPairs][2]
   long long o_sr, o_sh;
   int rows, heads_kv, group, tokens;  // tokens of a row tile: 128 / group
   int box_shift, slots;               // slots: row tiles of the grid
@@ -179,11 +181,26 @@ struct RowPlace {
   int b, r, hk, tile;
 };
 
-// kShares: lists the sequences in seq, then finds the shares and the place of
-// this CTA's first tile; scratch: 16 ints. Rows of row tiles that see no key
+// How a call in shares is dealt out. Whole parts: every pair is cut into equal
+// parts of its own and a CTA has one of them, when that leaves none with more
+// than kSlack key tiles above the mean. Else the tiles of all pairs, in order,
+// are cut into equal shares: a CTA may then finish one pair and begin another,
+// which costs it a second start and read-out, about kSlack tiles' time (300
+// rows on 4000 at 16/16 heads, 48 pairs of 66 tiles: 31 us a call in parts, 38
+// in shares; 512 rows on 15872 at 56/8 heads, 232 pairs of 250 tiles: 304 us
+// uncut, 285 in shares; 8 sequences of 32 rows on 2000 to 4000: 72 and 55).
+constexpr int kSlack = 6;
+struct RowShares : Shares {
+  bool whole;
+  int parts;        // whole: parts of the pair if this CTA has the first of several, else 0
+  long long units;  // key tiles of this CTA
+};
+
+// kShares: lists the sequences in seq, then finds this CTA's share and the
+// place of its first tile; scratch: 16 ints. Rows of row tiles that see no key
 // are zeroed on the way. False without a share.
 template <typename T>
-__device__ __forceinline__ bool find_share(const Params& p, int* seq, int* scratch, Shares& sh, RowPlace& at) {
+__device__ __forceinline__ bool find_share(const Params& p, int* seq, int* scratch, RowShares& sh, RowPlace& at) {
   const int tid = threadIdx.x;
   int* const first_slot = seq + 3 * kShareBatch;
   int slots = 0;
@@ -218,35 +235,88 @@ __device__ __forceinline__ bool find_share(const Params& p, int* seq, int* scrat
   int all = 0;
   const int ahead = prefix_sum(mine, scratch, all);
   const int units = p.heads_kv * p.group * (kD / 8);  // 16-byte stores of a row
-  for (int s = blockIdx.x; s < nslots; s += p.ctas) {
-    const Job job = job_of(s);
+  for (int s = blockIdx.x; s < p.slots; s += p.ctas) {
+    const Job job = s < nslots ? job_of(s) : Job{};
     if (job.tiles > 0) continue;
+    for (int h = tid; h < p.heads_kv; h += kThreads) p.joins[2 * (s * p.heads_kv + h)] = make_int4(0, 0, 0, 0);
     for (int i = tid; i < job.count * units; i += kThreads) {
       const int u = i % units;
       *reinterpret_cast<uint4*>(static_cast<T*>(p.o) + static_cast<long long>(job.row0 + i / units) * p.o_sr +
                                 u / (kD / 8) * p.o_sh + u % (kD / 8) * 8) = make_uint4(0u, 0u, 0u, 0u);
     }
   }
+  if (all == 0) return false;
   sh.total = static_cast<long long>(all) * p.heads_kv;
-  sh.ctas = static_cast<int>(max(1ll, min(static_cast<long long>(p.ctas), sh.total / kMinShare)));
-  if (all == 0 || static_cast<int>(blockIdx.x) >= sh.ctas) return false;
-  long long left = sh.first(blockIdx.x) - static_cast<long long>(ahead) * p.heads_kv;
-  if (left >= 0 && left < static_cast<long long>(mine) * p.heads_kv) {
-    for (int s = s0; s < s1; ++s) {
-      const Job job = job_of(s);
-      const long long here = static_cast<long long>(job.tiles) * p.heads_kv;
-      if (left < here) {
-        scratch[8] = job.b;
-        scratch[9] = (s - first_slot[job.b]) * p.tokens;
-        scratch[10] = static_cast<int>(left / job.tiles);
-        scratch[11] = static_cast<int>(left % job.tiles);
-        break;
+  // Parts of whole pairs of at most most + i tiles each, when so many CTAs do
+  // for them all: the smallest i.
+  const int most = static_cast<int>(max(static_cast<long long>(kMinShare), (sh.total + p.ctas - 1) / p.ctas));
+  int count[kSlack + 1] = {};
+  for (int s = s0; s < s1; ++s) {
+    const int tiles = job_of(s).tiles;
+#pragma unroll
+    for (int i = 0; i <= kSlack; ++i) count[i] += (tiles + most + i - 1) / (most + i);
+  }
+  int* const counts = seq + 4 * kShareBatch;  // [kSlack + 1][8]
+#pragma unroll
+  for (int i = 0; i <= kSlack; ++i) {
+    const int sum = __reduce_add_sync(0xffffffffu, count[i]);
+    if ((tid & 31) == 0) counts[i * 8 + (tid >> 5)] = sum;
+  }
+  __syncthreads();
+  int slack = kSlack + 1, mine_parts = 0;
+#pragma unroll
+  for (int i = kSlack; i >= 0; --i) {
+    long long sum = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) sum += counts[i * 8 + w];
+    if (sum * p.heads_kv <= p.ctas) slack = i, mine_parts = count[i];
+  }
+  sh.whole = slack <= kSlack;
+  if (sh.whole) {
+    int parts_all = 0;
+    int left = static_cast<int>(blockIdx.x) - prefix_sum(mine_parts, scratch, parts_all) * p.heads_kv;
+    sh.ctas = parts_all * p.heads_kv;
+    if (static_cast<int>(blockIdx.x) >= sh.ctas) return false;
+    if (left >= 0 && left < mine_parts * p.heads_kv) {
+      for (int s = s0; s < s1; ++s) {
+        const Job job = job_of(s);
+        const int parts = (job.tiles + most + slack - 1) / (most + slack);
+        if (left < parts * p.heads_kv) {
+          const int k = left % parts;
+          const long long from = static_cast<long long>(job.tiles) * k / parts;
+          scratch[8] = job.b;
+          scratch[9] = (s - first_slot[job.b]) * p.tokens;
+          scratch[10] = left / parts;
+          scratch[11] = static_cast<int>(from);
+          scratch[12] = static_cast<int>(static_cast<long long>(job.tiles) * (k + 1) / parts - from);
+          scratch[13] = k == 0 && parts > 1 ? parts : 0;
+          break;
+        }
+        left -= parts * p.heads_kv;
       }
-      left -= here;
+    }
+  } else {
+    sh.ctas = p.ctas;  // all busy: most > kMinShare, else parts would do
+    long long left = sh.first(blockIdx.x) - static_cast<long long>(ahead) * p.heads_kv;
+    if (left >= 0 && left < static_cast<long long>(mine) * p.heads_kv) {
+      for (int s = s0; s < s1; ++s) {
+        const Job job = job_of(s);
+        const long long here = static_cast<long long>(job.tiles) * p.heads_kv;
+        if (left < here) {
+          scratch[8] = job.b;
+          scratch[9] = (s - first_slot[job.b]) * p.tokens;
+          scratch[10] = static_cast<int>(left / job.tiles);
+          scratch[11] = static_cast<int>(left % job.tiles);
+          break;
+        }
+        left -= here;
+      }
     }
   }
   __syncthreads();
   at = RowPlace{scratch[8], scratch[9], scratch[10], scratch[11]};
+  sh.units = sh.whole ? scratch[12] : sh.first(blockIdx.x + 1) - sh.first(blockIdx.x);
+  sh.parts = scratch[13];
   return true;
 }
 
@@ -288,16 +358,14 @@ __global__ void __launch_bounds__(kThreads, 2)
   int* const scratch = reinterpret_cast<int*>(smem + kMiscOff + 8);
   int* const seq = reinterpret_cast<int*>(smem + kSeqOff);
   Job job;
-  Shares sh;
+  RowShares sh;
   RowPlace at;
   long long units = 0;  // key tiles of the share still to be done
   int hk = 0;
   bool some;
   if constexpr (kShares) {
-    // Nothing to join, unless the last segment says so.
-    if (tid == 0) p.joins[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
     some = find_share<T>(p, seq, scratch, sh, at);
-    if (some) units = sh.first(blockIdx.x + 1) - sh.first(blockIdx.x);
+    if (some) units = sh.units;
   } else {
     // Later row tiles of a sequence see more keys: heaviest first. Row-major
     // (grid x = head) or head-major (grid x = row tile), as in prefill_bsa.cu.
@@ -310,365 +378,378 @@ __global__ void __launch_bounds__(kThreads, 2)
   const int box_rows = 1 << p.box_shift;
   const bool start_ok = (*abort_flag == 0);
 
-  // The barriers' phases run on over the segments: every completion of a segment
-  // has been waited for when it ends, so a wait's parity is that of a first
-  // segment plus what the earlier ones completed: one phase a segment (Q_FULL,
-  // PRO[0], MMA_DONE), one for each with a second tile (PRO[1]: twos), one for
-  // each even (d0) or odd (d1) tile (K_FULL, V_FULL, P_FULL, DONE), one for
-  // each tile that was zeroed (V_RAW: raws).
+  // The barriers' phases run on over the segments: a wait's parity is that of a
+  // first segment plus what the earlier ones completed: one phase a segment
+  // (Q_FULL, PRO[0], MMA_DONE), one for each with a second tile (PRO[1]: twos),
+  // one for each even (d0) or odd (d1) tile (K_FULL, V_FULL, P_FULL, DONE), one
+  // for each tile that was zeroed (V_RAW: raws). No barrier can complete two
+  // phases ahead of a waiter: the next segment's first loads wait for MMA_DONE,
+  // which is committed after every other completion has been seen.
   int d0 = 0, d1 = 0, twos = 0, raws = 0;
   for (int segment = 0; some; ++segment) {
-  const int seg_par = segment & 1, two_par = twos & 1;
-  // Parity of the completion for the k-th tile of stage s (0 or 1).
-  auto par = [&](int s, int k) -> uint32_t { return static_cast<uint32_t>(k + (s ? d1 : d0)) & 1u; };
-  // This segment: key tiles [j0, j0 + nt) of the pair.
-  int j0 = 0, nt = job.tiles, place = 0;
-  bool part = false;
-  if constexpr (kShares) {
-    if (segment > 0) {
-      at.tile = 0;
-      if (++at.hk == p.heads_kv) {
-        at.hk = 0;
+    const int seg_par = segment & 1, two_par = twos & 1;
+    // After a timeout the walk goes on without work: every pair's record is written.
+    const bool going = start_ok && (!kShares || __all_sync(0xffffffffu, *abort_flag == 0));
+    // Parity of the completion for the k-th tile of stage s (0 or 1).
+    auto par = [&](int s, int k) -> uint32_t { return static_cast<uint32_t>(k + (s ? d1 : d0)) & 1u; };
+    // This segment: key tiles [j0, j0 + nt) of the pair.
+    int j0 = 0, nt = job.tiles, place = 0;
+    bool part = false;
+    if constexpr (kShares) {
+      if (segment > 0) {
+        at.tile = 0;
+        if (++at.hk == p.heads_kv) {
+          at.hk = 0;
+          at.r += p.tokens;
+        }
+      }
+      for (;;) {  // the next row tile that sees a key; units > 0: there is one
+        while (at.b < p.c.batch - 1 && at.r >= seq[kShareBatch + at.b]) {
+          ++at.b;
+          at.r = 0;
+        }
+        job = make_job(p, at.b, at.r, seq[at.b], seq[kShareBatch + at.b], seq[2 * kShareBatch + at.b]);
+        if (job.tiles > 0 || job.count <= 0) break;
         at.r += p.tokens;
       }
-    }
-    for (;;) {  // the next row tile that sees a key; units > 0: there is one
-      while (at.b < p.c.batch - 1 && at.r >= seq[kShareBatch + at.b]) {
-        ++at.b;
-        at.r = 0;
+      hk = at.hk;
+      j0 = at.tile;
+      nt = static_cast<int>(min(static_cast<long long>(job.tiles - j0), units));
+      units -= nt;
+      part = nt < job.tiles;
+      // A part is kept as the share's first (0) or last (1) segment.
+      place = 2 * static_cast<int>(blockIdx.x) + (segment > 0 ? 1 : 0);
+      if (j0 == 0 && tid == 0) {
+        // The pair begins here: does it end here too?
+        const int rest = job.tiles - nt;
+        int parts = sh.parts;
+        if (!sh.whole)
+          parts = rest > 0 ? sh.owner(sh.first(blockIdx.x + 1) + rest - 1) - static_cast<int>(blockIdx.x) + 1 : 0;
+        const int pair = (seq[3 * kShareBatch + at.b] + at.r / p.tokens) * p.heads_kv + hk;
+        p.joins[2 * pair] = make_int4(parts, static_cast<int>(blockIdx.x), place, 0);
+        p.joins[2 * pair + 1] = make_int4(job.row0, job.count, 0, 0);
       }
-      job = make_job(p, at.b, at.r, seq[at.b], seq[kShareBatch + at.b], seq[2 * kShareBatch + at.b]);
-      if (job.tiles > 0 || job.count <= 0) break;
-      at.r += p.tokens;
     }
-    hk = at.hk;
-    j0 = at.tile;
-    nt = static_cast<int>(min(static_cast<long long>(job.tiles - j0), units));
-    units -= nt;
-    part = nt < job.tiles;
-    // A part is kept as the share's first (0) or last (1) segment.
-    place = 2 * static_cast<int>(blockIdx.x) + (segment > 0 ? 1 : 0);
-    if (units == 0 && tid == 0) {
-      // When the share ends inside a pair that began in it, the pair is joined for it.
-      const int rest = j0 == 0 ? job.tiles - nt : 0;
-      const int parts = rest > 0 ? sh.owner(sh.first(blockIdx.x + 1) + rest - 1) - static_cast<int>(blockIdx.x) + 1 : 0;
-      p.joins[2 * blockIdx.x] = make_int4(parts, hk, place, 0);
-      p.joins[2 * blockIdx.x + 1] = make_int4(job.row0, job.count, 0, 0);
-    }
-    __syncthreads();
-  }
 
-  constexpr uint32_t kIdescQK = idesc_f16(128, 64, DT<T>::kBf16, false);
-  constexpr uint32_t kIdescPV = idesc_f16(128, 128, DT<T>::kBf16, true);
+    constexpr uint32_t kIdescQK = idesc_f16(128, 64, DT<T>::kBf16, false);
+    constexpr uint32_t kIdescPV = idesc_f16(128, 128, DT<T>::kBf16, true);
 
-  if (warp == 4 || warp == 6) {
-    // ---------------- TMA producers (warp 4: K, warp 6: V) ----------------
-    const bool is_k = (warp == 4);
-    const int full0 = is_k ? K_FULL : V_FULL;
-    const uint32_t ring = sbase + (is_k ? kKOff : kVOff);
-    const CUtensorMap* map = is_k ? &tmK : &tmV;
-    if (is_k && lane == 0 && start_ok) {
-      mbar_arrive_expect_tx(bar(Q_FULL), static_cast<uint32_t>(p.group * p.tokens) * 256u);
-      const uint64_t pol = l2_policy_evict_first();
-      tma_load_4d_hint(sbase + kQOff, &tmQ, bar(Q_FULL), 0, 0, job.row0, hk, pol);
-      tma_load_4d_hint(sbase + kQOff + kQBytes / 2, &tmQ, bar(Q_FULL), 64, 0, job.row0, hk, pol);
-    }
-    int issued = 0;    // tiles
-    bool raw = false;  // the last one went through V_RAW
-    bool ok = start_ok;
-    for (int i0 = 0; ok && i0 < nt * boxes; i0 += 32) {
-      // The pages of the next 32 boxes, one per lane; num_pages reads zeros.
-      int page = p.c.num_pages, off = 0;
-      if (i0 + lane < nt * boxes) {
-        const int t = job.pos(j0 + (i0 + lane) / boxes) + (((i0 + lane) % boxes) << p.box_shift);
-        off = t & ((1 << p.c.page_shift) - 1);
-        if (job.any(p.w, t, box_rows)) {
-          const int pg = p.c.page_of(job.b, t);
-          if (pg >= 0) page = pg;
-        }
+    if (warp == 4 || warp == 6) {
+      // ---------------- TMA producers (warp 4: K, warp 6: V) ----------------
+      const bool is_k = (warp == 4);
+      const int full0 = is_k ? K_FULL : V_FULL;
+      const uint32_t ring = sbase + (is_k ? kKOff : kVOff);
+      const CUtensorMap* map = is_k ? &tmK : &tmV;
+      // The segment before is done with the Q tile and both stages (while its O is
+      // still read out).
+      bool ok = going;
+      if (kShares && segment > 0 && ok) ok = mbar_wait_warp(bar(MMA_DONE), seg_par ^ 1, abort_flag);
+      if (is_k && lane == 0 && ok) {
+        mbar_arrive_expect_tx(bar(Q_FULL), static_cast<uint32_t>(p.group * p.tokens) * 256u);
+        const uint64_t pol = l2_policy_evict_first();
+        tma_load_4d_hint(sbase + kQOff, &tmQ, bar(Q_FULL), 0, 0, job.row0, hk, pol);
+        tma_load_4d_hint(sbase + kQOff + kQBytes / 2, &tmQ, bar(Q_FULL), 64, 0, job.row0, hk, pol);
       }
-      for (int i = i0; i < min(i0 + 32, nt * boxes); i += boxes) {
-        const int j = i / boxes;
-        const int s = j & 1;
-        if (j >= 2) {
-          // As in prefill_bsa.cu: K(j) may overwrite its stage after S(j-2)
-          // (PRO[j-2] for j < 4, else in C(j-4)), V(j) after P.V(j-2) (C(j-2)).
-          if (is_k && j < 4)
-            ok = mbar_wait_warp(bar(PRO + (j - 2)), j == 2 ? seg_par : two_par, abort_flag);
-          else
-            ok = mbar_wait_warp(bar(DONE + s), par(s, (j >> 1) - (is_k ? 2 : 1)), abort_flag);
-          if (!ok) break;
-        }
-        // Rows of V at and past the sequence's end inside a box are zeroed.
-        const int over = job.n - job.pos(j0 + j);
-        const bool clean = !is_k && over < kTile && (over & (box_rows - 1)) != 0;
-        const uint32_t full = bar(clean ? V_RAW : full0 + s);
-        if (lane == 0) mbar_arrive_expect_tx(full, kTileBytes);
-        __syncwarp();
-        const int x = lane - (i - i0);
-        const uint32_t dst = ring + s * kTileBytes;
-        if (x >= 0 && x < boxes) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-            tma_load_page(dst + h * (kTileBytes / 2) + x * box_rows * 128, map, full, off, h, hk, page);
-        }
-        issued = j + 1;
-        if (clean) {
-          raw = true;
-          const int raw_par = raws++ & 1;
-          ok = mbar_wait_warp(bar(V_RAW), raw_par, abort_flag);
-          if (!ok) break;
-          (void)mbar_test_wait(bar(V_RAW), raw_par);  // each lane's own acquire of the copied bytes
-          const int end = (over + box_rows) & ~(box_rows - 1);
-          for (int c = lane; c < (end - over) * 16; c += 32) {
-            const int row = over + (c >> 4);
-            *reinterpret_cast<uint4*>(smem + kVOff + s * kTileBytes + ((c >> 3) & 1) * (kTileBytes / 2) + row * 128 +
-                                      (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+      int issued = 0;    // tiles
+      bool raw = false;  // the last one went through V_RAW
+      const bool began = ok;
+      for (int i0 = 0; ok && i0 < nt * boxes; i0 += 32) {
+        // The pages of the next 32 boxes, one per lane; num_pages reads zeros.
+        int page = p.c.num_pages, off = 0;
+        if (i0 + lane < nt * boxes) {
+          const int t = job.pos(j0 + (i0 + lane) / boxes) + (((i0 + lane) % boxes) << p.box_shift);
+          off = t & ((1 << p.c.page_shift) - 1);
+          if (job.any(p.w, t, box_rows)) {
+            const int pg = p.c.page_of(job.b, t);
+            if (pg >= 0) page = pg;
           }
-          fence_proxy_async_smem();
+        }
+        for (int i = i0; i < min(i0 + 32, nt * boxes); i += boxes) {
+          const int j = i / boxes;
+          const int s = j & 1;
+          if (j >= 2) {
+            // As in prefill_bsa.cu: K(j) may overwrite its stage after S(j-2)
+            // (PRO[j-2] for j < 4, else in C(j-4)), V(j) after P.V(j-2) (C(j-2)).
+            if (is_k && j < 4)
+              ok = mbar_wait_warp(bar(PRO + (j - 2)), j == 2 ? seg_par : two_par, abort_flag);
+            else
+              ok = mbar_wait_warp(bar(DONE + s), par(s, (j >> 1) - (is_k ? 2 : 1)), abort_flag);
+            if (!ok) break;
+          }
+          // Rows of V at and past the sequence's end inside a box are zeroed.
+          const int over = job.n - job.pos(j0 + j);
+          const bool clean = !is_k && over < kTile && (over & (box_rows - 1)) != 0;
+          const uint32_t full = bar(clean ? V_RAW : full0 + s);
+          if (lane == 0) mbar_arrive_expect_tx(full, kTileBytes);
           __syncwarp();
-          if (lane == 0) mbar_arrive(bar(full0 + s));
+          const int x = lane - (i - i0);
+          const uint32_t dst = ring + s * kTileBytes;
+          if (x >= 0 && x < boxes) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              tma_load_page(dst + h * (kTileBytes / 2) + x * box_rows * 128, map, full, off, h, hk, page);
+          }
+          issued = j + 1;
+          if (clean) {
+            raw = true;
+            const int raw_par = raws++ & 1;
+            ok = mbar_wait_warp(bar(V_RAW), raw_par, abort_flag);
+            if (!ok) break;
+            (void)mbar_test_wait(bar(V_RAW), raw_par);  // each lane's own acquire of the copied bytes
+            const int end = (over + box_rows) & ~(box_rows - 1);
+            for (int c = lane; c < (end - over) * 16; c += 32) {
+              const int row = over + (c >> 4);
+              *reinterpret_cast<uint4*>(smem + kVOff + s * kTileBytes + ((c >> 3) & 1) * (kTileBytes / 2) + row * 128 +
+                                        (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar(full0 + s));
+          }
         }
       }
-    }
-    // Every issued copy must land before the CTA may exit. (The tile that ends
-    // the sequence is the last one: only it can have gone through V_RAW.)
-    if (lane == 0 && start_ok) {
-      if (is_k) mbar_wait_drain(bar(Q_FULL), seg_par);
-      for (int j = max(0, issued - 2); j < issued; ++j) {
-        if (raw && j == issued - 1)
-          mbar_wait_drain(bar(V_RAW), (raws - 1) & 1);
-        else
-          mbar_wait_drain(bar(full0 + (j & 1)), par(j & 1, j >> 1));
-      }
-    }
-  } else if (warp == 5) {
-    // ---------------- MMA issuer ----------------
-    if (lane == 0 && start_ok) {
-      const uint64_t qd = smem_desc_sw128(sbase + kQOff, 16, 1024);
-      const uint64_t kd0 = smem_desc_sw128(sbase + kKOff, 16, 1024);
-      const uint64_t vd0 = smem_desc_sw128(sbase + kVOff, kTileBytes / 2, 1024);
-      const uint32_t s_tmem = tmem + kTmemS;
-      bool ok = mbar_wait(bar(Q_FULL), seg_par, abort_flag);
-      auto issue_s = [&](int j) -> bool {
-        const int ks = j & 1;
-        if (!mbar_wait(bar(K_FULL + ks), par(ks, j >> 1), abort_flag)) return false;
-        tc_fence_after();
-        const uint64_t kd = kd0 + static_cast<uint64_t>(ks * (kTileBytes >> 4));
-        const uint32_t dst = s_tmem + 64 * ks;
-#pragma unroll
-        for (int kk = 0; kk < 8; ++kk) {
-          const uint64_t qo = ((kk >> 2) * (kQBytes / 2) + (kk & 3) * 32) >> 4;
-          const uint64_t ko = ((kk >> 2) * (kTileBytes / 2) + (kk & 3) * 32) >> 4;
-          mma_f16_ss(dst, qd + qo, kd + ko, kIdescQK, kk > 0 ? 1u : 0u);
+      // Every issued copy must land before the CTA may exit. (The tile that ends
+      // the sequence is the last one: only it can have gone through V_RAW.)
+      if (lane == 0 && began) {
+        if (is_k) mbar_wait_drain(bar(Q_FULL), seg_par);
+        for (int j = max(0, issued - 2); j < issued; ++j) {
+          if (raw && j == issued - 1)
+            mbar_wait_drain(bar(V_RAW), (raws - 1) & 1);
+          else
+            mbar_wait_drain(bar(full0 + (j & 1)), par(j & 1, j >> 1));
         }
-        return true;
-      };
-      auto issue_pv = [&](int i) -> bool {
-        const int pb = i & 1;
-        if (!mbar_wait(bar(P_FULL + pb), par(pb, i >> 1), abort_flag)) return false;
-        if (!mbar_wait(bar(V_FULL + pb), par(pb, i >> 1), abort_flag)) return false;
-        tc_fence_after();
-        const uint64_t vd = vd0 + static_cast<uint64_t>(pb * (kTileBytes >> 4));
-        const uint32_t pa = s_tmem + 64 * pb;
-        mma_f16_ts(tmem, pa, vd, kIdescPV, i > 0 ? 1u : 0u);
-#pragma unroll
-        for (int kk = 1; kk < 4; ++kk) mma_f16_ts(tmem, pa + 8 * kk, vd + kk * (2048 >> 4), kIdescPV, 1u);
-        return true;
-      };
-      for (int j = 0; ok && j < 2 && j < nt; ++j) {
-        ok = issue_s(j);
-        if (ok) mma_commit(bar(PRO + j));
       }
+    } else if (warp == 5) {
+      // ---------------- MMA issuer ----------------
+      if (lane == 0 && going) {
+        const uint64_t qd = smem_desc_sw128(sbase + kQOff, 16, 1024);
+        const uint64_t kd0 = smem_desc_sw128(sbase + kKOff, 16, 1024);
+        const uint64_t vd0 = smem_desc_sw128(sbase + kVOff, kTileBytes / 2, 1024);
+        const uint32_t s_tmem = tmem + kTmemS;
+        bool ok = mbar_wait(bar(Q_FULL), seg_par, abort_flag);
+        auto issue_s = [&](int j) -> bool {
+          const int ks = j & 1;
+          if (!mbar_wait(bar(K_FULL + ks), par(ks, j >> 1), abort_flag)) return false;
+          tc_fence_after();
+          const uint64_t kd = kd0 + static_cast<uint64_t>(ks * (kTileBytes >> 4));
+          const uint32_t dst = s_tmem + 64 * ks;
+#pragma unroll
+          for (int kk = 0; kk < 8; ++kk) {
+            const uint64_t qo = ((kk >> 2) * (kQBytes / 2) + (kk & 3) * 32) >> 4;
+            const uint64_t ko = ((kk >> 2) * (kTileBytes / 2) + (kk & 3) * 32) >> 4;
+            mma_f16_ss(dst, qd + qo, kd + ko, kIdescQK, kk > 0 ? 1u : 0u);
+          }
+          return true;
+        };
+        auto issue_pv = [&](int i) -> bool {
+          const int pb = i & 1;
+          if (!mbar_wait(bar(P_FULL + pb), par(pb, i >> 1), abort_flag)) return false;
+          if (!mbar_wait(bar(V_FULL + pb), par(pb, i >> 1), abort_flag)) return false;
+          tc_fence_after();
+          const uint64_t vd = vd0 + static_cast<uint64_t>(pb * (kTileBytes >> 4));
+          const uint32_t pa = s_tmem + 64 * pb;
+          mma_f16_ts(tmem, pa, vd, kIdescPV, i > 0 ? 1u : 0u);
+#pragma unroll
+          for (int kk = 1; kk < 4; ++kk) mma_f16_ts(tmem, pa + 8 * kk, vd + kk * (2048 >> 4), kIdescPV, 1u);
+          return true;
+        };
+        for (int j = 0; ok && j < 2 && j < nt; ++j) {
+          ok = issue_s(j);
+          if (ok) mma_commit(bar(PRO + j));
+        }
+        for (int j = 0; ok && j < nt; ++j) {
+          if (!issue_pv(j)) { ok = false; break; }
+          if (j + 2 < nt && !issue_s(j + 2)) { ok = false; break; }
+          mma_commit(bar(DONE + (j & 1)));
+        }
+        if constexpr (kShares) {
+          // The next segment's waiters start from known phases: C(nt-2), which
+          // nobody else may wait for, has arrived too.
+          for (int x = 0; ok && x < 2; ++x)
+            if (nt > x) mbar_wait_drain(bar(DONE + x), par(x, (nt - x - 1) >> 1));
+        }
+        // Whatever was issued must finish before tensor memory is released.
+        mma_commit(bar(MMA_DONE));
+        mbar_wait_drain(bar(MMA_DONE), seg_par);
+      }
+    } else {
+      // ---------------- softmax + epilogue (warps 0-3) ----------------
+      const int tok = tid / p.group;
+      const int head = hk * p.group + tid - tok * p.group;
+      const bool real = tok < job.count;
+      const int pos = job.pos0 + tok;
+      const int seen = real ? min(pos + 1, job.n) : 0;  // keys [0, seen), less the window's gap
+      const int wlo = p.w.first(pos);
+      const uint32_t tl = tmem + (static_cast<uint32_t>(warp * 32) << 16);
+      const float sl2 = p.scale_log2;
+      float m_run = -INFINITY;
+      float l_run = 0.f;
+      bool ok = going;
+      // Absent pages are not visible: the boxes of the next 32 / boxes tiles are
+      // looked up by the lanes, a batch ahead.
+      auto lookup = [&](int i) -> int {
+        const int t = job.pos(j0 + i / boxes) + ((i % boxes) << p.box_shift);
+        return i < nt * boxes && job.any(p.w, t, box_rows) ? p.c.entry(job.b, t) : 0;
+      };
+      int entry_ahead = lookup(lane);
+      uint32_t absent = 0;
       for (int j = 0; ok && j < nt; ++j) {
-        if (!issue_pv(j)) { ok = false; break; }
-        if (j + 2 < nt && !issue_s(j + 2)) { ok = false; break; }
-        mma_commit(bar(DONE + (j & 1)));
-      }
-      // Whatever was issued must finish before tensor memory is released.
-      mma_commit(bar(MMA_DONE));
-      mbar_wait_drain(bar(MMA_DONE), seg_par);
-      if constexpr (kShares) {
-        // C(nt-2), which nobody else may wait for, has arrived too.
-        for (int x = 0; ok && x < 2; ++x)
-          if (nt > x) mbar_wait_drain(bar(DONE + x), par(x, (nt - x - 1) >> 1));
-      }
-    }
-  } else {
-    // ---------------- softmax + epilogue (warps 0-3) ----------------
-    const int tok = tid / p.group;
-    const int head = hk * p.group + tid - tok * p.group;
-    const bool real = tok < job.count;
-    const int pos = job.pos0 + tok;
-    const int seen = real ? min(pos + 1, job.n) : 0;  // keys [0, seen), less the window's gap
-    const int wlo = p.w.first(pos);
-    const uint32_t tl = tmem + (static_cast<uint32_t>(warp * 32) << 16);
-    const float sl2 = p.scale_log2;
-    float m_run = -INFINITY;
-    float l_run = 0.f;
-    bool ok = start_ok;
-    // Absent pages are not visible: the boxes of the next 32 / boxes tiles are
-    // looked up by the lanes, a batch ahead.
-    auto lookup = [&](int i) -> int {
-      const int t = job.pos(j0 + i / boxes) + ((i % boxes) << p.box_shift);
-      return i < nt * boxes && job.any(p.w, t, box_rows) ? p.c.entry(job.b, t) : 0;
-    };
-    int entry_ahead = lookup(lane);
-    uint32_t absent = 0;
-    for (int j = 0; ok && j < nt; ++j) {
-      const int t = job.pos(j0 + j);
-      const int i = j * boxes;
-      if ((i & 31) == 0) {
-        absent = __ballot_sync(0xffffffffu, p.c.checked(entry_ahead) < 0);
-        entry_ahead = lookup(i + 32 + lane);
-      }
-      unsigned long long see = low_bits(seen - t) & (~low_bits(wlo - t) | low_bits(p.w.prefix - t));
-      const uint32_t missing = (absent >> (i & 31)) & ((1u << boxes) - 1u);
-      if (missing != 0u) {
+        const int t = job.pos(j0 + j);
+        const int i = j * boxes;
+        if ((i & 31) == 0) {
+          absent = __ballot_sync(0xffffffffu, p.c.checked(entry_ahead) < 0);
+          entry_ahead = lookup(i + 32 + lane);
+        }
+        unsigned long long see = low_bits(seen - t) & (~low_bits(wlo - t) | low_bits(p.w.prefix - t));
+        const uint32_t missing = (absent >> (i & 31)) & ((1u << boxes) - 1u);
+        if (missing != 0u) {
 #pragma unroll 1
-        for (int x = 0; x < boxes; ++x)
-          if ((missing >> x) & 1u) see &= ~(low_bits(box_rows) << (x << p.box_shift));
-      }
-      // A warp whose rows see no key of this tile stores P = 0 and leaves the
-      // exponential unit to the others.
-      const bool dead = __all_sync(0xffffffffu, see == 0ull);
-      const int sb = j & 1;
-      const uint32_t ts = tl + kTmemS + 64 * sb;
-      // S(j): PRO[j] for j < 2, else in C(j-2)
-      ok = j < 2 ? mbar_wait_warp(bar(PRO + j), j == 0 ? seg_par : two_par, abort_flag)
-                 : mbar_wait_warp(bar(DONE + sb), par(sb, (j >> 1) - 1), abort_flag);
-      if (!ok) break;
-      tc_fence_after();
-      uint32_t pk[32];
-      bool rescale = false;
-      float alpha = 1.0f;
-      if (dead) {
-#pragma unroll
-        for (int c = 0; c < 32; ++c) pk[c] = 0u;
-      } else {
-        uint32_t sr0[32], sr1[32];
-        tmem_ld32(ts, sr0);
-        tmem_ld32(ts + 32, sr1);
-        tmem_wait_ld();
-        float x[64];
-#pragma unroll
-        for (int c = 0; c < 32; ++c) {
-          x[c] = __uint_as_float(sr0[c]);
-          x[c + 32] = __uint_as_float(sr1[c]);
+          for (int x = 0; x < boxes; ++x)
+            if ((missing >> x) & 1u) see &= ~(low_bits(box_rows) << (x << p.box_shift));
         }
-        if (see != ~0ull) {
-#pragma unroll
-          for (int c = 0; c < 64; ++c)
-            if (!((see >> c) & 1ull)) x[c] = -INFINITY;
-        }
-        const float m_tile = row_max64(x) * sl2;
-        // The maximum used to scale P is only raised when it grows by more
-        // than 2^8 (exact: O and l share it).
-        rescale = m_tile > m_run + 8.0f;
-        const float m_use = rescale ? m_tile : m_run;
-        alpha = rescale ? ex2(m_run - m_use) : 1.0f;
-        const float moff = (m_use == -INFINITY) ? 0.0f : m_use;
-        const float rs = exp_tile<T>(x, sl2, moff, pk);
-        l_run = l_run * alpha + rs;
-        m_run = m_use;
-      }
-      // O must not change under a running P.V: rescale only after P.V(j-1).
-      if (j >= 1 && __any_sync(0xffffffffu, rescale)) {
-        ok = mbar_wait_warp(bar(DONE + ((j - 1) & 1)), par((j - 1) & 1, (j - 1) >> 1), abort_flag);
+        // A warp whose rows see no key of this tile stores P = 0 and leaves the
+        // exponential unit to the others.
+        const bool dead = __all_sync(0xffffffffu, see == 0ull);
+        const int sb = j & 1;
+        const uint32_t ts = tl + kTmemS + 64 * sb;
+        // S(j): PRO[j] for j < 2, else in C(j-2)
+        ok = j < 2 ? mbar_wait_warp(bar(PRO + j), j == 0 ? seg_par : two_par, abort_flag)
+                   : mbar_wait_warp(bar(DONE + sb), par(sb, (j >> 1) - 1), abort_flag);
         if (!ok) break;
         tc_fence_after();
+        uint32_t pk[32];
+        bool rescale = false;
+        float alpha = 1.0f;
+        if (dead) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) pk[c] = 0u;
+        } else {
+          uint32_t sr0[32], sr1[32];
+          tmem_ld32(ts, sr0);
+          tmem_ld32(ts + 32, sr1);
+          tmem_wait_ld();
+          float x[64];
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            x[c] = __uint_as_float(sr0[c]);
+            x[c + 32] = __uint_as_float(sr1[c]);
+          }
+          if (see != ~0ull) {
+#pragma unroll
+            for (int c = 0; c < 64; ++c)
+              if (!((see >> c) & 1ull)) x[c] = -INFINITY;
+          }
+          const float m_tile = row_max64(x) * sl2;
+          // The maximum used to scale P is only raised when it grows by more
+          // than 2^8 (exact: O and l share it).
+          rescale = m_tile > m_run + 8.0f;
+          const float m_use = rescale ? m_tile : m_run;
+          alpha = rescale ? ex2(m_run - m_use) : 1.0f;
+          const float moff = (m_use == -INFINITY) ? 0.0f : m_use;
+          const float rs = exp_tile<T>(x, sl2, moff, pk);
+          l_run = l_run * alpha + rs;
+          m_run = m_use;
+        }
+        // O must not change under a running P.V: rescale only after P.V(j-1).
+        if (j >= 1 && __any_sync(0xffffffffu, rescale)) {
+          ok = mbar_wait_warp(bar(DONE + ((j - 1) & 1)), par((j - 1) & 1, (j - 1) >> 1), abort_flag);
+          if (!ok) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int ch = 0; ch < 4; ++ch) {
+            uint32_t ov[32];
+            tmem_ld32(tl + ch * 32, ov);
+            tmem_wait_ld();
+#pragma unroll
+            for (int c = 0; c < 32; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * alpha);
+            tmem_st32(tl + ch * 32, ov);
+          }
+          tmem_wait_st();
+        }
+        tmem_st32(ts, pk);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar(P_FULL + sb));
+      }
+      if (ok && nt >= 1) {
+        ok = mbar_wait(bar(DONE + ((nt - 1) & 1)), par((nt - 1) & 1, (nt - 1) >> 1), abort_flag);
+        ok = __all_sync(0xffffffffu, ok);
+        tc_fence_after();
+      }
+      ok = __all_sync(0xffffffffu, ok);
+      // After a timeout anywhere in the CTA the tile is incomplete: store nothing.
+      if (ok && *abort_flag == 0) {
+        T* orow = static_cast<T*>(p.o) + static_cast<long long>(job.row0 + tok) * p.o_sr + head * p.o_sh;
+        const long long prow = static_cast<long long>(place) * kRows + tid;
+        const float inv = 1.0f / l_run;  // unused where the row saw nothing: it is zero
+        const uint64_t opol = l2_policy_evict_first();
 #pragma unroll 1
         for (int ch = 0; ch < 4; ++ch) {
           uint32_t ov[32];
-          tmem_ld32(tl + ch * 32, ov);
-          tmem_wait_ld();
+          if (nt >= 1) {
+            tmem_ld32(tl + ch * 32, ov);
+            tmem_wait_ld();
+          } else {
 #pragma unroll
-          for (int c = 0; c < 32; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * alpha);
-          tmem_st32(tl + ch * 32, ov);
-        }
-        tmem_wait_st();
-      }
-      tmem_st32(ts, pk);
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(bar(P_FULL + sb));
-    }
-    if (ok && nt >= 1) {
-      ok = mbar_wait(bar(DONE + ((nt - 1) & 1)), par((nt - 1) & 1, (nt - 1) >> 1), abort_flag);
-      ok = __all_sync(0xffffffffu, ok);
-      tc_fence_after();
-    }
-    ok = __all_sync(0xffffffffu, ok);
-    // After a timeout anywhere in the CTA the tile is incomplete: store nothing.
-    if (ok && *abort_flag == 0) {
-      T* orow = static_cast<T*>(p.o) + static_cast<long long>(job.row0 + tok) * p.o_sr + head * p.o_sh;
-      const long long prow = static_cast<long long>(place) * kRows + tid;
-      const float inv = 1.0f / l_run;  // unused where the row saw nothing: it is zero
-      const uint64_t opol = l2_policy_evict_first();
-#pragma unroll 1
-      for (int ch = 0; ch < 4; ++ch) {
-        uint32_t ov[32];
-        if (nt >= 1) {
-          tmem_ld32(tl + ch * 32, ov);
-          tmem_wait_ld();
-        } else {
+            for (int c = 0; c < 32; ++c) ov[c] = 0u;
+          }
+          if (!real) continue;
+          if (part) {
+            uint4* dst = reinterpret_cast<uint4*>(p.part_acc + prow * kD + ch * 32);
 #pragma unroll
-          for (int c = 0; c < 32; ++c) ov[c] = 0u;
-        }
-        if (!real) continue;
-        if (part) {
-          uint4* dst = reinterpret_cast<uint4*>(p.part_acc + prow * kD + ch * 32);
+            for (int q4 = 0; q4 < 8; ++q4)
+              dst[q4] = make_uint4(ov[4 * q4], ov[4 * q4 + 1], ov[4 * q4 + 2], ov[4 * q4 + 3]);
+          } else {
+            uint4* dst = reinterpret_cast<uint4*>(orow + ch * 32);
 #pragma unroll
-          for (int q4 = 0; q4 < 8; ++q4)
-            dst[q4] = make_uint4(ov[4 * q4], ov[4 * q4 + 1], ov[4 * q4 + 2], ov[4 * q4 + 3]);
-        } else {
-          uint4* dst = reinterpret_cast<uint4*>(orow + ch * 32);
+            for (int q4 = 0; q4 < 4; ++q4) {
+              uint32_t w[4];
 #pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) {
-            uint32_t w[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              w[e] = l_run > 0.f ? DT<T>::pack(__uint_as_float(ov[8 * q4 + 2 * e]) * inv,
-                                               __uint_as_float(ov[8 * q4 + 2 * e + 1]) * inv)
-                                 : 0u;
-            st_global_v4_hint(dst + q4, make_uint4(w[0], w[1], w[2], w[3]), opol);
+              for (int e = 0; e < 4; ++e)
+                w[e] = l_run > 0.f ? DT<T>::pack(__uint_as_float(ov[8 * q4 + 2 * e]) * inv,
+                                                 __uint_as_float(ov[8 * q4 + 2 * e + 1]) * inv)
+                                   : 0u;
+              st_global_v4_hint(dst + q4, make_uint4(w[0], w[1], w[2], w[3]), opol);
+            }
           }
         }
+        if (real && part) *reinterpret_cast<float2*>(p.part_ml + prow * 2) = make_float2(m_run, l_run);
       }
-      if (real && part) *reinterpret_cast<float2*>(p.part_ml + prow * 2) = make_float2(m_run, l_run);
     }
+
+    // Each role goes on to the next segment by itself: the producers wait for
+    // MMA_DONE, S(0) and S(1) are made while this segment's O is read out, and
+    // P.V(0) waits for P(0), which the softmax stores after that.
+    if (!kShares || units == 0) break;
+    d0 += (nt + 1) >> 1;
+    d1 += nt >> 1;
+    twos += nt >= 2 ? 1 : 0;
   }
 
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  if (!kShares || units == 0 || *abort_flag != 0) break;
-  d0 += (nt + 1) >> 1;
-  d1 += nt >> 1;
-  twos += nt >= 2 ? 1 : 0;
-  }  // segments
-
   if (warp == 5) tmem_dealloc(tmem, kTmemCols);
 }
 
-// Joins the parts of the pair whose first part ends share blockIdx.x, if there
-// is one, in share order: a warp per row, four columns a lane, eight parts in
-// flight.
+// Joins the parts of pair blockIdx.x, if it has several, in share order: a warp
+// per row, four columns a lane, eight parts in flight.
 template <typename T>
 __global__ void __launch_bounds__(256) paged_combine_kernel(const Params p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int x = blockIdx.x;
   const int lane = threadIdx.x & 31;
   const int row = blockIdx.y * 8 + (threadIdx.x >> 5);
-  const int4 pair = p.joins[2 * x];
+  const int4 pair = p.joins[2 * blockIdx.x];
   const int parts = pair.x;
   if (parts == 0) return;
-  const int4 rows = p.joins[2 * x + 1];
+  const int4 rows = p.joins[2 * blockIdx.x + 1];
   const int tok = row / p.group;
   if (tok >= rows.y) return;
   // The first part is the last segment of its share, the others open theirs.
-  auto slot = [&](int i) -> long long { return static_cast<long long>(i == 0 ? pair.z : 2 * (x + i)) * kRows + row; };
+  auto slot = [&](int i) -> long long {
+    return static_cast<long long>(i == 0 ? pair.z : 2 * (pair.y + i)) * kRows + row;
+  };
   constexpr int kBatch = 8;
   float M = -INFINITY, L = 0.f;
   float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -701,7 +782,7 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const Params p) {
     }
   }
   store_row<T>(static_cast<T*>(p.o) + static_cast<long long>(rows.x + tok) * p.o_sr +
-                   (pair.y * p.group + row - tok * p.group) * p.o_sh,
+                   (static_cast<int>(blockIdx.x) % p.heads_kv * p.group + row - tok * p.group) * p.o_sh,
                lane, A, L);
 }
 
@@ -714,7 +795,9 @@ static inline long long row_slots(int rows, int batch, int tokens) {
 
 // Whether a call runs in shares, as far as the host can tell: few pairs (row
 // tile, KV head) that are long, 32 key tiles or more, counted for a row tile in
-// the middle of its sequence's new rows.
+// the middle of its sequence's new rows. 64 rows on 16000 at 16/16 heads (16
+// pairs) take 37 us a call so and 235 as a CTA each; 1000 rows on none (128
+// pairs of 8 tiles on average) run 21 us as a CTA each and 25 in two parts.
 static bool in_shares(int rows, int batch, int heads_q, int heads_kv, int page_size, int max_pages, int window,
                       int prefix) {
   const int tokens = kRows / (heads_q / heads_kv);
@@ -724,12 +807,12 @@ static bool in_shares(int rows, int batch, int heads_q, int heads_kv, int page_s
     const long long seen = static_cast<long long>(window) + tokens + prefix;
     if (seen < span) span = seen;
   }
-  return batch <= kShareBatch && row_slots(rows, batch, tokens) * heads_kv <= 2 * kDecCtas && span >= 32 * kTile;
+  return batch <= kShareBatch && row_slots(rows, batch, tokens) * heads_kv <= kMaxPairs && span >= 32 * kTile;
 }
 
 // Joins, then the parts of two segments of every share.
 static constexpr size_t kShareWorkspace =
-    kDecCtas * 2 * sizeof(int4) + static_cast<size_t>(2) * kDecCtas * kRows * (kD + 2) * sizeof(float);
+    kMaxPairs * 2 * sizeof(int4) + static_cast<size_t>(2) * kDecCtas * kRows * (kD + 2) * sizeof(float);
 
 // Tensor map of q [rows, Hq, D]: dims (128 d, g heads of a group, rows, KV
 // heads); box = (64 d, g, tokens, 1): one d-half of a row tile, token by token.
@@ -764,7 +847,7 @@ static cudaError_t launch(const CUtensorMap& mq, const CUtensorMap& mk, const CU
   e = launch_dependent(grid, kThreads, smem, s, kernel, mq, mk, mv, p);
   if (e != cudaSuccess || p.ctas == 0) return e;
   const int tile_rows = (p.rows < p.tokens ? p.rows : p.tokens) * p.group;
-  return launch_dependent(dim3(p.ctas, (tile_rows + 7) / 8), 256, 0, s, paged_combine_kernel<T>, p);
+  return launch_dependent(dim3(p.slots * p.heads_kv, (tile_rows + 7) / 8), 256, 0, s, paged_combine_kernel<T>, p);
 }
 
 }  // namespace pre
@@ -818,7 +901,7 @@ int sabre_paged_prefill(const void* q, const void* k_pages, const void* v_pages,
   if (shares && !aligned16(workspace))
     return sabre_fail(SABRE_ERR_ALIGNMENT, "%s: workspace must be 16-byte aligned", fn);
   p.joins = static_cast<int4*>(workspace);
-  p.part_acc = shares ? reinterpret_cast<float*>(p.joins + 2 * kDecCtas) : nullptr;
+  p.part_acc = shares ? reinterpret_cast<float*>(p.joins + 2 * pre::kMaxPairs) : nullptr;
   p.part_ml = shares ? p.part_acc + static_cast<size_t>(2) * kDecCtas * pre::kRows * kD : nullptr;
   const long long slots = pre::row_slots(rows, batch, p.tokens);
   // The rule of prefill_bsa.cu: K/V larger than this -> head-major order.
