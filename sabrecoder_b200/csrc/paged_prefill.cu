@@ -793,11 +793,20 @@ static inline long long row_slots(int rows, int batch, int tokens) {
   return static_cast<long long>(rows - k) / tokens + k;
 }
 
-// Whether a call runs in shares, as far as the host can tell: few pairs (row
-// tile, KV head) that are long, 32 key tiles or more, counted for a row tile in
-// the middle of its sequence's new rows. 64 rows on 16000 at 16/16 heads (16
-// pairs) take 37 us a call so and 235 as a CTA each; 1000 rows on none (128
-// pairs of 8 tiles on average) run 21 us as a CTA each and 25 in two parts.
+// Whether a call runs in shares, as far as the host can tell: by the pairs (row
+// tile, KV head) there may be and the key tiles of one, counted for a row tile
+// in the middle of its sequence's new rows. Where a pair can be cut in k >= 2
+// parts, when that saves it 13 tiles or more: less does not pay for the larger
+// start and the joining. Where it cannot, equal shares fill the places that
+// the last pairs leave empty, which only long pairs are worth. Measured, us a
+// call, a CTA each against shares (pairs x tiles):
+//   64 rows on 1000, 16/16 heads (16 x 16)          19.8 / 16.1
+//   64 rows on 16000, 16/16 heads (16 x 250)         235 / 37
+//   256 rows on 1000, 56/8 heads (120 x 18)         25.4 / 31.4
+//   1000 rows on 1000, 16/16 heads (128 x 23)       35.6 / 36.5
+//   1000 rows on 1000, 56/8 heads (448 x 23)        63.8 / 91.8
+//   512 rows on 15872, 56/8 heads (232 x 252)        304 / 285
+//   16 sequences of 1..200 rows on 100..8000, 16/16  152 / 141
 static bool in_shares(int rows, int batch, int heads_q, int heads_kv, int page_size, int max_pages, int window,
                       int prefix) {
   const int tokens = kRows / (heads_q / heads_kv);
@@ -807,7 +816,10 @@ static bool in_shares(int rows, int batch, int heads_q, int heads_kv, int page_s
     const long long seen = static_cast<long long>(window) + tokens + prefix;
     if (seen < span) span = seen;
   }
-  return batch <= kShareBatch && row_slots(rows, batch, tokens) * heads_kv <= kMaxPairs && span >= 32 * kTile;
+  const long long pairs = row_slots(rows, batch, tokens) * heads_kv, tiles = span / kTile;
+  if (batch > kShareBatch || pairs > kMaxPairs) return false;
+  const long long k = kDecCtas / pairs;
+  return k >= 2 ? tiles - tiles / k >= 13 : tiles >= 96;
 }
 
 // Joins, then the parts of two segments of every share.
