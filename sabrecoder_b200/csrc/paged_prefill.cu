@@ -804,8 +804,10 @@ static inline long long row_slots(int rows, int batch, int tokens) {
 //   64 rows on 16000, 16/16 heads (16 x 250)         235 / 37
 //   256 rows on 1000, 56/8 heads (120 x 18)         25.4 / 31.4
 //   1000 rows on 1000, 16/16 heads (128 x 23)       35.6 / 36.5
-//   1000 rows on 1000, 56/8 heads (448 x 23)        63.8 / 91.8
+//   400 rows on 4000, 56/8 heads (184 x 66)         84.4 / 80.1
 //   512 rows on 15872, 56/8 heads (232 x 252)        304 / 285
+//   4 x 512 rows on 4000, 16/16 heads (304 x 66)    87.2 / 112
+//   1000 rows on 1000, 56/8 heads (448 x 23)        63.8 / 91.8
 //   16 sequences of 1..200 rows on 100..8000, 16/16  152 / 141
 static bool in_shares(int rows, int batch, int heads_q, int heads_kv, int page_size, int max_pages, int window,
                       int prefix) {
@@ -819,7 +821,7 @@ static bool in_shares(int rows, int batch, int heads_q, int heads_kv, int page_s
   const long long pairs = row_slots(rows, batch, tokens) * heads_kv, tiles = span / kTile;
   if (batch > kShareBatch || pairs > kMaxPairs) return false;
   const long long k = kDecCtas / pairs;
-  return k >= 2 ? tiles - tiles / k >= 13 : tiles >= 96;
+  return k >= 2 ? tiles - tiles / k >= 13 : tiles >= (k == 1 ? 48 : 96);
 }
 
 // Joins, then the parts of two segments of every share.
