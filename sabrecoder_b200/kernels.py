@@ -743,7 +743,7 @@ def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                 seq_lens.data_ptr(), q_start.data_ptr(), N, B, Hq, Hkv, D, P, ps, cols, window, prefix,
                 _S2(*q.stride()[:2]), _S3(*k_pages.stride()[:3]), _S3(*v_pages.stride()[:3]), _S2(*out.stride()[:2]),
                 page_table.stride(0), softmax_scale or 0.0, DTYPE_CODE[q.dtype], ws, ws_bytes)
-    LAUNCHES[0] += 1
+    LAUNCHES[0] += 2 if ws else 1  # in parts: and their joining
     return out
 
 

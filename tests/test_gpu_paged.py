@@ -364,3 +364,62 @@ def test_empty_calls(K):
     assert K.paged_prefill(e, kp, vp, none, zero[:0], zero).shape == (0, 2, D)
     K.paged_store(e[:, :1], e[:, :1], kp, vp, none, zero[:0], zero)
     K.copy_pages(kp, [], [])
+
+
+@pytest.mark.parametrize("call", ["decode", "prefill", "shares"])
+def test_waits_that_run_out_end_the_call_and_the_next_one_is_correct(K, call):
+    """Under a wait limit of 1 us the waits for copies and MMAs run out: the call
+    completes, the status word says so, and a call at the default limit is right.
+    (Every wait is bounded; nothing faults or hangs.)"""
+    lens, news = ([9000, 3000], [1, 1]) if call == "decode" else ([2000, 900], [1900, 900])
+    args = make(15, lens, news if call != "shares" else [70, 30], 8, 2, 64, BF)
+    q, kp, vp, table, sl, starts = args
+
+    def run():
+        if call == "decode":
+            return K.paged_decode(q, kp, vp, table, sl)
+        return K.paged_prefill(q, kp, vp, table, sl, starts)
+
+    K.device_status(clear=True)
+    K.set_wait_limit_ns(1000)
+    try:
+        run()
+        torch.cuda.synchronize()
+    finally:
+        K.set_wait_limit_ns(0)
+    assert K.device_status(clear=True) & 1
+    out = run()
+    assert K.device_status(clear=True) == 0
+    check(out, args, starts=None if call == "decode" else starts)
+
+
+def test_two_streams_and_two_captured_graphs_at_once(K):
+    """Calls on two streams, and two captured calls replayed at once, each with the
+    workspace of its own that it allocates."""
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    jobs = [make(16 + i, [3000 + 77 * i, 2900], [60, 5], 4, 2, 64, BF) for i in range(2)]
+    graphs, outs = [], []
+    for (q, kp, vp, table, sl, starts), side in zip(jobs, sides):
+        K.paged_prefill(q, kp, vp, table, sl, starts)
+        K.paged_decode(q[:2], kp, vp, table, sl)
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            outs.append((K.paged_prefill(q, kp, vp, table, sl, starts), K.paged_decode(q[:2], kp, vp, table, sl)))
+        graphs.append(g)
+    for kind in ("streams", "graphs"):
+        got = [None, None]
+        for _ in range(5):
+            for i, side in enumerate(sides):
+                with torch.cuda.stream(side):
+                    if kind == "graphs":
+                        graphs[i].replay()
+                        got[i] = outs[i]
+                    else:
+                        q, kp, vp, table, sl, starts = jobs[i]
+                        got[i] = (K.paged_prefill(q, kp, vp, table, sl, starts), K.paged_decode(q[:2], kp, vp, table, sl))
+        torch.cuda.synchronize()
+        for job, (a, b) in zip(jobs, got):
+            check(a, job, starts=job[5])
+            check(b, (job[0][:2],) + job[1:])
+    assert K.device_status(clear=True) == 0
