@@ -90,6 +90,26 @@ def lib() -> ctypes.CDLL:
     return _lib
 
 
+_paged = None
+
+
+def paged_call():
+    """The compiled calls of the paged entry points (csrc/paged_call.cpp; raises
+    SabreError if they are not built)."""
+    global _paged
+    if _paged is None:
+        lib()
+        try:
+            import torch  # noqa: F401  (its libraries, before the extension that needs them)
+
+            from . import _paged_call
+        except ImportError as e:
+            raise SabreError(f"{os.path.join(_PKG, '_paged_call.so')} is missing or does not load: build it with "
+                             f"`python -m sabrecoder_b200.build` ({e})") from e
+        _paged = _paged_call
+    return _paged
+
+
 def check(status: int, what: str) -> None:
     if status != 0:
         L = lib()

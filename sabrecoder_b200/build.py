@@ -1,4 +1,5 @@
-"""Build libsabre_b200.so in-tree with nvcc for sm_100a.
+"""Build libsabre_b200.so in-tree with nvcc for sm_100a, and with the host compiler
+the extension that calls its paged entry points from torch (_paged_call.so).
 
     python -m sabrecoder_b200.build          # build if sources changed
     python -m sabrecoder_b200.build --force  # always rebuild
@@ -17,6 +18,8 @@ PKG = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(PKG)
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libsabre_b200.so")
+CALL = os.path.join(PKG, "_paged_call.so")
+CALL_SOURCE = os.path.join(CSRC, "paged_call.cpp")
 HEADER = os.path.join(ROOT, "include", "sabre_b200.h")
 
 NVCC_FLAGS = [
@@ -44,17 +47,39 @@ def up_to_date() -> bool:
     return all(os.path.getmtime(s) <= t for s in sources())
 
 
-def build(force: bool = False, verbose: bool = False) -> str:
-    if not force and up_to_date():
-        return LIB
-    tmp = LIB + ".tmp"
-    cmd = [nvcc(), *NVCC_FLAGS, "-o", tmp, os.path.join(CSRC, "sabre_capi.cu")]
+def _run(cmd, tmp: str, out: str, verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd))
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
-        raise RuntimeError(f"nvcc failed ({r.returncode}):\n{r.stdout}\n{r.stderr}")
-    os.replace(tmp, LIB)
+        raise RuntimeError(f"{os.path.basename(cmd[0])} failed ({r.returncode}):\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, out)
+
+
+def build_call(force: bool = False, verbose: bool = False) -> str:
+    """The torch extension; linked to libsabre_b200.so beside it."""
+    if not force and os.path.exists(CALL) and all(os.path.getmtime(f) <= os.path.getmtime(CALL)
+                                                  for f in (CALL_SOURCE, HEADER)):
+        return CALL
+    import sysconfig
+
+    import torch
+    home = os.path.dirname(torch.__file__)
+    inc = [os.path.join(home, "include"), os.path.join(home, "include", "torch", "csrc", "api", "include"),
+           sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")]
+    tmp = CALL + ".tmp"
+    _run([os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
+          f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in inc), CALL_SOURCE,
+          "-o", tmp, f"-L{PKG}", "-l:" + os.path.basename(LIB), f"-L{os.path.join(home, 'lib')}", "-lc10",
+          "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"], tmp, CALL, verbose)
+    return CALL
+
+
+def build(force: bool = False, verbose: bool = False) -> str:
+    if force or not up_to_date():
+        tmp = LIB + ".tmp"
+        _run([nvcc(), *NVCC_FLAGS, "-o", tmp, os.path.join(CSRC, "sabre_capi.cu")], tmp, LIB, verbose)
+    build_call(force, verbose)
     return LIB
 
 

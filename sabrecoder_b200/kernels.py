@@ -9,13 +9,12 @@ allocates. There is no CPU path: non-CUDA tensors raise.
 from __future__ import annotations
 
 import ctypes
-import functools
 import math
 from typing import Optional, Sequence, Tuple
 
 import torch
 
-from ._lib import SabreError, check, i64, lib
+from ._lib import SabreError, check, i64, lib, paged_call
 
 DTYPE_CODE = {torch.bfloat16: 0, torch.float16: 1}
 
@@ -546,49 +545,9 @@ def token_tile_masks(tok_chunk: torch.Tensor, tok_group: torch.Tensor, tok_globa
 # (4) paged K/V cache
 # ---------------------------------------------------------------------------
 
-_S2, _S3 = ctypes.c_int64 * 2, ctypes.c_int64 * 3
-
-
-@functools.lru_cache(maxsize=1024)
-def _paged_workspace(what: str, *sizes: int) -> int:
-    """Workspace bytes of a paged call: a function of these sizes alone."""
-    return int(getattr(lib(), f"sabre_{what}_workspace_size")(*sizes))
-
-
-# The current stream's handle without building a Stream object (3 us of a
-# decode step), where this torch has it.
-_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
-    lambda dev: torch.cuda.current_stream(dev).cuda_stream)
-
-
-def _paged_ok(k_pages, v_pages, page_table, seq_lens, q_start, rows) -> bool:
-    """The conditions of :func:`_paged_refuse` in one pass (a decode step on the
-    device is as short as a few of these lookups). ``rows``: the ``[N, H, D]``
-    tensors of the new rows, some of them None."""
-    dt, dev = k_pages.dtype, k_pages.get_device()
-    ks, ts = k_pages.shape, page_table.shape
-    if dev < 0 or dt not in DTYPE_CODE or v_pages.dtype is not dt or len(ks) != 4 or v_pages.shape != ks or len(ts) != 2:
-        return False
-    B, cols = ts
-    if cols < 1 or (cols > 1 and page_table.stride(1) != 1) or k_pages.stride(3) != 1 or v_pages.stride(3) != 1:
-        return False
-    if (page_table.dtype is not torch.int32 or seq_lens.dtype is not torch.int32 or seq_lens.shape != (B,)
-            or not seq_lens.is_contiguous()):
-        return False
-    if not dev == v_pages.get_device() == page_table.get_device() == seq_lens.get_device():
-        return False
-    if q_start is not None and (q_start.shape != (B + 1,) or q_start.dtype is not torch.int32
-                                or not q_start.is_contiguous() or q_start.get_device() != dev):
-        return False
-    for t in rows:
-        if t is not None and (t.dtype is not dt or t.dim() != 3 or t.shape[2] != ks[3] or t.stride(2) != 1
-                              or t.get_device() != dev):
-            return False
-    return True
-
-
-def _paged_refuse(what: str, k_pages, v_pages, page_table, seq_lens, q_start, rows) -> None:
-    """Raises with what is wrong about the arguments the paged calls share."""
+def _paged_refuse(what: str, k_pages, v_pages, page_table, seq_lens, q_start, rows, workspace=None) -> None:
+    """Raises with what is wrong about the arguments of a paged call (``rows``: its
+    ``[N, H, D]`` tensors)."""
     ts = dict(k_pages=k_pages, v_pages=v_pages, page_table=page_table, seq_lens=seq_lens, q_start=q_start, **rows)
     if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
         raise SabreError(f"{what}: k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} must both be "
@@ -617,19 +576,17 @@ def _paged_refuse(what: str, k_pages, v_pages, page_table, seq_lens, q_start, ro
     for name, t in ts.items():
         if t is not None and t.device != k_pages.device:
             raise SabreError(f"{what}: {name} is on {t.device}, the pages are on {k_pages.device}")
-    raise SabreError(f"{what}: invalid arguments")
-
-
-def _paged_call(what: str, dev: int, fn, *args) -> None:
-    """Calls a C entry point on the current stream of CUDA device `dev`, with
-    that device current."""
-    if torch.cuda.current_device() == dev:
-        st = fn(*args, _raw_stream(dev))
-    else:
-        with torch.cuda.device(dev):
-            st = fn(*args, _raw_stream(dev))
-    if st != 0:
-        check(st, what)
+    first = next(iter(rows.values()))
+    if any(t is not None and t.shape != first.shape for t in rows.values()):
+        raise SabreError(f"{what}: {' and '.join(rows)} must have the same shape")
+    if what == "paged_store" and first.shape[1] != k_pages.shape[1]:
+        raise SabreError(f"{what}: rows of {first.shape[1]} heads, pages of {k_pages.shape[1]}")
+    if q_start is None and first.shape[0] != B:
+        raise SabreError(f"{what}: {first.shape[0]} rows for {B} sequences need q_start")
+    if workspace is not None:
+        raise SabreError(f"{what}: workspace must be contiguous on {k_pages.device} and hold what "
+                         f"sabre_{what}_workspace_size asks for")
+    raise SabreError(f"{what}: a size exceeds 2^31 - 1")
 
 
 def _window_code(what: str, window_size: Optional[int], num_prefix_tokens: int) -> Tuple[int, int]:
@@ -641,19 +598,17 @@ def _window_code(what: str, window_size: Optional[int], num_prefix_tokens: int) 
     return w, min(int(num_prefix_tokens), 2 ** 31 - 1)
 
 
-def _workspace(what: str, workspace: Optional[torch.Tensor], need: int, device):
-    """(pointer, bytes, keep-alive) of the caller's workspace or of a new one."""
-    if workspace is None:
-        if not need:
-            return None, 0, None
-        workspace = torch.empty(need, dtype=torch.uint8, device=device)
-        return workspace.data_ptr(), need, workspace
-    nbytes = workspace.numel() * workspace.element_size()
-    if workspace.device != device or not workspace.is_contiguous():
-        raise SabreError(f"{what}: workspace must be contiguous on {device}")
-    if nbytes < need:
-        raise SabreError(f"{what}: workspace holds {nbytes} < {need} bytes")
-    return workspace.data_ptr(), nbytes, workspace
+def _attend(what: str, q, k_pages, v_pages, page_table, seq_lens, q_start, window_size, num_prefix_tokens,
+            softmax_scale, out, workspace) -> torch.Tensor:
+    window, prefix = _window_code(what, window_size, num_prefix_tokens)
+    res = paged_call().attend(q, k_pages, v_pages, page_table, seq_lens, q_start, window, prefix,
+                              softmax_scale or 0.0, out, workspace)
+    if res is None:
+        _paged_refuse(what, k_pages, v_pages, page_table, seq_lens, q_start, dict(q=q, out=out), workspace)
+    if type(res) is int:
+        check(res, "sabre_" + what)
+    LAUNCHES[0] += 2  # and the joining of parts, where there may be some
+    return res
 
 
 def paged_store(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -666,20 +621,10 @@ def paged_store(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages
     with the new rows; q_start int32 ``[B + 1]``: rows ``q_start[b] ..
     q_start[b+1]-1`` are the last rows of sequence b (default: one row each,
     ``N == B``). Rows from ``q_start[B]`` on are padding."""
-    if not _paged_ok(k_pages, v_pages, page_table, seq_lens, q_start, (k, v)):
+    st = paged_call().store(k, v, k_pages, v_pages, page_table, seq_lens, q_start)
+    if st is None:
         _paged_refuse("paged_store", k_pages, v_pages, page_table, seq_lens, q_start, dict(k=k, v=v))
-    (P, Hkv, ps, D), (B, cols), (N, heads, _) = k_pages.shape, page_table.shape, k.shape
-    if v.shape != k.shape or heads != Hkv:
-        raise SabreError(f"paged_store: k {tuple(k.shape)} and v {tuple(v.shape)} must both be [N, {Hkv}, {D}]")
-    if q_start is None and N != B:
-        raise SabreError(f"paged_store: {N} rows for {B} sequences need q_start")
-    if N == 0 or B == 0:
-        return
-    _paged_call("sabre_paged_store", k.get_device(), lib().sabre_paged_store,
-                k.data_ptr(), v.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(),
-                seq_lens.data_ptr(), _ptr(q_start), N, B, Hkv, D, P, ps, cols, _S2(*k.stride()[:2]),
-                _S2(*v.stride()[:2]), _S3(*k_pages.stride()[:3]), _S3(*v_pages.stride()[:3]), page_table.stride(0),
-                DTYPE_CODE[k.dtype])
+    check(st, "sabre_paged_store")
     LAUNCHES[0] += 1
 
 
@@ -693,25 +638,8 @@ def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, 
     tables as in :func:`paged_store`. With a window the query at position i
     sees key j <= i when ``i - j <= window_size`` or ``j < num_prefix_tokens``.
     A sequence that sees nothing (length 0) gives zeros. Deterministic."""
-    window, prefix = _window_code("paged_decode", window_size, num_prefix_tokens)
-    if not _paged_ok(k_pages, v_pages, page_table, seq_lens, None, (q, out)):
-        _paged_refuse("paged_decode", k_pages, v_pages, page_table, seq_lens, None, dict(q=q, out=out))
-    (P, Hkv, ps, D), (B, cols), Hq = k_pages.shape, page_table.shape, q.shape[1]
-    if q.shape[0] != B or (out is not None and out.shape != q.shape):
-        raise SabreError(f"paged_decode: q {tuple(q.shape)} and out must be [B={B}, Hq, D]")
-    if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    if q.numel() == 0:
-        return out
-    ws, ws_bytes, _keep = _workspace("paged_decode", workspace, _paged_workspace("paged_decode", B, Hq, Hkv, D),
-                                     q.device)
-    _paged_call("sabre_paged_decode", q.get_device(), lib().sabre_paged_decode,
-                q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), page_table.data_ptr(),
-                seq_lens.data_ptr(), B, Hq, Hkv, D, P, ps, cols, window, prefix, _S2(*q.stride()[:2]),
-                _S3(*k_pages.stride()[:3]), _S3(*v_pages.stride()[:3]), _S2(*out.stride()[:2]), page_table.stride(0),
-                softmax_scale or 0.0, DTYPE_CODE[q.dtype], ws, ws_bytes)
-    LAUNCHES[0] += 2
-    return out
+    return _attend("paged_decode", q, k_pages, v_pages, page_table, seq_lens, None, window_size, num_prefix_tokens,
+                   softmax_scale, out, workspace)
 
 
 def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -724,27 +652,10 @@ def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
     q: ``[N, Hq, D]``; rows ``q_start[b] .. q_start[b+1]-1`` are the last
     rows of sequence b, the rest as in :func:`paged_decode`. Rows of ``out``
     from ``q_start[B]`` on are left as they are."""
-    window, prefix = _window_code("paged_prefill", window_size, num_prefix_tokens)
     if q_start is None:
         raise SabreError("paged_prefill needs q_start")
-    if not _paged_ok(k_pages, v_pages, page_table, seq_lens, q_start, (q, out)):
-        _paged_refuse("paged_prefill", k_pages, v_pages, page_table, seq_lens, q_start, dict(q=q, out=out))
-    (P, Hkv, ps, D), (B, cols), (N, Hq, _) = k_pages.shape, page_table.shape, q.shape
-    if out is not None and out.shape != q.shape:
-        raise SabreError(f"paged_prefill: out {tuple(out.shape)} must have q's shape {tuple(q.shape)}")
-    if out is None:
-        out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    if q.numel() == 0 or B == 0:
-        return out
-    ws, ws_bytes, _keep = _workspace("paged_prefill", workspace, _paged_workspace(
-        "paged_prefill", N, B, Hq, Hkv, D, ps, cols, window, prefix), q.device)
-    _paged_call("sabre_paged_prefill", q.get_device(), lib().sabre_paged_prefill,
-                q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), out.data_ptr(), page_table.data_ptr(),
-                seq_lens.data_ptr(), q_start.data_ptr(), N, B, Hq, Hkv, D, P, ps, cols, window, prefix,
-                _S2(*q.stride()[:2]), _S3(*k_pages.stride()[:3]), _S3(*v_pages.stride()[:3]), _S2(*out.stride()[:2]),
-                page_table.stride(0), softmax_scale or 0.0, DTYPE_CODE[q.dtype], ws, ws_bytes)
-    LAUNCHES[0] += 2 if ws else 1  # in parts: and their joining
-    return out
+    return _attend("paged_prefill", q, k_pages, v_pages, page_table, seq_lens, q_start, window_size,
+                   num_prefix_tokens, softmax_scale, out, workspace)
 
 
 def copy_pages(pages: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -> None:
@@ -756,42 +667,21 @@ def copy_pages(pages: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -> N
     synchronises nor copies to the device and can be captured. Pages are
     copied in no order: a page outside the pool, written twice, or both read
     and written raises and nothing is copied."""
-    moves = []
     for name, t in (("src", src), ("dst", dst)):
-        if isinstance(t, torch.Tensor):
-            if t.is_cuda or t.dim() != 1 or t.is_floating_point():
-                raise SabreError(f"copy_pages: {name} must be a list of ints or a 1-D CPU integer tensor")
-            t = t.tolist()
-        moves.append(t)
-    src, dst = moves
-    n = len(src)
-    if n != len(dst):
-        raise SabreError(f"copy_pages: {n} sources for {len(dst)} destinations")
-    if pages.dim() < 4:
-        raise SabreError(f"copy_pages: pages {tuple(pages.shape)} must be [..., num_pages, Hkv, page_size, D]")
-    shape, strides = pages.shape, pages.stride()
-    P = shape[-4]
-    for page in (*src, *dst):
-        if not 0 <= page < P:
-            raise SabreError(f"copy_pages: page {page} is outside the pool of {P} pages")
-    _need_cuda(pages=pages)
-    if pages.numel() == 0 or n == 0:
-        return
-    unit = 1
-    for size, stride in zip(shape[:-4:-1], strides[:-4:-1]):
-        if size > 1 and stride != unit:
-            raise SabreError("copy_pages: each page [Hkv, page_size, D] must be contiguous")
-        unit *= size
-    # The leading dimensions, flattened: buffers at one stride.
-    buffers, step = 1, 0
-    for size, stride in zip(shape[-5::-1], strides[-5::-1]):
-        if size > 1 and buffers > 1 and stride != buffers * step:
-            raise SabreError(f"copy_pages: the pools {tuple(shape[:-4])} are not at one stride")
-        if size > 1 and buffers == 1:
-            step = stride
-        buffers *= size
-    es = pages.element_size()
-    ids = ctypes.c_int32 * n
-    _paged_call("sabre_copy_pages", pages.get_device(), lib().sabre_copy_pages, pages.data_ptr(), buffers, step * es,
-                P, strides[-4] * es, unit * es, ids(*src), ids(*dst), n)
-    LAUNCHES[0] += -(-n // 480)
+        if isinstance(t, torch.Tensor) and (t.is_cuda or t.dim() != 1 or t.is_floating_point()):
+            raise SabreError(f"copy_pages: {name} must be a list of ints or a 1-D CPU integer tensor")
+    src = src.tolist() if isinstance(src, torch.Tensor) else list(src)
+    dst = dst.tolist() if isinstance(dst, torch.Tensor) else list(dst)
+    st = paged_call().copy(pages, src, dst)
+    if st is None:
+        if len(src) != len(dst):
+            raise SabreError(f"copy_pages: {len(src)} sources for {len(dst)} destinations")
+        if pages.dim() < 4:
+            raise SabreError(f"copy_pages: pages {tuple(pages.shape)} must be [..., num_pages, Hkv, page_size, D]")
+        for page in (*src, *dst):
+            if not 0 <= page < pages.shape[-4]:
+                raise SabreError(f"copy_pages: page {page} is outside the pool of {pages.shape[-4]} pages")
+        _need_cuda(pages=pages)
+        raise SabreError("copy_pages: each page [Hkv, page_size, D] must be contiguous, and the pools at one stride")
+    check(st, "sabre_copy_pages")
+    LAUNCHES[0] += -(-len(src) // 480)
