@@ -396,11 +396,11 @@ int sabre_prefill_bsa_tokenmask(const void* q, const void* k, const void* v, voi
  * j < seq_lens[b], page j is present and (window < 0, or i - j <= window, or
  * j < num_prefix_tokens). A query that sees nothing gives zeros. Rows that
  * the sequence does not have, or whose page is absent, never reach a result,
- * whatever they hold; nor, in decode, do rows outside the window. The rows it
- * has are taken to be finite in prefill: a NaN or an infinity in a V row
- * reaches every row of the call that shares its 64-key tile. heads_q /
- * heads_kv must be an integer <= 8; query head h reads KV head h / (Hq / Hkv).
- * softmax_scale <= 0 selects 1/sqrt(head_dim).
+ * whatever they hold; nor do rows that no query of the call sees (outside the
+ * window). In prefill a NaN or an infinity in a V row that some query sees may
+ * reach the other queries of its 128-row tile, those before it included.
+ * heads_q / heads_kv must be an integer <= 8; query head h reads KV head
+ * h / (Hq / Hkv). softmax_scale <= 0 selects 1/sqrt(head_dim).
  *
  * sabre_paged_store: new rows k, v [rows, Hkv, D] (strides {row, head}) into
  *   their pages. q_start NULL: one row per sequence (rows == batch). A row

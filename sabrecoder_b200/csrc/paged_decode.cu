@@ -14,18 +14,19 @@
 // share is finished there, the others leave (m, l, acc) per head and
 // paged_join_kernel adds them in share order: results do not depend on timing.
 //
-// A CTA: warp 4 fetches K and V tiles by TMA into a three-stage ring (one box
-// of 16 rows at a time; absent pages and boxes that nobody sees are not
-// fetched) and runs ahead over segment ends; warps 0..3 each take 16
-// of a tile's 64 keys on the tensor cores with their own softmax state, so
-// the tile loop has no barrier but the ring's:
+// A CTA: warp 4 fetches K and V tiles by TMA into a three-stage ring (boxes of
+// 16 rows; absent pages and boxes that nobody sees are not fetched) and runs
+// ahead over segment ends; warps 0..3 each take 16 of a tile's 64 keys on the
+// tensor cores with their own softmax state, so the tile loop has no barrier
+// but the ring's:
 //   S^T = K Q^T   (16 keys x 8 heads, K by ldmatrix, Q kept in registers)
 //   O^T += V^T P^T (128 d x 8 heads, V by transposed ldmatrix; P^T is S^T's
 //                   layout after one movmatrix per 8 keys)
 // Eight heads fill the instruction's N: groups of up to eight cost the same.
-// mma.sync is used rather than tcgen05: the work is a sixteenth of what the
-// HBM rate needs of it, and there is no tensor memory to allocate, fill and
-// read back per segment.
+// mma.sync is used rather than tcgen05: at the HBM rate the matrix work keeps
+// the tensor pipe busy a tenth of the time (ncu), and there is no tensor memory
+// to allocate, fill and read back per segment. 32 sequences of 1..16384 rows at
+// 56/8 heads (917 MB) take 143 us, 6.4 TB/s.
 // P is rounded to the type of V for the product (half a step of a weight,
 // below the rounding of the output); scores, sums and acc are fp32.
 namespace sabre {

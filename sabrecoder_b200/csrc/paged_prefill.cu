@@ -25,9 +25,9 @@
 // of a share to the next each role goes on by itself (model-checked:
 // tests/test_paged_prefill_protocol.py). Different here: tiles come box by box from pages (a TMA
 // box is min(page_size, 64) rows; absent pages and boxes that no row sees are
-// read outside the pool and give zeros), and rows past the sequence's end
-// inside a page are zeroed in V before its tile is handed to the MMA, since
-// 0 * NaN would reach the result.
+// read outside the pool and give zeros), and V rows that none of the CTA's rows
+// sees (past the sequence's end, before the window) are zeroed in shared memory
+// before their tile is handed to the MMA, since 0 * NaN would reach the result.
 // P is rounded to the type of V for the product; scores, sums and O are fp32.
 namespace sabre {
 namespace paged {
@@ -53,7 +53,7 @@ enum Bar {
   PRO = 5,     // [2] S(0), S(1) done
   DONE = 7,    // [2] commit C(j) on DONE[j%2]: P.V(j) and S(j+2) done
   P_FULL = 9,  // [2] P(j) stored over S buffer j%2 (one arrival per softmax warp)
-  V_RAW = 11,  // the copies of the tile that ends inside a page, before its rows are zeroed
+  V_RAW = 11,  // the copies of a V tile some of whose rows are zeroed before V_FULL
   MMA_DONE = 12,
   NUM_BARS = 13
 };
@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(kThreads, 2)
         tma_load_4d_hint(sbase + kQOff + kQBytes / 2, &tmQ, bar(Q_FULL), 64, 0, job.row0, hk, pol);
       }
       int issued = 0;    // tiles
-      bool raw = false;  // the last one went through V_RAW
+      bool raw = false;  // the last tile went through V_RAW
       const bool began = ok;
       for (int i0 = 0; ok && i0 < nt * boxes; i0 += 32) {
         // The pages of the next 32 boxes, one per lane; num_pages reads zeros.
@@ -476,9 +476,18 @@ __global__ void __launch_bounds__(kThreads, 2)
               ok = mbar_wait_warp(bar(DONE + s), par(s, (j >> 1) - (is_k ? 2 : 1)), abort_flag);
             if (!ok) break;
           }
-          // Rows of V at and past the sequence's end inside a box are zeroed.
-          const int over = job.n - job.pos(j0 + j);
-          const bool clean = !is_k && over < kTile && (over & (box_rows - 1)) != 0;
+          // Rows of V that none of this CTA's rows sees (past the end, before the
+          // window) but that share a box with some that one does are zeroed.
+          unsigned long long hidden = 0;
+          if (!is_k) {
+            const int t = job.pos(j0 + j);
+            hidden = ~low_bits(job.n - t) | (low_bits(job.lo - t) & ~low_bits(p.w.prefix - t));
+            for (int x = 0; x < boxes && hidden != 0ull; ++x) {  // a box that is hidden as a whole is zero already
+              const unsigned long long box = low_bits(box_rows) << (x << p.box_shift);
+              if ((hidden & box) == box) hidden &= ~box;
+            }
+          }
+          const bool clean = hidden != 0ull;
           const uint32_t full = bar(clean ? V_RAW : full0 + s);
           if (lane == 0) mbar_arrive_expect_tx(full, kTileBytes);
           __syncwarp();
@@ -490,26 +499,23 @@ __global__ void __launch_bounds__(kThreads, 2)
               tma_load_page(dst + h * (kTileBytes / 2) + x * box_rows * 128, map, full, off, h, hk, page);
           }
           issued = j + 1;
+          raw = clean;
           if (clean) {
-            raw = true;
             const int raw_par = raws++ & 1;
             ok = mbar_wait_warp(bar(V_RAW), raw_par, abort_flag);
             if (!ok) break;
             (void)mbar_test_wait(bar(V_RAW), raw_par);  // each lane's own acquire of the copied bytes
-            const int end = (over + box_rows) & ~(box_rows - 1);
-            for (int c = lane; c < (end - over) * 16; c += 32) {
-              const int row = over + (c >> 4);
-              *reinterpret_cast<uint4*>(smem + kVOff + s * kTileBytes + ((c >> 3) & 1) * (kTileBytes / 2) + row * 128 +
-                                        (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-            }
+            // Half a warp zeroes the even rows, half the odd ones, 16 bytes a lane.
+            uint8_t* const at16 = smem + kVOff + s * kTileBytes + ((lane >> 3) & 1) * (kTileBytes / 2) + (lane & 7) * 16;
+            for (unsigned long long m = hidden & (0x5555555555555555ull << (lane >> 4)); m != 0ull; m &= m - 1ull)
+              *reinterpret_cast<uint4*>(at16 + (__ffsll(m) - 1) * 128) = make_uint4(0u, 0u, 0u, 0u);
             fence_proxy_async_smem();
             __syncwarp();
             if (lane == 0) mbar_arrive(bar(full0 + s));
           }
         }
       }
-      // Every issued copy must land before the CTA may exit. (The tile that ends
-      // the sequence is the last one: only it can have gone through V_RAW.)
+      // Every issued copy must land before the CTA may exit.
       if (lane == 0 && began) {
         if (is_k) mbar_wait_drain(bar(Q_FULL), seg_par);
         for (int j = max(0, issued - 2); j < issued; ++j) {

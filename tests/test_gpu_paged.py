@@ -184,6 +184,30 @@ def test_absent_pages_inside_a_tile(K, ps, extra_cols):
     assert K.device_status(clear=True) == 0
 
 
+@pytest.mark.parametrize("ps,window,prefix", [(16, 100, 33), (64, 129, 0), (128, 700, 70), (32, 0, 1), (64, 127, 64)])
+@pytest.mark.parametrize("extra_cols", [1, 200])
+def test_rows_no_query_sees_may_hold_anything(K, ps, window, prefix, extra_cols):
+    """NaN and infinities in rows of present pages that lie before every query's
+    window and behind the prefix."""
+    lens, news = [1500, 2100, 901], [300, 1, 130]
+    args = make(18, lens, news, 6, 2, ps, BF, window, prefix, drop=False, extra_cols=extra_cols)
+    q, kp, vp, table, sl, starts = args
+    for b, (n, new) in enumerate(zip(lens, news)):
+        for j in range(prefix, n - new - window):
+            bad = float("nan") if j % 3 else float("inf")
+            kp[table[b, j // ps], :, j % ps] = bad
+            vp[table[b, j // ps], :, j % ps] = bad
+    clean = (q, torch.nan_to_num(kp, 0.0, 0.0), torch.nan_to_num(vp, 0.0, 0.0), table, sl, starts)
+    kw = dict(window_size=window, num_prefix_tokens=prefix)
+    check(K.paged_prefill(q, kp, vp, table, sl, starts, **kw), clean, window, prefix, starts=starts)
+    for b, (n, new) in enumerate(zip(lens, news)):  # and what the last row alone does not see
+        for j in range(max(prefix, n - new - window), n - 1 - window):
+            kp[table[b, j // ps], :, j % ps] = vp[table[b, j // ps], :, j % ps] = float("nan")
+    last = (q[starts[1:].long() - 1],) + clean[1:]
+    check(K.paged_decode(last[0], kp, vp, table, sl, **kw), last, window, prefix)
+    assert K.device_status(clear=True) == 0
+
+
 def test_pages_outside_the_pool_are_absent_and_recorded(K):
     args = make(7, [200, 300], [1, 1], 4, 2, 32, BF)
     q, kp, vp, table, sl, _ = args
