@@ -79,6 +79,9 @@ __global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(const StoreP
   const int r0 = blockIdx.x * p.cta_rows;
   const int tid = threadIdx.x;
   const int lane = tid & 31;
+  // The next kernel (a decode over these pages, say) may start its set-up now;
+  // it waits for this grid before touching memory.
+  if (tid == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");  // a programmatic dependent launch: inputs are ready from here on
   for (int r = tid >> 5; r < p.cta_rows; r += kStoreThreads / 32) {
     const int row = r0 + r;
