@@ -586,6 +586,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int pos = job.pos0 + tok;
       const int seen = real ? min(pos + 1, job.n) : 0;  // keys [0, seen), less the window's gap
       const int wlo = p.w.first(pos);
+      // Every row of the warp, if it has any, sees the keys [all_wlo, all_seen).
+      const int all_seen = __any_sync(0xffffffffu, real) ? __reduce_min_sync(0xffffffffu, real ? seen : INT_MAX) : 0;
+      const int all_wlo = __reduce_max_sync(0xffffffffu, wlo);
       const uint32_t tl = tmem + (static_cast<uint32_t>(warp * 32) << 16);
       const float sl2 = p.scale_log2;
       float m_run = -INFINITY;
@@ -606,21 +609,31 @@ __global__ void __launch_bounds__(kThreads, 2)
           absent = __ballot_sync(0xffffffffu, p.c.checked(entry_ahead) < 0);
           entry_ahead = lookup(i + 32 + lane);
         }
-        unsigned long long see = low_bits(seen - t) & (~low_bits(wlo - t) | low_bits(p.w.prefix - t));
         const uint32_t missing = (absent >> (i & 31)) & ((1u << boxes) - 1u);
-        if (missing != 0u) {
+        // Which keys the row sees; most tiles are seen whole by the whole warp (the
+        // masks left out there: 592 -> 574 us for the prompt below).
+        unsigned long long see = ~0ull;
+        bool dead = false;
+        if (t + kTile > all_seen || (t < all_wlo && t + kTile > p.w.prefix) || missing != 0u) {
+          see = low_bits(seen - t) & (~low_bits(wlo - t) | low_bits(p.w.prefix - t));
+          if (missing != 0u) {
 #pragma unroll 1
-          for (int x = 0; x < boxes; ++x)
-            if ((missing >> x) & 1u) see &= ~(low_bits(box_rows) << (x << p.box_shift));
+            for (int x = 0; x < boxes; ++x)
+              if ((missing >> x) & 1u) see &= ~(low_bits(box_rows) << (x << p.box_shift));
+          }
+          // A warp whose rows see no key of this tile stores P = 0 and leaves the
+          // exponential unit to the others.
+          dead = __all_sync(0xffffffffu, see == 0ull);
         }
-        // A warp whose rows see no key of this tile stores P = 0 and leaves the
-        // exponential unit to the others.
-        const bool dead = __all_sync(0xffffffffu, see == 0ull);
         const int sb = j & 1;
         const uint32_t ts = tl + kTmemS + 64 * sb;
         // S(j): PRO[j] for j < 2, else in C(j-2)
-        ok = j < 2 ? mbar_wait_warp(bar(PRO + j), j == 0 ? seg_par : two_par, abort_flag)
-                   : mbar_wait_warp(bar(DONE + sb), par(sb, (j >> 1) - 1), abort_flag);
+        const uint32_t s_bar = bar(j < 2 ? PRO + j : DONE + sb);
+        const uint32_t s_par = j < 2 ? (j == 0 ? seg_par : two_par) : par(sb, (j >> 1) - 1);
+        // Mostly there already: every lane looks, which spares the hand-over from
+        // lane 0 (a 12288-row prompt at 16/16 heads: 574 -> 560 us; looking on
+        // instead of waiting takes issue slots from the other warps, 567).
+        if (!__all_sync(0xffffffffu, mbar_test_wait(s_bar, s_par))) ok = mbar_wait_warp(s_bar, s_par, abort_flag);
         if (!ok) break;
         tc_fence_after();
         uint32_t pk[32];
