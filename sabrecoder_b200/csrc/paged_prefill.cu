@@ -33,7 +33,6 @@ namespace sabre {
 namespace paged {
 namespace pre {
 
-using prefill::exp_tile;
 using prefill::row_max64;
 
 constexpr int kThreads = 224;
@@ -82,6 +81,37 @@ struct Params {
   int head_major, ctas;               // ctas: of a call in shares, else 0
   float scale_log2;
 };
+
+// P = 2^(x * sl2 - moff) for one row of 64 scores (-inf gives 0), rounded to the
+// storage type and stored at column `col` of tensor memory, half a row at a time
+// so that the first half's store runs under the exponentials of the second;
+// returns the sum of the fp32 values.
+template <typename T>
+__device__ __forceinline__ float exp_store(const float (&x)[64], float sl2, float moff, uint32_t col) {
+  const uint64_t sc = f2_pack(sl2, sl2);
+  const uint64_t off = f2_pack(-moff, -moff);
+  uint64_t acc[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) acc[i] = f2_pack(0.f, 0.f);
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    uint32_t pk[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+      float y0, y1;
+      f2_unpack(f2_fma(f2_pack(x[32 * half + 2 * i], x[32 * half + 2 * i + 1]), sc, off), y0, y1);
+      const float p0 = ex2(y0);
+      const float p1 = ex2(y1);
+      acc[i & 3] = f2_add(acc[i & 3], f2_pack(p0, p1));
+      pk[i] = DT<T>::pack(p0, p1);
+    }
+    tmem_st16(col + 16 * half, pk);
+  }
+  float s[8];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) f2_unpack(acc[i], s[2 * i], s[2 * i + 1]);
+  return ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+}
 
 // Bits [0, x) of a 64-bit mask, x clamped to [0, 64].
 __device__ __forceinline__ unsigned long long low_bits(int x) {
@@ -532,10 +562,12 @@ __global__ void __launch_bounds__(kThreads, 2)
         const uint64_t kd0 = smem_desc_sw128(sbase + kKOff, 16, 1024);
         const uint64_t vd0 = smem_desc_sw128(sbase + kVOff, kTileBytes / 2, 1024);
         const uint32_t s_tmem = tmem + kTmemS;
-        bool ok = mbar_wait(bar(Q_FULL), seg_par, abort_flag);
+        const unsigned long long lim = wait_limit_ns();
+        auto wait = [&](int i, uint32_t parity) -> bool { return mbar_wait_lim<8>(bar(i), parity, abort_flag, lim); };
+        bool ok = wait(Q_FULL, seg_par);
         auto issue_s = [&](int j) -> bool {
           const int ks = j & 1;
-          if (!mbar_wait(bar(K_FULL + ks), par(ks, j >> 1), abort_flag)) return false;
+          if (!wait(K_FULL + ks, par(ks, j >> 1))) return false;
           tc_fence_after();
           const uint64_t kd = kd0 + static_cast<uint64_t>(ks * (kTileBytes >> 4));
           const uint32_t dst = s_tmem + 64 * ks;
@@ -549,8 +581,8 @@ __global__ void __launch_bounds__(kThreads, 2)
         };
         auto issue_pv = [&](int i) -> bool {
           const int pb = i & 1;
-          if (!mbar_wait(bar(P_FULL + pb), par(pb, i >> 1), abort_flag)) return false;
-          if (!mbar_wait(bar(V_FULL + pb), par(pb, i >> 1), abort_flag)) return false;
+          if (!wait(V_FULL + pb, par(pb, i >> 1))) return false;
+          if (!wait(P_FULL + pb, par(pb, i >> 1))) return false;
           tc_fence_after();
           const uint64_t vd = vd0 + static_cast<uint64_t>(pb * (kTileBytes >> 4));
           const uint32_t pa = s_tmem + 64 * pb;
@@ -636,12 +668,13 @@ __global__ void __launch_bounds__(kThreads, 2)
         if (!__all_sync(0xffffffffu, mbar_test_wait(s_bar, s_par))) ok = mbar_wait_warp(s_bar, s_par, abort_flag);
         if (!ok) break;
         tc_fence_after();
-        uint32_t pk[32];
         bool rescale = false;
         float alpha = 1.0f;
         if (dead) {
+          uint32_t zero[32];
 #pragma unroll
-          for (int c = 0; c < 32; ++c) pk[c] = 0u;
+          for (int c = 0; c < 32; ++c) zero[c] = 0u;
+          tmem_st32(ts, zero);
         } else {
           uint32_t sr0[32], sr1[32];
           tmem_ld32(ts, sr0);
@@ -665,8 +698,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           const float m_use = rescale ? m_tile : m_run;
           alpha = rescale ? ex2(m_run - m_use) : 1.0f;
           const float moff = (m_use == -INFINITY) ? 0.0f : m_use;
-          const float rs = exp_tile<T>(x, sl2, moff, pk);
-          l_run = l_run * alpha + rs;
+          l_run = l_run * alpha + exp_store<T>(x, sl2, moff, ts);
           m_run = m_use;
         }
         // O must not change under a running P.V: rescale only after P.V(j-1).
@@ -685,7 +717,6 @@ __global__ void __launch_bounds__(kThreads, 2)
           }
           tmem_wait_st();
         }
-        tmem_st32(ts, pk);
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
