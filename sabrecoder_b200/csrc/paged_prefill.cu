@@ -727,13 +727,47 @@ __global__ void __launch_bounds__(kThreads, 2)
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();
       }
-      ok = __all_sync(0xffffffffu, ok);
       // After a timeout anywhere in the CTA the tile is incomplete: store nothing.
-      if (ok && *abort_flag == 0) {
+      ok = __all_sync(0xffffffffu, ok && *abort_flag == 0);
+      if (ok) {
         T* orow = static_cast<T*>(p.o) + static_cast<long long>(job.row0 + tok) * p.o_sr + head * p.o_sh;
         const long long prow = static_cast<long long>(place) * kRows + tid;
         const float inv = 1.0f / l_run;  // unused where the row saw nothing: it is zero
         const uint64_t opol = l2_policy_evict_first();
+        auto quad = [&](const uint32_t (&ov)[32], int q4) -> uint4 {  // 8 columns of the result
+          uint32_t w[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            w[e] = l_run > 0.f ? DT<T>::pack(__uint_as_float(ov[8 * q4 + 2 * e]) * inv,
+                                             __uint_as_float(ov[8 * q4 + 2 * e + 1]) * inv)
+                               : 0u;
+          return make_uint4(w[0], w[1], w[2], w[3]);
+        };
+        if (!kShares && nt >= 1) {
+          // Every S is done, so the Q tile is free: the warp turns its rows in
+          // their place and writes two whole rows at a time.
+          uint8_t* const turn = smem + kQOff + warp * (32 * kD * 2);
+#pragma unroll 1
+          for (int ch = 0; ch < 4; ++ch) {
+            uint32_t ov[32];
+            tmem_ld32(tl + ch * 32, ov);
+            tmem_wait_ld();
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4)
+              *reinterpret_cast<uint4*>(turn + lane * 256 + (((ch * 4 + q4) ^ (lane & 7)) << 4)) = quad(ov, q4);
+          }
+          __syncwarp();
+          const uint32_t rows = __ballot_sync(0xffffffffu, real);
+          const unsigned long long mine = reinterpret_cast<unsigned long long>(orow);
+#pragma unroll 4
+          for (int i = 0; i < 32; i += 2) {
+            const int r = i + (lane >> 4);
+            uint4* const dst = reinterpret_cast<uint4*>(__shfl_sync(0xffffffffu, mine, r)) + (lane & 15);
+            const uint4 v = *reinterpret_cast<const uint4*>(turn + r * 256 + (((lane & 15) ^ (r & 7)) << 4));
+            if ((rows >> r) & 1u) st_global_v4_hint(dst, v, opol);
+          }
+          break;
+        }
 #pragma unroll 1
         for (int ch = 0; ch < 4; ++ch) {
           uint32_t ov[32];
@@ -753,15 +787,7 @@ __global__ void __launch_bounds__(kThreads, 2)
           } else {
             uint4* dst = reinterpret_cast<uint4*>(orow + ch * 32);
 #pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4) {
-              uint32_t w[4];
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                w[e] = l_run > 0.f ? DT<T>::pack(__uint_as_float(ov[8 * q4 + 2 * e]) * inv,
-                                                 __uint_as_float(ov[8 * q4 + 2 * e + 1]) * inv)
-                                   : 0u;
-              st_global_v4_hint(dst + q4, make_uint4(w[0], w[1], w[2], w[3]), opol);
-            }
+            for (int q4 = 0; q4 < 4; ++q4) st_global_v4_hint(dst + q4, quad(ov, q4), opol);
           }
         }
         if (real && part) *reinterpret_cast<float2*>(p.part_ml + prow * 2) = make_float2(m_run, l_run);
