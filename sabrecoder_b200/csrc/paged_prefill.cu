@@ -216,9 +216,9 @@ struct RowPlace {
 // than kSlack key tiles above the mean. Else the tiles of all pairs, in order,
 // are cut into equal shares: a CTA may then finish one pair and begin another,
 // which costs it a second start and read-out, about kSlack tiles' time (300
-// rows on 4000 at 16/16 heads, 48 pairs of 66 tiles: 31 us a call in parts, 38
-// in shares; 512 rows on 15872 at 56/8 heads, 232 pairs of 250 tiles: 304 us
-// uncut, 285 in shares; 8 sequences of 32 rows on 2000 to 4000: 72 and 55).
+// rows on 4000 at 16/16 heads, 48 pairs of 66 tiles: 30 us a call in parts, 35
+// in shares; 256 rows on 1000 at 56/8 heads, 120 pairs of 18: 31 and 38; 8
+// sequences of 32 rows on 2000 to 4000, ragged, in shares: 52).
 constexpr int kSlack = 6;
 struct RowShares : Shares {
   bool whole;
@@ -873,17 +873,22 @@ static inline long long row_slots(int rows, int batch, int tokens) {
 // tile, KV head) there may be and the key tiles of one, counted for a row tile
 // in the middle of its sequence's new rows. Where a pair can be cut in k >= 2
 // parts, when that saves it 13 tiles or more: less does not pay for the larger
-// start and the joining. Where it cannot, equal shares fill the places that
-// the last pairs leave empty, which only long pairs are worth. Measured, us a
-// call, a CTA each against shares (pairs x tiles):
-//   64 rows on 1000, 16/16 heads (16 x 16)          19.8 / 16.1
-//   64 rows on 16000, 16/16 heads (16 x 250)         235 / 37
-//   256 rows on 1000, 56/8 heads (120 x 18)         25.4 / 31.4
-//   1000 rows on 1000, 16/16 heads (128 x 23)       35.6 / 36.5
-//   400 rows on 4000, 56/8 heads (184 x 66)         84.4 / 80.1
-//   512 rows on 15872, 56/8 heads (232 x 252)        304 / 285
-//   4 x 512 rows on 4000, 16/16 heads (304 x 66)    87.2 / 112
-//   1000 rows on 1000, 56/8 heads (448 x 23)        63.8 / 91.8
+// start and the joining. Else equal shares fill the places that the last pairs
+// leave empty (counted for the pairs there are when row tiles end anywhere),
+// which pays when those are many and the pairs long: a CTA alone on its SM is
+// faster than one of two. Measured, us a call, a CTA each against shares (pairs
+// x tiles):
+//   64 rows on 1000, 16/16 heads (16 x 16)          18.6 / 16.1
+//   64 rows on 16000, 16/16 heads (16 x 250)         240 / 36
+//   256 rows on 1000, 56/8 heads (120 x 18)         22.3 / 31.4
+//   1000 rows on 1000, 16/16 heads (128 x 23)       31.0 / 35.5
+//   400 rows on 4000, 56/8 heads (184 x 66)         72.1 / 78.5
+//   400 rows on 8000, 56/8 heads (184 x 129)         133 / 118
+//   512 rows on 12000, 56/8 heads (232 x 192)        195 / 203
+//   512 rows on 15872, 56/8 heads (232 x 252)        257 / 251
+//   2300 rows on 8000, 16/16 heads (288 x 143)       174 / 220
+//   1280 rows on 6000, 32/32 heads (320 x 104)       198 / 190
+//   1500 rows on 12000, 32/32 heads (384 x 199)      370 / 410
 //   16 sequences of 1..200 rows on 100..8000, 16/16  152 / 141
 static bool in_shares(int rows, int batch, int heads_q, int heads_kv, int page_size, int max_pages, int window,
                       int prefix) {
@@ -897,7 +902,10 @@ static bool in_shares(int rows, int batch, int heads_q, int heads_kv, int page_s
   const long long pairs = row_slots(rows, batch, tokens) * heads_kv, tiles = span / kTile;
   if (batch > kShareBatch || pairs > kMaxPairs) return false;
   const long long k = kDecCtas / pairs;
-  return k >= 2 ? tiles - tiles / k >= 13 : tiles >= (k == 1 ? 48 : 96);
+  if (k >= 2) return tiles - tiles / k >= 13;
+  const long long likely = (2ll * rows + static_cast<long long>(batch) * tokens) * heads_kv / (2 * tokens);
+  if (likely <= kDecCtas) return tiles * (kDecCtas - likely) >= 48 * kDecCtas;
+  return tiles >= 96 && 2 * kDecCtas - likely >= 250;
 }
 
 // Joins, then the parts of two segments of every share.
