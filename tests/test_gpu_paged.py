@@ -149,6 +149,23 @@ def test_paged_prefill_vs_oracle(K, case):
     assert K.device_status(clear=True) == 0
 
 
+@pytest.mark.parametrize("lens,news,Hq,Hkv,ps,window,prefix", [
+    ([8400], [400], 56, 8, 64, None, 0),              # equal shares that cut pairs anywhere
+    ([900, 1300, 77], [900, 211, 77], 7, 1, 32, None, 0),
+    ([900, 1300, 77], [900, 211, 77], 16, 2, 64, 300, 40),
+])
+def test_results_into_any_layout(K, lens, news, Hq, Hkv, ps, window, prefix):
+    """Outputs with heads outermost and rows apart; what lies between stays."""
+    args = make(31, lens, news, Hq, Hkv, ps, BF, window, prefix)
+    q, kp, vp, table, sl, starts = args
+    base = torch.full((Hq, q.shape[0] + 2, 2 * D), 7.0, dtype=BF, device="cuda")
+    out = base[:, 1:-1, D:].transpose(0, 1)
+    K.paged_prefill(q, kp, vp, table, sl, starts, window_size=window, num_prefix_tokens=prefix, out=out)
+    check(out, args, window, prefix, starts=starts)
+    assert (base[..., :D] == 7.0).all() and (base[:, 0] == 7.0).all() and (base[:, -1] == 7.0).all()
+    assert K.device_status(clear=True) == 0
+
+
 @pytest.mark.parametrize("extra_cols", [1, 300])  # 300: the call runs in shares
 def test_rows_that_see_nothing_give_zeros(K, extra_cols):
     """Sequences shorter than their new rows, absent pages under every visible

@@ -60,8 +60,8 @@ def _programs(nts, rnd, flawed=False, rescale_prob=0.3):
                 yield from s_(j)
                 yield ("commit", ("PRO", j))
             for j in range(n):
-                yield ("wait", ("PF", j & 1), par(g, j & 1, j >> 1))
                 yield ("wait", ("VF", j & 1), par(g, j & 1, j >> 1))
+                yield ("wait", ("PF", j & 1), par(g, j & 1, j >> 1))
                 yield ("check", lambda s, j=j: ("V", g, j) in s and all(("P", g, j, w) in s for w in range(T.WARPS)),
                        f"PV{g}.{j} before P / V")
                 yield ("check", lambda s, j=j: j > 0 or g == 0 or all(("O", g - 1, w) in s for w in range(T.WARPS)),
