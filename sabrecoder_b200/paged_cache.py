@@ -32,6 +32,11 @@ from transformers.cache_utils import Cache, CacheLayerMixin
 from . import kernels as K
 
 
+def _capturing(pool: torch.Tensor) -> bool:
+    """Whether calls on the current stream are being captured into a graph."""
+    return pool.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
 class SabrePagedCacheLayer(CacheLayerMixin):
     """One layer of a :class:`SabrePagedKVCache`: its pages and the step it is at."""
 
@@ -306,12 +311,15 @@ class SabrePagedKVCache(Cache):
                       self.page_table, self.seq_lens, self._row_starts(n))
 
     def _row_starts(self, n: int) -> torch.Tensor:
+        """Row starts of a step of n rows each. Kept while the number of sequences
+        stays, since a captured call holds their address (at most max_seq_len small
+        tensors). First asked for inside a capture they belong to its graph, which
+        fills them on every replay, and to nobody else."""
         t = self._starts.get(n)
         if t is None:
-            if len(self._starts) > 64:
-                self._starts.clear()
             t = torch.arange(0, n * self.batch_size + 1, n, dtype=torch.int32, device=self.pool.device)
-            self._starts[n] = t
+            if not _capturing(self.pool):
+                self._starts[n] = t
         return t
 
     def decode(self, layer_idx: int, q: torch.Tensor, softmax_scale: Optional[float] = None,

@@ -201,3 +201,47 @@ def test_sparse_generation_refuses_pages(cuda):
     with pytest.raises(ValueError, match="contiguous cache"):
         model(input_ids=torch.zeros(1, 8, dtype=torch.long, device=cuda), past_key_values=cache, use_cache=True)
     assert cache.get_seq_length() == 0
+
+
+@pytest.mark.parametrize("eager_first", [True, False])
+def test_captured_prefill_replays_after_many_other_lengths(cuda, eager_first):
+    """A captured step of 6 rows (store and attention) keeps answering right after
+    the cache served 99 other row counts and the memory they left was reused; and
+    when 6 rows were first seen inside the capture, an eager step before the first
+    replay is right too."""
+    from sabrecoder_b200 import kernels as K
+    from sabrecoder_b200.paged_cache import SabrePagedKVCache
+    B, Hq, Hkv, n = 3, 4, 2, 6
+    gen = torch.Generator().manual_seed(9)
+    c = SabrePagedKVCache(batch_size=B, max_seq_len=512, page_size=16, num_layers=1, num_kv_heads=Hkv, head_dim=D)
+    c.pool.zero_()
+    layer = c.layers[0]
+    q = torch.randn(B, n, Hq, D, generator=gen).to(BF).cuda()
+    c.extend([40, 3, 100])
+    c.pool.normal_()
+    c.extend([n] * B)
+
+    def right(out):
+        starts = torch.tensor([0, n, 2 * n, 3 * n], dtype=torch.int32, device=cuda)
+        check(out.reshape(B * n, Hq, D), (q.view(B * n, Hq, D), layer.k_pages, layer.v_pages, c.page_table, c.seq_lens,
+                                          None), starts=starts)
+
+    if eager_first:
+        right(c.prefill(0, q))
+    else:
+        c.prefill(0, q[:, :1])  # the kernels are loaded
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = c.prefill(0, q)
+    right(c.prefill(0, q))
+    for m in range(1, 100):
+        c._row_starts(m)
+    junk = [torch.full((B + 1,), 10 ** 6, dtype=torch.int32, device=cuda) for _ in range(200)]
+    for _ in range(3):
+        c.extend([n, n, n])
+        q.copy_(torch.randn(q.shape, generator=gen).to(BF))
+        graph.replay()
+        right(out)
+    del junk
+    assert K.device_status(clear=True) == 0

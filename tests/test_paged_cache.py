@@ -259,3 +259,20 @@ def test_the_pool_goes_with_the_cache():
         assert ref() is None
     finally:
         gc.enable()
+
+
+def test_row_starts_stay_where_a_captured_call_found_them(monkeypatch):
+    """A captured prefill keeps the address of its row starts: they are the same
+    tensor after any number of other row counts, and those first asked for inside
+    a capture (whose fill only runs on replay) are not handed to eager calls."""
+    c = cache(batch_size=2)
+    first = c._row_starts(5)
+    for n in range(1, 150):
+        assert c._row_starts(n).tolist() == [0, n, 2 * n]
+    assert c._row_starts(5) is first
+    capturing = True
+    monkeypatch.setattr(PC, "_capturing", lambda pool: capturing, raising=False)
+    inside = c._row_starts(170)
+    assert c._row_starts(5) is first
+    capturing = False
+    assert c._row_starts(170) is not inside and c._row_starts(170) is c._row_starts(170)
