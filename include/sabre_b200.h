@@ -394,7 +394,9 @@ int sabre_prefill_bsa_tokenmask(const void* q, const void* k, const void* v, voi
  *
  * Visibility: the query at position i sees key j when j <= i,
  * j < seq_lens[b], page j is present and (window < 0, or i - j <= window, or
- * j < num_prefix_tokens). A query that sees nothing gives zeros. Rows that
+ * j < num_prefix_tokens). A query that sees nothing gives zeros; a score of
+ * -inf has weight zero (and a query with no other gives zeros), one of NaN or
+ * +inf makes its query's result NaN, however the work is split. Rows that
  * the sequence does not have, or whose page is absent, never reach a result,
  * whatever they hold; nor do rows that no query of the call sees (outside the
  * window). In prefill a NaN or an infinity in a V row that some query sees may

@@ -221,13 +221,64 @@ __device__ __forceinline__ void mma_16x8x16(float (&c)[4], const uint32_t (&a)[4
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// out[4 lane ..] = a / l, zeros where nothing was visible.
+// out[4 lane ..] = a / l, zeros where nothing was visible (l is exactly 0; a NaN
+// sum is a NaN result).
 template <typename T>
 __device__ __forceinline__ void store_row(T* out, int lane, const float4& a, float l) {
-  const float inv = l > 0.f ? 1.0f / l : 0.f;
+  const float inv = 1.0f / l;
   *reinterpret_cast<uint2*>(out + lane * 4) =
-      make_uint2(DT<T>::pack(a.x * inv, a.y * inv), DT<T>::pack(a.z * inv, a.w * inv));
+      l == 0.f ? make_uint2(0u, 0u)
+               : make_uint2(DT<T>::pack(a.x * inv, a.y * inv), DT<T>::pack(a.z * inv, a.w * inv));
 }
+
+// The running sum of a row's parts: maximum m, sum l and four columns a of the
+// accumulator. Scores of NaN never raise m but make l and a NaN, also where m
+// is still -inf, so no part is skipped for its m.
+struct PartSum {
+  float m = -INFINITY, l = 0.f;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  // The offset of the exponentials once m is raised to mn.
+  __device__ __forceinline__ float raise(float mn) {
+    const float off = mn == -INFINITY ? 0.f : mn;
+    const float r = ex2(m - off);
+    m = mn;
+    l *= r;
+    a = make_float4(a.x * r, a.y * r, a.z * r, a.w * r);
+    return off;
+  }
+  __device__ __forceinline__ void add(float off, float pm, float pl, const float4& pa) {
+    const float w = ex2(pm - off);
+    l += w * pl;
+    a.x += w * pa.x;
+    a.y += w * pa.y;
+    a.z += w * pa.z;
+    a.w += w * pa.w;
+  }
+  // Parts first, first + step, .. below `parts`, eight in flight; slot(i): the
+  // row of part i in ml and acc, this lane's columns from 4 lane on.
+  template <typename S>
+  __device__ __forceinline__ void add_parts(const float* part_ml, const float* part_acc, int first, int step, int parts,
+                                            int lane, S slot) {
+    constexpr int kBatch = 8;
+    for (int i0 = first; i0 < parts; i0 += step * kBatch) {
+      float2 ml[kBatch];
+      float4 x[kBatch];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int i = i0 + u * step;
+        ml[u] = i < parts ? *reinterpret_cast<const float2*>(part_ml + slot(i) * 2) : make_float2(-INFINITY, 0.f);
+        x[u] = i < parts ? *reinterpret_cast<const float4*>(part_acc + slot(i) * kD + lane * 4)
+                         : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+      float mn = m;
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) mn = fmaxf(mn, ml[u].x);
+      const float off = raise(mn);
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) add(off, ml[u].x, ml[u].y, x[u]);
+    }
+  }
+};
 
 template <typename T>
 __global__ void __launch_bounds__(kDecThreads, 2)
@@ -529,61 +580,27 @@ __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const Decod
   const int4 job = p.joins[x];
   const int parts = job.x;
   if (parts == 0) return;
-  constexpr int kBatch = 8;
-  const int warps = min(kJoinWarps, (parts + kBatch - 1) / kBatch);
+  const int warps = min(kJoinWarps, (parts + 7) / 8);
   // The first part is the last segment of its share, the others open theirs.
-  auto slot = [&](int i) -> long long { return (i == 0 ? job.w : 2ll * (x + i)) * p.group + g; };
-  float M = -INFINITY, L = 0.f;
-  float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = warp; warp < warps && i0 < parts; i0 += warps * kBatch) {
-    float2 ml[kBatch];
-    float4 a[kBatch];
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int i = i0 + u * warps;
-      ml[u] = i < parts ? *reinterpret_cast<const float2*>(p.part_ml + slot(i) * 2) : make_float2(-INFINITY, 0.f);
-      a[u] = i < parts ? *reinterpret_cast<const float4*>(p.part_acc + slot(i) * kD + lane * 4)
-                       : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    float mn = M;
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) mn = fmaxf(mn, ml[u].x);
-    if (mn == -INFINITY) continue;
-    const float r = ex2(M - mn);
-    M = mn;
-    L *= r;
-    A = make_float4(A.x * r, A.y * r, A.z * r, A.w * r);
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const float w = ex2(ml[u].x - mn);
-      L += w * ml[u].y;
-      A.x += w * a[u].x;
-      A.y += w * a[u].y;
-      A.z += w * a[u].z;
-      A.w += w * a[u].w;
-    }
-  }
+  PartSum sum;
+  if (warp < warps)
+    sum.add_parts(p.part_ml, p.part_acc, warp, warps, parts, lane,
+                  [&](int i) -> long long { return (i == 0 ? job.w : 2ll * (x + i)) * p.group + g; });
   if (warps > 1) {
     if (lane == 0) {
-      sm_m[warp] = M;
-      sm_l[warp] = L;
+      sm_m[warp] = sum.m;
+      sm_l[warp] = sum.l;
     }
-    sm_a[warp][lane] = A;
+    sm_a[warp][lane] = sum.a;
     __syncthreads();
     float mn = -INFINITY;
     for (int w = 0; w < warps; ++w) mn = fmaxf(mn, sm_m[w]);
-    L = 0.f;
-    A = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int w = 0; w < warps && mn != -INFINITY; ++w) {
-      const float r = ex2(sm_m[w] - mn);
-      L += r * sm_l[w];
-      A.x += r * sm_a[w][lane].x;
-      A.y += r * sm_a[w][lane].y;
-      A.z += r * sm_a[w][lane].z;
-      A.w += r * sm_a[w][lane].w;
-    }
+    sum = PartSum();
+    const float off = sum.raise(mn);
+    for (int w = 0; w < warps; ++w) sum.add(off, sm_m[w], sm_l[w], sm_a[w][lane]);
   }
-  if (warp == 0) store_row<T>(static_cast<T*>(p.o) + job.y * p.o_sb + (job.z * p.group + g) * p.o_sh, lane, A, L);
+  if (warp == 0)
+    store_row<T>(static_cast<T*>(p.o) + job.y * p.o_sb + (job.z * p.group + g) * p.o_sh, lane, sum.a, sum.l);
 }
 
 // Tensor map of a pool [num_pages, H, page_size, D]: dims (64 d, page rows, 2

@@ -735,15 +735,15 @@ __global__ void __launch_bounds__(kThreads, 2)
       if (ok) {
         T* orow = static_cast<T*>(p.o) + static_cast<long long>(job.row0 + tok) * p.o_sr + head * p.o_sh;
         const long long prow = static_cast<long long>(place) * kRows + tid;
-        const float inv = 1.0f / l_run;  // unused where the row saw nothing: it is zero
+        const float inv = 1.0f / l_run;  // unused where the row saw nothing (l_run is exactly 0): it is zero
         const uint64_t opol = l2_policy_evict_first();
         auto quad = [&](const uint32_t (&ov)[32], int q4) -> uint4 {  // 8 columns of the result
           uint32_t w[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            w[e] = l_run > 0.f ? DT<T>::pack(__uint_as_float(ov[8 * q4 + 2 * e]) * inv,
-                                             __uint_as_float(ov[8 * q4 + 2 * e + 1]) * inv)
-                               : 0u;
+            w[e] = l_run == 0.f ? 0u
+                                : DT<T>::pack(__uint_as_float(ov[8 * q4 + 2 * e]) * inv,
+                                              __uint_as_float(ov[8 * q4 + 2 * e + 1]) * inv);
           return make_uint4(w[0], w[1], w[2], w[3]);
         };
         if (!kShares && nt >= 1) {
@@ -827,43 +827,13 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const Params p) {
   const int tok = row / p.group;
   if (tok >= rows.y) return;
   // The first part is the last segment of its share, the others open theirs.
-  auto slot = [&](int i) -> long long {
+  PartSum sum;
+  sum.add_parts(p.part_ml, p.part_acc, 0, 1, parts, lane, [&](int i) -> long long {
     return static_cast<long long>(i == 0 ? pair.z : 2 * (pair.y + i)) * kRows + row;
-  };
-  constexpr int kBatch = 8;
-  float M = -INFINITY, L = 0.f;
-  float4 A = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0; i0 < parts; i0 += kBatch) {
-    float2 ml[kBatch];
-    float4 a[kBatch];
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const int i = i0 + u;
-      ml[u] = i < parts ? *reinterpret_cast<const float2*>(p.part_ml + slot(i) * 2) : make_float2(-INFINITY, 0.f);
-      a[u] = i < parts ? *reinterpret_cast<const float4*>(p.part_acc + slot(i) * kD + lane * 4)
-                       : make_float4(0.f, 0.f, 0.f, 0.f);
-    }
-    float mn = M;
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) mn = fmaxf(mn, ml[u].x);
-    if (mn == -INFINITY) continue;
-    const float r = ex2(M - mn);
-    M = mn;
-    L *= r;
-    A = make_float4(A.x * r, A.y * r, A.z * r, A.w * r);
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u) {
-      const float w = ex2(ml[u].x - mn);
-      L += w * ml[u].y;
-      A.x += w * a[u].x;
-      A.y += w * a[u].y;
-      A.z += w * a[u].z;
-      A.w += w * a[u].w;
-    }
-  }
+  });
   store_row<T>(static_cast<T*>(p.o) + static_cast<long long>(rows.x + tok) * p.o_sr +
                    (static_cast<int>(blockIdx.x) % p.heads_kv * p.group + row - tok * p.group) * p.o_sh,
-               lane, A, L);
+               lane, sum.a, sum.l);
 }
 
 // Row tiles that `rows` rows of `batch` sequences need at most: a sequence of

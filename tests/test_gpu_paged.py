@@ -464,3 +464,54 @@ def test_two_streams_and_two_captured_graphs_at_once(K):
             check(a, job, starts=job[5])
             check(b, (job[0][:2],) + job[1:])
     assert K.device_status(clear=True) == 0
+
+
+def poisoned(got, args, clean, window=None, prefix=0, starts=None):
+    """NaN in exactly the results where the oracle has it; the others within the
+    bound of `check` (score magnitudes without the bad values: a score of -inf is
+    exact, its weight zero)."""
+    kw = dict(window=window, prefix=prefix)
+    want, spread, _ = PO.attention(*args[:5], starts, **kw)
+    ds = PO.attention(*clean[:5], starts, **kw)[2]
+    u = torch.finfo(got.dtype).eps / 2
+    n = float(args[4].max())
+    rel = u + 2 * (129 * ds + 16) * 2.0 ** -23 + n * 2.0 ** -23
+    tol = rel[..., None] * spread + u * want.abs() + 2.0 ** -25 * n * (got.dtype == FP) * 6.0 + 1e-7
+    bad = want.isnan()
+    assert not bad.all()
+    assert torch.equal(got.isnan(), bad), f"{int(got.isnan().sum())} NaN for {int(bad.sum())}"
+    err = (got.double() - want).abs()
+    assert (err <= tol * 1.01)[~bad].all(), f"worst {(err / tol)[~bad].max():.2f} of its bound"
+    return int(bad.sum())
+
+
+@pytest.mark.parametrize("what", ["q", "q inf", "k", "k inf"])
+@pytest.mark.parametrize("lens,news,Hq,Hkv,ps,dtype,window,extra_cols", [
+    ([130, 128, 70], [130, 128, 70], 4, 2, 32, BF, None, 1),        # a CTA each
+    ([900, 1300, 80], [300, 200, 80], 4, 2, 64, BF, 100, 1),
+    ([9000, 31], [20, 9], 7, 1, 16, FP, None, 1),                   # parts of pairs
+    ([8400], [400], 56, 8, 64, BF, None, 1),                        # equal shares
+    ([300, 20], [1, 1], 16, 8, 16, BF, None, 1),                    # decode: pairs whole and cut
+    ([40000, 33], [1, 1], 7, 1, 64, BF, None, 1),
+    ([2000, 900, 77] * 20, [1] * 60, 2, 2, 32, FP, 300, 1),
+])
+def test_nan_in_what_a_query_sees_reaches_its_result(K, what, lens, news, Hq, Hkv, ps, dtype, window, extra_cols):
+    """A query with a NaN or an infinity, and a visible K row with one: the queries
+    that meet it answer NaN, whatever way the work is split, and no other does."""
+    clean = make(40, lens, news, Hq, Hkv, ps, dtype, window, extra_cols=extra_cols, drop=False)
+    q, kp, vp, table, sl, starts = clean
+    bad = float("inf") if "inf" in what else float("nan")
+    if what[0] == "q":
+        q = q.clone()
+        q[q.shape[0] // 2, Hq - 1, 17] = bad
+    else:  # in the first window of the last row of sequence 0, and in sight of few rows or many
+        kp = kp.clone()
+        j = lens[0] - 1 - min(news[0], 7)
+        kp[table[0, j // ps], 0, j % ps, 100] = bad
+    args = (q, kp, vp, table, sl, starts)
+    calls = [(K.paged_prefill(*args, window_size=window), starts)]
+    if max(news) == 1:
+        calls.append((K.paged_decode(*args[:5], window_size=window), None))
+    for got, st in calls:
+        assert poisoned(got, args, clean, window, starts=st) or what == "k inf"
+    assert K.device_status(clear=True) == 0
