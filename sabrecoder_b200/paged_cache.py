@@ -18,7 +18,8 @@ follows them) are what the kernels read.
 As a transformers ``Cache`` it takes the same number of new rows for every
 sequence of the batch; the patched attention writes its rows through
 :meth:`append` and attends with :meth:`decode` / :meth:`prefill`. Padding masks
-are not applied: sequences of different lengths keep their own lengths.
+are not applied: sequences of different lengths keep their own lengths, and a
+model that continues them needs ``position_ids`` that go on from each.
 """
 
 from __future__ import annotations
@@ -72,6 +73,9 @@ class SabrePagedCacheLayer(CacheLayerMixin):
         c = self._cache
         if c.window_size is not None:
             raise ValueError("SabrePagedKVCache with a window serves the patched attention only (pages are dropped)")
+        if len(set(c.lengths)) > 1:
+            raise ValueError(f"SabrePagedKVCache: sequences of different lengths ({c.lengths}) serve the patched "
+                             f"attention only (its mask knows one length)")
         c.append(self.index, key_states.transpose(1, 2), value_states.transpose(1, 2))
         return c.gather(self.index)
 
@@ -293,6 +297,18 @@ class SabrePagedKVCache(Cache):
         return len(src)
 
     # -- one step ---------------------------------------------------------
+
+    def check_step(self, layer_idx: int, n: int, position_ids: Optional[torch.Tensor]) -> None:
+        """Raises ValueError when a step of n rows cannot be what the model takes it
+        for. A model derives its positions from the longest sequence; when the lengths
+        differ it must have been given each sequence's own (read from the device, once
+        a step)."""
+        if self.layers[layer_idx].step != self.step or len(set(self.lengths)) <= 1:
+            return
+        own = [[length + i for i in range(n)] for length in self.lengths]
+        if position_ids is None or position_ids.tolist() != own:
+            raise ValueError(f"SabrePagedKVCache holds sequences of different lengths ({self.lengths}): their new rows "
+                             f"need position_ids that go on from each one's length")
 
     def append(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor) -> None:
         """Stores the rows k, v ``[B, n, Hkv, D]`` of a step in one layer; the

@@ -245,3 +245,31 @@ def test_captured_prefill_replays_after_many_other_lengths(cuda, eager_first):
         right(out)
     del junk
     assert K.device_status(clear=True) == 0
+
+
+def test_model_steps_on_sequences_of_different_lengths(cuda):
+    """A batch whose second sequence was cut back continues as two separate ones
+    when it is given each sequence's positions, and is refused without them."""
+    from transformers import DynamicCache
+
+    from sabrecoder_b200.paged_cache import SabrePagedKVCache
+    model = _model(cuda)
+    ids = torch.randint(0, 512, (2, 90), generator=torch.Generator().manual_seed(5)).to(cuda)
+    cache = SabrePagedKVCache(model.config, batch_size=2, max_seq_len=200, page_size=16, device=cuda)
+    with torch.no_grad():
+        model(input_ids=ids[:, :70], past_key_values=cache, use_cache=True)
+        cache.truncate(1, 33)
+        with pytest.raises(ValueError, match="position_ids"):
+            model(input_ids=ids[:, 70:75], past_key_values=cache, use_cache=True)
+        assert cache.lengths == [70, 33]
+        tokens = [list(ids[0, :70].tolist()), list(ids[1, :33].tolist())]
+        for n in (5, 1, 1, 12):
+            new = torch.stack([ids[0, 70:70 + n], ids[1, 40:40 + n]])
+            at = torch.tensor([[len(t)] for t in tokens], device=cuda) + torch.arange(n, device=cuda)
+            got = model(input_ids=new, past_key_values=cache, use_cache=True, position_ids=at).logits
+            for b in range(2):
+                tokens[b] += new[b].tolist()
+                want = model(input_ids=torch.tensor([tokens[b]], device=cuda), past_key_values=DynamicCache(),
+                             use_cache=True).logits[0, -n:]
+                _close(got[b], want)
+    assert cache.lengths == [89, 52]

@@ -276,3 +276,26 @@ def test_row_starts_stay_where_a_captured_call_found_them(monkeypatch):
     assert c._row_starts(5) is first
     capturing = False
     assert c._row_starts(170) is not inside and c._row_starts(170) is c._row_starts(170)
+
+
+def test_sequences_of_different_lengths_in_a_model():
+    """Attention that does not read pages cannot tell the rows a shorter sequence
+    does not have; the patched one needs every sequence's own positions."""
+    c = cache(batch_size=2)
+    k = torch.randn(2, H, 20, D)
+    for i in (0, 1):
+        c.update(k, k, i)
+    c.check_step(0, 3, torch.arange(20, 23)[None])
+    c.truncate(1, 10)
+    with pytest.raises(ValueError, match="different lengths"):
+        c.update(k[:, :, :1], k[:, :, :1], 0)
+    assert c.lengths == [20, 10]
+    for ids in (None, torch.tensor([[20, 21]]), torch.tensor([[20, 21], [20, 21]]), torch.tensor([[20], [10]])):
+        with pytest.raises(ValueError, match="position_ids"):
+            c.check_step(0, 2, ids)
+    own = torch.tensor([[20, 21], [10, 11]])
+    c.check_step(0, 2, own)
+    c.append(0, k[:, :, :2].transpose(1, 2), k[:, :, :2].transpose(1, 2))
+    c.check_step(1, 2, own)  # the same step: nothing new to check
+    c.append(1, k[:, :, :2].transpose(1, 2), k[:, :, :2].transpose(1, 2))
+    assert c.lengths == [22, 12]
