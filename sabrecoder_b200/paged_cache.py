@@ -18,8 +18,8 @@ follows them) are what the kernels read.
 As a transformers ``Cache`` it takes the same number of new rows for every
 sequence of the batch; the patched attention writes its rows through
 :meth:`append` and attends with :meth:`decode` / :meth:`prefill`. Padding masks
-are not applied: sequences of different lengths keep their own lengths, and a
-model that continues them needs ``position_ids`` that go on from each.
+are refused: sequences of different lengths keep their own lengths, and a model
+that continues them needs ``position_ids`` that go on from each.
 """
 
 from __future__ import annotations
@@ -298,17 +298,44 @@ class SabrePagedKVCache(Cache):
 
     # -- one step ---------------------------------------------------------
 
-    def check_step(self, layer_idx: int, n: int, position_ids: Optional[torch.Tensor]) -> None:
+    def check_step(self, layer_idx: int, n: int, position_ids: Optional[torch.Tensor],
+                   attention_mask: Optional[torch.Tensor] = None) -> None:
         """Raises ValueError when a step of n rows cannot be what the model takes it
         for. A model derives its positions from the longest sequence; when the lengths
-        differ it must have been given each sequence's own (read from the device, once
-        a step)."""
-        if self.layers[layer_idx].step != self.step or len(set(self.lengths)) <= 1:
+        differ it must have been given each sequence's own. A mask (if there is one:
+        additive, boolean, or one flag a key) may not say more than the cache does:
+        it must show the keys that each query sees here and none of its future. Both
+        are read from the device, once a step."""
+        if self.layers[layer_idx].step != self.step:
             return
-        own = [[length + i for i in range(n)] for length in self.lengths]
-        if position_ids is None or position_ids.tolist() != own:
-            raise ValueError(f"SabrePagedKVCache holds sequences of different lengths ({self.lengths}): their new rows "
-                             f"need position_ids that go on from each one's length")
+        if len(set(self.lengths)) > 1:
+            own = [[length + i for i in range(n)] for length in self.lengths]
+            if position_ids is None or position_ids.tolist() != own:
+                raise ValueError(f"SabrePagedKVCache holds sequences of different lengths ({self.lengths}): their new "
+                                 f"rows need position_ids that go on from each one's length")
+        if attention_mask is not None and not self._mask_fits(attention_mask, n):
+            raise ValueError("SabrePagedKVCache: attention over pages is causal (within the cache's window) over all "
+                             "rows of a sequence; this attention mask is not (padding must not be stored: give each "
+                             "sequence its own rows)")
+
+    def _mask_fits(self, mask: torch.Tensor, n: int) -> bool:
+        top = max(self.lengths)
+        if mask.shape[-1] < top + n or mask.dim() not in (2, 4) or (mask.dim() == 4 and mask.shape[2] != n):
+            return False
+        see = (mask == 0 if mask.is_floating_point() and mask.dim() == 4 else mask != 0)[..., :top + n]
+        if mask.dim() == 2:
+            see = see[:, None, None]
+        lengths = torch.tensor(self.lengths if len(set(self.lengths)) > 1 else self.lengths[:1], device=mask.device)
+        row = torch.arange(n, device=mask.device)[:, None]
+        j = torch.arange(top + n, device=mask.device)
+        i = lengths[:, None, None, None] + row
+        own = j <= i
+        if self.window_size is not None:
+            own = own & ((i - j <= self.window_size) | (j < self.num_prefix_tokens))
+        wrong = own & ~see
+        if mask.dim() == 4:
+            wrong = wrong | (see & (j > top + row))
+        return not bool(wrong.any())
 
     def append(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor) -> None:
         """Stores the rows k, v ``[B, n, Hkv, D]`` of a step in one layer; the

@@ -343,7 +343,7 @@ class StructureAwareAttentionWrapper(nn.Module):
             if self.use_sparse_for_generation:
                 raise ValueError("use_sparse_for_generation needs a contiguous cache: a SabrePagedKVCache decodes over "
                                  "all rows or its window")
-            cache.check_step(self.layer_idx, L, kwargs.get("position_ids"))
+            cache.check_step(self.layer_idx, L, kwargs.get("position_ids"), attention_mask)
             fresh = cache.get_seq_length(self.layer_idx) == 0
             kn = torch.empty(B, L, Hkv, D, dtype=q.dtype, device=q.device)
             vn = torch.empty_like(kn)

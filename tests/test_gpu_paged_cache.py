@@ -273,3 +273,30 @@ def test_model_steps_on_sequences_of_different_lengths(cuda):
                              use_cache=True).logits[0, -n:]
                 _close(got[b], want)
     assert cache.lengths == [89, 52]
+
+
+def test_padded_batches_are_refused_and_plain_masks_are_not(cuda):
+    """A left-padded batch in generate raises before a row is stored; the mask that
+    eager attention always builds changes nothing."""
+    from sabrecoder_b200.paged_cache import SabrePagedKVCache
+    model = _model(cuda)
+    ids = torch.randint(1, 512, (2, 50), generator=torch.Generator().manual_seed(6)).to(cuda)
+    mask = torch.ones_like(ids)
+    mask[1, :9] = 0
+
+    def new():
+        return SabrePagedKVCache(model.config, batch_size=2, max_seq_len=80, page_size=16, device=cuda)
+
+    cache = new()
+    with pytest.raises(ValueError, match="mask"):
+        model.generate(input_ids=ids, attention_mask=mask, past_key_values=cache, max_new_tokens=4, do_sample=False,
+                       pad_token_id=0)
+    assert cache.lengths == [0, 0]
+    with torch.no_grad():
+        ca, cb = new(), new()
+        for part in ids.split([30, 1, 19], 1):
+            a = model(input_ids=part, past_key_values=ca, use_cache=True).logits
+            model.config._attn_implementation = "eager"
+            b = model(input_ids=part, past_key_values=cb, use_cache=True).logits
+            model.config._attn_implementation = "sdpa"
+            assert torch.equal(a, b)

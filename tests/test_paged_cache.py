@@ -299,3 +299,58 @@ def test_sequences_of_different_lengths_in_a_model():
     c.check_step(1, 2, own)  # the same step: nothing new to check
     c.append(1, k[:, :, :2].transpose(1, 2), k[:, :, :2].transpose(1, 2))
     assert c.lengths == [22, 12]
+
+
+def test_masks_that_say_more_than_the_cache_are_refused():
+    """Attention over pages is causal within the cache's window: a mask that hides
+    more, shows more or adds a bias would be dropped without a word."""
+    lo = torch.finfo(torch.float32).min
+
+    def causal(B=2, n=4, T=24, window=None):
+        i, j = torch.arange(T - n, T)[:, None], torch.arange(T)[None]
+        see = (j <= i) & (i - j <= (T if window is None else window))
+        return see.expand(B, 1, n, T).clone()
+
+    c = cache(batch_size=2)
+    k = torch.randn(2, H, 20, D)
+    for i in (0, 1):
+        c.update(k, k, i)
+    ids = torch.arange(20, 24)[None]
+    good = causal()
+    left, right, future, bias = good.clone(), good.clone(), good.clone(), torch.where(good, 0.0, lo)
+    left[1, :, :, :3] = False
+    right[0, :, :, 22:] = False
+    future[:, :, 0] = True
+    assert (bias == 0).any()
+    bias[0, 0, 2, 5] = -0.5
+    pad = torch.ones(2, 24, dtype=torch.long)
+    pad[1, :3] = 0
+
+    def added(see):
+        return torch.where(see, 0.0, lo)
+
+    for ok in (None, good, good[:1], added(good), added(good).expand(2, H, 4, 24), torch.ones(2, 24, dtype=torch.long),
+               torch.nn.functional.pad(good, (0, 8))):
+        c.check_step(0, 4, ids, ok)
+    for wrong in (left, right, future, bias, added(left), added(future), pad, pad.bool(), causal(window=10), good[..., :20],
+                  good[0, 0], good[:, 0]):
+        with pytest.raises(ValueError, match="mask"):
+            c.check_step(0, 4, ids, wrong)
+    w = cache(batch_size=2, window_size=10)
+    for i in (0, 1):
+        w.append(i, k.transpose(1, 2), k.transpose(1, 2))
+    for ok in (good, causal(window=10), added(causal(window=15))):
+        w.check_step(0, 4, ids, ok)
+    for wrong in (left & causal(window=2), causal(window=9)):
+        with pytest.raises(ValueError, match="mask"):
+            w.check_step(0, 4, ids, wrong)
+    # Each sequence's own rows and positions, the mask of the longest.
+    c.truncate(1, 10)
+    own = torch.tensor([[20, 21, 22, 23], [10, 11, 12, 13]])
+    c.check_step(0, 4, own, good)
+    short = good.clone()
+    short[1, :, :, 14:] = False
+    c.check_step(0, 4, own, short)
+    short[1, :, :, 13:] = False
+    with pytest.raises(ValueError, match="mask"):
+        c.check_step(0, 4, own, short)
