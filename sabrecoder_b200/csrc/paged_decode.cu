@@ -78,7 +78,8 @@ struct Tiles {
     n = p.c.length(b);
     lo = n > 0 ? p.w.first(p.c.seq_lens[b] - 1) : 0;
     from = lo / kTile;
-    head = min((min(p.w.prefix, lo) + kTile - 1) / kTile, from);
+    // No tile past n: lengths and prefixes reach to the end of int32, tables do not.
+    head = min((min(min(p.w.prefix, lo), n) + kTile - 1) / kTile, from);
     count = head + max(0, (n + kTile - 1) / kTile - from);
   }
   __device__ __forceinline__ int pos(int i) const { return (i < head ? i : from + i - head) * kTile; }

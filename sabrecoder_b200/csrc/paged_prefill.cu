@@ -143,7 +143,7 @@ __device__ __forceinline__ Job make_job(const Params& p, int b, int r, int first
   job.lo = p.w.first(job.pos0);
   job.from = job.lo / kTile;
   const int whole = (job.n + kTile - 1) / kTile;
-  job.head = min(min((min(p.w.prefix, job.lo) + kTile - 1) / kTile, job.from), whole);
+  job.head = min((min(min(p.w.prefix, job.lo), job.n) + kTile - 1) / kTile, job.from);
   job.tiles = job.head + max(0, whole - job.from);
   return job;
 }

@@ -466,22 +466,26 @@ def test_two_streams_and_two_captured_graphs_at_once(K):
     assert K.device_status(clear=True) == 0
 
 
+def within(got, want, spread, ds, n):
+    """The bound of `check` over n keys for results whose exact value is a number."""
+    u = torch.finfo(got.dtype).eps / 2
+    rel = u + 2 * (129 * ds + 16) * 2.0 ** -23 + n * 2.0 ** -23
+    tol = rel[..., None] * spread + u * want.abs() + 2.0 ** -25 * n * (got.dtype == FP) * 6.0 + 1e-7
+    some = ~want.isnan()
+    err = (got.double() - want).abs()
+    assert (err <= tol * 1.01)[some].all(), f"worst {(err / tol)[some].max():.2f} of its bound"
+
+
 def poisoned(got, args, clean, window=None, prefix=0, starts=None):
     """NaN in exactly the results where the oracle has it; the others within the
     bound of `check` (score magnitudes without the bad values: a score of -inf is
     exact, its weight zero)."""
     kw = dict(window=window, prefix=prefix)
     want, spread, _ = PO.attention(*args[:5], starts, **kw)
-    ds = PO.attention(*clean[:5], starts, **kw)[2]
-    u = torch.finfo(got.dtype).eps / 2
-    n = float(args[4].max())
-    rel = u + 2 * (129 * ds + 16) * 2.0 ** -23 + n * 2.0 ** -23
-    tol = rel[..., None] * spread + u * want.abs() + 2.0 ** -25 * n * (got.dtype == FP) * 6.0 + 1e-7
     bad = want.isnan()
     assert not bad.all()
     assert torch.equal(got.isnan(), bad), f"{int(got.isnan().sum())} NaN for {int(bad.sum())}"
-    err = (got.double() - want).abs()
-    assert (err <= tol * 1.01)[~bad].all(), f"worst {(err / tol)[~bad].max():.2f} of its bound"
+    within(got, want, spread, PO.attention(*clean[:5], starts, **kw)[2], float(args[4].max()))
     return int(bad.sum())
 
 
@@ -514,4 +518,29 @@ def test_nan_in_what_a_query_sees_reaches_its_result(K, what, lens, news, Hq, Hk
         calls.append((K.paged_decode(*args[:5], window_size=window), None))
     for got, st in calls:
         assert poisoned(got, args, clean, window, starts=st) or what == "k inf"
+    assert K.device_status(clear=True) == 0
+
+
+FAR = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("window,prefix", [(100, 5000), (0, FAR), (FAR - 300, 33), (FAR - 300, FAR), (FAR - 1, 0),
+                                           (100, 0), (None, 0)])
+@pytest.mark.parametrize("times,extra_cols", [(40, 0), (10, 60)])  # 60: wide windows run in shares
+def test_lengths_far_past_the_table(K, window, prefix, times, extra_cols):
+    """Lengths up to the largest int32 over a table of a few rows: what the table
+    holds of the window and the prefix is seen, the other sequences are as ever."""
+    lens, news = [128, 256, 70] * times, [1, 3, 1] * times
+    args = make(19, lens, news, 4, 2, 64, BF, extra_cols=extra_cols, drop=False)
+    q, kp, vp, table, sl, starts = args
+    sl[::3] = FAR
+    sl[1::9] = FAR - 40
+    n = table.shape[1] * 64
+    table[:, 4:] = table[:, :1]  # the places past the rows hold some page of the pool
+    kp.nan_to_num_(0.25), vp.nan_to_num_(0.5)
+    kw = dict(window_size=window, num_prefix_tokens=prefix)
+    o = dict(window=window, prefix=prefix)
+    within(K.paged_prefill(q, kp, vp, table, sl, starts, **kw), *PO.attention(*args[:5], starts, **o), n)
+    last = q[starts[1:].long() - 1]
+    within(K.paged_decode(last, kp, vp, table, sl, **kw), *PO.attention(last, *args[1:5], **o), n)
     assert K.device_status(clear=True) == 0
