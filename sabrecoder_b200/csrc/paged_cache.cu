@@ -40,8 +40,9 @@ struct Cache {
 // i - j <= window, or j < prefix).
 struct Window {
   int window, prefix;  // window < 0: none
-  // First position inside the window of query i.
-  __device__ __forceinline__ int first(int i) const { return window < 0 ? 0 : max(0, i - window); }
+  // First position inside the window of query i (0 for a row before its sequence,
+  // i < 0, which sees nothing: i - window could pass the end of int32).
+  __device__ __forceinline__ int first(int i) const { return window < 0 ? 0 : max(0, max(i, 0) - window); }
 };
 
 // First row of sequence b in a ragged batch of `rows` rows (one row each

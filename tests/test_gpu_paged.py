@@ -544,3 +544,17 @@ def test_lengths_far_past_the_table(K, window, prefix, times, extra_cols):
     last = q[starts[1:].long() - 1]
     within(K.paged_decode(last, kp, vp, table, sl, **kw), *PO.attention(last, *args[1:5], **o), n)
     assert K.device_status(clear=True) == 0
+
+
+@pytest.mark.parametrize("window", [FAR - 1, FAR - 2, FAR - 5, None])
+@pytest.mark.parametrize("extra_cols", [1, 100])
+def test_rows_before_their_sequence_under_the_widest_windows(K, window, extra_cols):
+    """New rows that lie before their sequence see nothing, and hide nothing from the
+    others of their row tile."""
+    args = make(20, [40, 100, 64], [40, 100, 64], 4, 2, 16, BF, extra_cols=extra_cols)
+    q, kp, vp, table, sl, starts = args
+    sl[0], sl[2] = 10, 63
+    out = K.paged_prefill(q, kp, vp, table, sl, starts, window_size=window)
+    assert (out[:30] == 0).all() and (out[30:40] != 0).any(-1).all()
+    check(out, args, window, starts=starts)
+    assert K.device_status(clear=True) == 0
