@@ -873,8 +873,10 @@ static bool in_shares(int rows, int batch, int heads_q, int heads_kv, int page_s
     const long long seen = static_cast<long long>(window) + tokens + prefix;
     if (seen < span) span = seen;
   }
-  const long long pairs = row_slots(rows, batch, tokens) * heads_kv, tiles = span / kTile;
+  const long long slots = row_slots(rows, batch, tokens), pairs = slots * heads_kv, tiles = span / kTile;
   if (batch > kShareBatch || pairs > kMaxPairs) return false;
+  // find_share() counts the tiles of all row tiles in 32 bits.
+  if (slots * ((static_cast<long long>(page_size) * max_pages + kTile - 1) / kTile) > INT_MAX) return false;
   const long long k = kDecCtas / pairs;
   if (k >= 2) return tiles - tiles / k >= 13;
   const long long likely = (2ll * rows + static_cast<long long>(batch) * tokens) * heads_kv / (2 * tokens);

@@ -193,3 +193,16 @@ def test_copy_pages_refusals():
             K.copy_pages(pages, a, b)
     with pytest.raises(_lib.SabreError, match="must be"):
         K.copy_pages(pages[0, 0], [0], [1])
+
+
+def test_prompts_whose_key_tiles_pass_int32_do_not_run_in_shares():
+    """A call in shares counts the key tiles of all its row tiles in 32 bits (one row
+    tile sees up to 2^24 of them): the plan, seen in the workspace it asks for, is a
+    CTA for each pair where the sum could pass."""
+    def size(rows, ps, cols, batch=1, hq=8, hkv=1):
+        return _lib.lib().sabre_paged_prefill_workspace_size(rows, batch, hq, hkv, D, ps, cols, -1, 0)
+
+    assert size(16, 1024, 1 << 20) > 0 and size(127 * 16, 1024, 1 << 20) > 0  # 127 tiles of 2^24
+    assert size(128 * 16, 1024, 1 << 20) == 0 and size(148 * 16, 1024, 1 << 20) == 0
+    assert size(148 * 16, 1024, 1 << 19) > 0
+    assert size(147, 1024, 1 << 20, batch=128) == 0
