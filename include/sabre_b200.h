@@ -412,6 +412,9 @@ int sabre_prefill_bsa_tokenmask(const void* q, const void* k, const void* v, voi
  * sabre_paged_decode: one query row per sequence, q, o [batch, Hq, D]
  *   (strides {b, h}), at position seq_lens[b] - 1.
  * sabre_paged_prefill: q, o [rows, Hq, D] (strides {row, head}).
+ *   The work is planned by max_pages, so a call over short sequences passes
+ *   the columns in use (table_stride says where the rows are) and not the
+ *   whole table of a long cache.
  *   workspace: sabre_paged_*_workspace_size(...) bytes (may be 0, then NULL
  *   is fine), 16-byte aligned; calls that may overlap on the GPU need their own.
  * sabre_copy_pages: for each move m < moves, page dst[m] = page src[m] in

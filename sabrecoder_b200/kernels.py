@@ -651,7 +651,9 @@ def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
 
     q: ``[N, Hq, D]``; rows ``q_start[b] .. q_start[b+1]-1`` are the last
     rows of sequence b, the rest as in :func:`paged_decode`. Rows of ``out``
-    from ``q_start[B]`` on are left as they are."""
+    from ``q_start[B]`` on are left as they are. The work is planned by the
+    width of ``page_table``: pass the columns in use
+    (``page_table[:, :n]``) rather than all of a long cache's."""
     if q_start is None:
         raise SabreError("paged_prefill needs q_start")
     return _attend("paged_prefill", q, k_pages, v_pages, page_table, seq_lens, q_start, window_size,

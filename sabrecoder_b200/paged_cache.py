@@ -153,6 +153,7 @@ class SabrePagedKVCache(Cache):
             self.page_table = self._host.to(dev, copy=True)
             self.seq_lens = torch.zeros(len(tables), dtype=torch.int32, device=dev)
             self._starts.clear()
+            self._columns = self.max_pages, self.page_table
         self._upload(range(len(tables)))
 
     def _upload(self, seqs) -> None:
@@ -373,13 +374,24 @@ class SabrePagedKVCache(Cache):
                               window_size=self.window_size, num_prefix_tokens=self.num_prefix_tokens,
                               softmax_scale=softmax_scale, out=out)
 
+    def _columns_in_use(self) -> torch.Tensor:
+        """The columns of the page table that are in use: the prompt kernel plans its
+        work by the table's width. Inside a capture all of them, since a replay may find
+        more rows."""
+        if _capturing(self.pool):
+            return self.page_table
+        n = max(1, -(-max(self.lengths) // self.page_size))
+        if self._columns[0] != n:
+            self._columns = n, self.page_table[:, :n]
+        return self._columns[1]
+
     def prefill(self, layer_idx: int, q: torch.Tensor, softmax_scale: Optional[float] = None,
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Causal attention of a step's rows, q ``[B, n, Hq, D]``, over a layer."""
         layer = self.layers[layer_idx]
         B, n, Hq, D = q.shape
-        res = K.paged_prefill(q.reshape(B * n, Hq, D), layer.k_pages, layer.v_pages, self.page_table, self.seq_lens,
-                              self._row_starts(n), window_size=self.window_size,
+        res = K.paged_prefill(q.reshape(B * n, Hq, D), layer.k_pages, layer.v_pages, self._columns_in_use(),
+                              self.seq_lens, self._row_starts(n), window_size=self.window_size,
                               num_prefix_tokens=self.num_prefix_tokens, softmax_scale=softmax_scale,
                               out=None if out is None else out.view(B * n, Hq, D))
         return res.view(B, n, Hq, D)

@@ -354,3 +354,35 @@ def test_masks_that_say_more_than_the_cache_are_refused():
     short[1, :, :, 13:] = False
     with pytest.raises(ValueError, match="mask"):
         c.check_step(0, 4, own, short)
+
+
+def test_attention_is_planned_by_the_rows_that_are_there(monkeypatch):
+    """The prompt kernel plans its work by the table's width: eager calls pass the
+    columns in use, captured ones the whole table, which may fill by the replay."""
+    seen, capturing = [], False
+    monkeypatch.setattr(PC, "_capturing", lambda pool: capturing)
+    monkeypatch.setattr(PC.K, "paged_prefill", lambda q, kp, vp, table, *a, **kw: seen.append(table) or q)
+    c = cache(batch_size=2, max_seq_len=1000)
+
+    def width():
+        seen.clear()
+        c.prefill(0, torch.zeros(c.batch_size, 1, 4, D))
+        t, = seen
+        assert t.data_ptr() == c.page_table.data_ptr() and t.stride() == c.page_table.stride()
+        assert t.shape[0] == c.batch_size
+        return t.shape[1]
+
+    assert width() == 1
+    c.extend([16, 3])
+    assert width() == 1
+    c.extend([1, 1])
+    assert width() == 2
+    capturing = True
+    assert width() == 63
+    capturing = False
+    c.extend([200, 300])
+    assert width() == 19
+    c.batch_select_indices([0])
+    assert width() == 14
+    c.truncate(0, 0)
+    assert width() == 1
