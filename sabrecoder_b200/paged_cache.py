@@ -433,9 +433,8 @@ class SabrePagedKVCache(Cache):
         return new
 
     def crop(self, max_length: int) -> None:
-        top = max(self.lengths, default=0)
-        keep = max_length if max_length >= 0 else top + max_length
-        self._truncate({b: keep for b in range(self.batch_size)})
+        """Cuts every sequence to max_length rows; -n drops the last n of each."""
+        self._truncate({b: max_length if max_length >= 0 else n + max_length for b, n in enumerate(self.lengths)})
 
     def batch_select_indices(self, indices) -> None:
         """The sequences become copies (shared pages) of the listed ones."""

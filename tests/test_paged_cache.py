@@ -386,3 +386,18 @@ def test_attention_is_planned_by_the_rows_that_are_there(monkeypatch):
     assert width() == 14
     c.truncate(0, 0)
     assert width() == 1
+
+
+def test_crop_takes_the_last_rows_of_every_sequence():
+    c = cache(num_pages=30)
+    m = Mirror(c)
+    m.add([40, 7, 90])
+    c.crop(-10)
+    m.rows = [r[:max(0, len(r) - 10)] for r in m.rows]
+    assert c.lengths == [30, 0, 80]
+    m.check()
+    c.crop(50)
+    m.rows = [r[:50] for r in m.rows]
+    m.check()
+    c.crop(0)
+    assert c.lengths == [0, 0, 0] and c.pages_in_use == 0
