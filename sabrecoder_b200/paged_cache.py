@@ -172,6 +172,13 @@ class SabrePagedKVCache(Cache):
             if self.refs[page] == 0:
                 self.unused.append(page)
 
+    def _seq(self, seq: int) -> int:
+        """A sequence's index (from the end when negative)."""
+        n = self.batch_size
+        if not -n <= seq < n:
+            raise ValueError(f"SabrePagedKVCache has no sequence {seq} (it holds {n})")
+        return int(seq) % n
+
     @property
     def batch_size(self) -> int:
         return len(self.lengths)
@@ -242,6 +249,7 @@ class SabrePagedKVCache(Cache):
     def fork(self, src: int, dst: int) -> None:
         """Sequence ``dst`` gives its rows back and continues those of ``src``; the
         pages are shared until one of them writes."""
+        src, dst = self._seq(src), self._seq(dst)
         if src == dst:
             return
         for page in self.tables[src]:
@@ -254,7 +262,7 @@ class SabrePagedKVCache(Cache):
 
     def truncate(self, seq: int, length: int) -> None:
         """Drops the rows of a sequence from ``length`` on."""
-        self._truncate({seq: length})
+        self._truncate({self._seq(seq): length})
 
     def _truncate(self, lengths: Dict[int, int]) -> None:
         """{sequence: new length}; raises, changing nothing, where rows that the new
@@ -438,7 +446,9 @@ class SabrePagedKVCache(Cache):
 
     def batch_select_indices(self, indices) -> None:
         """The sequences become copies (shared pages) of the listed ones."""
-        idx = [int(i) for i in (indices.tolist() if isinstance(indices, torch.Tensor) else indices)]
+        idx = [self._seq(int(i)) for i in (indices.tolist() if isinstance(indices, torch.Tensor) else indices)]
+        if not idx:
+            raise ValueError("SabrePagedKVCache needs at least one sequence")
         for i in idx:
             for page in self.tables[i]:
                 if page >= 0:

@@ -401,3 +401,20 @@ def test_crop_takes_the_last_rows_of_every_sequence():
     m.check()
     c.crop(0)
     assert c.lengths == [0, 0, 0] and c.pages_in_use == 0
+
+
+@pytest.mark.parametrize("call", [lambda c: c.batch_select_indices([0, 3]), lambda c: c.reorder_cache(torch.tensor([1, 7, 0])),
+                                  lambda c: c.batch_select_indices([-4, 0]), lambda c: c.batch_select_indices([]),
+                                  lambda c: c.batch_repeat_interleave(0), lambda c: c.fork(0, 3), lambda c: c.fork(-4, 1),
+                                  lambda c: c.truncate(3, 0), lambda c: c.free(5)])
+def test_sequences_that_are_not_there_change_nothing(call):
+    c = cache(num_pages=20)
+    m = Mirror(c)
+    m.add([40, 16, 5])
+    c.fork(0, 2)
+    m.rows[2] = list(m.rows[0])
+    with pytest.raises((ValueError, IndexError), match="sequence"):
+        call(c)
+    m.check()
+    m.add([1, 2, 3])
+    m.check()
