@@ -354,13 +354,18 @@ class SabrePagedKVCache(Cache):
         if B != self.batch_size:
             raise ValueError(f"SabrePagedKVCache holds {self.batch_size} sequences (got rows of {B})")
         if layer.step == self.step:
+            pool = self.pool
+            for x in (k, v):  # before room is made for them
+                if x.shape != (B, n, pool.shape[3], pool.shape[5]) or x.dtype != pool.dtype or x.device != pool.device:
+                    raise ValueError(f"SabrePagedKVCache: rows {tuple(x.shape)} ({x.dtype}, {x.device}) for pages of "
+                                     f"{pool.shape[3]} heads of {pool.shape[5]} ({pool.dtype}, {pool.device})")
             self.extend([n] * B)
             self.step, self.step_rows = self.step + 1, n
         elif layer.step != self.step - 1 or n != self.step_rows:
             raise ValueError(f"SabrePagedKVCache: layer {layer_idx} is out of step")
-        layer.step = self.step
         K.paged_store(k.reshape(B * n, *k.shape[2:]), v.reshape(B * n, *v.shape[2:]), layer.k_pages, layer.v_pages,
                       self.page_table, self.seq_lens, self._row_starts(n))
+        layer.step = self.step
 
     def _row_starts(self, n: int) -> torch.Tensor:
         """Row starts of a step of n rows each. Kept while the number of sequences

@@ -418,3 +418,27 @@ def test_sequences_that_are_not_there_change_nothing(call):
     m.check()
     m.add([1, 2, 3])
     m.check()
+
+
+def test_refused_rows_leave_the_step_undone(monkeypatch):
+    """Rows that the store would refuse do not make room: the same step can be given
+    again."""
+    c = cache(batch_size=2, num_pages=20)
+    m = Mirror(c)
+    m.add([10, 3, 0][:2])
+    k = torch.randn(2, 4, H, D)
+    for kk, vv in ((k[:, :, :1], k[:, :, :1]), (k, k[:, :3]), (k.double(), k.double()), (k[..., :4], k[..., :4]),
+                   (k, k.double()), (k[:1], k[:1]), (k.to("meta"), k.to("meta"))):
+        with pytest.raises(ValueError, match="SabrePagedKVCache"):
+            c.append(0, kk, vv)
+        m.check()
+        assert (c.step, c.layers[0].step) == (0, 0)
+    c.append(0, k, -k)
+    c.append(1, k, -k)
+    assert c.lengths == [14, 7]
+    c.append(0, k, k)
+    monkeypatch.setattr(PC.K, "paged_store", lambda *a: (_ for _ in ()).throw(RuntimeError("refused")))
+    with pytest.raises(RuntimeError, match="refused"):
+        c.append(1, k, k)
+    monkeypatch.undo()
+    assert c.lengths == [18, 11] and (c.step, c.layers[1].step) == (2, 1)
