@@ -374,7 +374,7 @@ class SabrePagedKVCache(Cache):
         fills them on every replay, and to nobody else."""
         t = self._starts.get(n)
         if t is None:
-            t = torch.arange(0, n * self.batch_size + 1, n, dtype=torch.int32, device=self.pool.device)
+            t = torch.arange(self.batch_size + 1, dtype=torch.int32, device=self.pool.device) * n
             if not _capturing(self.pool):
                 self._starts[n] = t
         return t

@@ -442,3 +442,12 @@ def test_refused_rows_leave_the_step_undone(monkeypatch):
         c.append(1, k, k)
     monkeypatch.undo()
     assert c.lengths == [18, 11] and (c.step, c.layers[1].step) == (2, 1)
+
+
+def test_a_step_without_rows():
+    c = cache(batch_size=2)
+    k = torch.randn(2, 3, H, D)
+    for n in (3, 0, 1):
+        for i in (0, 1):
+            c.append(i, k[:, :n], k[:, :n])
+    assert c._row_starts(0).tolist() == [0, 0, 0] and c.lengths == [4, 4]
