@@ -172,6 +172,13 @@ class SabrePagedKVCache(Cache):
             if self.refs[page] == 0:
                 self.unused.append(page)
 
+    def _outside_captures(self) -> None:
+        """Tables and lengths change on the host and the device together: inside a
+        capture the device's part would only be recorded, and run at every replay."""
+        if _capturing(self.pool):
+            raise ValueError("SabrePagedKVCache: sequences do not change inside a capture (extend, and the like, go "
+                             "between replays; a captured step stores with paged_store)")
+
     def _seq(self, seq: int) -> int:
         """A sequence's index (from the end when negative)."""
         n = self.batch_size
@@ -193,6 +200,7 @@ class SabrePagedKVCache(Cache):
         """Makes room for ``new[b]`` more rows of each sequence (to be stored at
         its end). Raises ValueError, changing nothing, when a sequence or the
         pool is full."""
+        self._outside_captures()
         ps, w = self.page_size, self.window_size
         if len(new) != self.batch_size or min(new, default=0) < 0:
             raise ValueError(f"extend needs {self.batch_size} row counts >= 0")
@@ -249,6 +257,7 @@ class SabrePagedKVCache(Cache):
     def fork(self, src: int, dst: int) -> None:
         """Sequence ``dst`` gives its rows back and continues those of ``src``; the
         pages are shared until one of them writes."""
+        self._outside_captures()
         src, dst = self._seq(src), self._seq(dst)
         if src == dst:
             return
@@ -267,6 +276,7 @@ class SabrePagedKVCache(Cache):
     def _truncate(self, lengths: Dict[int, int]) -> None:
         """{sequence: new length}; raises, changing nothing, where rows that the new
         last row sees are dropped already."""
+        self._outside_captures()
         ps = self.page_size
         for b, length in lengths.items():
             lengths[b] = length = max(0, min(int(length), self.lengths[b]))
@@ -290,6 +300,7 @@ class SabrePagedKVCache(Cache):
     def compact(self) -> int:
         """Moves the live pages to the lowest places of the pool (all layers in one
         launch per 480 pages); returns how many moved."""
+        self._outside_captures()
         live = self.pages_in_use
         src = [p for p in range(live, self.num_pages) if self.refs[p]]
         dst = [p for p in range(live) if not self.refs[p]]
@@ -451,6 +462,7 @@ class SabrePagedKVCache(Cache):
 
     def batch_select_indices(self, indices) -> None:
         """The sequences become copies (shared pages) of the listed ones."""
+        self._outside_captures()
         idx = [self._seq(int(i)) for i in (indices.tolist() if isinstance(indices, torch.Tensor) else indices)]
         if not idx:
             raise ValueError("SabrePagedKVCache needs at least one sequence")

@@ -451,3 +451,22 @@ def test_a_step_without_rows():
         for i in (0, 1):
             c.append(i, k[:, :n], k[:, :n])
     assert c._row_starts(0).tolist() == [0, 0, 0] and c.lengths == [4, 4]
+
+
+@pytest.mark.parametrize("call", [lambda c: c.extend([1, 1, 1]), lambda c: c.fork(0, 1), lambda c: c.truncate(0, 3),
+                                  lambda c: c.compact(), lambda c: c.reorder_cache(torch.tensor([1, 0, 2])),
+                                  lambda c: c.crop(2), lambda c: c.reset(),
+                                  lambda c: c.append(0, torch.zeros(3, 1, H, D), torch.zeros(3, 1, H, D))])
+def test_the_host_state_does_not_change_inside_a_capture(monkeypatch, call):
+    """Inside a capture the device's tables and lengths are only recorded: the host's
+    would run ahead of them, and every replay would move them once more."""
+    c = cache(num_pages=20)
+    m = Mirror(c)
+    m.add([40, 16, 5])
+    c.free(1)
+    m.rows[1] = []
+    monkeypatch.setattr(PC, "_capturing", lambda pool: True)
+    with pytest.raises(ValueError, match="capture"):
+        call(c)
+    m.check()
+    assert c.step == 0
