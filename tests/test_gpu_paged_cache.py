@@ -300,3 +300,64 @@ def test_padded_batches_are_refused_and_plain_masks_are_not(cuda):
             b = model(input_ids=part, past_key_values=cb, use_cache=True).logits
             model.config._attn_implementation = "sdpa"
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("window,prefix", [(None, 0), (70, 20)])
+def test_captured_step_stores_new_rows_where_the_tables_now_say(cuda, window, prefix):
+    """Store and decode captured once: every replay writes the rows that k and v then
+    hold to the places that table and lengths then name, and nothing else; decode sees
+    them. Between replays extend takes pages, a sequence is forked, cut and the pool
+    compacted. A decode on another stream at the same time answers as it would alone."""
+    from sabrecoder_b200 import kernels as K
+    from sabrecoder_b200.paged_cache import SabrePagedKVCache
+    B, Hq, Hkv = 3, 8, 2
+    gen = torch.Generator().manual_seed(21)
+    c = SabrePagedKVCache(batch_size=B, max_seq_len=400, num_pages=60, page_size=16, num_layers=1, num_kv_heads=Hkv,
+                          head_dim=D, window_size=window, num_prefix_tokens=prefix)
+    layer = c.layers[0]
+
+    def rand(*shape):
+        return torch.randn(*shape, generator=gen).to(BF).cuda()
+
+    c.pool.copy_(rand(*c.pool.shape))
+    k, v, q = rand(B, Hkv, D), rand(B, Hkv, D), rand(B, Hq, D)
+    c.extend([100, 31, 203])
+    c.extend([1, 1, 1])
+    K.paged_store(k, v, layer.k_pages, layer.v_pages, c.page_table, c.seq_lens)
+    c.decode(0, q)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(ValueError, match="capture"):
+            c.append(0, k[:, None], v[:, None])
+        K.paged_store(k, v, layer.k_pages, layer.v_pages, c.page_table, c.seq_lens)
+        out = c.decode(0, q)
+    side = torch.cuda.Stream()
+    for step in range(20):
+        if step == 5:
+            c.fork(2, 0)
+        if step == 9:
+            c.truncate(1, 3)
+        if step == 12:
+            c.compact()
+        c.extend([1, 1, 1])
+        for t in (k, v, q):
+            t.copy_(rand(*t.shape))
+        out.fill_(9.0)
+        table = c.page_table
+        want = c.pool.clone()
+        placed = PO.slots(table, c.seq_lens, None, 16, c.num_pages)
+        assert len(placed) == B and len({p[1:] for p in placed}) == B
+        for r, page, off in placed:
+            want[0, 0, page, :, off], want[0, 1, page, :, off] = k[r], v[r]
+        # Another decode meanwhile, over a copy of the pool and all rows but the last.
+        before = (c.seq_lens - 1).clamp(min=0)
+        torch.cuda.synchronize()
+        graph.replay()
+        with torch.cuda.stream(side):
+            beside = K.paged_decode(q, want[0, 0], want[0, 1], table, before)
+        torch.cuda.synchronize()
+        assert torch.equal(c.pool, want)
+        check(out, (q, want[0, 0], want[0, 1], table, c.seq_lens, None), window, prefix)
+        check(beside, (q, want[0, 0], want[0, 1], table, before, None))
+    assert K.device_status(clear=True) == 0
