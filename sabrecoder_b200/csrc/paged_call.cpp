@@ -6,8 +6,9 @@
 // copy; here 5.1, 8.5, 5.0 and 4.5, of which a launch is 2.
 //
 // Every function returns None when an argument is not what the kernels take
-// (kernels.py then raises with what is wrong), an int status when the C entry
-// refused or failed (kernels.py raises with its message), else the result.
+// (kernels.py then raises with what is wrong), a negative int, the status, when
+// the C entry refused or failed (kernels.py raises with its message), else the
+// number of kernels launched, attend behind its result.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -85,7 +86,11 @@ float number(PyObject* o) {
   return static_cast<float>(x);
 }
 
-// store(k, v, k_pages, v_pages, page_table, seq_lens, q_start) -> 0
+PyObject* launched(int status, int64_t kernels) { return PyLong_FromLongLong(status == SABRE_OK ? kernels : status); }
+
+PyObject* result(const at::Tensor& out, int kernels) { return Py_BuildValue("Ni", THPVariable_Wrap(out), kernels); }
+
+// store(k, v, k_pages, v_pages, page_table, seq_lens, q_start) -> kernels
 PyObject* store(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Pages p;
@@ -97,15 +102,16 @@ PyObject* store(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (rows == 0 || p.batch == 0) return PyLong_FromLong(0);
   const int64_t kr[2] = {k->stride(0), k->stride(1)}, vr[2] = {v->stride(0), v->stride(1)};
   const c10::cuda::CUDAGuard guard(p.dev);
-  return PyLong_FromLong(sabre_paged_store(
-      k->const_data_ptr(), v->const_data_ptr(), p.k->data_ptr(), p.v->data_ptr(), p.i32(p.table), p.i32(p.lens),
-      p.i32(p.starts), rows, p.batch, p.heads, p.dim, p.pages, p.page_size, p.cols, kr, vr, p.ks, p.vs,
-      p.table->stride(0), p.dtype, c10::cuda::getCurrentCUDAStream(p.dev).stream()));
+  return launched(sabre_paged_store(k->const_data_ptr(), v->const_data_ptr(), p.k->data_ptr(), p.v->data_ptr(),
+                                    p.i32(p.table), p.i32(p.lens), p.i32(p.starts), rows, p.batch, p.heads, p.dim,
+                                    p.pages, p.page_size, p.cols, kr, vr, p.ks, p.vs, p.table->stride(0), p.dtype,
+                                    c10::cuda::getCurrentCUDAStream(p.dev).stream()),
+                  1);
   END_HANDLE_TH_ERRORS
 }
 
-// attend(q, k_pages, v_pages, page_table, seq_lens, q_start, window, prefix, scale, out, workspace) -> out;
-// decode without q_start.
+// attend(q, k_pages, v_pages, page_table, seq_lens, q_start, window, prefix, scale, out, workspace) ->
+// (out, kernels); decode without q_start.
 PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Pages p;
@@ -122,7 +128,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   const c10::cuda::CUDAGuard guard(p.dev);
   if (!out.defined()) out = at::empty(q->sizes(), q->options());
-  if (q->numel() == 0 || p.batch == 0) return THPVariable_Wrap(out);
+  if (q->numel() == 0 || p.batch == 0) return result(out, 0);
   const int rows = q->size(0), heads_q = q->size(1);
   const size_t need = p.starts ? sabre_paged_prefill_workspace_size(rows, p.batch, heads_q, p.heads, p.dim,
                                                                     p.page_size, p.cols, window, prefix)
@@ -148,11 +154,14 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                     p.page_size, p.cols, window, prefix, qr, p.ks, p.vs, orr, p.table->stride(0),
                                     scale, p.dtype, wp, wb, stream);
   if (st != SABRE_OK) return PyLong_FromLong(st);
-  return THPVariable_Wrap(out);
+  // Parts are joined by a second kernel: in prompts that run in shares, which is
+  // when they ask for a workspace; in decodes over more than one key tile.
+  const bool joined = p.starts ? need > 0 : p.batch > 1 || p.heads > 1 || int64_t{p.cols} * p.page_size > 64;
+  return result(out, joined ? 2 : 1);
   END_HANDLE_TH_ERRORS
 }
 
-// copy(pages, src, dst) -> 0; src and dst lists of ints.
+// copy(pages, src, dst) -> kernels; src and dst lists of ints.
 PyObject* copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   const at::Tensor* t = n == 3 ? tensor(a[0]) : nullptr;
@@ -182,10 +191,10 @@ PyObject* copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
   }
   if (t->numel() == 0 || moves == 0) return PyLong_FromLong(0);
   const c10::cuda::CUDAGuard guard(t->get_device());
-  return PyLong_FromLong(sabre_copy_pages(t->data_ptr(), static_cast<int>(buffers), step * es,
-                                          static_cast<int>(pages), t->stride(d - 4) * es, unit * es, ids.data(),
-                                          ids.data() + moves, static_cast<int>(moves),
-                                          c10::cuda::getCurrentCUDAStream(t->get_device()).stream()));
+  return launched(sabre_copy_pages(t->data_ptr(), static_cast<int>(buffers), step * es, static_cast<int>(pages),
+                                   t->stride(d - 4) * es, unit * es, ids.data(), ids.data() + moves,
+                                   static_cast<int>(moves), c10::cuda::getCurrentCUDAStream(t->get_device()).stream()),
+                  (moves + 479) / 480);
   END_HANDLE_TH_ERRORS
 }
 

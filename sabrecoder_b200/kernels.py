@@ -607,8 +607,9 @@ def _attend(what: str, q, k_pages, v_pages, page_table, seq_lens, q_start, windo
         _paged_refuse(what, k_pages, v_pages, page_table, seq_lens, q_start, dict(q=q, out=out), workspace)
     if type(res) is int:
         check(res, "sabre_" + what)
-    LAUNCHES[0] += 2  # and the joining of parts, where there may be some
-    return res
+    out, kernels = res
+    LAUNCHES[0] += kernels
+    return out
 
 
 def paged_store(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
@@ -624,8 +625,9 @@ def paged_store(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages
     st = paged_call().store(k, v, k_pages, v_pages, page_table, seq_lens, q_start)
     if st is None:
         _paged_refuse("paged_store", k_pages, v_pages, page_table, seq_lens, q_start, dict(k=k, v=v))
-    check(st, "sabre_paged_store")
-    LAUNCHES[0] += 1
+    if st < 0:
+        check(st, "sabre_paged_store")
+    LAUNCHES[0] += st
 
 
 def paged_decode(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
@@ -685,5 +687,6 @@ def copy_pages(pages: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -> N
                 raise SabreError(f"copy_pages: page {page} is outside the pool of {pages.shape[-4]} pages")
         _need_cuda(pages=pages)
         raise SabreError("copy_pages: each page [Hkv, page_size, D] must be contiguous, and the pools at one stride")
-    check(st, "sabre_copy_pages")
-    LAUNCHES[0] += -(-len(src) // 480)
+    if st < 0:
+        check(st, "sabre_copy_pages")
+    LAUNCHES[0] += st

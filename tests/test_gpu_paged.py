@@ -558,3 +558,40 @@ def test_rows_before_their_sequence_under_the_widest_windows(K, window, extra_co
     assert (out[:30] == 0).all() and (out[30:40] != 0).any(-1).all()
     check(out, args, window, starts=starts)
     assert K.device_status(clear=True) == 0
+
+
+def test_launches_are_counted_as_they_are(K):
+    """LAUNCHES grows by the kernels of a call: those of its captured graph."""
+    from cuda.bindings import runtime
+
+    def kernels(call):
+        graph = torch.cuda.CUDAGraph(keep_graph=True)
+        before = K.LAUNCHES[0]
+        with torch.cuda.graph(graph):
+            call()
+        counted = K.LAUNCHES[0] - before
+        err, _, n = runtime.cudaGraphGetNodes(graph.raw_cuda_graph())
+        assert err == runtime.cudaError_t.cudaSuccess
+        assert counted == n
+        return n
+
+    def one(lens, news, Hq, Hkv, ps, extra_cols=0):
+        return make(22, lens, news, Hq, Hkv, ps, BF, extra_cols=extra_cols)
+
+    q, kp, vp, table, sl, starts = one([1], [1], 2, 1, 16)
+    assert kernels(lambda: K.paged_decode(q, kp, vp, table, sl)) == 1
+    assert kernels(lambda: K.paged_store(q[:, :1], q[:, 1:], kp, vp, table, sl)) == 1
+    assert kernels(lambda: K.copy_pages(kp, [0, 1], [2, 3])) == 1
+    assert kernels(lambda: K.copy_pages(kp, [], [])) == 0
+    none, zero = table[:0], torch.zeros(1, dtype=torch.int32, device="cuda")
+    assert kernels(lambda: K.paged_decode(q[:0], kp, vp, none, sl[:0])) == 0
+    assert kernels(lambda: K.paged_prefill(q[:0], kp, vp, none, sl[:0], zero)) == 0
+    assert kernels(lambda: K.paged_store(q[:0, :1], q[:0, :1], kp, vp, none, sl[:0], zero)) == 0
+    pool = torch.zeros(2000, 1, 16, D, device="cuda", dtype=BF)
+    assert kernels(lambda: K.copy_pages(pool, list(range(961)), list(range(1000, 1961)))) == 3
+    for shape in (([70], [1], 2, 1, 16), ([9, 5], [1, 1], 2, 1, 16), ([9], [1], 2, 2, 16)):
+        q, kp, vp, table, sl, starts = one(*shape)
+        assert kernels(lambda: K.paged_decode(q, kp, vp, table, sl)) == 2
+    for shape, n in ((([300], [300], 2, 1, 16), 1), (([9000], [20], 2, 2, 64), 2), (([100], [100], 2, 1, 16, 200), 2)):
+        q, kp, vp, table, sl, starts = one(*shape)
+        assert kernels(lambda: K.paged_prefill(q, kp, vp, table, sl, starts)) == n
