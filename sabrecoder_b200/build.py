@@ -57,13 +57,18 @@ def _run(cmd, tmp: str, out: str, verbose: bool) -> None:
 
 
 def build_call(force: bool = False, verbose: bool = False) -> str:
-    """The torch extension; linked to libsabre_b200.so beside it."""
-    if not force and os.path.exists(CALL) and all(os.path.getmtime(f) <= os.path.getmtime(CALL)
-                                                  for f in (CALL_SOURCE, HEADER)):
-        return CALL
+    """The torch extension; linked to libsabre_b200.so beside it. It holds torch's and
+    Python's ABI, so the file beside it says which ones it was built for."""
     import sysconfig
 
     import torch
+    stamp = CALL + ".for"
+    key = f"torch {torch.__version__} python {sys.version}"
+    if not force and os.path.exists(CALL) and os.path.exists(stamp):
+        with open(stamp) as f:
+            same = f.read() == key
+        if same and all(os.path.getmtime(f) <= os.path.getmtime(CALL) for f in (CALL_SOURCE, HEADER)):
+            return CALL
     home = os.path.dirname(torch.__file__)
     inc = [os.path.join(home, "include"), os.path.join(home, "include", "torch", "csrc", "api", "include"),
            sysconfig.get_paths()["include"], os.path.join(os.path.dirname(os.path.dirname(nvcc())), "include")]
@@ -72,6 +77,8 @@ def build_call(force: bool = False, verbose: bool = False) -> str:
           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in inc), CALL_SOURCE,
           "-o", tmp, f"-L{PKG}", "-l:" + os.path.basename(LIB), f"-L{os.path.join(home, 'lib')}", "-lc10",
           "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_python", "-Wl,-rpath,$ORIGIN"], tmp, CALL, verbose)
+    with open(stamp, "w") as f:
+        f.write(key)
     return CALL
 
 
