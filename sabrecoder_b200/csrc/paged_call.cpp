@@ -12,6 +12,7 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <ATen/MemoryOverlap.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -123,7 +124,7 @@ PyObject* attend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   at::Tensor out, ws;
   if (a[9] != Py_None) {
     const at::Tensor* o = tensor(a[9]);
-    if (!p.rows(o) || o->sizes() != q->sizes()) Py_RETURN_NONE;
+    if (!p.rows(o) || o->sizes() != q->sizes() || at::has_internal_overlap(*o) == at::MemOverlap::Yes) Py_RETURN_NONE;
     out = *o;
   }
   const c10::cuda::CUDAGuard guard(p.dev);

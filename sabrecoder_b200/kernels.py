@@ -568,6 +568,9 @@ def _paged_refuse(what: str, k_pages, v_pages, page_table, seq_lens, q_start, ro
                              f"stride")
         if t is not None and t.dtype != k_pages.dtype:
             raise SabreError(f"{what}: {name} is {t.dtype}, the pages are {k_pages.dtype}")
+    out = rows.get("out")
+    if out is not None and any(n > 1 and st == 0 for n, st in zip(out.shape, out.stride())):
+        raise SabreError(f"{what}: rows or heads of out overlap (strides {out.stride()})")
     if k_pages.dtype not in DTYPE_CODE or v_pages.dtype != k_pages.dtype:
         raise SabreError(f"{what}: pages must share dtype bf16 or f16 (got {k_pages.dtype}, {v_pages.dtype})")
     if k_pages.stride(3) != 1 or v_pages.stride(3) != 1:

@@ -595,3 +595,17 @@ def test_launches_are_counted_as_they_are(K):
     for shape, n in ((([300], [300], 2, 1, 16), 1), (([9000], [20], 2, 2, 64), 2), (([100], [100], 2, 1, 16, 200), 2)):
         q, kp, vp, table, sl, starts = one(*shape)
         assert kernels(lambda: K.paged_prefill(q, kp, vp, table, sl, starts)) == n
+
+
+def test_outputs_that_overlap_themselves_are_refused(K):
+    q, kp, vp, table, sl, starts = make(23, [20, 9], [1, 1], 4, 2, 16, BF)
+    for out in (q[:1].clone().expand(2, 4, D), q[:, :1].clone().expand(2, 4, D)):
+        before = out.clone()
+        with pytest.raises(K.SabreError, match="overlap"):
+            K.paged_decode(q, kp, vp, table, sl, out=out)
+        with pytest.raises(K.SabreError, match="overlap"):
+            K.paged_prefill(q, kp, vp, table, sl, starts, out=out)
+        assert torch.equal(out, before)
+    one = torch.empty(1, 4, D, dtype=BF, device="cuda").expand(1, 4, D)  # a size of one repeats nothing
+    K.paged_decode(q[:1], kp, vp, table[:1], sl[:1], out=one)
+    check(one, (q[:1], kp, vp, table[:1], sl[:1], None))

@@ -206,3 +206,13 @@ def test_prompts_whose_key_tiles_pass_int32_do_not_run_in_shares():
     assert size(128 * 16, 1024, 1 << 20) == 0 and size(148 * 16, 1024, 1 << 20) == 0
     assert size(148 * 16, 1024, 1 << 19) > 0
     assert size(147, 1024, 1 << 20, batch=128) == 0
+
+
+def test_outputs_that_overlap_themselves_are_refused():
+    """Rows or heads of an expanded output would be written by several CTAs at once."""
+    row = torch.zeros(1, 4, D, dtype=torch.bfloat16).expand(3, 4, D)
+    head = torch.zeros(3, 1, D, dtype=torch.bfloat16).expand(3, 4, D)
+    for call in (decode, prefill):
+        for out in (row, head):
+            with pytest.raises(_lib.SabreError, match="overlap"):
+                call(args(), out=out)
