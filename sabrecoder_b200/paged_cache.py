@@ -340,6 +340,8 @@ class SabrePagedKVCache(Cache):
 
     def _mask_fits(self, mask: torch.Tensor, n: int) -> bool:
         top = max(self.lengths)
+        if not isinstance(mask, torch.Tensor):
+            return False
         if mask.shape[-1] < top + n or mask.dim() not in (2, 4) or (mask.dim() == 4 and mask.shape[2] != n):
             return False
         see = (mask == 0 if mask.is_floating_point() and mask.dim() == 4 else mask != 0)[..., :top + n]

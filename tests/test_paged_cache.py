@@ -470,3 +470,9 @@ def test_the_host_state_does_not_change_inside_a_capture(monkeypatch, call):
         call(c)
     m.check()
     assert c.step == 0
+
+
+def test_masks_that_are_not_tensors_are_refused():
+    c = cache(batch_size=2)
+    with pytest.raises(ValueError, match="mask"):
+        c.check_step(0, 4, None, {"full_attention": None})
