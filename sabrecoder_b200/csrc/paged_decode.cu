@@ -26,7 +26,7 @@
 // mma.sync is used rather than tcgen05: at the HBM rate the matrix work keeps
 // the tensor pipe busy a tenth of the time (ncu), and there is no tensor memory
 // to allocate, fill and read back per segment. 32 sequences of 1..16384 rows at
-// 56/8 heads (917 MB) take 143 us, 6.4 TB/s.
+// 56/8 heads (917 MB) take 145 us, 6.3 TB/s.
 // P is rounded to the type of V for the product (half a step of a weight,
 // below the rounding of the output); scores, sums and acc are fp32.
 namespace sabre {
@@ -567,8 +567,9 @@ __global__ void __launch_bounds__(kDecThreads, 2)
 // parts, up to four) take the parts in turn, four columns a lane and eight
 // parts in flight; the warps' sums are then added in order, so the result is
 // the same every time. A CTA for each head rather than a warp of one CTA: 12289
-// rows at 56/8 heads (37 parts a pair) take 13.2 us a call instead of 16.5,
-// 300 rows at 16/16 heads 6.6 instead of 7.0; the batches run alike.
+// rows at 56/8 heads (37 parts a pair; 50 MB that stay in L2 from call to call)
+// take 13.2 us a call instead of 16.5, 300 rows at 16/16 heads 6.6 instead of
+// 7.0; the batches run alike.
 constexpr int kJoinWarps = 4;
 template <typename T>
 __global__ void __launch_bounds__(kJoinWarps * 32) paged_join_kernel(const DecodeParams p) {

@@ -10,8 +10,8 @@
 // that a group's heads share each K/V tile, a short continuation fills its
 // rows, and a window's span grows by fewer tokens. Its key tiles (64 keys) are
 // the prefix tiles, then those of the window: nothing else is visited. Many
-// (row tile, KV head) pairs run as one CTA each, heaviest first. When there are
-// too few of them to fill the card evenly, and they are long, their key tiles
+// (row tile, KV head) pairs run as one CTA each, in the batch's reverse order and
+// so heaviest first within a sequence. When there are too few of them to fill the card evenly, and they are long, their key tiles
 // are dealt out to two CTAs per SM instead (kShares, see RowShares): a CTA
 // walks its share as segments, a pair inside one share is finished there, the
 // others leave (m, l, O) per row and paged_combine_kernel adds them in share
@@ -23,15 +23,18 @@
 // producer, 5 MMA issuer, 6 V producer; S = Q K^T of M=128 N=64 into two
 // buffers, P over its S, O += P V with P from tensor memory); from one segment
 // of a share to the next each role goes on by itself (model-checked:
-// tests/test_paged_prefill_protocol.py). Different here: tiles come box by box from pages (a TMA
+// tests/test_paged_prefill_protocol.py, the V tiles below in
+// tests/test_paged_prefill_zeroing_protocol.py). Different here: tiles come box by box from pages (a TMA
 // box is min(page_size, 64) rows; absent pages and boxes that no row sees are
 // read outside the pool and give zeros), and V rows that none of the CTA's rows
 // sees (past the sequence's end, before the window) are zeroed in shared memory
 // before their tile is handed to the MMA, since 0 * NaN would reach the result.
 // P is rounded to the type of V for the product; scores, sums and O are fp32.
-// A 12288-row prompt at 16/16 heads takes 553 us (1.12 PFLOP/s): neither the
-// tensor pipe nor the exponential unit is busy more than about half the time,
-// the softmax warps' own latencies bound each CTA's chain.
+// A 12288-row prompt at 16/16 heads takes 555 us (1.11 PFLOP/s) in bursts of
+// replays and 650 us (950 TFLOP/s) in a loop that holds the card at its power
+// cap; the times in the comments below are of bursts. Neither the tensor pipe nor
+// the exponential unit is busy more than about half the time: what bounds a CTA
+// is its chain from S over the softmax to P.V.
 namespace sabre {
 namespace paged {
 namespace pre {
@@ -400,7 +403,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     some = find_share<T>(p, seq, scratch, sh, at);
     if (some) units = sh.units;
   } else {
-    // Later row tiles of a sequence see more keys: heaviest first. Row-major
+    // Later row tiles of a sequence see more keys: its heaviest first (sequences
+    // come in the batch's reverse order, whatever their lengths). Row-major
     // (grid x = head) or head-major (grid x = row tile), as in prefill_bsa.cu.
     hk = p.head_major ? static_cast<int>(blockIdx.y) : static_cast<int>(blockIdx.x);
     some = find_job(p, p.slots - 1 - static_cast<int>(p.head_major ? blockIdx.x : blockIdx.y), scratch, job);
@@ -845,7 +849,10 @@ static inline long long row_slots(int rows, int batch, int tokens) {
 
 // Whether a call runs in shares, as far as the host can tell: by the pairs (row
 // tile, KV head) there may be and the key tiles of one, counted for a row tile
-// in the middle of its sequence's new rows. Where a pair can be cut in k >= 2
+// in the middle of its sequence's new rows. The table's width stands for the
+// sequences' length, so callers pass the columns in use: with the table of a
+// 16384-row cache 1280 fresh rows at 32/32 heads take 66 us instead of 24, 256 on
+// 1000 at 56/8 31.5 instead of 19.6. Where a pair can be cut in k >= 2
 // parts, when that saves it 13 tiles or more: less does not pay for the larger
 // start and the joining. Else equal shares fill the places that the last pairs
 // leave empty (counted for the pairs there are when row tiles end anywhere),
