@@ -195,7 +195,7 @@ PyObject* copy(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return launched(sabre_copy_pages(t->data_ptr(), static_cast<int>(buffers), step * es, static_cast<int>(pages),
                                    t->stride(d - 4) * es, unit * es, ids.data(), ids.data() + moves,
                                    static_cast<int>(moves), c10::cuda::getCurrentCUDAStream(t->get_device()).stream()),
-                  (moves + 479) / 480);
+                  (moves + 479) / 480);  // 480 moves travel with a launch
   END_HANDLE_TH_ERRORS
 }
 
