@@ -10,13 +10,14 @@
 // that a group's heads share each K/V tile, a short continuation fills its
 // rows, and a window's span grows by fewer tokens. Its key tiles (64 keys) are
 // the prefix tiles, then those of the window: nothing else is visited. Many
-// (row tile, KV head) pairs run as one CTA each, in the batch's reverse order and
-// so heaviest first within a sequence. When there are too few of them to fill the card evenly, and they are long, their key tiles
-// are dealt out to two CTAs per SM instead (kShares, see RowShares): a CTA
-// walks its share as segments, a pair inside one share is finished there, the
-// others leave (m, l, O) per row and paged_combine_kernel adds them in share
-// order. Sequences, lengths and pages are only read on the
-// device, so a captured call follows them.
+// (row tile, KV head) pairs run as one CTA each, in the batch's reverse order
+// and so heaviest first within a sequence. When there are too few of them to
+// fill the card evenly, and they are long, their key tiles are dealt out to two
+// CTAs per SM instead (kShares, see RowShares): a CTA walks its share as
+// segments, a pair inside one share is finished there, the others leave (m, l,
+// O) per row and paged_combine_kernel adds them in share order. Sequences,
+// lengths and pages are only read on the device, so a captured call follows
+// them.
 //
 // Roles, tensor-memory layout and barrier protocol are those of
 // prefill_bsa.cu (224 threads, two CTAs per SM: warps 0-3 softmax, 4 Q and K
@@ -24,11 +25,12 @@
 // buffers, P over its S, O += P V with P from tensor memory); from one segment
 // of a share to the next each role goes on by itself (model-checked:
 // tests/test_paged_prefill_protocol.py, the V tiles below in
-// tests/test_paged_prefill_zeroing_protocol.py). Different here: tiles come box by box from pages (a TMA
-// box is min(page_size, 64) rows; absent pages and boxes that no row sees are
-// read outside the pool and give zeros), and V rows that none of the CTA's rows
-// sees (past the sequence's end, before the window) are zeroed in shared memory
-// before their tile is handed to the MMA, since 0 * NaN would reach the result.
+// tests/test_paged_prefill_zeroing_protocol.py). Different here: tiles come box
+// by box from pages (a TMA box is min(page_size, 64) rows; absent pages and
+// boxes that no row sees are read outside the pool and give zeros), and V rows
+// that none of the CTA's rows sees (past the sequence's end, before the window)
+// are zeroed in shared memory before their tile is handed to the MMA, since 0 *
+// NaN would reach the result.
 // P is rounded to the type of V for the product; scores, sums and O are fp32.
 // A 12288-row prompt at 16/16 heads takes 555 us (1.11 PFLOP/s) in bursts of
 // replays and 650 us (950 TFLOP/s) in a loop that holds the card at its power

@@ -332,8 +332,8 @@ def test_masks_that_say_more_than_the_cache_are_refused():
     for ok in (None, good, good[:1], added(good), added(good).expand(2, H, 4, 24), torch.ones(2, 24, dtype=torch.long),
                torch.nn.functional.pad(good, (0, 8))):
         c.check_step(0, 4, ids, ok)
-    for wrong in (left, right, future, bias, added(left), added(future), pad, pad.bool(), causal(window=10), good[..., :20],
-                  good[0, 0], good[:, 0]):
+    for wrong in (left, right, future, bias, added(left), added(future), pad, pad.bool(), causal(window=10),
+                  good[..., :20], good[0, 0], good[:, 0]):
         with pytest.raises(ValueError, match="mask"):
             c.check_step(0, 4, ids, wrong)
     w = cache(batch_size=2, window_size=10)
@@ -403,9 +403,11 @@ def test_crop_takes_the_last_rows_of_every_sequence():
     assert c.lengths == [0, 0, 0] and c.pages_in_use == 0
 
 
-@pytest.mark.parametrize("call", [lambda c: c.batch_select_indices([0, 3]), lambda c: c.reorder_cache(torch.tensor([1, 7, 0])),
+@pytest.mark.parametrize("call", [lambda c: c.batch_select_indices([0, 3]),
+                                  lambda c: c.reorder_cache(torch.tensor([1, 7, 0])),
                                   lambda c: c.batch_select_indices([-4, 0]), lambda c: c.batch_select_indices([]),
-                                  lambda c: c.batch_repeat_interleave(0), lambda c: c.fork(0, 3), lambda c: c.fork(-4, 1),
+                                  lambda c: c.batch_repeat_interleave(0), lambda c: c.fork(0, 3),
+                                  lambda c: c.fork(-4, 1),
                                   lambda c: c.truncate(3, 0), lambda c: c.free(5)])
 def test_sequences_that_are_not_there_change_nothing(call):
     c = cache(num_pages=20)

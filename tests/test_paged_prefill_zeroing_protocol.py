@@ -81,7 +81,7 @@ def test_zeroed_tiles_never_deadlock_or_reorder(monkeypatch, first):
 
 @pytest.mark.parametrize("flaw,what", [("phases restart", ("violation", "deadlock")), ("zeroed unseen", ("violation",)),
                                        ("handed over first", ("violation",))])
-def test_the_checker_catches(monkeypatch, flaw, what):
+def test_a_planted_mistake_is_caught(monkeypatch, flaw, what):
     rnd = random.Random(0)
     shapes = [tuple(rnd.randint(1, 5) for _ in range(3)) for _ in range(20)]
     results = set(_results(monkeypatch, shapes, 25, flaw).values())
