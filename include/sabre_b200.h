@@ -40,7 +40,8 @@ enum { SABRE_BF16 = 0, SABRE_F16 = 1, SABRE_F32 = 2 /* sabre_chunk_vectors embed
 enum {
   SABRE_DEV_TIMEOUT = 1u,
   SABRE_DEV_BAD_SMEM_ALIGN = 2u,
-  SABRE_DEV_BAD_PAGE = 4u /* a paged entry met a position or page outside the table or the pool */
+  SABRE_DEV_BAD_PAGE = 4u, /* a paged entry met a position or page outside the table or the pool */
+  SABRE_DEV_NO_ROOM = 8u   /* sabre_paged_extend found no room and changed nothing */
 };
 
 int sabre_version(void);
@@ -448,6 +449,91 @@ int sabre_paged_prefill(const void* q, const void* k_pages, const void* v_pages,
                         float softmax_scale, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 int sabre_copy_pages(void* pages, int buffers, int64_t buffer_stride, int num_pages, int64_t page_stride,
                      int64_t page_bytes, const int32_t* src, const int32_t* dst, int moves, void* stream);
+
+/* --------------------------------------------------------------------------
+ * (5) Paged K/V cache: steps without the host, and attention over selected
+ * pages. Tables, lengths, row starts and pools as in (4).
+ *
+ * sabre_paged_extend: block tables and slot maps from request lengths. The
+ *   sequences grow by new_rows [batch] (>= 0): the i-th page that they need,
+ *   by sequence and then position, is free_pages[free_count[0] - 1 - i] of a
+ *   stack of free_size entries, and goes to its column of page_table.
+ *   seq_lens_out, free_count_out [1]: the new lengths and count (may be the
+ *   old ones' buffers; seq_lens_out may not be new_rows). q_start [batch + 1]:
+ *   row starts of the new rows. For row r of `rows` (>= their number):
+ *   slots[r] = page * page_size + row of the page, positions[r] its position;
+ *   -1 and 0 for rows past the last, and slot -1 for rows whose page is absent
+ *   or outside the pool (the latter recorded as SABRE_DEV_BAD_PAGE; its table
+ *   entry becomes -1). When the pages, a table row or the `rows` are too few,
+ *   or a length is negative, nothing changes, all starts are 0, all slots -1
+ *   and SABRE_DEV_NO_ROOM is recorded. At most 16384 sequences and 2^30 rows.
+ * sabre_paged_store_slots: rows k, v [rows, Hkv, D] into the places slots[r] =
+ *   page * page_size + row of the page; a negative slot drops its row, one past
+ *   the pool too and records SABRE_DEV_BAD_PAGE. No slot may be given twice.
+ * sabre_paged_key_means: key_means [num_pages, Hkv, D] fp32 (strides
+ *   km_strides = {page, head}, positive multiples of 4; 16-byte aligned): the
+ *   mean key of every page that the new rows (already stored) fill; other pages
+ *   stay. q_start NULL: one new row per sequence (rows == batch).
+ * Query blocks: each sequence's new rows in blocks of up to query_block, numbered
+ *   over the batch; sabre_paged_query_blocks(...) of them at most (batch blocks
+ *   of one row without q_start).
+ * sabre_paged_select: for each query block and KV head the table columns it
+ *   reads: those of the first num_prefix_tokens tokens, those that hold a key at
+ *   most `window` before one of the block's queries, its own included, and the
+ *   topk best of the others by (sum of the block's q over rows and heads of the
+ *   group) . key_means[page]; ties to the lower column, NaN last. Sums are 64
+ *   bits wide, a score is rounded to fp32 once. Absent pages are not listed.
+ *   lists int32 [blocks, Hkv, width] (contiguous, ascending, -1 behind the
+ *   end), width = sabre_paged_select_width(...); counts int32 [blocks, Hkv]. All
+ *   entries are written; blocks past the last have none. At most 32768 columns,
+ *   query_block <= 1024.
+ * sabre_paged_decode_listed / sabre_paged_prefill_listed: sabre_paged_decode /
+ *   _prefill over listed pages: key j is visible to the query at position i
+ *   when j <= i and its column is in the block's list. lists, counts: element
+ *   strides {block, head}, 0 = shared; list_entries: entries of a list. Lists
+ *   ascend: an entry that is not above the one before it is skipped, as is one
+ *   outside the table (recorded as SABRE_DEV_BAD_PAGE). query_block times
+ *   heads_q / heads_kv <= 128; rows of a block that see nothing are zero, rows
+ *   from q_start[batch] on are left. Decode's workspace:
+ *   sabre_paged_decode_workspace_size.
+ * ---------------------------------------------------------------------- */
+int sabre_paged_extend(const int32_t* new_rows, int32_t* page_table, const int32_t* seq_lens, int32_t* seq_lens_out,
+                       const int32_t* free_pages, const int32_t* free_count, int32_t* free_count_out,
+                       int32_t* q_start, int64_t* slots, int64_t* positions, int rows, int batch, int num_pages,
+                       int page_size, int max_pages, int free_size, int64_t table_stride, void* stream);
+int sabre_paged_store_slots(const void* k, const void* v, void* k_pages, void* v_pages, const int64_t* slots, int rows,
+                            int heads_kv, int head_dim, int num_pages, int page_size, const int64_t* k_strides,
+                            const int64_t* v_strides, const int64_t* kp_strides, const int64_t* vp_strides, int dtype,
+                            void* stream);
+int sabre_paged_key_means(const void* k_pages, float* key_means, const int32_t* page_table, const int32_t* seq_lens,
+                          const int32_t* q_start, int rows, int batch, int heads_kv, int head_dim, int num_pages,
+                          int page_size, int max_pages, const int64_t* kp_strides, const int64_t* km_strides,
+                          int64_t table_stride, int dtype, void* stream);
+int sabre_paged_query_blocks(int rows, int batch, int query_block);
+int sabre_paged_select_width(int page_size, int max_pages, int topk, int query_block, int window,
+                             int num_prefix_tokens);
+int sabre_paged_select(const void* q, const float* key_means, const int32_t* page_table, const int32_t* seq_lens,
+                       const int32_t* q_start, int32_t* lists, int32_t* counts, int rows, int batch, int heads_q,
+                       int heads_kv, int head_dim, int num_pages, int page_size, int max_pages, int topk,
+                       int query_block, int window, int num_prefix_tokens, const int64_t* q_strides,
+                       const int64_t* km_strides, int64_t table_stride, int dtype, void* stream);
+int sabre_paged_decode_listed(const void* q, const void* k_pages, const void* v_pages, void* o,
+                              const int32_t* page_table, const int32_t* seq_lens, const int32_t* lists,
+                              const int32_t* counts, int list_entries, int batch, int heads_q, int heads_kv,
+                              int head_dim, int num_pages, int page_size, int max_pages, const int64_t* q_strides,
+                              const int64_t* kp_strides, const int64_t* vp_strides, const int64_t* o_strides,
+                              const int64_t* list_strides, const int64_t* count_strides, int64_t table_stride,
+                              float softmax_scale, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+size_t sabre_paged_prefill_listed_workspace_size(int rows, int batch, int heads_q, int heads_kv, int head_dim,
+                                                 int page_size, int query_block, int list_entries);
+int sabre_paged_prefill_listed(const void* q, const void* k_pages, const void* v_pages, void* o,
+                               const int32_t* page_table, const int32_t* seq_lens, const int32_t* q_start,
+                               const int32_t* lists, const int32_t* counts, int list_entries, int rows, int batch,
+                               int heads_q, int heads_kv, int head_dim, int num_pages, int page_size, int max_pages,
+                               int query_block, const int64_t* q_strides, const int64_t* kp_strides,
+                               const int64_t* vp_strides, const int64_t* o_strides, const int64_t* list_strides,
+                               const int64_t* count_strides, int64_t table_stride, float softmax_scale, int dtype,
+                               void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

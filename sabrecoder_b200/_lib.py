@@ -62,6 +62,22 @@ SIGNATURES = {
     "sabre_paged_prefill_workspace_size": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
     "sabre_paged_prefill": (c_int, [P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                                     c_int, c_int, I64P, I64P, I64P, I64P, c_int64, c_float, c_int, P, c_size_t, P]),
+    "sabre_paged_extend": (c_int, [P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int64, P]),
+    "sabre_paged_store_slots": (c_int, [P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, I64P, I64P, I64P, I64P,
+                                        c_int, P]),
+    "sabre_paged_key_means": (c_int, [P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, I64P, I64P,
+                                      c_int64, c_int, P]),
+    "sabre_paged_query_blocks": (c_int, [c_int, c_int, c_int]),
+    "sabre_paged_select_width": (c_int, [c_int, c_int, c_int, c_int, c_int, c_int]),
+    "sabre_paged_select": (c_int, [P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                   c_int, c_int, c_int, I64P, I64P, c_int64, c_int, P]),
+    "sabre_paged_decode_listed": (c_int, [P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                          c_int, I64P, I64P, I64P, I64P, I64P, I64P, c_int64, c_float, c_int, P,
+                                          c_size_t, P]),
+    "sabre_paged_prefill_listed_workspace_size": (c_size_t, [c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int]),
+    "sabre_paged_prefill_listed": (c_int, [P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                           c_int, c_int, c_int, I64P, I64P, I64P, I64P, I64P, I64P, c_int64, c_float,
+                                           c_int, P, c_size_t, P]),
     "sabre_copy_pages": (c_int, [P, c_int, c_int64, c_int, c_int64, c_int64, I32P, I32P, c_int, P]),
 }
 

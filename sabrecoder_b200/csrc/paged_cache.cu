@@ -45,10 +45,105 @@ struct Window {
   __device__ __forceinline__ int first(int i) const { return window < 0 ? 0 : max(0, max(i, 0) - window); }
 };
 
+// Lists of table columns, ascending: which pages a query block reads for one KV
+// head. A list's rows are its pages', one after another ("list rows"). An entry
+// that is not above the one before it or that lies past the table is no page
+// (the latter is recorded).
+struct Lists {
+  const int32_t* entries;
+  const int32_t* counts;
+  long long e_sq, e_sh, c_sq, c_sh;  // strides {query block, head}
+  int cap;
+
+  __device__ __forceinline__ int count(int block, int head) const {
+    return min(max(counts[block * c_sq + head * c_sh], 0), cap);
+  }
+  // Column of entry i < count, or -1.
+  __device__ __forceinline__ int column(int block, int head, int i, const Cache& c) const {
+    const int32_t* e = entries + block * e_sq + head * e_sh + i;
+    const int col = e[0];
+    const bool in = col >= 0 && col < c.max_pages;
+    if (!in) record_status(SABRE_DEV_BAD_PAGE);
+    return in && (i == 0 || e[-1] < col) ? col : -1;
+  }
+};
+
 // First row of sequence b in a ragged batch of `rows` rows (one row each
 // without starts). Clamped, so that no start reaches past the rows.
 __device__ __forceinline__ int row_start(const int32_t* starts, int b, int rows) {
   return starts ? min(max(starts[b], 0), rows) : min(b, rows);
+}
+
+// Exclusive prefix sum over the CTA's kThreads threads (a multiple of 32);
+// scratch: an int for each warp. `all`: the total.
+template <int kThreads>
+__device__ __forceinline__ int prefix_sum(int mine, int* scratch, int& all) {
+  const int tid = threadIdx.x;
+  int incl = mine;
+#pragma unroll
+  for (int s = 1; s < 32; s <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, incl, s);
+    if ((tid & 31) >= s) incl += up;
+  }
+  __syncthreads();  // scratch is free
+  if ((tid & 31) == 31) scratch[tid >> 5] = incl;
+  __syncthreads();
+  int before = 0;
+  all = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    before += w < (tid >> 5) ? scratch[w] : 0;
+    all += scratch[w];
+  }
+  return before + incl - mine;
+}
+
+// Rows r, r + 1, .. (at most `tokens`) of sequence b, whose `len` new rows begin
+// at row `first` and end its `length` rows.
+struct RowTile {
+  int b, r, first, len, length;
+};
+
+// Row tile `slot` of a ragged batch cut into tiles of `tokens` rows, found by
+// the whole CTA (kThreads threads, at most 256); scratch: 16 ints. False: there
+// are fewer.
+template <int kThreads>
+__device__ __forceinline__ bool find_rows(const Cache& c, const int32_t* starts, int rows, int tokens, int slot,
+                                          int* scratch, RowTile& tile) {
+  const int tid = threadIdx.x;
+  const int per = (c.batch + kThreads - 1) / kThreads;
+  const int b0 = min(tid * per, c.batch), b1 = min(b0 + per, c.batch);
+  // The first length comes with the starts, not after them: one round trip
+  // for as many sequences as threads.
+  const int len0 = b0 < b1 ? c.seq_lens[b0] : 0;
+  int mine = 0;
+  for (int b = b0; b < b1; ++b) {
+    const int len = row_start(starts, b + 1, rows) - row_start(starts, b, rows);
+    mine += (max(len, 0) + tokens - 1) / tokens;
+  }
+  if (tid == 0) scratch[8] = -1;
+  int all = 0;
+  int left = slot - prefix_sum<kThreads>(mine, scratch, all);
+  if (left >= 0 && left < mine) {
+    for (int b = b0; b < b1; ++b) {
+      const int first = row_start(starts, b, rows);
+      const int len = row_start(starts, b + 1, rows) - first;
+      const int nt = (max(len, 0) + tokens - 1) / tokens;
+      if (left < nt) {
+        scratch[8] = b;
+        scratch[9] = left * tokens;
+        scratch[10] = first;
+        scratch[11] = len;
+        scratch[12] = b == b0 ? len0 : c.seq_lens[b];
+        break;
+      }
+      left -= nt;
+    }
+  }
+  __syncthreads();
+  if (scratch[8] < 0) return false;
+  tile = RowTile{scratch[8], scratch[9], scratch[10], scratch[11], scratch[12]};
+  return true;
 }
 
 // ---------------------------------------------------------------------------
@@ -71,6 +166,7 @@ struct StoreParams {
   uint4* kp;
   uint4* vp;
   const int32_t* starts;
+  const long long* slots;            // the rows' places (page * page_size + row; negative: none), or null
   long long k_sr, k_sh, v_sr, v_sh;  // strides of the rows, in 16-byte units
   int rows, heads, cta_rows;
 };
@@ -89,7 +185,14 @@ __global__ void __launch_bounds__(kStoreThreads) paged_store_kernel(const StoreP
     int page = -1, off = 0;
     // Sequence b: start(b) <= row < start(b + 1).
     int b = -1;
-    if (row < p.rows) {
+    if (p.slots) {
+      const long long slot = row < p.rows ? p.slots[row] : -1;
+      if (slot >= 0) {
+        const long long pg = slot >> p.c.page_shift;
+        page = p.c.checked(pg < p.c.num_pages ? static_cast<int>(pg) : p.c.num_pages);
+        off = static_cast<int>(slot & ((1 << p.c.page_shift) - 1));
+      }
+    } else if (row < p.rows) {
       if (!p.starts) {
         b = row;
       } else {
@@ -187,6 +290,25 @@ static cudaError_t launch_dependent(dim3 grid, int threads, int smem, cudaStream
   return cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
+// The same with clusters of `ctas` CTAs along x.
+template <typename K, typename... A>
+static cudaError_t launch_cluster(dim3 grid, int ctas, int threads, int smem, cudaStream_t s, K kernel, A... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = ctas;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // Checks shared by the paged entry points; fills c. `kp` / `vp` strides are
 // {page, head, row} in elements.
 static int make_cache(Cache* c, const char* fn, const void* k_pages, const void* v_pages, const int32_t* page_table,
@@ -228,38 +350,21 @@ static int make_cache(Cache* c, const char* fn, const void* k_pages, const void*
   return SABRE_OK;
 }
 
-}  // namespace paged
-}  // namespace sabre
-
-extern "C" {
-
-int sabre_paged_store(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* page_table,
-                      const int32_t* seq_lens, const int32_t* q_start, int rows, int batch, int heads_kv,
-                      int head_dim, int num_pages, int page_size, int max_pages, const int64_t* k_strides,
-                      const int64_t* v_strides, const int64_t* kp_strides, const int64_t* vp_strides,
-                      int64_t table_stride, int dtype, void* stream) {
-  using namespace sabre::paged;
-  if (!k || !v || !k_strides || !v_strides)
-    return sabre_fail(SABRE_ERR_INVALID_ARG, "sabre_paged_store: null pointer argument");
-  StoreParams p;
-  const int st = make_cache(&p.c, "sabre_paged_store", k_pages, v_pages, page_table, seq_lens, batch, heads_kv,
-                            head_dim, num_pages, page_size, max_pages, kp_strides, vp_strides, table_stride, dtype);
-  if (st != SABRE_OK) return st;
-  if (rows <= 0) return sabre_fail(SABRE_ERR_INVALID_ARG, "sabre_paged_store: rows must be positive");
-  if (!q_start && rows != batch)
-    return sabre_fail(SABRE_ERR_INVALID_ARG, "sabre_paged_store: %d rows for %d sequences need q_start", rows, batch);
-  if (!aligned16(k) || !aligned16(v))
-    return sabre_fail(SABRE_ERR_ALIGNMENT, "sabre_paged_store: k/v must be 16-byte aligned");
+// Both store entries; p has its tables or slots.
+static int store(StoreParams& p, const char* fn, const void* k, const void* v, void* k_pages, void* v_pages, int rows,
+                 int heads_kv, const int64_t* k_strides, const int64_t* v_strides, void* stream) {
+  if (!k || !v || !k_strides || !v_strides) return sabre_fail(SABRE_ERR_INVALID_ARG, "%s: null pointer argument", fn);
+  if (rows <= 0) return sabre_fail(SABRE_ERR_INVALID_ARG, "%s: rows must be positive", fn);
+  if (!aligned16(k) || !aligned16(v)) return sabre_fail(SABRE_ERR_ALIGNMENT, "%s: k/v must be 16-byte aligned", fn);
   for (int i = 0; i < 2; ++i)
     if (k_strides[i] % 8 != 0 || v_strides[i] % 8 != 0)
-      return sabre_fail(SABRE_ERR_ALIGNMENT, "sabre_paged_store: k/v strides must be multiples of 8 elements");
+      return sabre_fail(SABRE_ERR_ALIGNMENT, "%s: k/v strides must be multiples of 8 elements", fn);
   long long* s[6] = {&p.c.k_sp, &p.c.k_sh, &p.c.k_st, &p.c.v_sp, &p.c.v_sh, &p.c.v_st};
   for (int i = 0; i < 6; ++i) *s[i] /= 8;
   p.k = static_cast<const uint4*>(k);
   p.v = static_cast<const uint4*>(v);
   p.kp = static_cast<uint4*>(k_pages);
   p.vp = static_cast<uint4*>(v_pages);
-  p.starts = q_start;
   p.k_sr = k_strides[0] / 8;
   p.k_sh = k_strides[1] / 8;
   p.v_sr = v_strides[0] / 8;
@@ -271,7 +376,58 @@ int sabre_paged_store(const void* k, const void* v, void* k_pages, void* v_pages
   p.cta_rows = kStoreBatch * (heads_kv < 8 ? 8 / heads_kv : 1);
   const cudaError_t e = launch_dependent(dim3((rows + p.cta_rows - 1) / p.cta_rows), kStoreThreads, 0,
                                          static_cast<cudaStream_t>(stream), paged_store_kernel, p);
-  return e == cudaSuccess ? SABRE_OK : sabre_cuda_fail(e, "sabre_paged_store launch");
+  return e == cudaSuccess ? SABRE_OK : sabre_cuda_fail(e, fn);
+}
+
+// Strides are {query block, KV head}; 0 is one list for all of them.
+static int make_lists(Lists* l, const char* fn, const int32_t* entries, const int32_t* counts, int cap,
+                      const int64_t* e, const int64_t* c) {
+  if (!entries || !counts || !e || !c) return sabre_fail(SABRE_ERR_INVALID_ARG, "%s: null pointer argument", fn);
+  if (cap <= 0) return sabre_fail(SABRE_ERR_INVALID_ARG, "%s: lists of %d entries", fn, cap);
+  if (e[0] < 0 || e[1] < 0 || c[0] < 0 || c[1] < 0)
+    return sabre_fail(SABRE_ERR_INVALID_ARG, "%s: list strides must not be negative", fn);
+  *l = Lists{entries, counts, e[0], e[1], c[0], c[1], cap};
+  return SABRE_OK;
+}
+
+}  // namespace paged
+}  // namespace sabre
+
+extern "C" {
+
+int sabre_paged_store(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* page_table,
+                      const int32_t* seq_lens, const int32_t* q_start, int rows, int batch, int heads_kv,
+                      int head_dim, int num_pages, int page_size, int max_pages, const int64_t* k_strides,
+                      const int64_t* v_strides, const int64_t* kp_strides, const int64_t* vp_strides,
+                      int64_t table_stride, int dtype, void* stream) {
+  using namespace sabre::paged;
+  const char* fn = "sabre_paged_store";
+  StoreParams p;
+  const int st = make_cache(&p.c, fn, k_pages, v_pages, page_table, seq_lens, batch, heads_kv, head_dim, num_pages,
+                            page_size, max_pages, kp_strides, vp_strides, table_stride, dtype);
+  if (st != SABRE_OK) return st;
+  if (!q_start && rows > 0 && rows != batch)
+    return sabre_fail(SABRE_ERR_INVALID_ARG, "%s: %d rows for %d sequences need q_start", fn, rows, batch);
+  p.starts = q_start;
+  p.slots = nullptr;
+  return store(p, fn, k, v, k_pages, v_pages, rows, heads_kv, k_strides, v_strides, stream);
+}
+
+int sabre_paged_store_slots(const void* k, const void* v, void* k_pages, void* v_pages, const int64_t* slots, int rows,
+                            int heads_kv, int head_dim, int num_pages, int page_size, const int64_t* k_strides,
+                            const int64_t* v_strides, const int64_t* kp_strides, const int64_t* vp_strides, int dtype,
+                            void* stream) {
+  using namespace sabre::paged;
+  const char* fn = "sabre_paged_store_slots";
+  if (!slots) return sabre_fail(SABRE_ERR_INVALID_ARG, "%s: null pointer argument", fn);
+  StoreParams p;
+  const int32_t* none = reinterpret_cast<const int32_t*>(slots);  // not read
+  const int st = make_cache(&p.c, fn, k_pages, v_pages, none, none, 1, heads_kv, head_dim, num_pages, page_size, 1,
+                            kp_strides, vp_strides, 0, dtype);
+  if (st != SABRE_OK) return st;
+  p.starts = nullptr;
+  p.slots = reinterpret_cast<const long long*>(slots);
+  return store(p, fn, k, v, k_pages, v_pages, rows, heads_kv, k_strides, v_strides, stream);
 }
 
 int sabre_copy_pages(void* pages, int buffers, int64_t buffer_stride, int num_pages, int64_t page_stride,

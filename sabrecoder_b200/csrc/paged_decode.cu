@@ -68,6 +68,7 @@ struct DecodeParams {
   long long q_sb, q_sh, o_sb, o_sh;
   int heads_kv, group, ctas;
   float scale_log2;
+  Lists lists;  // of a call over listed pages
 };
 
 // The visible tiles of one sequence: `head` tiles from 0 (prefix tokens), then
@@ -88,6 +89,34 @@ struct Tiles {
   }
 };
 
+// The same over the listed pages of one (sequence, KV head) pair: 64 list rows a
+// tile, as many tiles as its list has entries for.
+struct ListedTiles {
+  int n, entries, count;
+  __device__ __forceinline__ ListedTiles(const DecodeParams& p, int b, int hk) {
+    n = p.c.length(b);
+    entries = n > 0 ? p.lists.count(b, hk) : 0;
+    count = static_cast<int>(((static_cast<long long>(entries) << p.c.page_shift) + kTile - 1) / kTile);
+  }
+};
+
+// What the shares are dealt out over, in order: without lists sequences, whose
+// KV heads all have the same tiles; with lists pairs.
+template <bool kListed>
+struct Work {
+  using Tiles_ = typename std::conditional<kListed, ListedTiles, Tiles>::type;
+  static __device__ __forceinline__ int count(const DecodeParams& p) {
+    return kListed ? p.c.batch * p.heads_kv : p.c.batch;
+  }
+  static __device__ __forceinline__ int heads(const DecodeParams& p) { return kListed ? 1 : p.heads_kv; }
+  static __device__ __forceinline__ Tiles_ tiles(const DecodeParams& p, int x) {
+    if constexpr (kListed)
+      return ListedTiles(p, x / p.heads_kv, x % p.heads_kv);
+    else
+      return Tiles(p, x);
+  }
+};
+
 // Shares: total tiles dealt to `ctas` CTAs; unit u belongs to CTA owner(u).
 struct Shares {
   long long total;
@@ -102,16 +131,18 @@ struct Place {
 
 // Finds the shares and the place of this CTA's first unit with the whole CTA
 // (kDecThreads threads); scratch: 16 ints of shared memory. False for a CTA
-// without a share. Calls on_empty(b) for sequences without a tile.
-template <typename E>
+// without a share. Calls on_empty(x) for the sequences (with lists: pairs)
+// without a tile.
+template <bool kListed, typename E>
 __device__ __forceinline__ bool locate(const DecodeParams& p, int* scratch, Shares& sh, Place& at, E on_empty) {
   constexpr int kThreads = kDecThreads;
+  using W = Work<kListed>;
   const int tid = threadIdx.x;
-  const int per = (p.c.batch + kThreads - 1) / kThreads;
-  const int b0 = min(tid * per, p.c.batch), b1 = min(b0 + per, p.c.batch);
+  const int per = (W::count(p) + kThreads - 1) / kThreads;
+  const int b0 = min(tid * per, W::count(p)), b1 = min(b0 + per, W::count(p));
   int mine = 0;
   for (int b = b0; b < b1; ++b) {
-    const int nt = Tiles(p, b).count;
+    const int nt = W::tiles(p, b).count;
     if (nt == 0) on_empty(b);
     mine += nt;
   }
@@ -129,16 +160,16 @@ __device__ __forceinline__ bool locate(const DecodeParams& p, int* scratch, Shar
     before += w < (tid >> 5) ? scratch[w] : 0;
     all += scratch[w];
   }
-  sh.total = static_cast<long long>(all) * p.heads_kv;
+  sh.total = static_cast<long long>(all) * W::heads(p);
   if (all == 0) return false;
   sh.ctas = static_cast<int>(min(static_cast<long long>(p.ctas), sh.total));
   if (static_cast<int>(blockIdx.x) >= sh.ctas) return false;
-  long long left = sh.first(blockIdx.x) - static_cast<long long>(before + incl - mine) * p.heads_kv;
+  long long left = sh.first(blockIdx.x) - static_cast<long long>(before + incl - mine) * W::heads(p);
   int* found = scratch + kThreads / 32;
-  if (left >= 0 && left < static_cast<long long>(mine) * p.heads_kv) {
+  if (left >= 0 && left < static_cast<long long>(mine) * W::heads(p)) {
     for (int b = b0; b < b1; ++b) {
-      const int nt = Tiles(p, b).count;
-      const long long here = static_cast<long long>(nt) * p.heads_kv;
+      const int nt = W::tiles(p, b).count;
+      const long long here = static_cast<long long>(nt) * W::heads(p);
       if (left < here) {
         found[0] = b;
         found[1] = static_cast<int>(left / nt);
@@ -149,25 +180,35 @@ __device__ __forceinline__ bool locate(const DecodeParams& p, int* scratch, Shar
     }
   }
   __syncthreads();
-  at.b = found[0];
-  at.hk = found[1];
+  at.b = kListed ? found[0] / p.heads_kv : found[0];
+  at.hk = kListed ? found[0] % p.heads_kv : found[1];
   at.tile = found[2];
   return true;
 }
 
 // Walks a share's segments: the same sequence for the producer and the consumers.
+template <bool kListed>
 struct Segments {
   const DecodeParams& p;
   int b, hk, t0, t1, seen;  // this segment: tiles [t0, t1) of pair (b, hk)
   long long left;
-  Tiles tiles;
+  typename Work<kListed>::Tiles_ tiles;
   __device__ __forceinline__ Segments(const DecodeParams& p_, const Place& at, long long units)
-      : p(p_), b(at.b), hk(at.hk), t0(at.tile), t1(0), seen(-1), left(units), tiles(p_, at.b) {}
+      : p(p_), b(at.b), hk(at.hk), t0(at.tile), t1(0), seen(-1), left(units),
+        tiles(Work<kListed>::tiles(p_, kListed ? at.b * p_.heads_kv + at.hk : at.b)) {}
   __device__ __forceinline__ bool next() {
     if (left <= 0) return false;
     if (++seen > 0) {
       t0 = 0;
-      if (++hk == p.heads_kv) {
+      if constexpr (kListed) {
+        do {  // left > 0: another pair has tiles
+          if (++hk == p.heads_kv) {
+            hk = 0;
+            ++b;
+          }
+          tiles = ListedTiles(p, b, hk);
+        } while (tiles.count == 0 && b * p.heads_kv + hk < p.c.batch * p.heads_kv - 1);
+      } else if (++hk == p.heads_kv) {
         hk = 0;
         do tiles = Tiles(p, ++b);  // left > 0: another sequence has tiles
         while (tiles.count == 0 && b < p.c.batch - 1);
@@ -285,7 +326,8 @@ struct PartSum {
   }
 };
 
-template <typename T>
+// kListed: over the pages of p.lists; else over all rows, or the window's.
+template <typename T, bool kListed>
 __global__ void __launch_bounds__(kDecThreads, 2)
     paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                         const DecodeParams p) {
@@ -297,7 +339,9 @@ __global__ void __launch_bounds__(kDecThreads, 2)
   const int warp = tid >> 5;
   const int lane = tid & 31;
   const uint32_t sbase = smem_u32(smem);
-  uint32_t* valid = reinterpret_cast<uint32_t*>(smem + kMiscOff);  // [kStages]: fetched boxes of the tile
+  // [kStages]: fetched boxes of the tile; with lists also, from bit 4 on, how many
+  // rows of each box the sequence has, in five bits each.
+  uint32_t* valid = reinterpret_cast<uint32_t*>(smem + kMiscOff);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kMiscOff + 16);
   auto full_bar = [&](int s) -> uint32_t { return sbase + kBarOff + 8u * s; };
   auto empty_bar = [&](int s) -> uint32_t { return sbase + kBarOff + 8u * (kStages + s); };
@@ -320,10 +364,12 @@ __global__ void __launch_bounds__(kDecThreads, 2)
   Shares sh;
   Place at;
   T* const out = static_cast<T*>(p.o);
-  const bool some = locate(p, reinterpret_cast<int*>(smem + kAccOff), sh, at, [&](int b) {
-    // No visible tile: the sequence's rows are zero.
-    if (b % p.ctas != static_cast<int>(blockIdx.x)) return;
-    for (int h = 0; h < p.heads_kv * p.group; ++h)
+  const bool some = locate<kListed>(p, reinterpret_cast<int*>(smem + kAccOff), sh, at, [&](int x) {
+    // No visible tile: the sequence's (with lists: the pair's) rows are zero.
+    if (x % p.ctas != static_cast<int>(blockIdx.x)) return;
+    const int b = kListed ? x / p.heads_kv : x;
+    const int h0 = kListed ? x % p.heads_kv * p.group : 0;
+    for (int h = h0; h < h0 + (kListed ? 1 : p.heads_kv) * p.group; ++h)
       for (int d = 0; d < kD; d += 8)
         *reinterpret_cast<uint4*>(out + b * p.o_sb + h * p.o_sh + d) = make_uint4(0u, 0u, 0u, 0u);
   });
@@ -332,7 +378,7 @@ __global__ void __launch_bounds__(kDecThreads, 2)
     if (tid == 0) p.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
     return;
   }
-  Segments seg(p, at, sh.first(blockIdx.x + 1) - sh.first(blockIdx.x));
+  Segments<kListed> seg(p, at, sh.first(blockIdx.x + 1) - sh.first(blockIdx.x));
   __syncthreads();  // the scratch of locate() is free
   bool ok = *abort_flag == 0;
 
@@ -345,7 +391,22 @@ __global__ void __launch_bounds__(kDecThreads, 2)
       for (int i0 = 0; ok && i0 < nbox; i0 += 32) {
         // The pages of the next 32 boxes, one per lane.
         int page = -1, off = 0;
-        if (i0 + lane < nbox) {
+        uint32_t rows = 0;  // kListed: of this tile's boxes
+        if constexpr (kListed) {
+          const int at_row = seg.t0 * kTile + (i0 + lane) * kBoxRows;
+          const int e = at_row >> p.c.page_shift;
+          if (i0 + lane < nbox && e < seg.tiles.entries) {
+            const int col = p.lists.column(seg.b, seg.hk, e, p.c);
+            off = at_row & ((1 << p.c.page_shift) - 1);
+            const int t = (col << p.c.page_shift) + off;
+            if (col >= 0 && t < seg.tiles.n) {
+              page = p.c.page_of(seg.b, t);
+              rows = static_cast<uint32_t>(min(seg.tiles.n - t, kBoxRows)) << (4 + 5 * (lane % kBoxes));
+            }
+          }
+          rows |= __shfl_xor_sync(0xffffffffu, rows, 1);
+          rows |= __shfl_xor_sync(0xffffffffu, rows, 2);
+        } else if (i0 + lane < nbox) {
           const int t = seg.tiles.pos(seg.t0 + (i0 + lane) / kBoxes) + (lane % kBoxes) * kBoxRows;
           if (seg.tiles.any(p.w, t, kBoxRows)) {
             page = p.c.page_of(seg.b, t);
@@ -358,8 +419,9 @@ __global__ void __launch_bounds__(kDecThreads, 2)
           ok = mbar_wait_warp_lim(empty_bar(s), ((it / kStages) & 1) ^ 1, abort_flag, wlim);
           if (!ok) break;
           const uint32_t mask = (have >> i) & ((1u << kBoxes) - 1u);
+          const uint32_t tile_rows = kListed ? __shfl_sync(0xffffffffu, rows, i) : 0u;
           if (lane == 0) {
-            valid[s] = mask;
+            valid[s] = mask | tile_rows;
             mbar_arrive_expect_tx(full_bar(s), __popc(mask) * 2u * kBoxBytes);
           }
           __syncwarp();
@@ -419,7 +481,11 @@ __global__ void __launch_bounds__(kDecThreads, 2)
       // The phase is complete; each lane's own probe gives it acquire order on the copied bytes.
       if (ok) (void)mbar_test_wait(full_bar(s), (it / kStages) & 1);
       if (ok && ((valid[s] >> warp) & 1u)) {
-        const int t = seg.tiles.pos(tile) + warp * 16;
+        int t = 0, rows = 0;  // the position of the 16 keys; kListed: how many of them there are
+        if constexpr (kListed)
+          rows = (valid[s] >> (4 + 5 * warp)) & 31u;
+        else
+          t = seg.tiles.pos(tile) + warp * 16;
         const uint32_t kb = sbase + kRingOff + s * 2 * kTileBytes + krow;
         const uint32_t vb = sbase + kRingOff + s * 2 * kTileBytes + kTileBytes + vrow;
         float sc[2][4] = {};
@@ -436,10 +502,19 @@ __global__ void __launch_bounds__(kDecThreads, 2)
         // Some of the 16 keys may be hidden (ends of the sequence, the window
         // and the prefix): their scores become -inf and their V rows zero,
         // whatever the page holds there.
-        const bool whole = t + 16 <= seg.tiles.n && (t >= seg.tiles.lo || t + 16 <= p.w.prefix);
+        bool whole;
+        if constexpr (kListed)
+          whole = rows == 16;
+        else
+          whole = t + 16 <= seg.tiles.n && (t >= seg.tiles.lo || t + 16 <= p.w.prefix);
         uint32_t vm0 = ~0u, vm1 = ~0u;
         if (!whole) {
-          auto see = [&](int k) { return t + k < seg.tiles.n && (t + k >= seg.tiles.lo || t + k < p.w.prefix); };
+          auto see = [&](int k) -> bool {
+            if constexpr (kListed)
+              return k < rows;
+            else
+              return t + k < seg.tiles.n && (t + k >= seg.tiles.lo || t + k < p.w.prefix);
+          };
           if (!see(r4)) x[0] = x[1] = -INFINITY;
           if (!see(r4 + 8)) x[2] = x[3] = -INFINITY;
           vm0 = (see(c2) ? 0xffffu : 0u) | (see(c2 + 1) ? 0xffff0000u : 0u);
@@ -654,14 +729,79 @@ static size_t decode_workspace(int group) {
   return kDecCtas * sizeof(int4) + static_cast<size_t>(2) * kDecCtas * group * (kD + 2) * sizeof(float);
 }
 
-template <typename T>
+template <typename T, bool kListed>
 static cudaError_t launch_paged_decode(const CUtensorMap& mk, const CUtensorMap& mv, const DecodeParams& p,
                                        cudaStream_t s) {
-  cudaError_t e = cudaFuncSetAttribute(paged_decode_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, kDecSmem);
+  const auto kernel = paged_decode_kernel<T, kListed>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDecSmem);
   if (e != cudaSuccess) return e;
-  e = launch_dependent(dim3(p.ctas), kDecThreads, kDecSmem, s, paged_decode_kernel<T>, mk, mv, p);
+  e = launch_dependent(dim3(p.ctas), kDecThreads, kDecSmem, s, kernel, mk, mv, p);
   if (e != cudaSuccess || p.ctas == 1) return e;  // a single share is finished where it is
   return launch_dependent(dim3(p.ctas - 1, p.group), kJoinWarps * 32, 0, s, paged_join_kernel<T>, p);
+}
+
+// Both decode entries: over the pages of `lists`, or (null) over all rows or the window's.
+static int decode_call(const char* fn, const void* q, const void* k_pages, const void* v_pages, void* o,
+                  const int32_t* page_table, const int32_t* seq_lens, const Lists* lists, int batch, int heads_q,
+                  int heads_kv, int head_dim, int num_pages, int page_size, int max_pages, int window,
+                  int num_prefix_tokens, const int64_t* q_strides, const int64_t* kp_strides,
+                  const int64_t* vp_strides, const int64_t* o_strides, int64_t table_stride, float softmax_scale,
+                  int dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  DecodeParams p;
+  int st = make_cache(&p.c, fn, k_pages, v_pages, page_table, seq_lens, batch, heads_kv, head_dim, num_pages,
+                      page_size, max_pages, kp_strides, vp_strides, table_stride, dtype);
+  if (st == SABRE_OK) st = check_queries(fn, q, o, heads_q, heads_kv, num_prefix_tokens, q_strides, o_strides);
+  if (st != SABRE_OK) return st;
+  p.lists = lists ? *lists : Lists{};
+  p.w = Window{window, window < 0 ? 0 : num_prefix_tokens};
+  p.q = q;
+  p.o = o;
+  p.q_sb = q_strides[0];
+  p.q_sh = q_strides[1];
+  p.o_sb = o_strides[0];
+  p.o_sh = o_strides[1];
+  p.heads_kv = heads_kv;
+  p.group = heads_q / heads_kv;
+  p.scale_log2 = scale_log2(softmax_scale);
+  if (!workspace || workspace_bytes < decode_workspace(p.group))
+    return sabre_fail(SABRE_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", fn, workspace_bytes,
+                      decode_workspace(p.group));
+  if (!aligned16(workspace)) return sabre_fail(SABRE_ERR_ALIGNMENT, "%s: workspace must be 16-byte aligned", fn);
+  // No more CTAs than the table has tiles, nor parts of a pair than pay for
+  // their joining (12000 rows of one KV head, 188 tiles: 11.2 us a call in 188
+  // parts, 9.3 in 94; below that a tile a CTA is the fastest).
+  if (lists && static_cast<long long>(page_size) * lists->cap > kMaxRows)
+    return sabre_fail(SABRE_ERR_UNSUPPORTED, "%s: page_size * list entries exceeds 2^30 rows", fn);
+  const long long span = lists ? static_cast<long long>(page_size) * lists->cap
+                               : static_cast<long long>(page_size) * max_pages;
+  const long long per_head = static_cast<long long>(batch) * ((span + kTile - 1) / kTile);
+  const long long tiles = per_head * heads_kv;
+  // The kernel adds up a sequence's (with lists: a pair's) tiles in 32 bits.
+  if ((lists ? tiles : per_head) > 0x7fffffffll)
+    return sabre_fail(SABRE_ERR_UNSUPPORTED, lists ? "%s: batch * heads_kv * page_size * list entries exceeds 2^37 rows"
+                                                   : "%s: batch * page_size * max_pages exceeds 2^37 rows", fn);
+  long long ctas = static_cast<long long>(batch) * heads_kv * kMaxParts;
+  if (ctas > tiles) ctas = tiles;
+  p.ctas = static_cast<int>(ctas < kDecCtas ? ctas : kDecCtas);
+  p.joins = static_cast<int4*>(workspace);
+  p.part_acc = reinterpret_cast<float*>(p.joins + kDecCtas);
+  p.part_ml = p.part_acc + static_cast<size_t>(2) * kDecCtas * p.group * kD;
+  CUtensorMap mk, mv;
+  if ((st = make_map_pages(&mk, k_pages, dtype, num_pages, heads_kv, page_size, p.c.k_sp, p.c.k_sh, p.c.k_st,
+                           kBoxRows, 2, "k_pages")) != SABRE_OK)
+    return st;
+  if ((st = make_map_pages(&mv, v_pages, dtype, num_pages, heads_kv, page_size, p.c.v_sp, p.c.v_sh, p.c.v_st,
+                           kBoxRows, 2, "v_pages")) != SABRE_OK)
+    return st;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  cudaError_t e;
+  if (lists)
+    e = dtype == SABRE_BF16 ? launch_paged_decode<__nv_bfloat16, true>(mk, mv, p, s)
+                            : launch_paged_decode<__half, true>(mk, mv, p, s);
+  else
+    e = dtype == SABRE_BF16 ? launch_paged_decode<__nv_bfloat16, false>(mk, mv, p, s)
+                            : launch_paged_decode<__half, false>(mk, mv, p, s);
+  return e == cudaSuccess ? SABRE_OK : sabre_cuda_fail(e, fn);
 }
 
 }  // namespace paged
@@ -681,51 +821,27 @@ int sabre_paged_decode(const void* q, const void* k_pages, const void* v_pages, 
                        const int64_t* kp_strides, const int64_t* vp_strides, const int64_t* o_strides,
                        int64_t table_stride, float softmax_scale, int dtype, void* workspace, size_t workspace_bytes,
                        void* stream) {
+  return sabre::paged::decode_call("sabre_paged_decode", q, k_pages, v_pages, o, page_table, seq_lens, nullptr, batch,
+                              heads_q, heads_kv, head_dim, num_pages, page_size, max_pages, window, num_prefix_tokens,
+                              q_strides, kp_strides, vp_strides, o_strides, table_stride, softmax_scale, dtype,
+                              workspace, workspace_bytes, stream);
+}
+
+int sabre_paged_decode_listed(const void* q, const void* k_pages, const void* v_pages, void* o,
+                              const int32_t* page_table, const int32_t* seq_lens, const int32_t* lists,
+                              const int32_t* counts, int list_entries, int batch, int heads_q, int heads_kv,
+                              int head_dim, int num_pages, int page_size, int max_pages, const int64_t* q_strides,
+                              const int64_t* kp_strides, const int64_t* vp_strides, const int64_t* o_strides,
+                              const int64_t* list_strides, const int64_t* count_strides, int64_t table_stride,
+                              float softmax_scale, int dtype, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace sabre::paged;
-  const char* fn = "sabre_paged_decode";
-  DecodeParams p;
-  int st = make_cache(&p.c, fn, k_pages, v_pages, page_table, seq_lens, batch, heads_kv, head_dim, num_pages,
-                      page_size, max_pages, kp_strides, vp_strides, table_stride, dtype);
-  if (st == SABRE_OK) st = check_queries(fn, q, o, heads_q, heads_kv, num_prefix_tokens, q_strides, o_strides);
+  const char* fn = "sabre_paged_decode_listed";
+  Lists l;
+  const int st = make_lists(&l, fn, lists, counts, list_entries, list_strides, count_strides);
   if (st != SABRE_OK) return st;
-  p.w = Window{window, window < 0 ? 0 : num_prefix_tokens};
-  p.q = q;
-  p.o = o;
-  p.q_sb = q_strides[0];
-  p.q_sh = q_strides[1];
-  p.o_sb = o_strides[0];
-  p.o_sh = o_strides[1];
-  p.heads_kv = heads_kv;
-  p.group = heads_q / heads_kv;
-  p.scale_log2 = scale_log2(softmax_scale);
-  if (!workspace || workspace_bytes < decode_workspace(p.group))
-    return sabre_fail(SABRE_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", fn, workspace_bytes,
-                      decode_workspace(p.group));
-  if (!aligned16(workspace)) return sabre_fail(SABRE_ERR_ALIGNMENT, "%s: workspace must be 16-byte aligned", fn);
-  // No more CTAs than the table has tiles, nor parts of a pair than pay for
-  // their joining (12000 rows of one KV head, 188 tiles: 11.2 us a call in 188
-  // parts, 9.3 in 94; below that a tile a CTA is the fastest).
-  const long long per_head = static_cast<long long>(batch) * ((page_size * max_pages + kTile - 1) / kTile);
-  if (per_head > 0x7fffffffll)
-    return sabre_fail(SABRE_ERR_UNSUPPORTED, "%s: batch * page_size * max_pages exceeds 2^37 rows", fn);
-  const long long tiles = per_head * heads_kv;
-  long long ctas = static_cast<long long>(batch) * heads_kv * kMaxParts;
-  if (ctas > tiles) ctas = tiles;
-  p.ctas = static_cast<int>(ctas < kDecCtas ? ctas : kDecCtas);
-  p.joins = static_cast<int4*>(workspace);
-  p.part_acc = reinterpret_cast<float*>(p.joins + kDecCtas);
-  p.part_ml = p.part_acc + static_cast<size_t>(2) * kDecCtas * p.group * kD;
-  CUtensorMap mk, mv;
-  if ((st = make_map_pages(&mk, k_pages, dtype, num_pages, heads_kv, page_size, p.c.k_sp, p.c.k_sh, p.c.k_st,
-                           kBoxRows, 2, "k_pages")) != SABRE_OK)
-    return st;
-  if ((st = make_map_pages(&mv, v_pages, dtype, num_pages, heads_kv, page_size, p.c.v_sp, p.c.v_sh, p.c.v_st,
-                           kBoxRows, 2, "v_pages")) != SABRE_OK)
-    return st;
-  const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  const cudaError_t e = dtype == SABRE_BF16 ? launch_paged_decode<__nv_bfloat16>(mk, mv, p, s)
-                                            : launch_paged_decode<__half>(mk, mv, p, s);
-  return e == cudaSuccess ? SABRE_OK : sabre_cuda_fail(e, fn);
+  return decode_call(fn, q, k_pages, v_pages, o, page_table, seq_lens, &l, batch, heads_q, heads_kv, head_dim, num_pages,
+                page_size, max_pages, -1, 0, q_strides, kp_strides, vp_strides, o_strides, table_stride,
+                softmax_scale, dtype, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

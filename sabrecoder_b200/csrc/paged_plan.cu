@@ -1,0 +1,217 @@
+// Block tables and slot maps of a paged cache, built on the device from request
+// lengths: a step that makes room for its own rows can be captured whole.
+//
+// Sequence b goes from len_b to len_b + new_b rows and owns ceil(. / page_size)
+// pages before and after; the i-th page that the batch needs (by sequence, then
+// position) is free_pages[free_count - 1 - i]. Row r of sequence b (its rows
+// follow those of the sequences before it) is at position pos = len_b + r -
+// q_start[b], in slot table[b][pos / page_size] * page_size + pos % page_size.
+//
+// Reads 8 bytes a sequence and writes 16 a row: a call is bound by its launch
+// and by the chain lengths -> prefix sums -> table or free page -> slot. One
+// cluster of up to eight CTAs does it: each sums the whole batch for itself (in
+// shared memory, so that rows and pages find their sequence by bisection), and
+// the cluster's barrier keeps the new lengths and the new count from being
+// written over the old ones before every CTA has read them. Separate kernels for
+// the plan and the rows would cost a second launch, a grid-wide counter memory
+// that is zero before every call.
+namespace sabre {
+namespace paged {
+namespace plan {
+
+constexpr int kThreads = 512;
+constexpr int kMaxCtas = 8;         // of the cluster: the portable size
+constexpr int kMaxBatch = 16384;    // three ints of shared memory a sequence
+constexpr int kCtaRows = 4 * kThreads;  // rows that make another CTA worth its place
+
+struct Params {
+  const int32_t* fresh;  // new rows of each sequence
+  const int32_t* lens;
+  const int32_t* free_pages;
+  const int32_t* free_count;
+  int32_t* table;
+  int32_t* lens_out;
+  int32_t* count_out;
+  int32_t* q_start;
+  long long* slots;
+  long long* positions;
+  long long table_sb;
+  int batch, max_pages, page_shift, num_pages, free_size, rows;
+};
+
+// Inclusive sum over the CTA of two counts at once; scratch: 2 * kThreads / 32.
+__device__ __forceinline__ void scan2(long long& a, long long& b, long long* scratch, long long& all_a,
+                                      long long& all_b) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int s = 1; s < 32; s <<= 1) {
+    const long long ua = __shfl_up_sync(0xffffffffu, a, s), ub = __shfl_up_sync(0xffffffffu, b, s);
+    if (lane >= s) a += ua, b += ub;
+  }
+  if (lane == 31) scratch[2 * warp] = a, scratch[2 * warp + 1] = b;
+  __syncthreads();
+  all_a = all_b = 0;
+  long long before_a = 0, before_b = 0;
+#pragma unroll
+  for (int w = 0; w < kThreads / 32; ++w) {
+    if (w == warp) before_a = all_a, before_b = all_b;
+    all_a += scratch[2 * w], all_b += scratch[2 * w + 1];
+  }
+  a += before_a;
+  b += before_b;
+}
+
+// The last i in [0, n) with first[i] <= x; first ascends from first[0] <= x.
+__device__ __forceinline__ int last_at(const int* first, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    (first[mid] <= x ? lo : hi) = mid;
+  }
+  return lo;
+}
+
+__global__ void __launch_bounds__(kThreads) paged_extend_kernel(const Params p) {
+  extern __shared__ int s_seq[];  // [3][batch]: rows and pages before the sequence, its old length
+  __shared__ long long s_scan[2 * kThreads / 32];
+  int* const s_rows = s_seq;
+  int* const s_pages = s_seq + p.batch;
+  int* const s_len = s_seq + 2 * p.batch;
+  const int tid = threadIdx.x;
+  if (tid == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int ps1 = (1 << p.page_shift) - 1;
+  const long long capacity = static_cast<long long>(p.max_pages) << p.page_shift;
+  auto page = [&](int id) -> int {
+    if (id < -1 || id >= p.num_pages) record_status(SABRE_DEV_BAD_PAGE);
+    return id >= 0 && id < p.num_pages ? id : -1;
+  };
+  auto have = [&](int len) -> int { return (len + ps1) >> p.page_shift; };
+
+  const int per = (p.batch + kThreads - 1) / kThreads;
+  const int b0 = min(tid * per, p.batch), b1 = min(b0 + per, p.batch);
+  const int count = *p.free_count;
+  long long rows = 0, pages = 0;
+  bool bad = count < 0 || count > p.free_size;
+  for (int b = b0; b < b1; ++b) {
+    const int len = p.lens[b], fresh = p.fresh[b];
+    // Refused below, with nothing of it used.
+    if (len < 0 || fresh < 0 || static_cast<long long>(len) + fresh > capacity) {
+      bad = true;
+      continue;
+    }
+    s_len[b] = len;
+    rows += fresh;
+    pages += have(len + fresh) - have(len);
+  }
+  long long row = rows, pg = pages, all_rows, all_pages;
+  scan2(row, pg, s_scan, all_rows, all_pages);
+  bad = __syncthreads_or(bad) != 0;
+  // A call that does not fit changes nothing and has no rows.
+  bad = bad || all_pages > count || all_rows > p.rows;
+  // Every CTA has read the old lengths and the old count.
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  if (!bad) {
+    row -= rows;
+    pg -= pages;
+    for (int b = b0; b < b1; ++b) {
+      s_rows[b] = static_cast<int>(row);
+      s_pages[b] = static_cast<int>(pg);
+      const int fresh = p.fresh[b];  // lens_out may not be fresh (refused on the host)
+      row += fresh;
+      pg += have(s_len[b] + fresh) - have(s_len[b]);
+    }
+  }
+  __syncthreads();
+  const int total = bad ? 0 : static_cast<int>(all_rows);
+  const int step = gridDim.x * kThreads;
+  for (int r = blockIdx.x * kThreads + tid; r < p.rows; r += step) {
+    long long slot = -1, pos = 0;
+    if (r < total) {
+      const int b = last_at(s_rows, p.batch, r);
+      const int at = s_len[b] + r - s_rows[b];
+      const int col = at >> p.page_shift, new_col = col - have(s_len[b]);
+      const int id = page(new_col < 0 ? p.table[b * p.table_sb + col] : p.free_pages[count - 1 - s_pages[b] - new_col]);
+      pos = at;
+      if (id >= 0) slot = (static_cast<long long>(id) << p.page_shift) + (at & ps1);
+    }
+    p.slots[r] = slot;
+    p.positions[r] = pos;
+  }
+  // Columns that no row's look-up above reads.
+  const int need = bad ? 0 : static_cast<int>(all_pages);
+  for (int i = blockIdx.x * kThreads + tid; i < need; i += step) {
+    const int b = last_at(s_pages, p.batch, i);
+    p.table[b * p.table_sb + have(s_len[b]) + i - s_pages[b]] = page(p.free_pages[count - 1 - i]);
+  }
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+  if (blockIdx.x == 0) {
+    if (tid == 0) {
+      if (bad) record_status(SABRE_DEV_NO_ROOM);
+      p.q_start[p.batch] = total;
+      *p.count_out = bad ? count : count - need;
+    }
+    for (int b = tid; b < p.batch; b += kThreads) {
+      p.q_start[b] = bad ? 0 : s_rows[b];
+      p.lens_out[b] = bad ? p.lens[b] : s_len[b] + (b + 1 < p.batch ? s_rows[b + 1] : total) - s_rows[b];
+    }
+  }
+}
+
+}  // namespace plan
+}  // namespace paged
+}  // namespace sabre
+
+extern "C" int sabre_paged_extend(const int32_t* new_rows, int32_t* page_table, const int32_t* seq_lens,
+                                  int32_t* seq_lens_out, const int32_t* free_pages, const int32_t* free_count,
+                                  int32_t* free_count_out, int32_t* q_start, int64_t* slots, int64_t* positions,
+                                  int rows, int batch, int num_pages, int page_size, int max_pages, int free_size,
+                                  int64_t table_stride, void* stream) {
+  using namespace sabre::paged;
+  const char* fn = "sabre_paged_extend";
+  if (!new_rows || !page_table || !seq_lens || !seq_lens_out || !free_count || !free_count_out || !q_start ||
+      (free_size > 0 && !free_pages) || (rows > 0 && (!slots || !positions)))
+    return sabre_fail(SABRE_ERR_INVALID_ARG, "%s: null pointer argument", fn);
+  if (new_rows == seq_lens_out)  // CTAs still read the one when the other is written
+    return sabre_fail(SABRE_ERR_INVALID_ARG, "%s: new_rows and seq_lens_out are the same", fn);
+  if (rows < 0 || batch <= 0 || num_pages <= 0 || max_pages <= 0 || free_size < 0)
+    return sabre_fail(SABRE_ERR_INVALID_ARG, "%s: sizes must be positive", fn);
+  if (page_size < 16 || page_size > 1024 || (page_size & (page_size - 1)) != 0)
+    return sabre_fail(SABRE_ERR_UNSUPPORTED, "%s: page_size %d (a power of two from 16 to 1024)", fn, page_size);
+  if (static_cast<long long>(page_size) * max_pages > kMaxRows)
+    return sabre_fail(SABRE_ERR_UNSUPPORTED, "%s: page_size * max_pages exceeds 2^30 rows", fn);
+  if (batch > plan::kMaxBatch)
+    return sabre_fail(SABRE_ERR_UNSUPPORTED, "%s: %d sequences (at most %d)", fn, batch, plan::kMaxBatch);
+  if (table_stride < (batch > 1 ? max_pages : 0))
+    return sabre_fail(SABRE_ERR_INVALID_ARG, "%s: page_table rows overlap (stride %lld < %d)", fn,
+                      static_cast<long long>(table_stride), max_pages);
+  if (rows > 1 << 30) return sabre_fail(SABRE_ERR_UNSUPPORTED, "%s: more than 2^30 rows", fn);
+  plan::Params p;
+  p.fresh = new_rows;
+  p.lens = seq_lens;
+  p.free_pages = free_pages;
+  p.free_count = free_count;
+  p.table = page_table;
+  p.lens_out = seq_lens_out;
+  p.count_out = free_count_out;
+  p.q_start = q_start;
+  p.slots = reinterpret_cast<long long*>(slots);
+  p.positions = reinterpret_cast<long long*>(positions);
+  p.table_sb = table_stride;
+  p.batch = batch;
+  p.max_pages = max_pages;
+  p.page_shift = 0;
+  while ((1 << p.page_shift) < page_size) ++p.page_shift;
+  p.num_pages = num_pages;
+  p.free_size = free_size;
+  p.rows = rows;
+  int ctas = 1;
+  while (ctas < plan::kMaxCtas && rows > ctas * plan::kCtaRows) ctas *= 2;
+  const int smem = 3 * batch * static_cast<int>(sizeof(int));
+  cudaError_t e = cudaFuncSetAttribute(plan::paged_extend_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       3 * plan::kMaxBatch * static_cast<int>(sizeof(int)));
+  if (e != cudaSuccess) return sabre_cuda_fail(e, fn);
+  e = launch_cluster(dim3(ctas), ctas, plan::kThreads, smem, static_cast<cudaStream_t>(stream),
+                     plan::paged_extend_kernel, p);
+  return e == cudaSuccess ? SABRE_OK : sabre_cuda_fail(e, fn);
+}

@@ -88,7 +88,16 @@ struct Params {
   int box_shift, slots;               // slots: row tiles of the grid
   int head_major, ctas;               // ctas: of a call in shares, else 0
   float scale_log2;
+  // kListed: a row tile is a query block and reads the pages of its list, in
+  // `parts` equal parts of its key tiles (64 list rows each). A part's place is
+  // pair * parts + part, and joins[2 * pair + 1] holds the pair's rows.
+  Lists lists;
+  int parts;
 };
+
+// What a CTA works on: a whole pair of row tile and KV head, a share of all key
+// tiles, or a part of a pair's listed pages.
+enum Mode { kWholePairs, kInShares, kOverLists };
 
 // P = 2^(x * sl2 - moff) for one row of 64 scores (-inf gives 0), rounded to the
 // storage type and stored at column `col` of tensor memory, half a row at a time
@@ -153,63 +162,11 @@ __device__ __forceinline__ Job make_job(const Params& p, int b, int r, int first
   return job;
 }
 
-// Exclusive prefix sum over the CTA's threads; scratch: 8 ints. `all`: the total.
-__device__ __forceinline__ int prefix_sum(int mine, int* scratch, int& all) {
-  const int tid = threadIdx.x;
-  int incl = mine;
-#pragma unroll
-  for (int s = 1; s < 32; s <<= 1) {
-    const int up = __shfl_up_sync(0xffffffffu, incl, s);
-    if ((tid & 31) >= s) incl += up;
-  }
-  __syncthreads();  // scratch is free
-  if ((tid & 31) == 31) scratch[tid >> 5] = incl;
-  __syncthreads();
-  int before = 0;
-  all = 0;
-#pragma unroll
-  for (int w = 0; w < kThreads / 32; ++w) {
-    before += w < (tid >> 5) ? scratch[w] : 0;
-    all += scratch[w];
-  }
-  return before + incl - mine;
-}
-
 // Row tile `slot` of the batch, found by the whole CTA; scratch: 16 ints.
 __device__ __forceinline__ bool find_job(const Params& p, int slot, int* scratch, Job& job) {
-  const int tid = threadIdx.x;
-  const int per = (p.c.batch + kThreads - 1) / kThreads;
-  const int b0 = min(tid * per, p.c.batch), b1 = min(b0 + per, p.c.batch);
-  // The first length comes with the starts, not after them: one round trip
-  // for as many sequences as threads.
-  const int len0 = b0 < b1 ? p.c.seq_lens[b0] : 0;
-  int mine = 0;
-  for (int b = b0; b < b1; ++b) {
-    const int len = row_start(p.starts, b + 1, p.rows) - row_start(p.starts, b, p.rows);
-    mine += (max(len, 0) + p.tokens - 1) / p.tokens;
-  }
-  if (tid == 0) scratch[8] = -1;
-  int all = 0;
-  int left = slot - prefix_sum(mine, scratch, all);
-  if (left >= 0 && left < mine) {
-    for (int b = b0; b < b1; ++b) {
-      const int first = row_start(p.starts, b, p.rows);
-      const int len = row_start(p.starts, b + 1, p.rows) - first;
-      const int nt = (max(len, 0) + p.tokens - 1) / p.tokens;
-      if (left < nt) {
-        scratch[8] = b;
-        scratch[9] = left * p.tokens;
-        scratch[10] = first;
-        scratch[11] = len;
-        scratch[12] = b == b0 ? len0 : p.c.seq_lens[b];
-        break;
-      }
-      left -= nt;
-    }
-  }
-  __syncthreads();
-  if (scratch[8] < 0) return false;
-  job = make_job(p, scratch[8], scratch[9], scratch[10], scratch[11], scratch[12]);
+  RowTile t;
+  if (!find_rows<kThreads>(p.c, p.starts, p.rows, p.tokens, slot, scratch, t)) return false;
+  job = make_job(p, t.b, t.r, t.first, t.len, t.length);
   return true;
 }
 
@@ -251,7 +208,7 @@ __device__ __forceinline__ bool find_share(const Params& p, int* seq, int* scrat
     seq[2 * kShareBatch + tid] = p.c.seq_lens[tid];
   }
   int nslots = 0;
-  const int before = prefix_sum(slots, scratch, nslots);
+  const int before = prefix_sum<kThreads>(slots, scratch, nslots);
   if (tid < p.c.batch) first_slot[tid] = before;
   __syncthreads();
   auto sequence = [&](int slot) -> int {  // the last b with first_slot[b] <= slot
@@ -271,7 +228,7 @@ __device__ __forceinline__ bool find_share(const Params& p, int* seq, int* scrat
   int mine = 0;
   for (int s = s0; s < s1; ++s) mine += job_of(s).tiles;
   int all = 0;
-  const int ahead = prefix_sum(mine, scratch, all);
+  const int ahead = prefix_sum<kThreads>(mine, scratch, all);
   const int units = p.heads_kv * p.group * (kD / 8);  // 16-byte stores of a row
   for (int s = blockIdx.x; s < p.slots; s += p.ctas) {
     const Job job = s < nslots ? job_of(s) : Job{};
@@ -312,7 +269,7 @@ __device__ __forceinline__ bool find_share(const Params& p, int* seq, int* scrat
   sh.whole = slack <= kSlack;
   if (sh.whole) {
     int parts_all = 0;
-    int left = static_cast<int>(blockIdx.x) - prefix_sum(mine_parts, scratch, parts_all) * p.heads_kv;
+    int left = static_cast<int>(blockIdx.x) - prefix_sum<kThreads>(mine_parts, scratch, parts_all) * p.heads_kv;
     sh.ctas = parts_all * p.heads_kv;
     if (static_cast<int>(blockIdx.x) >= sh.ctas) return false;
     if (left >= 0 && left < mine_parts * p.heads_kv) {
@@ -358,11 +315,12 @@ __device__ __forceinline__ bool find_share(const Params& p, int* seq, int* scrat
   return true;
 }
 
-// kShares: the CTA walks a share of all key tiles; else it owns a whole pair.
-template <typename T, bool kShares>
+template <typename T, Mode kMode>
 __global__ void __launch_bounds__(kThreads, 2)
     paged_prefill_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                          const __grid_constant__ CUtensorMap tmV, const Params p) {
+  constexpr bool kShares = kMode == kInShares;
+  constexpr bool kListed = kMode == kOverLists;
   extern __shared__ __align__(1024) uint8_t smem[];
   const int tid = threadIdx.x;
   const int warp = tid >> 5;
@@ -400,8 +358,17 @@ __global__ void __launch_bounds__(kThreads, 2)
   RowPlace at;
   long long units = 0;  // key tiles of the share still to be done
   int hk = 0;
+  int block = 0, entries = 0;  // kListed: the query block and its list's length
   bool some;
-  if constexpr (kShares) {
+  if constexpr (kListed) {
+    // Later blocks of a sequence have no shorter lists: its heaviest first.
+    block = p.slots - 1 - static_cast<int>(blockIdx.x / p.parts);
+    hk = static_cast<int>(blockIdx.y);
+    some = find_job(p, block, scratch, job);
+    if (some && job.n > 0) entries = p.lists.count(block, hk);
+    if (p.parts > 1 && blockIdx.x % p.parts == 0 && tid == 0)
+      p.joins[2 * (block * p.heads_kv + hk) + 1] = some ? make_int4(job.row0, job.count, 0, 0) : make_int4(0, 0, 0, 0);
+  } else if constexpr (kShares) {
     some = find_share<T>(p, seq, scratch, sh, at);
     if (some) units = sh.units;
   } else {
@@ -434,6 +401,28 @@ __global__ void __launch_bounds__(kThreads, 2)
     // This segment: key tiles [j0, j0 + nt) of the pair.
     int j0 = 0, nt = job.tiles, place = 0;
     bool part = false;
+    if constexpr (kListed) {
+      const int part_id = static_cast<int>(blockIdx.x) % p.parts;
+      const long long all = ((static_cast<long long>(entries) << p.c.page_shift) + kTile - 1) / kTile;
+      j0 = static_cast<int>(all * part_id / p.parts);
+      nt = static_cast<int>(all * (part_id + 1) / p.parts) - j0;
+      part = p.parts > 1;
+      place = (block * p.heads_kv + hk) * p.parts + part_id;
+    }
+    // kListed: the position of box i of this part (all of it past the sequence or in
+    // no page: kNowhere) and its page there, or -1.
+    constexpr int kNowhere = INT_MAX - 64;
+    auto listed_box = [&](int i, int& page) -> int {
+      page = -1;
+      const int row = j0 * kTile + (i << p.box_shift);
+      const int e = row >> p.c.page_shift;
+      if (i >= nt * boxes || e >= entries) return kNowhere;
+      const int col = p.lists.column(block, hk, e, p.c);
+      const int t = (col << p.c.page_shift) + (row & ((1 << p.c.page_shift) - 1));
+      if (col < 0 || t >= job.n) return kNowhere;
+      page = p.c.page_of(job.b, t);
+      return page >= 0 ? t : kNowhere;
+    };
     if constexpr (kShares) {
       if (segment > 0) {
         at.tile = 0;
@@ -495,7 +484,15 @@ __global__ void __launch_bounds__(kThreads, 2)
       for (int i0 = 0; ok && i0 < nt * boxes; i0 += 32) {
         // The pages of the next 32 boxes, one per lane; num_pages reads zeros.
         int page = p.c.num_pages, off = 0;
-        if (i0 + lane < nt * boxes) {
+        int at = kNowhere;  // kListed: the box's position
+        if constexpr (kListed) {
+          int pg;
+          at = listed_box(i0 + lane, pg);
+          if (pg >= 0) {
+            page = pg;
+            off = at & ((1 << p.c.page_shift) - 1);
+          }
+        } else if (i0 + lane < nt * boxes) {
           const int t = job.pos(j0 + (i0 + lane) / boxes) + (((i0 + lane) % boxes) << p.box_shift);
           off = t & ((1 << p.c.page_shift) - 1);
           if (job.any(p.w, t, box_rows)) {
@@ -518,7 +515,12 @@ __global__ void __launch_bounds__(kThreads, 2)
           // Rows of V that none of this CTA's rows sees (past the end, before the
           // window) but that share a box with some that one does are zeroed.
           unsigned long long hidden = 0;
-          if (!is_k) {
+          if (kListed && !is_k) {
+            for (int x = 0; x < boxes; ++x) {  // all of a box that is nowhere is zero already
+              const int rows = job.n - __shfl_sync(0xffffffffu, at, i - i0 + x);
+              if (rows > 0 && rows < box_rows) hidden |= (low_bits(box_rows) & ~low_bits(rows)) << (x << p.box_shift);
+            }
+          } else if (!is_k) {
             const int t = job.pos(j0 + j);
             hidden = ~low_bits(job.n - t) | (low_bits(job.lo - t) & ~low_bits(p.w.prefix - t));
             for (int x = 0; x < boxes && hidden != 0ull; ++x) {  // a box that is hidden as a whole is zero already
@@ -637,17 +639,30 @@ __global__ void __launch_bounds__(kThreads, 2)
       bool ok = going;
       // Absent pages are not visible: the boxes of the next 32 / boxes tiles are
       // looked up by the lanes, a batch ahead.
+      // kListed: the boxes' positions instead, and which boxes all rows of the warp
+      // see whole.
+      int at_ahead = 0, at = 0;
       auto lookup = [&](int i) -> int {
+        if constexpr (kListed) {
+          int pg;
+          at_ahead = listed_box(i, pg);
+          return 0;
+        }
         const int t = job.pos(j0 + i / boxes) + ((i % boxes) << p.box_shift);
         return i < nt * boxes && job.any(p.w, t, box_rows) ? p.c.entry(job.b, t) : 0;
       };
       int entry_ahead = lookup(lane);
       uint32_t absent = 0;
       for (int j = 0; ok && j < nt; ++j) {
-        const int t = job.pos(j0 + j);
+        const int t = kListed ? 0 : job.pos(j0 + j);
         const int i = j * boxes;
         if ((i & 31) == 0) {
-          absent = __ballot_sync(0xffffffffu, p.c.checked(entry_ahead) < 0);
+          if constexpr (kListed) {
+            at = at_ahead;
+            absent = __ballot_sync(0xffffffffu, at + box_rows > all_seen);
+          } else {
+            absent = __ballot_sync(0xffffffffu, p.c.checked(entry_ahead) < 0);
+          }
           entry_ahead = lookup(i + 32 + lane);
         }
         const uint32_t missing = (absent >> (i & 31)) & ((1u << boxes) - 1u);
@@ -655,7 +670,17 @@ __global__ void __launch_bounds__(kThreads, 2)
         // masks left out there: 592 -> 574 us for the prompt below).
         unsigned long long see = ~0ull;
         bool dead = false;
-        if (t + kTile > all_seen || (t < all_wlo && t + kTile > p.w.prefix) || missing != 0u) {
+        if constexpr (kListed) {
+          if (missing != 0u) {
+#pragma unroll 1
+            for (int x = 0; x < boxes; ++x) {
+              const int bt = __shfl_sync(0xffffffffu, at, (i & 31) + x);
+              const unsigned long long box = low_bits(box_rows);
+              see &= ~((box & ~low_bits(seen - bt)) << (x << p.box_shift));
+            }
+            dead = __all_sync(0xffffffffu, see == 0ull);
+          }
+        } else if (t + kTile > all_seen || (t < all_wlo && t + kTile > p.w.prefix) || missing != 0u) {
           see = low_bits(seen - t) & (~low_bits(wlo - t) | low_bits(p.w.prefix - t));
           if (missing != 0u) {
 #pragma unroll 1
@@ -752,7 +777,7 @@ __global__ void __launch_bounds__(kThreads, 2)
                                               __uint_as_float(ov[8 * q4 + 2 * e + 1]) * inv);
           return make_uint4(w[0], w[1], w[2], w[3]);
         };
-        if (!kShares && nt >= 1) {
+        if (!kShares && !part && nt >= 1) {
           // Every S is done, so the Q tile is free: the warp turns its rows in
           // their place and writes two whole rows at a time (windowed prompts 767
           // -> 752 us). In shares the next Q may be on its way there already.
@@ -842,13 +867,6 @@ __global__ void __launch_bounds__(256) paged_combine_kernel(const Params p) {
                lane, sum.a, sum.l);
 }
 
-// Row tiles that `rows` rows of `batch` sequences need at most: a sequence of
-// l > 0 rows takes (l - 1) / tokens + 1.
-static inline long long row_slots(int rows, int batch, int tokens) {
-  const int k = rows < batch ? rows : batch;
-  return static_cast<long long>(rows - k) / tokens + k;
-}
-
 // Whether a call runs in shares, as far as the host can tell: by the pairs (row
 // tile, KV head) there may be and the key tiles of one, counted for a row tile
 // in the middle of its sequence's new rows. The table's width stands for the
@@ -897,6 +915,38 @@ static bool in_shares(int rows, int batch, int heads_q, int heads_kv, int page_s
 static constexpr size_t kShareWorkspace =
     kMaxPairs * 2 * sizeof(int4) + static_cast<size_t>(2) * kDecCtas * kRows * (kD + 2) * sizeof(float);
 
+// Joins the parts of pair (block, KV head) blockIdx.x of a call over lists.
+template <typename T>
+__global__ void __launch_bounds__(256) paged_combine_listed_kernel(const Params p) {
+  if (threadIdx.x == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int lane = threadIdx.x & 31;
+  const int row = blockIdx.y * 8 + (threadIdx.x >> 5);
+  const int4 rows = p.joins[2ll * blockIdx.x + 1];
+  const int tok = row / p.group;
+  if (tok >= rows.y) return;
+  PartSum sum;
+  sum.add_parts(p.part_ml, p.part_acc, 0, 1, p.parts, lane, [&](int i) -> long long {
+    return (static_cast<long long>(blockIdx.x) * p.parts + i) * kRows + row;
+  });
+  store_row<T>(static_cast<T*>(p.o) + static_cast<long long>(rows.x + tok) * p.o_sr +
+                   (static_cast<int>(blockIdx.x) % p.heads_kv * p.group + row - tok * p.group) * p.o_sh,
+               lane, sum.a, sum.l);
+}
+
+// Parts that each pair of a call over lists is cut into: as many as leave every
+// CTA kMinShare key tiles and no more CTAs than two an SM, when that is two or
+// more.
+static inline int listed_parts(long long pairs, int page_size, int entries) {
+  const long long tiles = (static_cast<long long>(page_size) * entries + kTile - 1) / kTile;
+  const long long parts = kDecCtas / pairs < tiles / kMinShare ? kDecCtas / pairs : tiles / kMinShare;
+  return parts < 1 ? 1 : static_cast<int>(parts);
+}
+
+static inline size_t listed_workspace(long long pairs, int parts) {
+  return parts <= 1 ? 0 : pairs * (2 * sizeof(int4) + static_cast<size_t>(parts) * kRows * (kD + 2) * sizeof(float));
+}
+
 // Tensor map of q [rows, Hq, D]: dims (128 d, g heads of a group, rows, KV
 // heads); box = (64 d, g, tokens, 1): one d-half of a row tile, token by token.
 static int make_map_q(CUtensorMap* m, const void* q, int dtype, int rows, int heads_kv, int group, int tokens,
@@ -923,7 +973,7 @@ template <typename T>
 static cudaError_t launch(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Params& p,
                           cudaStream_t s) {
   const int smem = p.ctas > 0 ? kShareSmemBytes : kSmemBytes;
-  auto kernel = p.ctas > 0 ? paged_prefill_kernel<T, true> : paged_prefill_kernel<T, false>;
+  auto kernel = p.ctas > 0 ? paged_prefill_kernel<T, kInShares> : paged_prefill_kernel<T, kWholePairs>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != cudaSuccess) return e;
   const dim3 grid = p.ctas > 0 ? dim3(p.ctas) : p.head_major ? dim3(p.slots, p.heads_kv) : dim3(p.heads_kv, p.slots);
@@ -931,6 +981,18 @@ static cudaError_t launch(const CUtensorMap& mq, const CUtensorMap& mk, const CU
   if (e != cudaSuccess || p.ctas == 0) return e;
   const int tile_rows = (p.rows < p.tokens ? p.rows : p.tokens) * p.group;
   return launch_dependent(dim3(p.slots * p.heads_kv, (tile_rows + 7) / 8), 256, 0, s, paged_combine_kernel<T>, p);
+}
+
+template <typename T>
+static cudaError_t launch_listed(const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, const Params& p,
+                                 cudaStream_t s) {
+  const auto kernel = paged_prefill_kernel<T, kOverLists>;
+  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+  if (e != cudaSuccess) return e;
+  e = launch_dependent(dim3(p.slots * p.parts, p.heads_kv), kThreads, kSmemBytes, s, kernel, mq, mk, mv, p);
+  if (e != cudaSuccess || p.parts == 1) return e;
+  const int tile_rows = (p.rows < p.tokens ? p.rows : p.tokens) * p.group;
+  return launch_dependent(dim3(p.slots * p.heads_kv, (tile_rows + 7) / 8), 256, 0, s, paged_combine_listed_kernel<T>, p);
 }
 
 }  // namespace pre
@@ -976,6 +1038,8 @@ int sabre_paged_prefill(const void* q, const void* k_pages, const void* v_pages,
   p.tokens = pre::kRows / p.group;
   p.box_shift = p.c.page_shift < 6 ? p.c.page_shift : 6;
   p.scale_log2 = scale_log2(softmax_scale);
+  p.lists = Lists{};
+  p.parts = 1;
   const bool shares =
       pre::in_shares(rows, batch, heads_q, heads_kv, page_size, max_pages, window, num_prefix_tokens);
   p.ctas = shares ? kDecCtas : 0;
@@ -986,7 +1050,7 @@ int sabre_paged_prefill(const void* q, const void* k_pages, const void* v_pages,
   p.joins = static_cast<int4*>(workspace);
   p.part_acc = shares ? reinterpret_cast<float*>(p.joins + 2 * pre::kMaxPairs) : nullptr;
   p.part_ml = shares ? p.part_acc + static_cast<size_t>(2) * kDecCtas * pre::kRows * kD : nullptr;
-  const long long slots = pre::row_slots(rows, batch, p.tokens);
+  const long long slots = row_slots(rows, batch, p.tokens);
   // The rule of prefill_bsa.cu: K/V larger than this -> head-major order.
   const long long kv_bytes = 4ll * heads_kv * kD * batch * page_size * max_pages;
   p.head_major = kv_bytes > (112ll << 20) || slots > 65535 ? 1 : 0;
@@ -1003,6 +1067,80 @@ int sabre_paged_prefill(const void* q, const void* k_pages, const void* v_pages,
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t e = dtype == SABRE_BF16 ? pre::launch<__nv_bfloat16>(mq, mk, mv, p, s)
                                             : pre::launch<__half>(mq, mk, mv, p, s);
+  return e == cudaSuccess ? SABRE_OK : sabre_cuda_fail(e, fn);
+}
+
+size_t sabre_paged_prefill_listed_workspace_size(int rows, int batch, int heads_q, int heads_kv, int head_dim,
+                                                 int page_size, int query_block, int list_entries) {
+  using namespace sabre::paged;
+  if (rows <= 0 || batch <= 0 || heads_q <= 0 || heads_kv <= 0 || head_dim != kD || heads_q % heads_kv != 0 ||
+      page_size <= 0 || query_block <= 0 || list_entries <= 0)
+    return 0;
+  const long long pairs = row_slots(rows, batch, query_block) * heads_kv;
+  return pre::listed_workspace(pairs, pre::listed_parts(pairs, page_size, list_entries));
+}
+
+int sabre_paged_prefill_listed(const void* q, const void* k_pages, const void* v_pages, void* o,
+                               const int32_t* page_table, const int32_t* seq_lens, const int32_t* q_start,
+                               const int32_t* lists, const int32_t* counts, int list_entries, int rows, int batch,
+                               int heads_q, int heads_kv, int head_dim, int num_pages, int page_size, int max_pages,
+                               int query_block, const int64_t* q_strides, const int64_t* kp_strides,
+                               const int64_t* vp_strides, const int64_t* o_strides, const int64_t* list_strides,
+                               const int64_t* count_strides, int64_t table_stride, float softmax_scale, int dtype,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace sabre::paged;
+  const char* fn = "sabre_paged_prefill_listed";
+  if (!q_start) return sabre_fail(SABRE_ERR_INVALID_ARG, "%s: null pointer argument", fn);
+  pre::Params p;
+  int st = make_cache(&p.c, fn, k_pages, v_pages, page_table, seq_lens, batch, heads_kv, head_dim, num_pages,
+                      page_size, max_pages, kp_strides, vp_strides, table_stride, dtype);
+  if (st == SABRE_OK) st = check_queries(fn, q, o, heads_q, heads_kv, 0, q_strides, o_strides);
+  if (st == SABRE_OK) st = make_lists(&p.lists, fn, lists, counts, list_entries, list_strides, count_strides);
+  if (st != SABRE_OK) return st;
+  if (rows <= 0) return sabre_fail(SABRE_ERR_INVALID_ARG, "%s: rows must be positive", fn);
+  if (query_block <= 0 || query_block > pre::kRows || query_block * (heads_q / heads_kv) > pre::kRows)
+    return sabre_fail(SABRE_ERR_UNSUPPORTED, "%s: query_block %d times %d heads of a group (from 1 to %d rows)", fn,
+                      query_block, heads_q / heads_kv, pre::kRows);
+  if (static_cast<long long>(page_size) * list_entries > kMaxRows)
+    return sabre_fail(SABRE_ERR_UNSUPPORTED, "%s: page_size * list entries exceeds 2^30 rows", fn);
+  p.w = Window{-1, 0};
+  p.starts = q_start;
+  p.o = o;
+  p.o_sr = o_strides[0];
+  p.o_sh = o_strides[1];
+  p.rows = rows;
+  p.heads_kv = heads_kv;
+  p.group = heads_q / heads_kv;
+  p.tokens = query_block;
+  p.box_shift = p.c.page_shift < 6 ? p.c.page_shift : 6;
+  p.scale_log2 = scale_log2(softmax_scale);
+  p.ctas = 0;
+  p.head_major = 0;
+  const long long slots = row_slots(rows, batch, query_block), pairs = slots * heads_kv;
+  p.parts = pre::listed_parts(pairs, page_size, list_entries);
+  if (slots * p.parts > INT_MAX || pairs > INT_MAX)
+    return sabre_fail(SABRE_ERR_UNSUPPORTED, "%s: too many query blocks", fn);
+  const size_t need = pre::listed_workspace(pairs, p.parts);
+  if (need > 0 && (!workspace || workspace_bytes < need))
+    return sabre_fail(SABRE_ERR_WORKSPACE, "%s: workspace %zu < %zu bytes", fn, workspace_bytes, need);
+  if (need > 0 && !aligned16(workspace))
+    return sabre_fail(SABRE_ERR_ALIGNMENT, "%s: workspace must be 16-byte aligned", fn);
+  p.joins = need > 0 ? static_cast<int4*>(workspace) : nullptr;
+  p.part_acc = need > 0 ? reinterpret_cast<float*>(p.joins + 2 * pairs) : nullptr;
+  p.part_ml = need > 0 ? p.part_acc + static_cast<size_t>(pairs) * p.parts * pre::kRows * kD : nullptr;
+  p.slots = static_cast<int>(slots);
+  CUtensorMap mq, mk, mv;
+  if ((st = pre::make_map_q(&mq, q, dtype, rows, heads_kv, p.group, p.tokens, q_strides[0], q_strides[1])) != SABRE_OK)
+    return st;
+  if ((st = make_map_pages(&mk, k_pages, dtype, num_pages, heads_kv, page_size, p.c.k_sp, p.c.k_sh, p.c.k_st,
+                           1 << p.box_shift, 1, "k_pages")) != SABRE_OK)
+    return st;
+  if ((st = make_map_pages(&mv, v_pages, dtype, num_pages, heads_kv, page_size, p.c.v_sp, p.c.v_sh, p.c.v_st,
+                           1 << p.box_shift, 1, "v_pages")) != SABRE_OK)
+    return st;
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  const cudaError_t e = dtype == SABRE_BF16 ? pre::launch_listed<__nv_bfloat16>(mq, mk, mv, p, s)
+                                            : pre::launch_listed<__half>(mq, mk, mv, p, s);
   return e == cudaSuccess ? SABRE_OK : sabre_cuda_fail(e, fn);
 }
 

@@ -8,6 +8,7 @@
 #include <cstdlib>
 #include <cstring>
 #include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 #include "prefill_bsa.cu"
@@ -101,6 +102,8 @@ static int ensure_smem_attr(Kern kern, int bytes) {
 #include "decode_gqa.cu"
 #include "qkv_prefill.cu"
 #include "paged_cache.cu"
+#include "paged_plan.cu"
+#include "paged_select.cu"
 #include "paged_decode.cu"
 #include "paged_prefill.cu"
 

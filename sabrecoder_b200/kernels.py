@@ -665,6 +665,245 @@ def paged_prefill(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                    num_prefix_tokens, softmax_scale, out, workspace)
 
 
+# -- steps without the host, and attention over selected pages
+
+def _refuse_tables(what: str, page_table, seq_lens, q_start, ints: dict, **others) -> None:
+    """Raises for what is wrong with the tables of a paged call; ``ints``: {name:
+    (tensor, entries)} of further int32 vectors, ``others``: tensors that must be on
+    the tables' device. Returns when nothing is."""
+    for name, t in (("page_table", page_table), ("seq_lens", seq_lens)):
+        if not isinstance(t, torch.Tensor):
+            raise SabreError(f"{what}: {name} must be a tensor (got {type(t).__name__})")
+    if page_table.dim() != 2 or page_table.shape[1] < 1 or (page_table.shape[1] > 1 and page_table.stride(1) != 1):
+        raise SabreError(f"{what}: page_table {tuple(page_table.shape)} must be [B, max_pages >= 1] with unit column "
+                         f"stride")
+    B = page_table.shape[0]
+    _i32(page_table, "page_table")
+    for name, (t, n) in dict(seq_lens=(seq_lens, B), q_start=(q_start, B + 1), **ints).items():
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor) or t.dim() != 1 or (n is not None and t.shape[0] != n) or \
+                not t.is_contiguous():
+            shape = tuple(t.shape) if isinstance(t, torch.Tensor) else type(t).__name__
+            raise SabreError(f"{what}: {name} {shape} must be a contiguous [{'N' if n is None else n}]")
+        _i32(t, name)
+        others[name] = t
+    _need_cuda(page_table=page_table, **others)
+    for name, t in others.items():
+        if t is not None and t.device != page_table.device:
+            raise SabreError(f"{what}: {name} is on {t.device}, page_table is on {page_table.device}")
+
+
+def _size(what: str, name: str, value: int, low: int) -> int:
+    """An argument as the C ABI's int; values past int32 are held there."""
+    if value < low:
+        raise SabreError(f"{what}: {name} {value} must be at least {low}")
+    return min(int(value), 2 ** 31 - 1)
+
+
+def paged_extend(new_rows: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, free_pages: torch.Tensor,
+                 free_count: torch.Tensor, *, page_size: int, num_pages: int, num_rows: int,
+                 seq_lens_out: Optional[torch.Tensor] = None, free_count_out: Optional[torch.Tensor] = None
+                 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Block tables and slot maps from request lengths, without the host.
+
+    new_rows int32 ``[B]``: rows that each sequence grows by; page_table int32
+    ``[B, max_pages]`` and seq_lens int32 ``[B]``: the sequences as they are;
+    free_pages int32 ``[F]`` and free_count int32 ``[1]``: a stack of free pages,
+    the last of ``free_pages[:free_count]`` taken first. Writes the new pages into
+    page_table and the new lengths and count into ``seq_lens_out`` and
+    ``free_count_out`` (default: in place). num_rows: room for rows, at least the
+    sum of new_rows (known on the host, as a captured batch's is).
+
+    Returns ``(q_start int32 [B + 1], slots int64 [num_rows], positions int64
+    [num_rows])``: row starts; each row's place ``page * page_size + row of the
+    page`` for :func:`paged_store_slots` and its position. Rows past the last have
+    slot -1 and position 0. When pages, table columns or num_rows are too few, or a
+    length is negative, nothing changes, every start is 0 and every slot -1, and
+    bit 8 of the device status is set."""
+    what = "paged_extend"
+    ps, pool = _size(what, "page_size", page_size, 1), _size(what, "num_pages", num_pages, 1)
+    rows = _size(what, "num_rows", num_rows, 0)
+    res = paged_call().extend(new_rows, page_table, seq_lens, free_pages, free_count, ps, pool, rows, seq_lens_out,
+                              free_count_out)
+    if res is None:
+        B = page_table.shape[0] if page_table.dim() else 0
+        _refuse_tables(what, page_table, seq_lens, None, dict(
+            new_rows=(new_rows, B), free_pages=(free_pages, None), free_count=(free_count, 1),
+            seq_lens_out=(seq_lens_out, B), free_count_out=(free_count_out, 1)))
+        raise SabreError(f"{what}: no sequences, or a size exceeds 2^31 - 1")
+    if type(res) is int:
+        check(res, "sabre_" + what)
+    LAUNCHES[0] += 1
+    return res
+
+
+def paged_store_slots(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
+                      slots: torch.Tensor) -> None:
+    """Writes new K/V rows ``[N, Hkv, D]`` into the places that
+    :func:`paged_extend` gave them: int64 ``slots`` ``[N]``. Rows with a negative
+    slot are dropped, as are those past the pool (recorded); no slot may be given
+    twice. Pools as in :func:`paged_store`."""
+    what = "paged_store_slots"
+    st = paged_call().store_slots(k, v, k_pages, v_pages, slots)
+    if st is None:
+        if k_pages.dim() != 4 or v_pages.shape != k_pages.shape:
+            raise SabreError(f"{what}: k_pages {tuple(k_pages.shape)} and v_pages {tuple(v_pages.shape)} must both be "
+                             f"[num_pages, Hkv, page_size, D]")
+        if k_pages.dtype not in DTYPE_CODE or any(t.dtype != k_pages.dtype for t in (k, v, v_pages)):
+            raise SabreError(f"{what}: rows and pages must share dtype bf16 or f16")
+        if k.dim() != 3 or v.shape != k.shape or k.shape[1] != k_pages.shape[1] or k.shape[2] != k_pages.shape[3]:
+            raise SabreError(f"{what}: k {tuple(k.shape)} and v {tuple(v.shape)} must both be [N, {k_pages.shape[1]}, "
+                             f"{k_pages.shape[3]}]")
+        if any(t.stride(-1) != 1 for t in (k, v, k_pages, v_pages)):
+            raise SabreError(f"{what}: rows and pages need unit last stride")
+        if not isinstance(slots, torch.Tensor) or slots.dtype != torch.int64 or tuple(slots.shape) != k.shape[:1] or \
+                not slots.is_contiguous():
+            raise SabreError(f"{what}: slots must be a contiguous int64 [{k.shape[0]}]")
+        _need_cuda(k_pages=k_pages, v_pages=v_pages, k=k, v=v, slots=slots)
+        raise SabreError(f"{what}: all tensors must be on {k_pages.device}, with sizes below 2^31")
+    if st < 0:
+        check(st, "sabre_" + what)
+    LAUNCHES[0] += st
+
+
+def paged_key_means(k_pages: torch.Tensor, key_means: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
+                    q_start: Optional[torch.Tensor] = None, *, num_rows: Optional[int] = None) -> None:
+    """Mean key of every page that the new rows fill, into key_means fp32
+    ``[num_pages, Hkv, D]`` (the means of other pages stay as they are).
+
+    The rows are in the pool already and as in :func:`paged_store`: the last
+    ``q_start[b+1] - q_start[b]`` of sequence b, or one each. num_rows: at least
+    ``q_start[B]`` (needed with q_start)."""
+    what = "paged_key_means"
+    if num_rows is None:
+        if q_start is not None:
+            raise SabreError(f"{what} needs num_rows with q_start")
+        num_rows = page_table.shape[0]
+    st = paged_call().key_means(k_pages, key_means, page_table, seq_lens, q_start, _size(what, "num_rows", num_rows, 0))
+    if st is None:
+        if k_pages.dim() != 4 or k_pages.dtype not in DTYPE_CODE or k_pages.stride(3) != 1:
+            raise SabreError(f"{what}: k_pages {tuple(k_pages.shape)} must be [num_pages, Hkv, page_size, D] bf16 or "
+                             f"f16 with unit head-dim stride")
+        _refuse_means(what, key_means, (k_pages.shape[0], k_pages.shape[1], k_pages.shape[3]))
+        _refuse_tables(what, page_table, seq_lens, q_start, {}, k_pages=k_pages, key_means=key_means)
+        if q_start is None:
+            raise SabreError(f"{what}: {num_rows} rows for {page_table.shape[0]} sequences need q_start")
+        raise SabreError(f"{what}: a size exceeds 2^31 - 1")
+    if st < 0:
+        check(st, "sabre_" + what)
+    LAUNCHES[0] += st
+
+
+def _refuse_means(what: str, key_means, shape) -> None:
+    if not isinstance(key_means, torch.Tensor) or key_means.dtype != torch.float32 or key_means.dim() != 3 or \
+            any(w is not None and n != w for n, w in zip(key_means.shape, shape)) or key_means.stride(2) != 1:
+        raise SabreError(f"{what}: key_means must be fp32 [num_pages, Hkv, D] with unit last stride, as the pages "
+                         f"{tuple('any' if w is None else w for w in shape)}")
+
+
+def paged_select(q: torch.Tensor, key_means: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor,
+                 q_start: Optional[torch.Tensor] = None, *, page_size: int, topk: int, query_block: int = 1,
+                 window_size: int = 0, num_prefix_tokens: int = 0) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Which pages each query block reads, as lists for
+    :func:`paged_decode_listed` and :func:`paged_prefill_listed`.
+
+    q: ``[N, Hq, D]``, rows as in :func:`paged_prefill` (without q_start as in
+    :func:`paged_decode`, blocks of one row). A query block is up to
+    ``query_block`` consecutive new rows of one sequence; for each KV head it reads
+    the pages of the first ``num_prefix_tokens`` tokens, those with a key at most
+    ``window_size`` before one of its queries (their own positions included) and
+    the ``topk`` others whose mean key has the largest product with the sum of the
+    block's queries (over its rows and the group's heads). Sums are 64 bits wide, a
+    score is rounded to fp32 once; equal scores go to the earlier page, NaN last.
+    Absent pages are left out.
+
+    Returns ``(lists int32 [blocks, Hkv, width], counts int32 [blocks, Hkv])``:
+    ascending columns of page_table, -1 behind the end. Blocks are numbered over the
+    batch; there are as many as the rows can make, those past the last empty."""
+    what = "paged_select"
+    sizes = (_size(what, "page_size", page_size, 1), _size(what, "topk", topk, 0),
+             _size(what, "query_block", query_block, 1), _size(what, "window_size", window_size, 0),
+             _size(what, "num_prefix_tokens", num_prefix_tokens, 0))
+    if q_start is None and query_block != 1:
+        raise SabreError(f"{what}: query blocks of {query_block} rows need q_start")
+    res = paged_call().select(q, key_means, page_table, seq_lens, q_start, *sizes)
+    if res is None:
+        if q.dim() != 3 or q.dtype not in DTYPE_CODE or q.stride(2) != 1:
+            raise SabreError(f"{what}: q {tuple(q.shape)} must be [N, Hq, D] bf16 or f16 with unit last stride")
+        _refuse_means(what, key_means, (None, None, q.shape[2]))
+        _refuse_tables(what, page_table, seq_lens, q_start, {}, q=q, key_means=key_means)
+        if q_start is None and q.shape[0] != page_table.shape[0]:
+            raise SabreError(f"{what}: {q.shape[0]} rows for {page_table.shape[0]} sequences need q_start")
+        raise SabreError(f"{what}: key_means of no heads, or a size exceeds 2^31 - 1")
+    if type(res) is int:
+        check(res, "sabre_" + what)
+    LAUNCHES[0] += res[2]
+    return res[:2]
+
+
+def _attend_listed(what: str, q, k_pages, v_pages, page_table, seq_lens, q_start, lists, counts, query_block,
+                   softmax_scale, out, workspace) -> torch.Tensor:
+    block = _size(what, "query_block", query_block, 1)
+    res = paged_call().attend_listed(q, k_pages, v_pages, page_table, seq_lens, q_start, lists, counts, block,
+                                     softmax_scale or 0.0, out, workspace)
+    if res is None:
+        for name, t, dims in (("lists", lists, 3), ("counts", counts, 2)):
+            if not isinstance(t, torch.Tensor) or t.dim() != dims or t.dtype != torch.int32:
+                raise SabreError(f"{what}: {name} must be int32 {'[blocks, Hkv, n]' if dims == 3 else '[blocks, Hkv]'}")
+        _need_cuda(lists=lists, counts=counts)
+        if lists.device != k_pages.device or counts.device != k_pages.device:
+            raise SabreError(f"{what}: lists are on {lists.device}, counts on {counts.device}, the pages on "
+                             f"{k_pages.device}")
+        if lists.shape[2] < 1 or (lists.shape[2] > 1 and lists.stride(2) != 1):
+            raise SabreError(f"{what}: lists {tuple(lists.shape)} need entries, at unit stride")
+        B, H = page_table.shape[0], k_pages.shape[1] if k_pages.dim() == 4 else None
+        if q.dim() == 3 and lists.shape[:2] == counts.shape and \
+                (q_start is not None or q.shape[0] == B) and H is not None:
+            blocks = lib().sabre_paged_query_blocks(q.shape[0], B, block) if q_start is not None else B
+            if counts.shape[0] < blocks or counts.shape[1] != H:
+                raise SabreError(f"{what}: lists of {tuple(counts.shape)} (blocks, heads) for {blocks} query blocks of "
+                                 f"{H} KV heads")
+        elif lists.shape[:2] != counts.shape:
+            raise SabreError(f"{what}: lists {tuple(lists.shape)} and counts {tuple(counts.shape)} do not belong "
+                             f"together")
+        _paged_refuse(what, k_pages, v_pages, page_table, seq_lens, q_start, dict(q=q, out=out), workspace)
+    if type(res) is int:
+        check(res, "sabre_" + what)
+    out, kernels = res
+    LAUNCHES[0] += kernels
+    return out
+
+
+def paged_decode_listed(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                        seq_lens: torch.Tensor, lists: torch.Tensor, counts: torch.Tensor, *,
+                        softmax_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                        workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`paged_decode` over listed pages: the query of sequence b sees, for KV
+    head h, the rows of columns ``lists[b, h, :counts[b, h]]`` of its table (int32,
+    ascending; a stride of 0 shares a list). An entry that is not above the one
+    before it is skipped, as is one outside the table (recorded). The workspace is
+    that of :func:`paged_decode`. Deterministic."""
+    return _attend_listed("paged_decode_listed", q, k_pages, v_pages, page_table, seq_lens, None, lists, counts, 1,
+                          softmax_scale, out, workspace)
+
+
+def paged_prefill_listed(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor, page_table: torch.Tensor,
+                         seq_lens: torch.Tensor, q_start: torch.Tensor, lists: torch.Tensor, counts: torch.Tensor, *,
+                         query_block: int, softmax_scale: Optional[float] = None, out: Optional[torch.Tensor] = None,
+                         workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`paged_prefill` over listed pages: the query at position i of block n
+    sees, for KV head h, the rows j <= i of columns ``lists[n, h, :counts[n, h]]``
+    (as in :func:`paged_decode_listed`). Blocks as in :func:`paged_select`, with
+    ``query_block * (Hq / Hkv) <= 128``: the nearer to 128, the less of the work is
+    padding. A NaN or an infinity in a V row that some query of a block sees may
+    reach the other queries of that block."""
+    if q_start is None:
+        raise SabreError("paged_prefill_listed needs q_start")
+    return _attend_listed("paged_prefill_listed", q, k_pages, v_pages, page_table, seq_lens, q_start, lists, counts,
+                          query_block, softmax_scale, out, workspace)
+
+
 def copy_pages(pages: torch.Tensor, src: Sequence[int], dst: Sequence[int]) -> None:
     """Copies page ``src[m]`` to page ``dst[m]`` in every pool of ``pages``:
     one pool ``[num_pages, Hkv, page_size, D]`` or several at one stride
