@@ -58,13 +58,19 @@ struct Lists {
   __device__ __forceinline__ int count(int block, int head) const {
     return min(max(counts[block * c_sq + head * c_sh], 0), cap);
   }
-  // Column of entry i < count, or -1.
-  __device__ __forceinline__ int column(int block, int head, int i, const Cache& c) const {
+  // Entry i < cap and the one before it.
+  __device__ __forceinline__ int2 entry(int block, int head, int i) const {
     const int32_t* e = entries + block * e_sq + head * e_sh + i;
-    const int col = e[0];
-    const bool in = col >= 0 && col < c.max_pages;
+    return make_int2(e[0], i > 0 ? e[-1] : -1);
+  }
+  // The column of an entry below the list's count, or -1.
+  static __device__ __forceinline__ int column(int2 e, const Cache& c) {
+    const bool in = e.x >= 0 && e.x < c.max_pages;
     if (!in) record_status(SABRE_DEV_BAD_PAGE);
-    return in && (i == 0 || e[-1] < col) ? col : -1;
+    return in && e.y < e.x ? e.x : -1;
+  }
+  __device__ __forceinline__ int column(int block, int head, int i, const Cache& c) const {
+    return column(entry(block, head, i), c);
   }
 };
 
@@ -143,6 +149,34 @@ __device__ __forceinline__ bool find_rows(const Cache& c, const int32_t* starts,
   __syncthreads();
   if (scratch[8] < 0) return false;
   tile = RowTile{scratch[8], scratch[9], scratch[10], scratch[11], scratch[12]};
+  return true;
+}
+
+// The same for at most 32 sequences, by each warp for itself: one round trip and no
+// barrier. len: the new rows of sequence `lane` (0 behind the last). False: there are
+// fewer tiles.
+__device__ __forceinline__ bool find_rows_warp(const Cache& c, const int32_t* starts, int rows, int tokens, int slot,
+                                               RowTile& tile, int& len) {
+  const int lane = threadIdx.x & 31;
+  int first = 0, length = 0;
+  len = 0;
+  if (lane < c.batch) {
+    first = row_start(starts, lane, rows);
+    length = c.seq_lens[lane];
+    len = max(row_start(starts, lane + 1, rows) - first, 0);
+  }
+  const int nt = (len + tokens - 1) / tokens;
+  int incl = nt;
+#pragma unroll
+  for (int s = 1; s < 32; s <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, incl, s);
+    if (lane >= s) incl += up;
+  }
+  const uint32_t past = __ballot_sync(0xffffffffu, slot < incl);
+  if (past == 0u) return false;
+  const int b = __ffs(past) - 1;
+  tile = RowTile{b, (slot - __shfl_sync(0xffffffffu, incl - nt, b)) * tokens, __shfl_sync(0xffffffffu, first, b),
+                 __shfl_sync(0xffffffffu, len, b), __shfl_sync(0xffffffffu, length, b)};
   return true;
 }
 

@@ -359,13 +359,27 @@ __global__ void __launch_bounds__(kThreads, 2)
   long long units = 0;  // key tiles of the share still to be done
   int hk = 0;
   int block = 0, entries = 0;  // kListed: the query block and its list's length
+  int2 first_entry = make_int2(-1, -1);
   bool some;
   if constexpr (kListed) {
     // Later blocks of a sequence have no shorter lists: its heaviest first.
     block = p.slots - 1 - static_cast<int>(blockIdx.x / p.parts);
     hk = static_cast<int>(blockIdx.y);
-    some = find_job(p, block, scratch, job);
-    if (some && job.n > 0) entries = p.lists.count(block, hk);
+    // The list's length and, when the pair has no parts, its first entries (one a lane:
+    // that of its box) are asked for together with the rows.
+    const int asked = p.lists.count(block, hk);
+    const int e = (lane << p.box_shift) >> p.c.page_shift;
+    if (p.parts == 1 && e < p.lists.cap) first_entry = p.lists.entry(block, hk, e);
+    if (p.c.batch <= 32) {
+      RowTile t;
+      int len;
+      some = find_rows_warp(p.c, p.starts, p.rows, p.tokens, block, t, len);
+      if (some) job = make_job(p, t.b, t.r, t.first, t.len, t.length);
+      __syncthreads();  // orders the set-up above before its use, as find_job() does
+    } else {
+      some = find_job(p, block, scratch, job);
+    }
+    if (some && job.n > 0) entries = asked;
     if (p.parts > 1 && blockIdx.x % p.parts == 0 && tid == 0)
       p.joins[2 * (block * p.heads_kv + hk) + 1] = some ? make_int4(job.row0, job.count, 0, 0) : make_int4(0, 0, 0, 0);
   } else if constexpr (kShares) {
@@ -410,14 +424,14 @@ __global__ void __launch_bounds__(kThreads, 2)
       place = (block * p.heads_kv + hk) * p.parts + part_id;
     }
     // kListed: the position of box i of this part (all of it past the sequence or in
-    // no page: kNowhere) and its page there, or -1.
+    // no page: kNowhere) and its page there, or -1. i % 32 is the lane.
     constexpr int kNowhere = INT_MAX - 64;
     auto listed_box = [&](int i, int& page) -> int {
       page = -1;
       const int row = j0 * kTile + (i << p.box_shift);
       const int e = row >> p.c.page_shift;
       if (i >= nt * boxes || e >= entries) return kNowhere;
-      const int col = p.lists.column(block, hk, e, p.c);
+      const int col = p.parts == 1 && i < 32 ? Lists::column(first_entry, p.c) : p.lists.column(block, hk, e, p.c);
       const int t = (col << p.c.page_shift) + (row & ((1 << p.c.page_shift) - 1));
       if (col < 0 || t >= job.n) return kNowhere;
       page = p.c.page_of(job.b, t);

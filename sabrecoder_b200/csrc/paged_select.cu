@@ -434,19 +434,17 @@ __global__ void __launch_bounds__(kWarps * 32, kGroup == 1 ? 5 : 16 / kGroup) pa
   } else {
     const int tile = p.tokens * kGroup;
     int before = 0, all = 0;  // blocks of the sequences before this one, and of all
-    if (p.c.batch == 1) {  // a prompt: nothing to look for
-      t = RowTile{0, 0, row_start(p.starts, 0, p.rows), 0, p.c.seq_lens[0]};
-      t.len = max(row_start(p.starts, 1, p.rows) - t.first, 0);
-      all = (t.len + p.tokens - 1) / p.tokens;
-      if (static_cast<long long>(slot) * tile < t.len)
-        t.r = slot * tile;
-      else
-        t = RowTile{-1, 0, 0, 0, 0};
+    if (p.c.batch <= 32) {
+      int len;
+      if (!find_rows_warp(p.c, p.starts, p.rows, tile, slot, t, len)) t = RowTile{-1, 0, 0, 0, 0};
+      const int n = (len + p.tokens - 1) / p.tokens;
+      before = __reduce_add_sync(0xffffffffu, lane < t.b ? n : 0);
+      all = __reduce_add_sync(0xffffffffu, n);
     } else if (!find_rows<kThreads>(p.c, p.starts, p.rows, tile, slot, scratch, t)) {
       t = RowTile{-1, 0, 0, 0, 0};
     }
     if constexpr (kGroup > 1) {
-      if (p.c.batch > 1) {
+      if (p.c.batch > 32) {
         for (int b = tid; b < p.c.batch; b += kThreads) {
           const int len = max(row_start(p.starts, b + 1, p.rows) - row_start(p.starts, b, p.rows), 0);
           const int n = (len + p.tokens - 1) / p.tokens;
