@@ -235,7 +235,7 @@ PyObject* store_slots(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // extend(new_rows, page_table, seq_lens, free_pages, free_count, page_size, num_pages, rows, seq_lens_out or None,
-// free_count_out or None) -> (q_start, slots, positions)
+// free_count_out or None) -> (q_start, slots, positions, kernels)
 PyObject* extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Tables p;
@@ -261,7 +261,9 @@ PyObject* extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
       integer(a[6]), integer(a[5]), p.cols, free_pages->size(0), p.table->stride(0),
       c10::cuda::getCurrentCUDAStream(p.dev).stream());
   if (st != SABRE_OK) return PyLong_FromLong(st);
-  return Py_BuildValue("NNN", THPVariable_Wrap(starts), THPVariable_Wrap(slots), THPVariable_Wrap(positions));
+  // More than 2048 rows are placed by a kernel of their own.
+  return Py_BuildValue("NNNi", THPVariable_Wrap(starts), THPVariable_Wrap(slots), THPVariable_Wrap(positions),
+                       rows > 2048 ? 2 : 1);
   END_HANDLE_TH_ERRORS
 }
 

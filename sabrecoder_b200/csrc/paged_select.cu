@@ -670,10 +670,12 @@ template <typename T, int kGroup, int kWarps>
 static cudaError_t launch(const Params& p, long long slots, cudaStream_t s) {
   const auto kernel = paged_select_kernel<T, kGroup, kWarps>;
   const int most = kGroup > 1 ? kGroup * (kGroupPages + 1) : kMaxPages + 1;
-  cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       most * static_cast<int>(sizeof(uint32_t)));
-  if (e != cudaSuccess) return e;
   const int smem = kGroup * p.key_row * static_cast<int>(sizeof(uint32_t));
+  if (smem > 32 * 1024) {  // with the kernel's own past what every launch may have
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               most * static_cast<int>(sizeof(uint32_t)));
+    if (e != cudaSuccess) return e;
+  }
   const dim3 grid(static_cast<unsigned>(slots * p.ctas), p.heads_kv);
   if (p.ctas == 1) return launch_dependent(grid, kWarps * 32, smem, s, kernel, p);
   return launch_cluster(grid, p.ctas, kWarps * 32, smem, s, kernel, p);

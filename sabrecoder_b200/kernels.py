@@ -734,8 +734,8 @@ def paged_extend(new_rows: torch.Tensor, page_table: torch.Tensor, seq_lens: tor
         raise SabreError(f"{what}: no sequences, or a size exceeds 2^31 - 1")
     if type(res) is int:
         check(res, "sabre_" + what)
-    LAUNCHES[0] += 1
-    return res
+    LAUNCHES[0] += res[3]
+    return res[:3]
 
 
 def paged_store_slots(k: torch.Tensor, v: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
