@@ -14,6 +14,12 @@ follows them) are what the kernels read.
 * With ``window_size`` (and ``num_prefix_tokens`` first tokens that stay
   visible) a query at position i sees key j <= i when ``i - j <= window_size``
   or ``j < num_prefix_tokens``; pages that no later query can see are released.
+* With ``topk_pages`` queries read selected pages: those of the window and the
+  prefix (the window's pages are the query's own without ``window_size``) and the
+  ``topk_pages`` others whose mean key suits them best. All pages are kept.
+* :meth:`lend` hands free pages to the device, where :meth:`extend_on_device`
+  makes room for rows, also inside a capture, until :meth:`settle` brings the host
+  up to date.
 
 As a transformers ``Cache`` it takes the same number of new rows for every
 sequence of the batch; the patched attention writes its rows through
@@ -49,6 +55,7 @@ class SabrePagedCacheLayer(CacheLayerMixin):
         self._ref, self.index, self.step = weakref.ref(cache), index, 0
         self.max_cache_len = cache.max_seq_len
         self.k_pages, self.v_pages = cache.pool[index, 0], cache.pool[index, 1]
+        self.key_means = None if cache.key_means is None else cache.key_means[index]
         self.dtype, self.device = cache.pool.dtype, cache.pool.device
         self.keys = self.values = None  # never held as one tensor
         self.is_initialized = True
@@ -73,6 +80,8 @@ class SabrePagedCacheLayer(CacheLayerMixin):
         c = self._cache
         if c.window_size is not None:
             raise ValueError("SabrePagedKVCache with a window serves the patched attention only (pages are dropped)")
+        if c.topk_pages is not None:
+            raise ValueError("SabrePagedKVCache with topk_pages serves the patched attention only")
         if len(set(c.lengths)) > 1:
             raise ValueError(f"SabrePagedKVCache: sequences of different lengths ({c.lengths}) serve the patched "
                              f"attention only (its mask knows one length)")
@@ -105,12 +114,16 @@ class SabrePagedKVCache(Cache):
     with explicit ``num_layers`` / ``num_kv_heads`` / ``head_dim``.
 
     ``num_pages`` is shared by all sequences (default: enough for every
-    sequence at ``max_seq_len``)."""
+    sequence at ``max_seq_len``). ``topk_pages``: attention over selected pages,
+    one choice for each KV head and up to ``query_block`` new rows (default: the
+    largest power of two that fills a row tile of the prompt kernel, 128 rows over
+    the heads of a group)."""
 
     def __init__(self, config=None, *, batch_size: int = 1, max_seq_len: int, num_pages: Optional[int] = None,
                  page_size: int = 64, window_size: Optional[int] = None, num_prefix_tokens: int = 0, device="cuda",
                  dtype: torch.dtype = torch.bfloat16, num_layers: Optional[int] = None,
-                 num_kv_heads: Optional[int] = None, head_dim: Optional[int] = None):
+                 num_kv_heads: Optional[int] = None, head_dim: Optional[int] = None, topk_pages: Optional[int] = None,
+                 query_block: Optional[int] = None):
         if config is not None:
             num_layers = num_layers or config.num_hidden_layers
             num_kv_heads = num_kv_heads or config.num_key_value_heads
@@ -123,14 +136,30 @@ class SabrePagedKVCache(Cache):
             raise ValueError("SabrePagedKVCache needs batch_size >= 1 and max_seq_len >= 1")
         if (window_size is not None and window_size < 0) or num_prefix_tokens < 0:
             raise ValueError("window_size and num_prefix_tokens must not be negative")
+        if topk_pages is not None and topk_pages < 0:
+            raise ValueError(f"topk_pages {topk_pages} must not be negative")
+        if query_block is not None and (topk_pages is None or not 1 <= query_block <= 128):
+            raise ValueError(f"query_block {query_block} goes with topk_pages, from 1 to 128")
         self.page_size, self.max_seq_len = int(page_size), int(max_seq_len)
+        self.topk_pages, self.query_block = topk_pages, query_block
         self.window_size, self.num_prefix_tokens = window_size, int(num_prefix_tokens)
         self.max_pages = -(-self.max_seq_len // self.page_size)
         self.num_pages = int(num_pages) if num_pages is not None else batch_size * self.max_pages
         if self.num_pages < 1:
             raise ValueError("SabrePagedKVCache needs at least one page")
+        if topk_pages is not None and self.max_pages > 32768:
+            raise ValueError(f"topk_pages selects among at most 32768 pages of a sequence, not {self.max_pages}")
         self.pool = torch.empty(num_layers, 2, self.num_pages, num_kv_heads, self.page_size, head_dim, dtype=dtype,
                                 device=device)
+        # The mean key of every full page; other pages' are not read.
+        self.key_means = None
+        if topk_pages is not None:
+            self.key_means = torch.empty(num_layers, self.num_pages, num_kv_heads, head_dim, dtype=torch.float32,
+                                         device=device)
+        # Pages lent to the device, as a stack, and how many of them it still has.
+        self.free_pages = torch.zeros(self.num_pages, dtype=torch.int32, device=device)
+        self.free_count = torch.zeros(1, dtype=torch.int32, device=device)
+        self._lent: Optional[List[int]] = None
         self.refs: List[int] = [0] * self.num_pages
         self.unused: List[int] = list(range(self.num_pages - 1, -1, -1))  # the lowest page is taken first
         self.step = 0       # steps begun (a step: new rows of every layer)
@@ -178,6 +207,9 @@ class SabrePagedKVCache(Cache):
         if _capturing(self.pool):
             raise ValueError("SabrePagedKVCache: sequences do not change inside a capture (extend, and the like, go "
                              "between replays; a captured step stores with paged_store)")
+        if self._lent is not None:
+            raise ValueError("SabrePagedKVCache: pages are lent to the device, which changes the sequences; settle() "
+                             "comes first")
 
     def _seq(self, seq: int) -> int:
         """A sequence's index (from the end when negative)."""
@@ -194,6 +226,11 @@ class SabrePagedKVCache(Cache):
     def pages_in_use(self) -> int:
         return self.num_pages - len(self.unused)
 
+    @property
+    def _drop_window(self) -> Optional[int]:
+        """The window outside of which pages are given back."""
+        return self.window_size if self.topk_pages is None else None
+
     # -- sequences --------------------------------------------------------
 
     def extend(self, new: Sequence[int]) -> None:
@@ -201,7 +238,7 @@ class SabrePagedKVCache(Cache):
         its end). Raises ValueError, changing nothing, when a sequence or the
         pool is full."""
         self._outside_captures()
-        ps, w = self.page_size, self.window_size
+        ps, w = self.page_size, self._drop_window
         if len(new) != self.batch_size or min(new, default=0) < 0:
             raise ValueError(f"extend needs {self.batch_size} row counts >= 0")
         need, dropped, shared = 0, [], {}
@@ -280,7 +317,7 @@ class SabrePagedKVCache(Cache):
         ps = self.page_size
         for b, length in lengths.items():
             lengths[b] = length = max(0, min(int(length), self.lengths[b]))
-            if self.window_size is not None:
+            if self._drop_window is not None:
                 first = max(0, length - 1 - self.window_size) // ps
                 if any(p < 0 for p in self.tables[b][first:-(-length // ps)]):
                     raise ValueError(f"SabrePagedKVCache: rows in the window before {length} of sequence {b} are "
@@ -307,6 +344,8 @@ class SabrePagedKVCache(Cache):
         if not src:
             return 0
         K.copy_pages(self.pool, src, dst)
+        if self.key_means is not None:
+            K.copy_pages(self.key_means.unsqueeze(3), src, dst)
         to = dict(zip(src, dst))
         for a, b in to.items():
             self.refs[b], self.refs[a] = self.refs[a], 0
@@ -315,6 +354,93 @@ class SabrePagedKVCache(Cache):
         self.unused = list(range(self.num_pages - 1, live - 1, -1))
         self._upload(range(self.batch_size))
         return len(src)
+
+    # -- steps without the host -------------------------------------------
+
+    def lend(self, num_pages: Optional[int] = None) -> int:
+        """Hands free pages (all of them by default) to the device, which takes them
+        in :meth:`extend_on_device`; returns how many. Until :meth:`settle` the
+        sequences are the device's: calls that change them raise. Last pages that
+        sequences share are copied first."""
+        self._outside_captures()
+        ps = self.page_size
+        copies, count = [], {}
+        for b, n in enumerate(self.lengths):
+            if n % ps:
+                page = self.tables[b][n // ps]
+                count[page] = count.get(page, 0) + 1
+                if self.refs[page] - count[page] > 0:  # all but the last to share it get their own
+                    copies.append((b, page))
+        free = len(self.unused) - len(copies)
+        want = free if num_pages is None else int(num_pages)
+        if want < 0 or want > free:
+            raise ValueError(f"SabrePagedKVCache: {want} pages cannot be lent: {len(self.unused)} are free and "
+                             f"{len(copies)} are needed for copies of shared pages")
+        src, dst = [], []
+        for b, page in copies:
+            src.append(page)
+            dst.append(self.unused.pop())
+            self.refs[dst[-1]] = 1
+            self._release(page)
+            self.tables[b][self.lengths[b] // ps] = dst[-1]
+        if src:
+            K.copy_pages(self.pool, src, dst)
+            self._upload([b for b, _ in copies])
+        self._lent = self.unused[len(self.unused) - want:]
+        del self.unused[len(self.unused) - want:]
+        self.free_pages[:want].copy_(torch.tensor(self._lent, dtype=torch.int32))
+        self.free_count.fill_(want)
+        return want
+
+    def extend_on_device(self, new_rows: torch.Tensor, num_rows: int
+                         ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """Makes room for ``new_rows`` (int32 ``[B]``, on the device) more rows of each
+        sequence, num_rows or fewer in all, from the pages lent: ``(q_start, slots,
+        positions)`` as :func:`kernels.paged_extend` gives them. May be captured."""
+        if self._lent is None:
+            raise ValueError("SabrePagedKVCache: lend() pages to the device first")
+        return K.paged_extend(new_rows, self.page_table, self.seq_lens, self.free_pages, self.free_count,
+                              page_size=self.page_size, num_pages=self.num_pages, num_rows=num_rows)
+
+    def store_rows(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor, q_start: torch.Tensor,
+                   slots: torch.Tensor) -> None:
+        """Stores the rows k, v ``[num_rows, Hkv, D]`` of a step on the device in one
+        layer, where :meth:`extend_on_device` made room for them."""
+        layer = self.layers[layer_idx]
+        K.paged_store_slots(k, v, layer.k_pages, layer.v_pages, slots)
+        if layer.key_means is not None:
+            K.paged_key_means(layer.k_pages, layer.key_means, self.page_table, self.seq_lens, q_start,
+                              num_rows=k.shape[0])
+
+    def settle(self) -> None:
+        """Takes over what the device did with the pages lent (waits for it) and takes
+        the others back. Nothing happens when none are lent."""
+        if _capturing(self.pool):
+            raise ValueError("SabrePagedKVCache: settle() reads from the device, which a capture cannot")
+        if self._lent is None:
+            return
+        ps, lent = self.page_size, self._lent
+        left = int(self.free_count)
+        lengths, rows = self.seq_lens.tolist(), self.page_table.tolist()
+        taken = {}
+        for b, n in enumerate(lengths):
+            if n < self.lengths[b] or n > self.max_pages * ps:
+                raise ValueError(f"SabrePagedKVCache: sequence {b} went from {self.lengths[b]} rows to {n} on the device")
+            for col in range(len(self.tables[b]), -(-n // ps)):
+                taken[rows[b][col]] = taken.get(rows[b][col], 0) + 1
+        if taken != {page: 1 for page in lent[left:]} or not 0 <= left <= len(lent):
+            raise ValueError("SabrePagedKVCache: the device's tables do not match the pages lent to it")
+        for b, n in enumerate(lengths):
+            self.tables[b] += rows[b][len(self.tables[b]):-(-n // ps)]
+        for page in taken:
+            self.refs[page] = 1
+        self.unused += lent[:left]
+        self.lengths, self._lent = lengths, None
+        self.free_count.zero_()
+        # The host's copies of the tables; the device has them.
+        host = self._host.numpy()
+        for b, t in enumerate(self.tables):
+            host[b, :len(t)] = t
 
     # -- one step ---------------------------------------------------------
 
@@ -352,7 +478,7 @@ class SabrePagedKVCache(Cache):
         j = torch.arange(top + n, device=mask.device)
         i = lengths[:, None, None, None] + row
         own = j <= i
-        if self.window_size is not None:
+        if self._drop_window is not None:
             own = own & ((i - j <= self.window_size) | (j < self.num_prefix_tokens))
         wrong = own & ~see
         if mask.dim() == 4:
@@ -378,6 +504,9 @@ class SabrePagedKVCache(Cache):
             raise ValueError(f"SabrePagedKVCache: layer {layer_idx} is out of step")
         K.paged_store(k.reshape(B * n, *k.shape[2:]), v.reshape(B * n, *v.shape[2:]), layer.k_pages, layer.v_pages,
                       self.page_table, self.seq_lens, self._row_starts(n))
+        if layer.key_means is not None:
+            K.paged_key_means(layer.k_pages, layer.key_means, self.page_table, self.seq_lens, self._row_starts(n),
+                              num_rows=B * n)
         layer.step = self.step
 
     def _row_starts(self, n: int) -> torch.Tensor:
@@ -396,15 +525,38 @@ class SabrePagedKVCache(Cache):
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Attention of one new token per sequence, q ``[B, Hq, D]``, over a layer."""
         layer = self.layers[layer_idx]
+        if self.topk_pages is not None:
+            table = self._columns_in_use()
+            lists, counts = self.select(layer_idx, q)
+            return K.paged_decode_listed(q, layer.k_pages, layer.v_pages, table, self.seq_lens, lists, counts,
+                                         softmax_scale=softmax_scale, out=out)
         return K.paged_decode(q, layer.k_pages, layer.v_pages, self.page_table, self.seq_lens,
                               window_size=self.window_size, num_prefix_tokens=self.num_prefix_tokens,
                               softmax_scale=softmax_scale, out=out)
 
+    def select(self, layer_idx: int, q: torch.Tensor, q_start: Optional[torch.Tensor] = None
+               ) -> Tuple[torch.Tensor, torch.Tensor]:
+        """The pages (as lists of table columns) that the rows q ``[N, Hq, D]`` of a
+        step read in a layer: one new token per sequence, or the last
+        ``q_start[b+1] - q_start[b]`` rows of each in blocks of :meth:`block_rows`."""
+        if self.topk_pages is None:
+            raise ValueError("SabrePagedKVCache selects pages with topk_pages only")
+        layer = self.layers[layer_idx]
+        return K.paged_select(q, layer.key_means, self._columns_in_use(), self.seq_lens, q_start,
+                              page_size=self.page_size, topk=self.topk_pages,
+                              query_block=1 if q_start is None else self.block_rows(q.shape[1]),
+                              window_size=self.window_size or 0, num_prefix_tokens=self.num_prefix_tokens)
+
+    def block_rows(self, num_heads: int) -> int:
+        """Rows of a query block for so many query heads."""
+        most = max(1, 128 // max(1, num_heads // self.pool.shape[3]))
+        return min(self.query_block or 128, 1 << (most.bit_length() - 1))
+
     def _columns_in_use(self) -> torch.Tensor:
         """The columns of the page table that are in use: the prompt kernel plans its
-        work by the table's width. Inside a capture all of them, since a replay may find
-        more rows."""
-        if _capturing(self.pool):
+        work by the table's width. Inside a capture, and while pages are lent, all of
+        them, since the device may find more rows."""
+        if _capturing(self.pool) or self._lent is not None:
             return self.page_table
         n = max(1, -(-max(self.lengths) // self.page_size))
         if self._columns[0] != n:
@@ -416,6 +568,13 @@ class SabrePagedKVCache(Cache):
         """Causal attention of a step's rows, q ``[B, n, Hq, D]``, over a layer."""
         layer = self.layers[layer_idx]
         B, n, Hq, D = q.shape
+        if self.topk_pages is not None:
+            rows, starts = q.reshape(B * n, Hq, D), self._row_starts(n)
+            lists, counts = self.select(layer_idx, rows, starts)
+            return K.paged_prefill_listed(rows, layer.k_pages, layer.v_pages, self._columns_in_use(), self.seq_lens,
+                                          starts, lists, counts, query_block=self.block_rows(Hq),
+                                          softmax_scale=softmax_scale,
+                                          out=None if out is None else out.view(B * n, Hq, D)).view(B, n, Hq, D)
         res = K.paged_prefill(q.reshape(B * n, Hq, D), layer.k_pages, layer.v_pages, self._columns_in_use(),
                               self.seq_lens, self._row_starts(n), window_size=self.window_size,
                               num_prefix_tokens=self.num_prefix_tokens, softmax_scale=softmax_scale,
@@ -443,14 +602,18 @@ class SabrePagedKVCache(Cache):
 
     def __deepcopy__(self, memo) -> "SabrePagedKVCache":
         """A cache of its own with the same contents, as prompts are reused."""
+        if self._lent is not None:
+            raise ValueError("SabrePagedKVCache: pages are lent to the device; settle() comes before a copy")
         _, _, n, heads, _, dim = self.pool.shape
         new = SabrePagedKVCache(batch_size=self.batch_size, max_seq_len=self.max_seq_len, num_pages=n,
                                 page_size=self.page_size, window_size=self.window_size,
                                 num_prefix_tokens=self.num_prefix_tokens, device=self.pool.device,
                                 dtype=self.pool.dtype, num_layers=self.pool.shape[0], num_kv_heads=heads,
-                                head_dim=dim)
+                                head_dim=dim, topk_pages=self.topk_pages, query_block=self.query_block)
         memo[id(self)] = new
         new.pool.copy_(self.pool)
+        if self.key_means is not None:
+            new.key_means.copy_(self.key_means)
         new.refs, new.unused = list(self.refs), list(self.unused)
         new.step, new.step_rows = self.step, self.step_rows
         for a, b in zip(new.layers, self.layers):

@@ -340,9 +340,9 @@ class StructureAwareAttentionWrapper(nn.Module):
         paged = isinstance(cache, SabrePagedKVCache)
         fresh = True
         if paged:
-            if self.use_sparse_for_generation:
+            if self.use_sparse_for_generation and cache.topk_pages is None:
                 raise ValueError("use_sparse_for_generation needs a contiguous cache: a SabrePagedKVCache decodes over "
-                                 "all rows or its window")
+                                 "all rows or its window (or, with topk_pages, over selected pages)")
             cache.check_step(self.layer_idx, L, kwargs.get("position_ids"), attention_mask)
             fresh = cache.get_seq_length(self.layer_idx) == 0
             kn = torch.empty(B, L, Hkv, D, dtype=q.dtype, device=q.device)
@@ -371,7 +371,8 @@ class StructureAwareAttentionWrapper(nn.Module):
         if paged and (L == 1 or get_current_code() is None or not fresh):
             # One new token, or prompt rows that continue cached ones (or have no
             # structure): attention over the pages.
-            _DENSE_CALL_COUNT += 1
+            _DENSE_CALL_COUNT += 1 if cache.topk_pages is None else 0
+            _SPARSE_CALL_COUNT += 0 if cache.topk_pages is None else 1
             attn = (cache.decode(self.layer_idx, q.view(B, Hq, D), self.scaling) if L == 1 else
                     cache.prefill(self.layer_idx, q, self.scaling)).view(B, L, Hq * D)
         elif L == 1:
