@@ -851,10 +851,7 @@ def _attend_listed(what: str, q, k_pages, v_pages, page_table, seq_lens, q_start
         for name, t, dims in (("lists", lists, 3), ("counts", counts, 2)):
             if not isinstance(t, torch.Tensor) or t.dim() != dims or t.dtype != torch.int32:
                 raise SabreError(f"{what}: {name} must be int32 {'[blocks, Hkv, n]' if dims == 3 else '[blocks, Hkv]'}")
-        _need_cuda(lists=lists, counts=counts)
-        if lists.device != k_pages.device or counts.device != k_pages.device:
-            raise SabreError(f"{what}: lists are on {lists.device}, counts on {counts.device}, the pages on "
-                             f"{k_pages.device}")
+        _refuse_tables(what, page_table, seq_lens, q_start, {}, lists=lists, counts=counts)
         if lists.shape[2] < 1 or (lists.shape[2] > 1 and lists.stride(2) != 1):
             raise SabreError(f"{what}: lists {tuple(lists.shape)} need entries, at unit stride")
         B, H = page_table.shape[0], k_pages.shape[1] if k_pages.dim() == 4 else None
