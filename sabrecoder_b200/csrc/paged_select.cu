@@ -25,7 +25,7 @@ namespace paged {
 // ---------------------------------------------------------------------------
 namespace means {
 
-constexpr int kMaxWarps = 8;
+constexpr int kMaxWarps = 4;
 
 struct Params {
   Cache c;  // k strides only
@@ -374,18 +374,27 @@ __device__ __forceinline__ void write_list(const Params& p, const Cut& cut, cons
   const int lane = threadIdx.x & 31;
   int32_t* const out = p.lists + (static_cast<long long>(block) * p.heads_kv + hk) * p.cap;
   int total = 0, equal = 0;
-  for (int i0 = 0; i0 < pages; i0 += 32) {
-    const uint32_t k = i0 + lane < pages ? key[i0 + lane] : 0u;
-    const uint32_t below = (1u << lane) - 1u;
-    uint32_t take = __ballot_sync(0xffffffffu, k > cut.limit);
+  const uint32_t below = (1u << lane) - 1u;
+  for (int i0 = 0; i0 < pages; i0 += 128) {  // four looks at a time
+    uint32_t k[4], take[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) k[u] = i0 + 32 * u + lane < pages ? key[i0 + 32 * u + lane] : 0u;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) take[u] = __ballot_sync(0xffffffffu, k[u] > cut.limit);
     if (cut.want > 0) {
-      const uint32_t same = __ballot_sync(0xffffffffu, k == cut.limit);
-      take |= __ballot_sync(0xffffffffu, k == cut.limit && equal + __popc(same & below) < cut.want);
-      equal += __popc(same);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const uint32_t same = __ballot_sync(0xffffffffu, k[u] == cut.limit);
+        take[u] |= __ballot_sync(0xffffffffu, k[u] == cut.limit && equal + __popc(same & below) < cut.want);
+        equal += __popc(same);
+      }
     }
-    const int place = total + __popc(take & below);
-    if ((take >> lane & 1u) && place < p.cap) out[place] = i0 + lane;
-    total += __popc(take);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int place = total + __popc(take[u] & below);
+      if ((take[u] >> lane & 1u) && place < p.cap) out[place] = i0 + 32 * u + lane;
+      total += __popc(take[u]);
+    }
   }
   total = min(total, p.cap);
   for (int i = total + lane; i < p.cap; i += 32) out[i] = -1;
