@@ -347,6 +347,8 @@ __global__ void __launch_bounds__(kThreads, 2)
     tmem_relinquish();
     tc_fence_before();
   }
+  // kListed: short CTAs, so the next kernel's set-up under the last of them counts.
+  if (kListed && tid == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // The set-up above overlaps the tail of the stream's previous kernel (this is
   // a programmatic dependent launch) and the loads below, whose barriers order
   // it before its use. Nothing before this line reads what that kernel wrote.
@@ -416,12 +418,15 @@ __global__ void __launch_bounds__(kThreads, 2)
     int j0 = 0, nt = job.tiles, place = 0;
     bool part = false;
     if constexpr (kListed) {
-      const int part_id = static_cast<int>(blockIdx.x) % p.parts;
-      const long long all = ((static_cast<long long>(entries) << p.c.page_shift) + kTile - 1) / kTile;
-      j0 = static_cast<int>(all * part_id / p.parts);
-      nt = static_cast<int>(all * (part_id + 1) / p.parts) - j0;
-      part = p.parts > 1;
-      place = (block * p.heads_kv + hk) * p.parts + part_id;
+      nt = static_cast<int>(((static_cast<long long>(entries) << p.c.page_shift) + kTile - 1) / kTile);
+      if (p.parts > 1) {
+        const long long all = nt;
+        const int part_id = static_cast<int>(blockIdx.x) % p.parts;
+        j0 = static_cast<int>(all * part_id / p.parts);
+        nt = static_cast<int>(all * (part_id + 1) / p.parts) - j0;
+        part = true;
+        place = (block * p.heads_kv + hk) * p.parts + part_id;
+      }
     }
     // kListed: the position of box i of this part (all of it past the sequence or in
     // no page: kNowhere) and its page there, or -1. i % 32 is the lane.
