@@ -14,6 +14,7 @@
 
 #include <ATen/MemoryOverlap.h>
 #include <ATen/core/Tensor.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <ATen/ops/empty.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -113,6 +114,11 @@ struct Tables {
            small(m->size(1)) && small(m->size(2));
   }
 };
+
+// A tensor on the device past the dispatcher.
+at::Tensor fresh_tensor(at::IntArrayRef size, at::ScalarType type, c10::DeviceIndex dev) {
+  return at::Tensor(at::detail::empty_cuda(size, type, c10::Device(c10::kCUDA, dev), std::nullopt));
+}
 
 int32_t* i32(const at::Tensor* t) { return t ? static_cast<int32_t*>(t->data_ptr()) : nullptr; }
 
@@ -252,9 +258,8 @@ PyObject* extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int rows = integer(a[7]);
   if (rows < 0) Py_RETURN_NONE;
   const c10::cuda::CUDAGuard guard(p.dev);
-  const auto longs = p.table->options().dtype(at::kLong);
-  at::Tensor starts = at::empty({int64_t{p.batch} + 1}, p.table->options());
-  at::Tensor slots = at::empty({rows}, longs), positions = at::empty({rows}, longs);
+  at::Tensor starts = fresh_tensor({int64_t{p.batch} + 1}, at::kInt, p.dev);
+  at::Tensor slots = fresh_tensor({rows}, at::kLong, p.dev), positions = fresh_tensor({rows}, at::kLong, p.dev);
   const int st = sabre_paged_extend(
       i32(fresh), i32(p.table), i32(p.lens), i32(lens_out), i32(free_pages), i32(count), i32(count_out), i32(&starts),
       static_cast<int64_t*>(slots.data_ptr()), static_cast<int64_t*>(positions.data_ptr()), rows, p.batch,
@@ -304,8 +309,8 @@ PyObject* select(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const c10::cuda::CUDAGuard guard(p.dev);
   const int blocks = sabre_paged_query_blocks(rows, p.batch, block);
   const int width = sabre_paged_select_width(page_size, p.cols, topk, block, window, prefix);
-  at::Tensor lists = at::empty({blocks, heads, width}, p.table->options());
-  at::Tensor counts = at::empty({blocks, heads}, p.table->options());
+  at::Tensor lists = fresh_tensor({blocks, heads, width}, at::kInt, p.dev);
+  at::Tensor counts = fresh_tensor({blocks, heads}, at::kInt, p.dev);
   if (rows > 0 && p.batch > 0) {
     const int64_t qr[2] = {q->stride(0), q->stride(1)}, ms[2] = {m->stride(0), m->stride(1)};
     const int st = sabre_paged_select(q->const_data_ptr(), static_cast<const float*>(m->const_data_ptr()), i32(p.table),
@@ -346,7 +351,7 @@ PyObject* attend_listed(PyObject*, PyObject* const* a, Py_ssize_t n) {
     out = *o;
   }
   const c10::cuda::CUDAGuard guard(p.dev);
-  if (!out.defined()) out = at::empty(q->sizes(), q->options());
+  if (!out.defined()) out = fresh_tensor(q->sizes(), q->scalar_type(), p.dev);
   if (q->numel() == 0 || p.batch == 0) return result(out, 0);
   const int entries = lists->size(2);
   const size_t need = p.starts ? sabre_paged_prefill_listed_workspace_size(rows, p.batch, heads_q, p.heads, p.dim,
@@ -357,7 +362,7 @@ PyObject* attend_listed(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (!w || !p.on(*w) || !w->is_contiguous() || w->nbytes() < need) Py_RETURN_NONE;
     ws = *w;
   } else if (need > 0) {
-    ws = at::empty({static_cast<int64_t>(need)}, q->options().dtype(at::kByte));
+    ws = fresh_tensor({static_cast<int64_t>(need)}, at::kByte, p.dev);
   }
   void* const wp = ws.defined() ? ws.data_ptr() : nullptr;
   const size_t wb = ws.defined() ? ws.nbytes() : 0;

@@ -27,6 +27,16 @@ namespace means {
 
 constexpr int kMaxWarps = 4;
 
+// volatile: eight of them go out before the first is used.
+__device__ __forceinline__ uint4 load_once(const void* p) {
+  uint4 x;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(x.x), "=r"(x.y), "=r"(x.z), "=r"(x.w)
+               : "l"(p)
+               : "memory");
+  return x;
+}
+
 struct Params {
   Cache c;  // k strides only
   const void* k;
@@ -85,7 +95,7 @@ __global__ void __launch_bounds__(kMaxWarps * 32) paged_key_means_kernel(const P
     for (int r = 0; r < pairs; r += 8) {
       uint4 x[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u) x[u] = *reinterpret_cast<const uint4*>(src + (r + u) * 2 * p.c.k_st);
+      for (int u = 0; u < 8; ++u) x[u] = load_once(src + (r + u) * 2 * p.c.k_st);
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
         const T* e = reinterpret_cast<const T*>(&x[u]);

@@ -701,6 +701,13 @@ def _size(what: str, name: str, value: int, low: int) -> int:
     return min(int(value), 2 ** 31 - 1)
 
 
+def _sizes(what: str, lowest: dict, values: tuple) -> tuple:
+    """:func:`_size` of several (``lowest``: {name: lowest value})."""
+    if all(low <= v < 2 ** 31 for low, v in zip(lowest.values(), values)):
+        return values
+    return tuple(_size(what, name, v, low) for (name, low), v in zip(lowest.items(), values))
+
+
 def paged_extend(new_rows: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, free_pages: torch.Tensor,
                  free_count: torch.Tensor, *, page_size: int, num_pages: int, num_rows: int,
                  seq_lens_out: Optional[torch.Tensor] = None, free_count_out: Optional[torch.Tensor] = None
@@ -722,9 +729,8 @@ def paged_extend(new_rows: torch.Tensor, page_table: torch.Tensor, seq_lens: tor
     length is negative, nothing changes, every start is 0 and every slot -1, and
     bit 8 of the device status is set."""
     what = "paged_extend"
-    ps, pool = _size(what, "page_size", page_size, 1), _size(what, "num_pages", num_pages, 1)
-    rows = _size(what, "num_rows", num_rows, 0)
-    res = paged_call().extend(new_rows, page_table, seq_lens, free_pages, free_count, ps, pool, rows, seq_lens_out,
+    sizes = _sizes(what, dict(page_size=1, num_pages=1, num_rows=0), (page_size, num_pages, num_rows))
+    res = paged_call().extend(new_rows, page_table, seq_lens, free_pages, free_count, *sizes, seq_lens_out,
                               free_count_out)
     if res is None:
         B = page_table.shape[0] if page_table.dim() else 0
@@ -822,9 +828,8 @@ def paged_select(q: torch.Tensor, key_means: torch.Tensor, page_table: torch.Ten
     ascending columns of page_table, -1 behind the end. Blocks are numbered over the
     batch; there are as many as the rows can make, those past the last empty."""
     what = "paged_select"
-    sizes = (_size(what, "page_size", page_size, 1), _size(what, "topk", topk, 0),
-             _size(what, "query_block", query_block, 1), _size(what, "window_size", window_size, 0),
-             _size(what, "num_prefix_tokens", num_prefix_tokens, 0))
+    sizes = _sizes(what, dict(page_size=1, topk=0, query_block=1, window_size=0, num_prefix_tokens=0),
+                   (page_size, topk, query_block, window_size, num_prefix_tokens))
     if q_start is None and query_block != 1:
         raise SabreError(f"{what}: query blocks of {query_block} rows need q_start")
     res = paged_call().select(q, key_means, page_table, seq_lens, q_start, *sizes)
