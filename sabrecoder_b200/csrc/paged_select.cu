@@ -11,10 +11,10 @@
 // as far as they are present. Only full pages are scored: every page that is
 // partly filled holds a query's own position.
 //
-// Both the queries' sum and s_p are summed in 64 bits and s_p is rounded once to
-// fp32: the order of the sums then changes a score, and so a list, only for values
-// that lie within 2^-50 or so of a border, where 32 bits would make the lists
-// depend on the order of every sum.
+// The order is that of sums in 64 bits, a score rounded once to fp32: it depends on the
+// order of a sum only for values that lie within 2^-30 or so of a border, where sums in
+// 32 bits would make a list in a thousand depend on it. (The queries' sum is kept in two
+// fp32 parts, which hold it exactly while the bits of its terms span no more than 48.)
 namespace sabre {
 namespace paged {
 
@@ -793,8 +793,8 @@ int sabre_paged_select(const void* q, const float* key_means, const int32_t* pag
   if (st != SABRE_OK) return st;
   if (!q || !lists || !counts || !q_strides) return sabre_fail(SABRE_ERR_INVALID_ARG, "%s: null pointer argument", fn);
   if (rows <= 0 || heads_q <= 0) return sabre_fail(SABRE_ERR_INVALID_ARG, "%s: sizes must be positive", fn);
-  if (heads_q % heads_kv != 0)
-    return sabre_fail(SABRE_ERR_UNSUPPORTED, "%s: heads_q/heads_kv must be an integer", fn);
+  if (heads_q % heads_kv != 0 || heads_q / heads_kv > 1024)  // rows of a block stay below 2^20
+    return sabre_fail(SABRE_ERR_UNSUPPORTED, "%s: heads_q/heads_kv must be an integer <= 1024", fn);
   if (topk < 0 || query_block <= 0 || query_block > 1024 || window < 0 || num_prefix_tokens < 0)
     return sabre_fail(SABRE_ERR_INVALID_ARG, "%s: topk %d, query_block %d, window %d, num_prefix_tokens %d", fn, topk,
                       query_block, window, num_prefix_tokens);

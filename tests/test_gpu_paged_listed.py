@@ -42,6 +42,8 @@ EXTEND = [
     ([(37 * i) % 300 for i in range(600)], [(i * i) % 4 for i in range(600)], 32, 9, 5, 1),
     ([(11 * i) % 40 for i in range(1500)], [1] * 1500, 16, 0, 0, 0),
     ([0] * 3, [40000, 1, 30000], 128, 1, 1, 1),
+    ([i % 33 for i in range(16384)], [i % 2 for i in range(16384)], 16, 3, 1, 0),
+    ([0, 0, 7, 0], [0, 2049, 0, 0], 16, 0, 0, 0),
 ]
 
 
@@ -242,6 +244,13 @@ SELECT = [
     ([900, 1300], [900, 200], 6, 2, 32, BF, 33, 4, 1000, 5000),
     ([600] * 40, [i % 5 for i in range(40)], 2, 2, 16, BF, 2, 3, 16, 16),
     ([3000, 260], [2049, 260], 2, 2, 32, BF, 64, 12, 31, 0),
+    # Enough blocks that groups of four share the means they read.
+    ([3000, 0, 777, 2500], [2900, 0, 700, 2500], 16, 16, 16, BF, 16, 6, 30, 20),
+    ([2600, 5, 900], [2600, 2, 800], 56, 8, 32, FP, 5, 9, 0, 0),
+    ([2600], [2600], 16, 2, 16, BF, 3, 200, 100, 64),
+    ([7 * i % 90 + 150 for i in range(200)], [i % 7 for i in range(200)], 4, 4, 16, BF, 2, 2, 16, 16),
+    ([20000], [1300], 4, 4, 16, FP, 4, 700, 0, 0),
+    ([4000, 900], [3000, 900], 32, 32, 1024, BF, 128, 1, 0, 0),
 ]
 
 
@@ -271,6 +280,50 @@ def test_select_vs_oracle(K, case):
     want = PO.select(q, means, table, sl, qs, block=block, window=window, prefix=prefix, **kw)
     check_lists(lists, counts, want)
     assert K.device_status(clear=True) == 0
+
+
+@pytest.mark.parametrize("lens,news,Hq,Hkv,block,topk", [
+    ([2000, 900], [1900, 700], 16, 16, 16, 5), ([2000, 900], [1900, 700], 16, 16, 16, 60), ([3000], [1], 4, 2, 1, 40),
+    ([3000, 2000], [40, 30], 8, 1, 16, 7)])
+def test_select_among_many_equal_scores(K, lens, news, Hq, Hkv, block, topk):
+    """Queries and means of small whole numbers: scores are exact and many are equal."""
+    q, kp, _, table, sl, starts = make(79, lens, news, Hq, Hkv, 16, BF)
+    gen = torch.Generator(device="cuda").manual_seed(7)
+    q = torch.randint(-1, 2, q.shape, generator=gen, device="cuda").to(BF)
+    means = torch.randint(-1, 2, (kp.shape[0], Hkv, D), generator=gen, device="cuda").float()
+    means[..., 8:] = 0
+    starts = starts if block > 1 else None
+    lists, counts = K.paged_select(q, means, table, sl, starts, page_size=16, topk=topk, query_block=block)
+    check_lists(lists, counts, PO.select(q, means, table, sl, starts, page_size=16, topk=topk, block=block))
+
+
+@pytest.mark.parametrize("lens,news,Hkv,block", [([2000, 900], [1900, 700], 16, 16), ([2000, 900], [2, 3], 2, 1)])
+def test_select_with_odd_values_in_queries_and_means(K, lens, news, Hkv, block):
+    """NaN, infinities and numbers at the ends of their ranges, in some queries and pages."""
+    q, kp, _, table, sl, starts = make(78, lens, news, Hkv, Hkv, 16, BF)
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    means = torch.randn(kp.shape[0], Hkv, D, generator=gen, device="cuda")
+    for x, bad in ((means, float("nan")), (means, float("inf")), (means, -float("inf")), (means, 3e38), (means, 1e-44),
+                   (q, float("nan")), (q, float("inf")), (q, 3e38), (q, -1e-38)):
+        for _ in range(3):
+            i, h, d = (int(torch.randint(0, n, (1,), generator=gen, device="cuda")) for n in x.shape)
+            x[i, h, d] = bad
+    lists, counts = K.paged_select(q, means, table, sl, starts, page_size=16, topk=9, query_block=block)
+    check_lists(lists, counts, PO.select(q, means, table, sl, starts, page_size=16, topk=9, block=block))
+
+
+def test_select_scores_that_only_64_bits_tell_apart(K):
+    """Means that differ in their last bit, and queries whose sum cancels."""
+    q, kp, _, table, sl, starts = make(77, [3000, 3000], [64, 64], 4, 4, 16, BF)
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    q[1::2] = -q[::2]
+    q[::16, :, :4] += 0.0625
+    base = torch.randn(4, D, generator=gen, device="cuda")
+    ulp = torch.randint(-3, 4, (kp.shape[0], 4, D), generator=gen, device="cuda").float() * 2.0 ** -24
+    means = base * (1 + ulp)
+    for block, starts_ in ((16, starts), (64, starts)):
+        lists, counts = K.paged_select(q, means, table, sl, starts_, page_size=16, topk=20, query_block=block)
+        check_lists(lists, counts, PO.select(q, means, table, sl, starts_, page_size=16, topk=20, block=block))
 
 
 def test_select_equal_scores_and_odd_ones(K):
