@@ -481,8 +481,11 @@ int sabre_copy_pages(void* pages, int buffers, int64_t buffer_stride, int num_pa
  *   reads: those of the first num_prefix_tokens tokens, those that hold a key at
  *   most `window` before one of the block's queries, its own included, and the
  *   topk best of the others by (sum of the block's q over rows and heads of the
- *   group) . key_means[page]; ties to the lower column, NaN last. Sums are 64
- *   bits wide, a score is rounded to fp32 once. Absent pages are not listed.
+ *   group) . key_means[page]; ties to the lower column, NaN last. Scores are
+ *   ordered as sums in 64 bits rounded to fp32 once (the sum of the queries in
+ *   two fp32 parts; one past fp32's range is infinite). Absent pages are not
+ *   listed; the mean of a page is read only when the page is full of rows before
+ *   the block's first.
  *   lists int32 [blocks, Hkv, width] (contiguous, ascending, -1 behind the
  *   end), width = sabre_paged_select_width(...); counts int32 [blocks, Hkv]. All
  *   entries are written; blocks past the last have none. At most 32768 columns,

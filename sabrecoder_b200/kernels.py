@@ -820,9 +820,10 @@ def paged_select(q: torch.Tensor, key_means: torch.Tensor, page_table: torch.Ten
     the pages of the first ``num_prefix_tokens`` tokens, those with a key at most
     ``window_size`` before one of its queries (their own positions included) and
     the ``topk`` others whose mean key has the largest product with the sum of the
-    block's queries (over its rows and the group's heads). Sums are 64 bits wide, a
-    score is rounded to fp32 once; equal scores go to the earlier page, NaN last.
-    Absent pages are left out.
+    block's queries (over its rows and the group's heads). Scores are ordered as sums
+    in 64 bits rounded to fp32 once; equal scores go to the earlier page, NaN last.
+    Absent pages are left out. Means are read of pages only that are full of rows
+    before the block's first.
 
     Returns ``(lists int32 [blocks, Hkv, width], counts int32 [blocks, Hkv])``:
     ascending columns of page_table, -1 behind the end. Blocks are numbered over the
