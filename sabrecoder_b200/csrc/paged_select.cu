@@ -130,7 +130,9 @@ struct Params {
   const int32_t* starts;
   int32_t* lists;
   int32_t* counts;
-  long long q_sr, q_sh, m_sp, m_sh;
+  long long m_sp, m_sh;
+  int q_sr, q_sh;       // one multiplication a row: sums of queries are bound by their instructions
+  uint32_t per_group;   // ceil(2^32 / group), for rows / group (group > 1)
   int rows, heads_kv, group, tokens, topk, window, prefix, cap;
   int blocks, ctas, key_row;  // ctas: of a cluster; key_row: keys of a block in shared memory
 };
@@ -262,13 +264,14 @@ __device__ __forceinline__ void sum_queries(const Params& p, const Block& blk, i
                                             float* lo) {
   const int lane = threadIdx.x & 31;
   const int many = blk.count * p.group;
-  const T* const q = static_cast<const T*>(p.q) + blk.row * p.q_sr + hk * p.group * p.q_sh + (lane & 15) * 8;
-  const float per = 1.0f / p.group;  // r < 2^20: (r + 1/2) / group is never within rounding of a whole number
+  const T* const q = static_cast<const T*>(p.q) + blk.row * p.q_sr + static_cast<long long>(hk) * p.group * p.q_sh +
+                     (lane & 15) * 8;
   uint64_t sum[4] = {}, rest[4] = {};
   auto load = [&](int r) -> uint4 {
     if (r >= many) return make_uint4(0u, 0u, 0u, 0u);
-    const int tok = static_cast<int>((r + 0.5f) * per);
-    return *reinterpret_cast<const uint4*>(q + tok * p.q_sr + (r - tok * p.group) * p.q_sh);
+    const int tok = p.group == 1 ? r : __umulhi(r, p.per_group);  // exact for r < 2^32 / group
+    return *reinterpret_cast<const uint4*>(q + (static_cast<long long>(tok) * p.q_sr +
+                                                static_cast<long long>(r - tok * p.group) * p.q_sh));
   };
   uint4 x[8];
 #pragma unroll
@@ -532,10 +535,10 @@ __global__ void __launch_bounds__(kWarps * 32, kGroup == 1 ? 5 : 16 / kGroup) pa
 
   // Scores: eight lanes share a page, 16 columns each (four of every 32).
   const int sub = lane & 7;
-  float4 q1[kGroup == 1 ? 4 : 1];
+  ulonglong2 q1[kGroup == 1 ? 4 : 1];  // four columns as two pairs, as everything below
   if constexpr (kGroup == 1) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) q1[j] = *reinterpret_cast<const float4*>(&s_hi[of][32 * j + 4 * sub]);
+    for (int j = 0; j < 4; ++j) q1[j] = *reinterpret_cast<const ulonglong2*>(&s_hi[of][32 * j + 4 * sub]);
   }
   // The first CTA has started when its shared memory is written to.
   uint32_t keys = smem_u32(s_key), told = smem_u32(s_told);
@@ -556,7 +559,7 @@ __global__ void __launch_bounds__(kWarps * 32, kGroup == 1 ? 5 : 16 / kGroup) pa
     const int next = g0 + 32 + lane;
     entry = next < p1 ? p.c.entry(t.b, next << p.c.page_shift) : -1;
     for (int u0 = 0; u0 < here; u0 += 4 * kInFlight) {
-      float4 m[kInFlight][4];
+      ulonglong2 m[kInFlight][4];
       int page[kInFlight];
 #pragma unroll
       for (int u = 0; u < kInFlight; ++u) {
@@ -567,29 +570,32 @@ __global__ void __launch_bounds__(kWarps * 32, kGroup == 1 ? 5 : 16 / kGroup) pa
         const float* src = p.means + page[u] * p.m_sp + hk * p.m_sh + 4 * sub;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
-          m[u][j] = scored ? *reinterpret_cast<const float4*>(src + 32 * j) : make_float4(0.f, 0.f, 0.f, 0.f);
+          m[u][j] = scored ? *reinterpret_cast<const ulonglong2*>(src + 32 * j) : make_ulonglong2(0ull, 0ull);
       }
 #pragma unroll
       for (int u = 0; u < kInFlight; ++u) {
-        float n2 = 0.f;
+        uint64_t n2 = 0ull;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          n2 = fmaf(m[u][j].x, m[u][j].x,
-                    fmaf(m[u][j].y, m[u][j].y, fmaf(m[u][j].z, m[u][j].z, fmaf(m[u][j].w, m[u][j].w, n2))));
-        size = n2 <= 1e37f ? fmaxf(size, n2) : INFINITY;
+        for (int j = 0; j < 4; ++j) n2 = f2_fma(m[u][j].x, m[u][j].x, f2_fma(m[u][j].y, m[u][j].y, n2));
+        float a, b;
+        f2_unpack(n2, a, b);
+        size = a + b <= 1e37f ? fmaxf(size, a + b) : INFINITY;
       }
       float acc[kInFlight][kGroup];
 #pragma unroll
       for (int g = 0; g < kGroup; ++g) {
-#pragma unroll
-        for (int u = 0; u < kInFlight; ++u) acc[u][g] = 0.f;
+        uint64_t two[kInFlight] = {};
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const float4 x = kGroup == 1 ? q1[j] : *reinterpret_cast<const float4*>(&s_hi[g][32 * j + 4 * sub]);
+          const ulonglong2 x = kGroup == 1 ? q1[j] : *reinterpret_cast<const ulonglong2*>(&s_hi[g][32 * j + 4 * sub]);
 #pragma unroll
-          for (int u = 0; u < kInFlight; ++u)
-            acc[u][g] = fmaf(x.x, m[u][j].x,
-                             fmaf(x.y, m[u][j].y, fmaf(x.z, m[u][j].z, fmaf(x.w, m[u][j].w, acc[u][g]))));
+          for (int u = 0; u < kInFlight; ++u) two[u] = f2_fma(x.x, m[u][j].x, f2_fma(x.y, m[u][j].y, two[u]));
+        }
+#pragma unroll
+        for (int u = 0; u < kInFlight; ++u) {
+          float a, b;
+          f2_unpack(two[u], a, b);
+          acc[u][g] = a + b;
         }
       }
 #pragma unroll
@@ -811,8 +817,11 @@ int sabre_paged_select(const void* q, const float* key_means, const int32_t* pag
   p.starts = q_start;
   p.lists = lists;
   p.counts = counts;
-  p.q_sr = q_strides[0];
-  p.q_sh = q_strides[1];
+  if (q_strides[0] < 0 || q_strides[1] < 0 || q_strides[0] > INT_MAX || q_strides[1] > INT_MAX)
+    return sabre_fail(SABRE_ERR_UNSUPPORTED, "%s: q strides must be from 0 to 2^31 - 1", fn);
+  p.q_sr = static_cast<int>(q_strides[0]);
+  p.q_sh = static_cast<int>(q_strides[1]);
+  p.per_group = static_cast<uint32_t>(((1ull << 32) + heads_q / heads_kv - 1) / (heads_q / heads_kv));
   p.m_sp = km_strides[0];
   p.m_sh = km_strides[1];
   p.rows = rows;

@@ -240,6 +240,7 @@ def c_select(**kw):
     (dict(block=1025), -1, b"query_block"), (dict(window=-1), -1, b"window"), (dict(starts=None), -1, b"q_start"),
     (dict(starts=None, block=1, rows=4), -1, b"q_start"), (dict(max_pages=32769, stride=32769), -2, b"32768"),
     (dict(q=8), -3, b"aligned"), (dict(qs=_lib.i64([512, 4])), -3, b"aligned"), (dict(means=4), -3, b"key_means"),
+    (dict(qs=_lib.i64([2 ** 31, 128])), -2, b"strides"), (dict(heads_q=2050), -2, b"1024"),
 ])
 def test_c_select_rejects(kw, code, match):
     got, msg = c_select(**kw)
