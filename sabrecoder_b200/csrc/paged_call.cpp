@@ -128,6 +128,14 @@ int integer(PyObject* o) {
   return static_cast<int>(x);
 }
 
+// A size of at least `low`, held to int32; false below that.
+bool sized(PyObject* o, long long low, int& out) {
+  const long long x = PyLong_AsLongLong(o);
+  if (x == -1 && PyErr_Occurred()) throw python_error();
+  out = x > INT_MAX ? INT_MAX : static_cast<int>(x);
+  return x >= low;
+}
+
 float number(PyObject* o) {
   const double x = PyFloat_AsDouble(o);
   if (x == -1.0 && PyErr_Occurred()) throw python_error();
@@ -255,15 +263,15 @@ PyObject* extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_RETURN_NONE;
   if (!lens_out) lens_out = p.lens;
   if (!count_out) count_out = count;
-  const int rows = integer(a[7]);
-  if (rows < 0) Py_RETURN_NONE;
+  int page_size, num_pages, rows;
+  if (!sized(a[5], 1, page_size) || !sized(a[6], 1, num_pages) || !sized(a[7], 0, rows)) Py_RETURN_NONE;
   const c10::cuda::CUDAGuard guard(p.dev);
   at::Tensor starts = fresh_tensor({int64_t{p.batch} + 1}, at::kInt, p.dev);
   at::Tensor slots = fresh_tensor({rows}, at::kLong, p.dev), positions = fresh_tensor({rows}, at::kLong, p.dev);
   const int st = sabre_paged_extend(
       i32(fresh), i32(p.table), i32(p.lens), i32(lens_out), i32(free_pages), i32(count), i32(count_out), i32(&starts),
       static_cast<int64_t*>(slots.data_ptr()), static_cast<int64_t*>(positions.data_ptr()), rows, p.batch,
-      integer(a[6]), integer(a[5]), p.cols, free_pages->size(0), p.table->stride(0),
+      num_pages, page_size, p.cols, free_pages->size(0), p.table->stride(0),
       c10::cuda::getCurrentCUDAStream(p.dev).stream());
   if (st != SABRE_OK) return PyLong_FromLong(st);
   // More than 2048 rows are placed by a kernel of their own.
@@ -281,8 +289,8 @@ PyObject* key_means(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!k || !p.on(*k) || k->dim() != 4 || code(*k) < 0 || k->stride(3) != 1 || !p.means(m) ||
       m->size(0) != k->size(0) || m->size(1) != k->size(1) || m->size(2) != k->size(3) || !small(k->size(2)))
     Py_RETURN_NONE;
-  const int rows = integer(a[5]);
-  if (rows < 0 || (!p.starts && rows != p.batch)) Py_RETURN_NONE;
+  int rows;
+  if (!sized(a[5], 0, rows) || (!p.starts && rows != p.batch)) Py_RETURN_NONE;
   if (rows == 0 || p.batch == 0) return PyLong_FromLong(0);
   const int64_t ks[3] = {k->stride(0), k->stride(1), k->stride(2)}, ms[2] = {m->stride(0), m->stride(1)};
   const c10::cuda::CUDAGuard guard(p.dev);
@@ -304,8 +312,11 @@ PyObject* select(PyObject*, PyObject* const* a, Py_ssize_t n) {
       q->size(2) != m->size(2) || !small(q->size(0)) || !small(q->size(1)) || m->size(1) == 0 ||
       (!p.starts && q->size(0) != p.batch))
     Py_RETURN_NONE;
-  const int rows = q->size(0), heads = m->size(1), page_size = integer(a[5]), topk = integer(a[6]);
-  const int block = integer(a[7]), window = integer(a[8]), prefix = integer(a[9]);
+  const int rows = q->size(0), heads = m->size(1);
+  int page_size, topk, block, window, prefix;
+  if (!sized(a[5], 1, page_size) || !sized(a[6], 0, topk) || !sized(a[7], 1, block) || !sized(a[8], 0, window) ||
+      !sized(a[9], 0, prefix) || (!p.starts && block != 1))
+    Py_RETURN_NONE;
   const c10::cuda::CUDAGuard guard(p.dev);
   const int blocks = sabre_paged_query_blocks(rows, p.batch, block);
   const int width = sabre_paged_select_width(page_size, p.cols, topk, block, window, prefix);
@@ -332,9 +343,9 @@ PyObject* attend_listed(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (n != 12 || !p.read(a[1], a[2], a[3], a[4], a[5])) Py_RETURN_NONE;
   const at::Tensor *q = tensor(a[0]), *lists = tensor(a[6]), *counts = tensor(a[7]);
   if (!p.rows(q) || (!p.starts && q->size(0) != p.batch)) Py_RETURN_NONE;
-  const int block = integer(a[8]);
+  int block;
+  if (!sized(a[8], 1, block)) Py_RETURN_NONE;
   const float scale = number(a[9]);
-  if (block <= 0) Py_RETURN_NONE;
   const int rows = q->size(0), heads_q = q->size(1);
   const int blocks = p.starts ? sabre_paged_query_blocks(rows, p.batch, block) : p.batch;
   for (const at::Tensor* t : {lists, counts})

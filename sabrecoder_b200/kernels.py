@@ -694,18 +694,12 @@ def _refuse_tables(what: str, page_table, seq_lens, q_start, ints: dict, **other
             raise SabreError(f"{what}: {name} is on {t.device}, page_table is on {page_table.device}")
 
 
-def _size(what: str, name: str, value: int, low: int) -> int:
-    """An argument as the C ABI's int; values past int32 are held there."""
-    if value < low:
-        raise SabreError(f"{what}: {name} {value} must be at least {low}")
-    return min(int(value), 2 ** 31 - 1)
-
-
-def _sizes(what: str, lowest: dict, values: tuple) -> tuple:
-    """:func:`_size` of several (``lowest``: {name: lowest value})."""
-    if all(low <= v < 2 ** 31 for low, v in zip(lowest.values(), values)):
-        return values
-    return tuple(_size(what, name, v, low) for (name, low), v in zip(lowest.items(), values))
+def _refuse_sizes(what: str, **sizes) -> None:
+    """Raises for sizes below their lowest values ({name: (value, lowest)}); those past
+    int32 are held there by the compiled calls."""
+    for name, (value, low) in sizes.items():
+        if value < low:
+            raise SabreError(f"{what}: {name} {value} must be at least {low}")
 
 
 def paged_extend(new_rows: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, free_pages: torch.Tensor,
@@ -729,10 +723,10 @@ def paged_extend(new_rows: torch.Tensor, page_table: torch.Tensor, seq_lens: tor
     length is negative, nothing changes, every start is 0 and every slot -1, and
     bit 8 of the device status is set."""
     what = "paged_extend"
-    sizes = _sizes(what, dict(page_size=1, num_pages=1, num_rows=0), (page_size, num_pages, num_rows))
-    res = paged_call().extend(new_rows, page_table, seq_lens, free_pages, free_count, *sizes, seq_lens_out,
-                              free_count_out)
+    res = paged_call().extend(new_rows, page_table, seq_lens, free_pages, free_count, page_size, num_pages, num_rows,
+                              seq_lens_out, free_count_out)
     if res is None:
+        _refuse_sizes(what, page_size=(page_size, 1), num_pages=(num_pages, 1), num_rows=(num_rows, 0))
         B = page_table.shape[0] if page_table.dim() else 0
         _refuse_tables(what, page_table, seq_lens, None, dict(
             new_rows=(new_rows, B), free_pages=(free_pages, None), free_count=(free_count, 1),
@@ -786,8 +780,9 @@ def paged_key_means(k_pages: torch.Tensor, key_means: torch.Tensor, page_table: 
         if q_start is not None:
             raise SabreError(f"{what} needs num_rows with q_start")
         num_rows = page_table.shape[0]
-    st = paged_call().key_means(k_pages, key_means, page_table, seq_lens, q_start, _size(what, "num_rows", num_rows, 0))
+    st = paged_call().key_means(k_pages, key_means, page_table, seq_lens, q_start, num_rows)
     if st is None:
+        _refuse_sizes(what, num_rows=(num_rows, 0))
         if k_pages.dim() != 4 or k_pages.dtype not in DTYPE_CODE or k_pages.stride(3) != 1:
             raise SabreError(f"{what}: k_pages {tuple(k_pages.shape)} must be [num_pages, Hkv, page_size, D] bf16 or "
                              f"f16 with unit head-dim stride")
@@ -829,12 +824,13 @@ def paged_select(q: torch.Tensor, key_means: torch.Tensor, page_table: torch.Ten
     ascending columns of page_table, -1 behind the end. Blocks are numbered over the
     batch; there are as many as the rows can make, those past the last empty."""
     what = "paged_select"
-    sizes = _sizes(what, dict(page_size=1, topk=0, query_block=1, window_size=0, num_prefix_tokens=0),
-                   (page_size, topk, query_block, window_size, num_prefix_tokens))
-    if q_start is None and query_block != 1:
-        raise SabreError(f"{what}: query blocks of {query_block} rows need q_start")
-    res = paged_call().select(q, key_means, page_table, seq_lens, q_start, *sizes)
+    res = paged_call().select(q, key_means, page_table, seq_lens, q_start, page_size, topk, query_block, window_size,
+                              num_prefix_tokens)
     if res is None:
+        _refuse_sizes(what, page_size=(page_size, 1), topk=(topk, 0), query_block=(query_block, 1),
+                      window_size=(window_size, 0), num_prefix_tokens=(num_prefix_tokens, 0))
+        if q_start is None and query_block != 1:
+            raise SabreError(f"{what}: query blocks of {query_block} rows need q_start")
         if q.dim() != 3 or q.dtype not in DTYPE_CODE or q.stride(2) != 1:
             raise SabreError(f"{what}: q {tuple(q.shape)} must be [N, Hq, D] bf16 or f16 with unit last stride")
         _refuse_means(what, key_means, (None, None, q.shape[2]))
@@ -850,10 +846,10 @@ def paged_select(q: torch.Tensor, key_means: torch.Tensor, page_table: torch.Ten
 
 def _attend_listed(what: str, q, k_pages, v_pages, page_table, seq_lens, q_start, lists, counts, query_block,
                    softmax_scale, out, workspace) -> torch.Tensor:
-    block = _size(what, "query_block", query_block, 1)
-    res = paged_call().attend_listed(q, k_pages, v_pages, page_table, seq_lens, q_start, lists, counts, block,
+    res = paged_call().attend_listed(q, k_pages, v_pages, page_table, seq_lens, q_start, lists, counts, query_block,
                                      softmax_scale or 0.0, out, workspace)
     if res is None:
+        _refuse_sizes(what, query_block=(query_block, 1))
         for name, t, dims in (("lists", lists, 3), ("counts", counts, 2)):
             if not isinstance(t, torch.Tensor) or t.dim() != dims or t.dtype != torch.int32:
                 raise SabreError(f"{what}: {name} must be int32 {'[blocks, Hkv, n]' if dims == 3 else '[blocks, Hkv]'}")
@@ -863,7 +859,7 @@ def _attend_listed(what: str, q, k_pages, v_pages, page_table, seq_lens, q_start
         B, H = page_table.shape[0], k_pages.shape[1] if k_pages.dim() == 4 else None
         if q.dim() == 3 and lists.shape[:2] == counts.shape and \
                 (q_start is not None or q.shape[0] == B) and H is not None:
-            blocks = lib().sabre_paged_query_blocks(q.shape[0], B, block) if q_start is not None else B
+            blocks = lib().sabre_paged_query_blocks(q.shape[0], B, query_block) if q_start is not None else B
             if counts.shape[0] < blocks or counts.shape[1] != H:
                 raise SabreError(f"{what}: lists of {tuple(counts.shape)} (blocks, heads) for {blocks} query blocks of "
                                  f"{H} KV heads")
