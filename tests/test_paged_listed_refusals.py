@@ -139,7 +139,8 @@ def test_key_means_refuses():
 
 
 @pytest.mark.parametrize("kw,match", [(dict(topk=-1), "topk"), (dict(window_size=-1), "window_size"),
-                                      (dict(num_prefix_tokens=-1), "num_prefix_tokens"), (dict(query_block=0), "query_block"),
+                                      (dict(num_prefix_tokens=-1), "num_prefix_tokens"),
+                                      (dict(query_block=0), "query_block"),
                                       (dict(page_size=0), "page_size")])
 def test_select_sizes_are_checked(kw, match):
     with pytest.raises(_lib.SabreError, match=match):
@@ -200,7 +201,8 @@ def c_extend(**kw):
 @pytest.mark.parametrize("kw,code,match", [
     (dict(new_rows=None), -1, b"null"), (dict(free=None), -1, b"null"), (dict(slots=None), -1, b"null"),
     (dict(lens_out=16), -1, b"same"), (dict(rows=-1), -1, b"sizes"), (dict(batch=0), -1, b"sizes"),
-    (dict(free_size=-1), -1, b"sizes"), (dict(page_size=24), -2, b"page_size"), (dict(page_size=2048), -2, b"page_size"),
+    (dict(free_size=-1), -1, b"sizes"), (dict(page_size=24), -2, b"page_size"),
+    (dict(page_size=2048), -2, b"page_size"),
     (dict(page_size=1024, max_pages=2 ** 21, stride=2 ** 21), -2, b"2^30"), (dict(batch=16385, stride=2), -2, b"16384"),
     (dict(stride=1), -1, b"overlap"), (dict(rows=2 ** 30 + 1), -2, b"2^30"),
 ])
@@ -217,7 +219,8 @@ def c_means(**kw):
 
 
 @pytest.mark.parametrize("kw,code,match", [
-    (dict(k=None), -1, b"null"), (dict(means=None), -1, b"null"), (dict(rows=0), -1, b"rows"), (dict(rows=4), -1, b"q_start"),
+    (dict(k=None), -1, b"null"), (dict(means=None), -1, b"null"), (dict(rows=0), -1, b"rows"),
+    (dict(rows=4), -1, b"q_start"),
     (dict(dim=64), -2, b"head_dim"), (dict(means=8), -3, b"key_means"), (dict(ms=_lib.i64([256, 126])), -3, b"key_means"),
     (dict(ms=_lib.i64([-256, 128])), -3, b"key_means"), (dict(dtype=2), -1, b"dtype"),
 ])
@@ -235,7 +238,8 @@ def c_select(**kw):
 
 
 @pytest.mark.parametrize("kw,code,match", [
-    (dict(q=None), -1, b"null"), (dict(lists=None), -1, b"null"), (dict(heads_q=0), -1, b"sizes"), (dict(rows=0), -1, b"sizes"),
+    (dict(q=None), -1, b"null"), (dict(lists=None), -1, b"null"), (dict(heads_q=0), -1, b"sizes"),
+    (dict(rows=0), -1, b"sizes"),
     (dict(heads_q=3), -2, b"integer"), (dict(topk=-1), -1, b"topk"), (dict(block=0), -1, b"query_block"),
     (dict(block=1025), -1, b"query_block"), (dict(window=-1), -1, b"window"), (dict(starts=None), -1, b"q_start"),
     (dict(starts=None, block=1, rows=4), -1, b"q_start"), (dict(max_pages=32769, stride=32769), -2, b"32768"),
@@ -265,7 +269,8 @@ def c_prefill(**kw):
 
 BOTH = [
     (dict(lists=None), -1, b"null"), (dict(counts=None), -1, b"null"), (dict(entries=0), -1, b"entries"),
-    (dict(ls=_lib.i64([-12, 6])), -1, b"strides"), (dict(cs=_lib.i64([2, -1])), -1, b"strides"), (dict(q=None), -1, b"null"),
+    (dict(ls=_lib.i64([-12, 6])), -1, b"strides"), (dict(cs=_lib.i64([2, -1])), -1, b"strides"),
+    (dict(q=None), -1, b"null"),
     (dict(heads_q=5), -2, b"integer"), (dict(heads_q=18), -2, b"integer"), (dict(dim=64), -2, b"head_dim"),
     (dict(page_size=1024, entries=2 ** 20 + 1), -2, b"2^30"),
 ]
