@@ -156,9 +156,10 @@ class SabrePagedKVCache(Cache):
         if topk_pages is not None:
             self.key_means = torch.empty(num_layers, self.num_pages, num_kv_heads, head_dim, dtype=torch.float32,
                                          device=device)
-        # Pages lent to the device, as a stack, and how many of them it still has.
+        # Pages lent to the device, as a stack, and how many of them it still has (-1:
+        # none are lent, and a graph that extends on the device changes nothing).
         self.free_pages = torch.zeros(self.num_pages, dtype=torch.int32, device=device)
-        self.free_count = torch.zeros(1, dtype=torch.int32, device=device)
+        self.free_count = torch.full((1,), -1, dtype=torch.int32, device=device)
         self._lent: Optional[List[int]] = None
         self.refs: List[int] = [0] * self.num_pages
         self.unused: List[int] = list(range(self.num_pages - 1, -1, -1))  # the lowest page is taken first
@@ -436,7 +437,7 @@ class SabrePagedKVCache(Cache):
             self.refs[page] = 1
         self.unused += lent[:left]
         self.lengths, self._lent = lengths, None
-        self.free_count.zero_()
+        self.free_count.fill_(-1)
         # The host's copies of the tables; the device has them.
         host = self._host.numpy()
         for b, t in enumerate(self.tables):

@@ -254,6 +254,16 @@ SELECT = [
 ]
 
 
+@pytest.mark.parametrize("lens,news,Hq,Hkv", [([900, 0, 30, 500], [200, 0, 30, 1], 8, 8), ([700], [600], 56, 8)])
+def test_select_for_each_row_of_a_prompt(K, lens, news, Hq, Hkv):
+    """Blocks of one row, alone and in groups."""
+    q, kp, _, table, sl, starts = make(83, lens, news, Hq, Hkv, 16, BF)
+    means = torch.randn(kp.shape[0], Hkv, D, device="cuda")
+    kw = dict(page_size=16, topk=4, window_size=20, num_prefix_tokens=16)
+    lists, counts = K.paged_select(q, means, table, sl, starts, query_block=1, **kw)
+    check_lists(lists, counts, PO.select(q, means, table, sl, starts, page_size=16, topk=4, block=1, window=20, prefix=16))
+
+
 def lists_of(lists, counts):
     return [[lists[i, h, :int(counts[i, h])].tolist() for h in range(lists.shape[1])] for i in range(lists.shape[0])]
 

@@ -238,3 +238,5 @@ def test_a_graph_that_runs_out_of_pages_stands_still(cuda):
     graph.replay()
     c.settle()
     assert c.lengths == [17, 17] and K.device_status(clear=True) == 0
+    graph.replay()  # nothing is lent: no row is added, although the last pages have room
+    assert slots.tolist() == [-1, -1] and c.seq_lens.tolist() == [17, 17] and K.device_status(clear=True) == 8

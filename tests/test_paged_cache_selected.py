@@ -282,6 +282,19 @@ def test_settling_refuses_tables_that_do_not_match():
         c.extend_on_device(torch.tensor([1, 1, 1], dtype=torch.int32), 3)
 
 
+def test_a_step_after_settling_changes_nothing():
+    """A graph of an earlier loan, replayed: also where a row fits into a last page."""
+    c = cache()
+    one = torch.ones(3, dtype=torch.int32)
+    c.lend()
+    c.extend_on_device(one, 3)
+    c.settle()
+    _, slots, _ = PC.K.paged_extend(one, c.page_table, c.seq_lens, c.free_pages, c.free_count, page_size=PS,
+                                    num_pages=c.num_pages, num_rows=3)
+    assert (slots == -1).all() and c.lengths == [1, 1, 1]
+    consistent(c)
+
+
 def test_lending_inside_a_capture_is_refused(monkeypatch):
     c = cache()
     monkeypatch.setattr(PC, "_capturing", lambda pool: True)
