@@ -392,8 +392,10 @@ PyObject* attend_listed(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                       p.batch, heads_q, p.heads, p.dim, p.pages, p.page_size, p.cols, qr, p.ks, p.vs,
                                       orr, ls, cs, p.table->stride(0), scale, p.dtype, wp, wb, stream);
   if (st != SABRE_OK) return PyLong_FromLong(st);
-  // As in attend: prompts whose pairs are cut into parts ask for a workspace.
-  const bool joined = p.starts ? need > 0 : p.batch > 1 || p.heads > 1 || int64_t{entries} * p.page_size > 64;
+  // As in attend: prompts whose pairs are cut into parts ask for a workspace; decodes of
+  // more than one key tile are joined by a second kernel, unless they run in clusters.
+  const int64_t tiles = (int64_t{entries} * p.page_size + 63) / 64, pairs = int64_t{p.batch} * p.heads;
+  const bool joined = p.starts ? need > 0 : tiles * pairs > 1 && !(pairs * 8 <= 296 && tiles > 1 && tiles <= 32);
   return result(out, joined ? 2 : 1);
   END_HANDLE_TH_ERRORS
 }

@@ -92,7 +92,7 @@ struct Tiles {
 // The same over the listed pages of one (sequence, KV head) pair: 64 list rows a
 // tile, as many tiles as its list has entries for. Bound by HBM as the dense decode:
 // 64 sequences at 56/8 heads over 22 pages of 128 rows (649 MB) take 106.5 us, 6.1
-// TB/s; one sequence of 14 pages at 16/16 heads 8.0, the latency of two kernels.
+// TB/s; one sequence of 14 pages at 16/16 heads 6.8 (a cluster a pair, below).
 struct ListedTiles {
   int n, entries, count;
   __device__ __forceinline__ ListedTiles(const DecodeParams& p, int b, int hk) {
@@ -328,11 +328,27 @@ struct PartSum {
   }
 };
 
-// kListed: over the pages of p.lists; else over all rows, or the window's.
-template <typename T, bool kListed>
+// A barrier over all threads of the cluster.
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// Short lists of few pairs run in clusters: kCluster CTAs take a pair's tiles in equal
+// runs and the first joins them over the cluster's shared memory, which spares the
+// joining kernel (one sequence of 14 pages at 16/16 heads 8.0 -> 6.8 us). A CTA then has
+// at most kClusterTiles tiles.
+constexpr int kCluster = 8;
+constexpr int kClusterTiles = 4;
+
+// kMode: over all rows, or the window's; over the pages of p.lists; the same in clusters.
+enum DecodeMode { kDense, kOverPages, kInClusters };
+template <typename T, DecodeMode kMode>
 __global__ void __launch_bounds__(kDecThreads, 2)
     paged_decode_kernel(const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                         const DecodeParams p) {
+  constexpr bool kListed = kMode != kDense;
+  constexpr bool kClustered = kMode == kInClusters;
   // paged_join_kernel (a programmatic dependent launch) may become resident
   // now; its griddepcontrol.wait still waits for this whole grid.
   if (threadIdx.x == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -366,21 +382,32 @@ __global__ void __launch_bounds__(kDecThreads, 2)
   Shares sh;
   Place at;
   T* const out = static_cast<T*>(p.o);
-  const bool some = locate<kListed>(p, reinterpret_cast<int*>(smem + kAccOff), sh, at, [&](int x) {
-    // No visible tile: the sequence's (with lists: the pair's) rows are zero.
-    if (x % p.ctas != static_cast<int>(blockIdx.x)) return;
-    const int b = kListed ? x / p.heads_kv : x;
-    const int h0 = kListed ? x % p.heads_kv * p.group : 0;
-    for (int h = h0; h < h0 + (kListed ? 1 : p.heads_kv) * p.group; ++h)
-      for (int d = 0; d < kD; d += 8)
-        *reinterpret_cast<uint4*>(out + b * p.o_sb + h * p.o_sh + d) = make_uint4(0u, 0u, 0u, 0u);
-  });
-  // locate()'s barriers order the mbarrier set-up above before its use.
-  if (!some) {
-    if (tid == 0) p.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
-    return;
+  long long units;
+  if constexpr (kClustered) {
+    const int pair = blockIdx.x / kCluster, rank = blockIdx.x % kCluster;
+    at.b = pair / p.heads_kv;
+    at.hk = pair % p.heads_kv;
+    const int n = ListedTiles(p, at.b, at.hk).count;
+    at.tile = n * rank / kCluster;
+    units = n * (rank + 1) / kCluster - at.tile;
+  } else {
+    const bool some = locate<kListed>(p, reinterpret_cast<int*>(smem + kAccOff), sh, at, [&](int x) {
+      // No visible tile: the sequence's (with lists: the pair's) rows are zero.
+      if (x % p.ctas != static_cast<int>(blockIdx.x)) return;
+      const int b = kListed ? x / p.heads_kv : x;
+      const int h0 = kListed ? x % p.heads_kv * p.group : 0;
+      for (int h = h0; h < h0 + (kListed ? 1 : p.heads_kv) * p.group; ++h)
+        for (int d = 0; d < kD; d += 8)
+          *reinterpret_cast<uint4*>(out + b * p.o_sb + h * p.o_sh + d) = make_uint4(0u, 0u, 0u, 0u);
+    });
+    // locate()'s barriers order the mbarrier set-up above before its use.
+    if (!some) {
+      if (tid == 0) p.joins[blockIdx.x] = make_int4(0, 0, 0, 0);
+      return;
+    }
+    units = sh.first(blockIdx.x + 1) - sh.first(blockIdx.x);
   }
-  Segments<kListed> seg(p, at, sh.first(blockIdx.x + 1) - sh.first(blockIdx.x));
+  Segments<kListed> seg(p, at, units);
   __syncthreads();  // the scratch of locate() is free
   bool ok = *abort_flag == 0;
 
@@ -440,6 +467,11 @@ __global__ void __launch_bounds__(kDecThreads, 2)
     if (lane == 0)
       for (int i = max(0, issued - kStages); i < issued; ++i)
         mbar_wait_drain(full_bar(i % kStages), (i / kStages) & 1);
+    if constexpr (kClustered) {  // the joining below
+      __syncwarp();
+      cluster_sync();
+      cluster_sync();
+    }
     return;
   }
 
@@ -465,6 +497,16 @@ __global__ void __launch_bounds__(kDecThreads, 2)
       qf[kk][1] = r4 < p.group ? *reinterpret_cast<const uint32_t*>(qp + kk * 16 + 8) : 0u;
     }
   };
+  // kClustered: what this CTA has of the two heads that a warp joins, four columns a lane.
+  float4 mine_a[kGroup / kConsumers];
+  float2 mine_ml[kGroup / kConsumers];
+  if constexpr (kClustered) {
+#pragma unroll
+    for (int u = 0; u < kGroup / kConsumers; ++u) {
+      mine_a[u] = make_float4(0.f, 0.f, 0.f, 0.f);
+      mine_ml[u] = make_float2(-INFINITY, 0.f);
+    }
+  }
   bool more = seg.next();
   if (more) load_q();
   while (more) {
@@ -574,7 +616,7 @@ __global__ void __launch_bounds__(kDecThreads, 2)
     const bool whole_pair = seg.t0 == 0 && seg.t1 == seg.tiles.count;
     // A part is kept as the share's first (0) or last (1) segment.
     const int place = 2 * static_cast<int>(blockIdx.x) + (seg.seen > 0 ? 1 : 0);
-    if (tid == 0 && seg.left == 0) {
+    if (!kClustered && tid == 0 && seg.left == 0) {
       // When the share ends inside a pair that began in it, the pair is joined for it.
       const int rest = seg.t0 == 0 ? seg.tiles.count - seg.t1 : 0;
       const int parts = rest > 0 ? sh.owner(sh.first(blockIdx.x + 1) + rest - 1) - static_cast<int>(blockIdx.x) + 1 : 0;
@@ -628,6 +670,11 @@ __global__ void __launch_bounds__(kDecThreads, 2)
           A.z += a * x.z;
           A.w += a * x.w;
         }
+        if constexpr (kClustered) {
+          mine_a[u] = A;
+          mine_ml[u] = make_float2(M, L);
+          continue;
+        }
         if (whole_pair)
           store_row<T>(out + b * p.o_sb + (hk * p.group + g) * p.o_sh, lane, A, L);
         else
@@ -636,6 +683,60 @@ __global__ void __launch_bounds__(kDecThreads, 2)
       }
     }
     named_bar_sync(1, kConsumers * 32);  // the joining buffers are free again
+  }
+
+  if constexpr (kClustered) {
+    // Every CTA is done with its ring when the first barrier lets it through; the parts
+    // then go into the first one's: [rank][head][kD], and (m, l, whether it is whole).
+    ok = ok && *abort_flag == 0;
+    const int rank = blockIdx.x % kCluster;
+    const int pair = blockIdx.x / kCluster;
+    constexpr int kMlAt = kCluster * kGroup * kD * 4;
+    cluster_sync();
+    uint32_t dst;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(dst) : "r"(sbase + kRingOff), "r"(0));
+#pragma unroll
+    for (int u = 0; u < kGroup / kConsumers; ++u) {
+      const int slot = rank * kGroup + warp + u * kConsumers;
+      asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(dst + slot * kD * 4 + lane * 16),
+                   "f"(mine_a[u].x), "f"(mine_a[u].y), "f"(mine_a[u].z), "f"(mine_a[u].w)
+                   : "memory");
+      if (lane == 0)
+        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %3};" ::"r"(dst + kMlAt + slot * 16),
+                     "f"(mine_ml[u].x), "f"(mine_ml[u].y), "f"(ok ? 1.f : 0.f)
+                     : "memory");
+    }
+    cluster_sync();
+    if (rank != 0) return;
+#pragma unroll
+    for (int u = 0; u < kGroup / kConsumers; ++u) {
+      const int g = warp + u * kConsumers;
+      if (g >= p.group) break;
+      float4 ml[kCluster];
+      float mn = -INFINITY;
+      bool whole = true;
+#pragma unroll
+      for (int r = 0; r < kCluster; ++r) {
+        ml[r] = *reinterpret_cast<const float4*>(smem + kRingOff + kMlAt + (r * kGroup + g) * 16);
+        mn = fmaxf(mn, ml[r].x);
+        whole = whole && ml[r].z != 0.f;
+      }
+      PartSum sum;
+      const float off = mn == -INFINITY ? 0.f : mn;
+#pragma unroll
+      for (int r = 0; r < kCluster; ++r) {
+        const float4 a = *reinterpret_cast<const float4*>(smem + kRingOff + (r * kGroup + g) * kD * 4 + lane * 16);
+        // A part without a maximum has sums of 0 or NaN, which are added as they are.
+        if (ml[r].x == -INFINITY)
+          sum.l += ml[r].y;
+        else
+          sum.add(off, ml[r].x, ml[r].y, a);
+      }
+      // After a timeout in any CTA the result is incomplete: store nothing.
+      if (whole)
+        store_row<T>(out + (pair / p.heads_kv) * p.o_sb + (pair % p.heads_kv * p.group + g) * p.o_sh, lane, sum.a,
+                     sum.l);
+    }
   }
 }
 
@@ -731,12 +832,15 @@ static size_t decode_workspace(int group) {
   return kDecCtas * sizeof(int4) + static_cast<size_t>(2) * kDecCtas * group * (kD + 2) * sizeof(float);
 }
 
-template <typename T, bool kListed>
+template <typename T, DecodeMode kMode>
 static cudaError_t launch_paged_decode(const CUtensorMap& mk, const CUtensorMap& mv, const DecodeParams& p,
                                        cudaStream_t s) {
-  const auto kernel = paged_decode_kernel<T, kListed>;
+  const auto kernel = paged_decode_kernel<T, kMode>;
   cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kDecSmem);
   if (e != cudaSuccess) return e;
+  if (kMode == kInClusters)
+    return launch_cluster(dim3(p.c.batch * p.heads_kv * kCluster), kCluster, kDecThreads, kDecSmem, s, kernel, mk, mv,
+                          p);
   e = launch_dependent(dim3(p.ctas), kDecThreads, kDecSmem, s, kernel, mk, mv, p);
   if (e != cudaSuccess || p.ctas == 1) return e;  // a single share is finished where it is
   return launch_dependent(dim3(p.ctas - 1, p.group), kJoinWarps * 32, 0, s, paged_join_kernel<T>, p);
@@ -797,12 +901,17 @@ static int decode_call(const char* fn, const void* q, const void* k_pages, const
     return st;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-  if (lists)
-    e = dtype == SABRE_BF16 ? launch_paged_decode<__nv_bfloat16, true>(mk, mv, p, s)
-                            : launch_paged_decode<__half, true>(mk, mv, p, s);
+  // Clusters for pairs whose CTAs all have a place at once (tiles: of all pairs).
+  const long long pairs = static_cast<long long>(batch) * heads_kv;
+  if (lists && pairs * kCluster <= kDecCtas && tiles > pairs && tiles <= pairs * kCluster * kClusterTiles)
+    e = dtype == SABRE_BF16 ? launch_paged_decode<__nv_bfloat16, kInClusters>(mk, mv, p, s)
+                            : launch_paged_decode<__half, kInClusters>(mk, mv, p, s);
+  else if (lists)
+    e = dtype == SABRE_BF16 ? launch_paged_decode<__nv_bfloat16, kOverPages>(mk, mv, p, s)
+                            : launch_paged_decode<__half, kOverPages>(mk, mv, p, s);
   else
-    e = dtype == SABRE_BF16 ? launch_paged_decode<__nv_bfloat16, false>(mk, mv, p, s)
-                            : launch_paged_decode<__half, false>(mk, mv, p, s);
+    e = dtype == SABRE_BF16 ? launch_paged_decode<__nv_bfloat16, kDense>(mk, mv, p, s)
+                            : launch_paged_decode<__half, kDense>(mk, mv, p, s);
   return e == cudaSuccess ? SABRE_OK : sabre_cuda_fail(e, fn);
 }
 

@@ -441,6 +441,13 @@ DECODE = [
     (list(range(0, 300)), 2, 2, 16, BF, 7, 0.4, "phtd"),
     ([40000], 32, 32, 128, BF, 200, 0.5, "phtd"),
     ([70001, 2], 7, 1, 64, FP, 900, 0.8, "phtd"),
+    # A cluster a pair: up to 37 pairs of two to 32 key tiles.
+    ([2000], 1, 1, 64, BF, 2, 0.9, "phtd"),
+    ([3000, 0, 5, 64, 2049], 7, 1, 64, BF, 32, 0.9, "ptkhd"),
+    ([3000, 700, 1], 24, 12, 16, FP, 128, 0.7, "phtd"),
+    ([100, 3000], 16, 16, 1024, BF, 2, 1.0, "phtd"),
+    ([2100] * 37, 8, 1, 32, FP, 9, 0.2, "phtd"),
+    ([2100] * 38, 8, 1, 32, FP, 9, 0.2, "phtd"),  # a pair too many
 ]
 
 
@@ -705,6 +712,79 @@ def test_two_streams_at_once(K):
     assert K.device_status(clear=True) == 0
 
 
+@pytest.mark.parametrize("call", ["clusters", "shares", "prompt", "parts"])
+def test_listed_waits_that_run_out_end_the_call(K, call):
+    """A wait limit shorter than any load: the call ends, records it and leaves the
+    device usable."""
+    lens, news = ([5000, 3000], [1, 1]) if call in ("clusters", "shares") else ([5000, 3000], [70, 40])
+    args = make(407, lens, news, 4, 2, 64, BF)
+    q, kp, vp, table, sl, starts = args
+    block = 1 if call in ("clusters", "shares") else 32
+    lists, counts = random_lists(5, args, 2, 64, block, starts, dict(clusters=20, shares=70, prompt=6, parts=70)[call],
+                                 0.9)
+
+    def run():
+        if block == 1:
+            return K.paged_decode_listed(q, kp, vp, table, sl, lists, counts)
+        return K.paged_prefill_listed(q, kp, vp, table, sl, starts, lists, counts, query_block=block)
+
+    K.device_status(clear=True)
+    K.set_wait_limit_ns(1000)
+    try:
+        run()
+        torch.cuda.synchronize()
+    finally:
+        K.set_wait_limit_ns(0)
+    assert K.device_status(clear=True) & 1
+    out = run()
+    assert K.device_status(clear=True) == 0
+    check(out, args, lists, counts, starts, block)
+
+
+def test_two_streams_and_two_captured_graphs_of_listed_calls(K):
+    """Calls on two streams, and two captured calls replayed at once, each with the
+    workspace of its own that it allocates."""
+    sides = [torch.cuda.Stream(), torch.cuda.Stream()]
+    jobs, graphs, outs = [], [], []
+    for i, side in enumerate(sides):
+        args = make(408 + i, [3000 + 77 * i, 2900], [60, 5], 4, 2, 64, BF)
+        q, kp, vp, table, sl, starts = args
+        long = random_lists(i, args, 2, 64, 32, starts, 40, 0.9)
+        short = [t[[0, 2]] for t in long]
+        wide = random_lists(9 + i, (q[:2],) + args[1:], 2, 64, 1, None, 46, 0.95)
+        jobs.append((args, long, short, wide))
+
+        def run(args=args, long=long, short=short, wide=wide):
+            q, kp, vp, table, sl, starts = args
+            return (K.paged_prefill_listed(q, kp, vp, table, sl, starts, *long, query_block=32),
+                    K.paged_decode_listed(q[:2], kp, vp, table, sl, short[0][:, :, :20], short[1]),
+                    K.paged_decode_listed(q[:2], kp, vp, table, sl, *wide))
+
+        run()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            outs.append(run())
+        graphs.append((g, run))
+    for kind in ("streams", "graphs"):
+        got = [None, None]
+        for _ in range(5):
+            for i, side in enumerate(sides):
+                with torch.cuda.stream(side):
+                    if kind == "graphs":
+                        graphs[i][0].replay()
+                        got[i] = outs[i]
+                    else:
+                        got[i] = graphs[i][1]()
+        torch.cuda.synchronize()
+        for (args, long, short, wide), (a, b, c) in zip(jobs, got):
+            check(a, args, *long, args[5], 32)
+            two = (args[0][:2],) + args[1:]
+            check(b, two, short[0][:, :, :20], short[1])
+            check(c, two, *wide)
+    assert K.device_status(clear=True) == 0
+
+
 def test_launches_of_listed_calls_are_counted(K):
     """LAUNCHES grows by the kernels of a call: those of its captured graph."""
     from cuda.bindings import runtime
@@ -738,6 +818,9 @@ def test_launches_of_listed_calls_are_counted(K):
     assert kernels(lambda: K.paged_prefill_listed(q, kp, vp, table, sl, starts, lists, counts, query_block=16)) == 2
     assert kernels(lambda: K.paged_prefill_listed(q, kp, vp, table, sl, starts, lists[:, :, :2], counts,
                                                   query_block=16)) == 1
-    assert kernels(lambda: K.paged_decode_listed(q[:2], kp, vp, table, sl, lists[:2], counts[:2])) == 2
+    # A cluster a pair up to 32 key tiles; parts and a joining kernel beyond them.
+    assert kernels(lambda: K.paged_decode_listed(q[:2], kp, vp, table, sl, lists[:2], counts[:2])) == 1
+    long = i32(list(range(132))).expand(2, 2, 132)
+    assert kernels(lambda: K.paged_decode_listed(q[:2], kp, vp, table, sl, long, counts[:2])) == 2
     assert kernels(lambda: K.paged_decode_listed(q[:1, :2], kp[:, :1], vp[:, :1], table[:1], sl[:1], lists[:1, :1, :4],
                                                  counts[:1, :1])) == 1
