@@ -727,7 +727,7 @@ def paged_extend(new_rows: torch.Tensor, page_table: torch.Tensor, seq_lens: tor
                               seq_lens_out, free_count_out)
     if res is None:
         _refuse_sizes(what, page_size=(page_size, 1), num_pages=(num_pages, 1), num_rows=(num_rows, 0))
-        B = page_table.shape[0] if page_table.dim() else 0
+        B = page_table.shape[0] if isinstance(page_table, torch.Tensor) and page_table.dim() else 0
         _refuse_tables(what, page_table, seq_lens, None, dict(
             new_rows=(new_rows, B), free_pages=(free_pages, None), free_count=(free_count, 1),
             seq_lens_out=(seq_lens_out, B), free_count_out=(free_count_out, 1)))

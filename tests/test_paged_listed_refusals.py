@@ -81,6 +81,8 @@ def test_row_starts_are_checked(call):
 
 
 EXTEND = [
+    (dict(page_table=None), {}, "page_table must be a tensor"),
+    (dict(seq_lens=[0, 0, 0]), {}, "seq_lens must be a tensor"),
     (dict(new_rows=i32(2)), {}, "new_rows"),
     (dict(new_rows=torch.zeros(3)), {}, "new_rows|int32"),
     (dict(free_pages=i32(7, 1)), {}, "free_pages"),
