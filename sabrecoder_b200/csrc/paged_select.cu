@@ -691,7 +691,9 @@ __global__ void __launch_bounds__(kWarps * 32, kGroup == 1 ? 5 : 16 / kGroup) pa
   for (int j = 0; j < 4; ++j) q2 = fmaf(s_hi[of][32 * j + lane], s_hi[of][32 * j + lane], q2);
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) q2 += __shfl_xor_sync(0xffffffffu, q2, o);
-  const float bound = 24.f * sqrtf(q2) * sqrtf(size) * 0x1.1p-24f + 1e-37f;
+  // 2^-120 is more than what underflow takes from 128 squares, so that the lengths of
+  // tiny vectors (below 2^-60) are bounded from above too; 1e-37 covers the products'.
+  const float bound = 24.f * sqrtf(q2 + 0x1p-120f) * sqrtf(size + 0x1p-120f) * 0x1.1p-24f + 1e-37f;
   const Cut cut = choose(p, key, mine.pages, lo, hi, candidates, bound, s_hi[of], s_lo[of], t.b, hk, s_near[pick]);
   write_list(p, cut, key, mine.pages, block + pick, hk);
 }
