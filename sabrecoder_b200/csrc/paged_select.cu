@@ -487,9 +487,10 @@ __global__ void __launch_bounds__(kWarps * 32, kGroup == 1 ? 5 : 16 / kGroup) pa
         for (int w = 0; w < kWarps; ++w) before += scratch[w], all += scratch[kWarps + w];
       }
       block = before + t.r / p.tokens;
-      // Blocks that the rows could make but do not hold have no pages.
-      for (int i = all + slot * kWarps + warp; i < p.blocks; i += gridDim.x * kWarps)
-        write_list(p, Cut{0u, 0}, s_key, 0, i, hk);
+      // Blocks that the rows could make but do not hold have no pages. (A count past
+      // int32, which only starts that do not ascend can make, is past them all.)
+      for (long long i = (all < 0 ? p.blocks : all) + 0ll + slot * kWarps + warp; i < p.blocks; i += gridDim.x * kWarps)
+        write_list(p, Cut{0u, 0}, s_key, 0, static_cast<int>(i), hk);
       if (t.b < 0) return;
     }
   }
@@ -669,9 +670,10 @@ __global__ void __launch_bounds__(kWarps * 32, kGroup == 1 ? 5 : 16 / kGroup) pa
     __syncthreads();
   }
 
-  // A warp picks for its block; kGroup = 1: the first one.
-  if (kGroup == 1 ? warp > 0 : mine.count == 0) return;
+  // A warp picks for its block; kGroup = 1: the first one. Starts that do not ascend
+  // count more blocks than there is room for.
   const int pick = kGroup > 1 ? warp : 0;
+  if (kGroup == 1 ? warp > 0 : mine.count == 0 || static_cast<uint32_t>(block + pick) >= p.blocks) return;
   uint32_t* const key = s_key + pick * p.key_row;
   uint4 sum = make_uint4(kAlways, 0u, 0u, 0u);
   for (int i = lane; i < p.ctas * kWarps; i += 32) {

@@ -6,6 +6,7 @@ import pytest
 import torch
 
 from oracle import paged_oracle as PO
+from sabrecoder_b200 import _lib
 from test_gpu_paged import BF, D, make
 from test_gpu_paged_listed import K, check, check_lists, i32  # noqa: F401 (K: a fixture)
 
@@ -27,3 +28,30 @@ def test_select_of_tiny_means_and_queries(K, lens, news, block, of_means, of_que
     starts = None if block == 1 else starts
     lists, counts = K.paged_select(q, means, table, sl, starts, page_size=16, topk=20, query_block=block)
     check_lists(lists, counts, PO.select(q, means, table, sl, starts, page_size=16, topk=20, block=block))
+
+
+@pytest.mark.parametrize("starts,rows,block", [([0, 12800, 0, 12800], 12800, 16), ([0, 700, 3, 700, 0, 700], 700, 1),
+                                               ([0, 640] * 20, 640, 4)])
+def test_select_with_row_starts_that_do_not_ascend(K, starts, rows, block):
+    """Sequences that share rows count more blocks than the rows can make: no list or
+    count behind the last is written."""
+    B, H, ps = len(starts) - 1, 16, 16
+    L = K.lib()
+    blocks, cols = L.sabre_paged_query_blocks(rows, B, block), -(-rows // ps)
+    width = L.sabre_paged_select_width(ps, cols, 3, block, 0, 0)
+    q = torch.randn(rows, H, D, device="cuda").to(BF)
+    means = torch.randn(cols, H, D, device="cuda")
+    table = torch.arange(cols, dtype=torch.int32, device="cuda").repeat(B, 1)
+    lens, start = i32([rows] * B), i32(starts)
+    lists = torch.full((2 * blocks + B * rows, H, width), -7, dtype=torch.int32, device="cuda")
+    counts = torch.full((2 * blocks + B * rows, H), -7, dtype=torch.int32, device="cuda")
+    st = L.sabre_paged_select(q.data_ptr(), means.data_ptr(), table.data_ptr(), lens.data_ptr(), start.data_ptr(),
+                              lists[blocks:].data_ptr(), counts[blocks:].data_ptr(), rows, B, H, H, D, cols, ps, cols, 3,
+                              block, 0, 0, _lib.i64([H * D, D]), _lib.i64([H * D, D]), cols, 0,
+                              torch.cuda.current_stream().cuda_stream)
+    assert st == 0
+    for t in (lists, counts):
+        assert (t[:blocks] == -7).all() and (t[2 * blocks:] == -7).all()
+    mine = counts[blocks:2 * blocks]
+    assert ((mine >= 0) & (mine <= width) | (mine == -7)).all() and (mine > 0).any()
+    assert K.device_status(clear=True) == 0
