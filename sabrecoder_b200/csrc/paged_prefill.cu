@@ -650,7 +650,9 @@ __global__ void __launch_bounds__(kThreads, 2)
       const int head = hk * p.group + tid - tok * p.group;
       const bool real = tok < job.count;
       const int pos = job.pos0 + tok;
-      const int seen = real ? min(pos + 1, job.n) : 0;  // keys [0, seen), less the window's gap
+      // Keys [0, seen), less the window's gap. Over lists never below 0, as for rows before
+      // their sequence: seen - kNowhere could pass the end of int32.
+      const int seen = real ? max(min(pos + 1, job.n), kListed ? 0 : INT_MIN) : 0;
       const int wlo = p.w.first(pos);
       // Every row of the warp, if it has any, sees the keys [all_wlo, all_seen).
       const int all_seen = __any_sync(0xffffffffu, real) ? __reduce_min_sync(0xffffffffu, real ? seen : INT_MAX) : 0;

@@ -55,3 +55,21 @@ def test_select_with_row_starts_that_do_not_ascend(K, starts, rows, block):
     mine = counts[blocks:2 * blocks]
     assert ((mine >= 0) & (mine <= width) | (mine == -7)).all() and (mine > 0).any()
     assert K.device_status(clear=True) == 0
+
+
+@pytest.mark.parametrize("width", [1, 300])
+def test_listed_rows_far_before_their_sequence_give_zeros(K, width):
+    """A block of 128 rows of which 108 lie before the sequence, whatever they hold; also
+    in parts of long lists."""
+    args = make(406, [128, 200], [128, 128], 2, 2, 16, BF)
+    q, kp, vp, table, sl, starts = args
+    sl[0] = 20
+    q[:108] = float("nan")
+    lists = torch.full((3, 2, width), -1, dtype=torch.int32, device="cuda")  # the rows could make three blocks
+    lists[:, :, 0] = 0
+    counts = i32([[1, 1]] * 3)
+    out = K.paged_prefill_listed(q, kp, vp, table, sl, starts, lists, counts, query_block=128)
+    assert (out[:108] == 0).all()
+    clean = (q.nan_to_num(0.0),) + args[1:]
+    check(out, clean, lists, counts, starts, 128)
+    assert K.device_status(clear=True) == 0
