@@ -414,12 +414,16 @@ class SabrePagedKVCache(Cache):
                               num_rows=k.shape[0])
 
     def settle(self) -> None:
-        """Takes over what the device did with the pages lent (waits for it) and takes
-        the others back. Nothing happens when none are lent."""
+        """Takes over what the device did with the pages lent and takes the others back.
+        Waits for all of the device's streams: steps may have been replayed on any of
+        them, and later ones, on any of them, find nothing lent. Nothing happens when
+        none are lent."""
         if _capturing(self.pool):
             raise ValueError("SabrePagedKVCache: settle() reads from the device, which a capture cannot")
         if self._lent is None:
             return
+        wait = torch.cuda.synchronize if self.pool.is_cuda else lambda device: None
+        wait(self.pool.device)
         ps, lent = self.page_size, self._lent
         left = int(self.free_count)
         lengths, rows = self.seq_lens.tolist(), self.page_table.tolist()
@@ -438,6 +442,7 @@ class SabrePagedKVCache(Cache):
         self.unused += lent[:left]
         self.lengths, self._lent = lengths, None
         self.free_count.fill_(-1)
+        wait(self.pool.device)
         # The host's copies of the tables; the device has them.
         host = self._host.numpy()
         for b, t in enumerate(self.tables):

@@ -73,3 +73,27 @@ def test_listed_rows_far_before_their_sequence_give_zeros(K, width):
     clean = (q.nan_to_num(0.0),) + args[1:]
     check(out, clean, lists, counts, starts, 128)
     assert K.device_status(clear=True) == 0
+
+
+def test_settling_waits_for_steps_on_other_streams(K):
+    from sabrecoder_b200.paged_cache import SabrePagedKVCache
+    c = SabrePagedKVCache(batch_size=3, max_seq_len=64, page_size=16, num_layers=1, num_kv_heads=1, head_dim=D)
+    new = i32([20, 0, 1])
+    c.lend()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        c.extend_on_device(new, 21)
+        torch.cuda._sleep(200_000_000)  # a tenth of a second or so
+        c.extend_on_device(new, 21)
+    c.settle()
+    assert c.lengths == [40, 0, 2] == c.seq_lens.tolist() and c.pages_in_use == 4
+    c.extend([1, 1, 1])
+    assert c.seq_lens.tolist() == [41, 1, 3] and K.device_status(clear=True) == 0
+    c.lend()
+    c.settle()
+    with torch.cuda.stream(side):  # not ordered behind it: nothing is lent all the same
+        _, slots, _ = K.paged_extend(new, c.page_table, c.seq_lens, c.free_pages, c.free_count, page_size=16,
+                                     num_pages=c.num_pages, num_rows=21)
+    side.synchronize()
+    assert (slots == -1).all() and c.seq_lens.tolist() == c.lengths and K.device_status(clear=True) == 8
