@@ -467,6 +467,8 @@ int sabre_copy_pages(void* pages, int buffers, int64_t buffer_stride, int num_pa
  *   entry becomes -1). When the pages, a table row or the `rows` are too few,
  *   or a length is negative, nothing changes, all starts are 0, all slots -1
  *   and SABRE_DEV_NO_ROOM is recorded. At most 16384 sequences and 2^30 rows.
+ * sabre_paged_extend_within: the same for sequences of at most max_len rows,
+ *   where that is less than their table rows hold: longer ones have no room.
  * sabre_paged_store_slots: rows k, v [rows, Hkv, D] into the places slots[r] =
  *   page * page_size + row of the page; a negative slot drops its row, one past
  *   the pool too and records SABRE_DEV_BAD_PAGE. No slot may be given twice.
@@ -504,6 +506,11 @@ int sabre_paged_extend(const int32_t* new_rows, int32_t* page_table, const int32
                        const int32_t* free_pages, const int32_t* free_count, int32_t* free_count_out,
                        int32_t* q_start, int64_t* slots, int64_t* positions, int rows, int batch, int num_pages,
                        int page_size, int max_pages, int free_size, int64_t table_stride, void* stream);
+int sabre_paged_extend_within(const int32_t* new_rows, int32_t* page_table, const int32_t* seq_lens,
+                              int32_t* seq_lens_out, const int32_t* free_pages, const int32_t* free_count,
+                              int32_t* free_count_out, int32_t* q_start, int64_t* slots, int64_t* positions, int rows,
+                              int batch, int num_pages, int page_size, int max_pages, int free_size, int max_len,
+                              int64_t table_stride, void* stream);
 int sabre_paged_store_slots(const void* k, const void* v, void* k_pages, void* v_pages, const int64_t* slots, int rows,
                             int heads_kv, int head_dim, int num_pages, int page_size, const int64_t* k_strides,
                             const int64_t* v_strides, const int64_t* kp_strides, const int64_t* vp_strides, int dtype,

@@ -79,13 +79,15 @@ def attention(q, k_pages, v_pages, table, seq_lens, q_start=None, *, window: Opt
 # block tables from lengths, and attention over selected pages
 # ---------------------------------------------------------------------------
 
-def extend(new, table, lens, free, count, page_size: int, num_pages: int, rows: int):
+def extend(new, table, lens, free, count, page_size: int, num_pages: int, rows: int, max_len: Optional[int] = None):
     """(fits, table, lens, count, starts, slots, positions) as lists; all arguments
-    lists too. Where it does not fit, everything is as before and no row has a place."""
+    lists too. Where it does not fit, everything is as before and no row has a place.
+    max_len: rows that a sequence may have, beside what its table row holds."""
     table, lens = [list(t) for t in table], list(lens)
     need = [-(-(n + m) // page_size) - -(-n // page_size) if n >= 0 and m >= 0 else 0 for n, m in zip(lens, new)]
     fits = all(n >= 0 and m >= 0 and n + m <= len(t) * page_size for n, m, t in zip(lens, new, table))
     fits = fits and 0 <= count <= len(free) and sum(need) <= count and sum(new) <= rows
+    fits = fits and (max_len is None or all(n + m <= max_len for n, m in zip(lens, new)))
     starts, slots, positions = [0], [], []
     for b, m in enumerate(new if fits else [0] * len(new)):
         for pos in range(lens[b], lens[b] + m):

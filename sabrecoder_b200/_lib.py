@@ -63,6 +63,8 @@ SIGNATURES = {
     "sabre_paged_prefill": (c_int, [P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
                                     c_int, c_int, I64P, I64P, I64P, I64P, c_int64, c_float, c_int, P, c_size_t, P]),
     "sabre_paged_extend": (c_int, [P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int64, P]),
+    "sabre_paged_extend_within": (c_int, [P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int,
+                                          c_int64, P]),
     "sabre_paged_store_slots": (c_int, [P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, I64P, I64P, I64P, I64P,
                                         c_int, P]),
     "sabre_paged_key_means": (c_int, [P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, I64P, I64P,

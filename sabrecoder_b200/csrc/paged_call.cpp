@@ -249,11 +249,11 @@ PyObject* store_slots(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 // extend(new_rows, page_table, seq_lens, free_pages, free_count, page_size, num_pages, rows, seq_lens_out or None,
-// free_count_out or None) -> (q_start, slots, positions, kernels)
+// free_count_out or None, max_seq_len or None) -> (q_start, slots, positions, kernels)
 PyObject* extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   Tables p;
-  if (n != 10 || !p.read(a[1], a[2], Py_None) || p.batch == 0) Py_RETURN_NONE;
+  if (n != 11 || !p.read(a[1], a[2], Py_None) || p.batch == 0) Py_RETURN_NONE;
   const at::Tensor *fresh = tensor(a[0]), *free_pages = tensor(a[3]), *count = tensor(a[4]);
   bool ok = true;
   const at::Tensor *lens_out = optional(a[8], ok), *count_out = optional(a[9], ok);
@@ -263,15 +263,17 @@ PyObject* extend(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_RETURN_NONE;
   if (!lens_out) lens_out = p.lens;
   if (!count_out) count_out = count;
-  int page_size, num_pages, rows;
-  if (!sized(a[5], 1, page_size) || !sized(a[6], 1, num_pages) || !sized(a[7], 0, rows)) Py_RETURN_NONE;
+  int page_size, num_pages, rows, max_len = INT_MAX;
+  if (!sized(a[5], 1, page_size) || !sized(a[6], 1, num_pages) || !sized(a[7], 0, rows) ||
+      (a[10] != Py_None && !sized(a[10], 1, max_len)))
+    Py_RETURN_NONE;
   const c10::cuda::CUDAGuard guard(p.dev);
   at::Tensor starts = fresh_tensor({int64_t{p.batch} + 1}, at::kInt, p.dev);
   at::Tensor slots = fresh_tensor({rows}, at::kLong, p.dev), positions = fresh_tensor({rows}, at::kLong, p.dev);
-  const int st = sabre_paged_extend(
+  const int st = sabre_paged_extend_within(
       i32(fresh), i32(p.table), i32(p.lens), i32(lens_out), i32(free_pages), i32(count), i32(count_out), i32(&starts),
       static_cast<int64_t*>(slots.data_ptr()), static_cast<int64_t*>(positions.data_ptr()), rows, p.batch,
-      num_pages, page_size, p.cols, free_pages->size(0), p.table->stride(0),
+      num_pages, page_size, p.cols, free_pages->size(0), max_len, p.table->stride(0),
       c10::cuda::getCurrentCUDAStream(p.dev).stream());
   if (st != SABRE_OK) return PyLong_FromLong(st);
   // More than 2048 rows are placed by a kernel of their own.

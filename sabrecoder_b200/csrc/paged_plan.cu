@@ -36,7 +36,8 @@ struct Params {
   long long* slots;
   long long* positions;
   long long table_sb;
-  int batch, max_pages, page_shift, num_pages, free_size, rows;
+  int batch, page_shift, num_pages, free_size, rows;
+  int limit;  // rows of a sequence at most
 
   __device__ __forceinline__ int page(int id) const {  // a page of the pool, or -1
     if (id < -1 || id >= num_pages) record_status(SABRE_DEV_BAD_PAGE);
@@ -88,7 +89,6 @@ __global__ void __launch_bounds__(kThreads) paged_extend_kernel(const Params p) 
   if (tid == 0) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int ps1 = (1 << p.page_shift) - 1;
-  const long long capacity = static_cast<long long>(p.max_pages) << p.page_shift;
   auto have = [&](int len) -> int { return (len + ps1) >> p.page_shift; };
 
   const int threads = blockDim.x;
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(kThreads) paged_extend_kernel(const Params p) 
   for (int b = b0; b < b1; ++b) {
     const int len = p.lens[b], fresh = p.fresh[b];
     // Refused below, with nothing of it used.
-    if (len < 0 || fresh < 0 || static_cast<long long>(len) + fresh > capacity) {
+    if (len < 0 || fresh < 0 || static_cast<long long>(len) + fresh > p.limit) {
       bad = true;
       continue;
     }
@@ -193,16 +193,13 @@ __global__ void __launch_bounds__(kRowThreads) paged_slots_kernel(const Params p
 }
 
 }  // namespace plan
-}  // namespace paged
-}  // namespace sabre
 
-extern "C" int sabre_paged_extend(const int32_t* new_rows, int32_t* page_table, const int32_t* seq_lens,
-                                  int32_t* seq_lens_out, const int32_t* free_pages, const int32_t* free_count,
-                                  int32_t* free_count_out, int32_t* q_start, int64_t* slots, int64_t* positions,
-                                  int rows, int batch, int num_pages, int page_size, int max_pages, int free_size,
-                                  int64_t table_stride, void* stream) {
-  using namespace sabre::paged;
-  const char* fn = "sabre_paged_extend";
+// Both entries; max_len: rows of a sequence at most, or -1: as many as its table row holds.
+static int extend_call(const char* fn, const int32_t* new_rows, int32_t* page_table, const int32_t* seq_lens,
+                       int32_t* seq_lens_out, const int32_t* free_pages, const int32_t* free_count,
+                       int32_t* free_count_out, int32_t* q_start, int64_t* slots, int64_t* positions, int rows,
+                       int batch, int num_pages, int page_size, int max_pages, int free_size, int max_len,
+                       int64_t table_stride, void* stream) {
   if (!new_rows || !page_table || !seq_lens || !seq_lens_out || !free_count || !free_count_out || !q_start ||
       (free_size > 0 && !free_pages) || (rows > 0 && (!slots || !positions)))
     return sabre_fail(SABRE_ERR_INVALID_ARG, "%s: null pointer argument", fn);
@@ -233,7 +230,8 @@ extern "C" int sabre_paged_extend(const int32_t* new_rows, int32_t* page_table, 
   p.positions = reinterpret_cast<long long*>(positions);
   p.table_sb = table_stride;
   p.batch = batch;
-  p.max_pages = max_pages;
+  p.limit = page_size * max_pages;
+  if (max_len >= 0 && max_len < p.limit) p.limit = max_len;
   p.page_shift = 0;
   while ((1 << p.page_shift) < page_size) ++p.page_shift;
   p.num_pages = num_pages;
@@ -252,3 +250,31 @@ extern "C" int sabre_paged_extend(const int32_t* new_rows, int32_t* page_table, 
     e = launch_dependent(dim3((rows + kCtaRows - 1) / kCtaRows), plan::kRowThreads, 0, st, plan::paged_slots_kernel, p);
   return e == cudaSuccess ? SABRE_OK : sabre_cuda_fail(e, fn);
 }
+
+}  // namespace paged
+}  // namespace sabre
+
+extern "C" {
+
+int sabre_paged_extend(const int32_t* new_rows, int32_t* page_table, const int32_t* seq_lens, int32_t* seq_lens_out,
+                       const int32_t* free_pages, const int32_t* free_count, int32_t* free_count_out,
+                       int32_t* q_start, int64_t* slots, int64_t* positions, int rows, int batch, int num_pages,
+                       int page_size, int max_pages, int free_size, int64_t table_stride, void* stream) {
+  return sabre::paged::extend_call("sabre_paged_extend", new_rows, page_table, seq_lens, seq_lens_out, free_pages,
+                                   free_count, free_count_out, q_start, slots, positions, rows, batch, num_pages,
+                                   page_size, max_pages, free_size, -1, table_stride, stream);
+}
+
+int sabre_paged_extend_within(const int32_t* new_rows, int32_t* page_table, const int32_t* seq_lens,
+                              int32_t* seq_lens_out, const int32_t* free_pages, const int32_t* free_count,
+                              int32_t* free_count_out, int32_t* q_start, int64_t* slots, int64_t* positions, int rows,
+                              int batch, int num_pages, int page_size, int max_pages, int free_size, int max_len,
+                              int64_t table_stride, void* stream) {
+  const char* fn = "sabre_paged_extend_within";
+  if (max_len < 0) return sabre_fail(SABRE_ERR_INVALID_ARG, "%s: max_len must not be negative", fn);
+  return sabre::paged::extend_call(fn, new_rows, page_table, seq_lens, seq_lens_out, free_pages, free_count,
+                                   free_count_out, q_start, slots, positions, rows, batch, num_pages, page_size,
+                                   max_pages, free_size, max_len, table_stride, stream);
+}
+
+}  // extern "C"

@@ -704,8 +704,8 @@ def _refuse_sizes(what: str, **sizes) -> None:
 
 def paged_extend(new_rows: torch.Tensor, page_table: torch.Tensor, seq_lens: torch.Tensor, free_pages: torch.Tensor,
                  free_count: torch.Tensor, *, page_size: int, num_pages: int, num_rows: int,
-                 seq_lens_out: Optional[torch.Tensor] = None, free_count_out: Optional[torch.Tensor] = None
-                 ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+                 seq_lens_out: Optional[torch.Tensor] = None, free_count_out: Optional[torch.Tensor] = None,
+                 max_seq_len: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """Block tables and slot maps from request lengths, without the host.
 
     new_rows int32 ``[B]``: rows that each sequence grows by; page_table int32
@@ -714,19 +714,21 @@ def paged_extend(new_rows: torch.Tensor, page_table: torch.Tensor, seq_lens: tor
     the last of ``free_pages[:free_count]`` taken first. Writes the new pages into
     page_table and the new lengths and count into ``seq_lens_out`` and
     ``free_count_out`` (default: in place). num_rows: room for rows, at least the
-    sum of new_rows (known on the host, as a captured batch's is).
+    sum of new_rows (known on the host, as a captured batch's is). max_seq_len: rows
+    that a sequence may have (default: as many as its row of the table holds).
 
     Returns ``(q_start int32 [B + 1], slots int64 [num_rows], positions int64
     [num_rows])``: row starts; each row's place ``page * page_size + row of the
     page`` for :func:`paged_store_slots` and its position. Rows past the last have
-    slot -1 and position 0. When pages, table columns or num_rows are too few, or a
-    length is negative, nothing changes, every start is 0 and every slot -1, and
-    bit 8 of the device status is set."""
+    slot -1 and position 0. When pages, table columns or num_rows are too few, a
+    sequence would pass max_seq_len or a length is negative, nothing changes, every
+    start is 0 and every slot -1, and bit 8 of the device status is set."""
     what = "paged_extend"
     res = paged_call().extend(new_rows, page_table, seq_lens, free_pages, free_count, page_size, num_pages, num_rows,
-                              seq_lens_out, free_count_out)
+                              seq_lens_out, free_count_out, max_seq_len)
     if res is None:
-        _refuse_sizes(what, page_size=(page_size, 1), num_pages=(num_pages, 1), num_rows=(num_rows, 0))
+        _refuse_sizes(what, page_size=(page_size, 1), num_pages=(num_pages, 1), num_rows=(num_rows, 0),
+                      max_seq_len=(1 if max_seq_len is None else max_seq_len, 1))
         B = page_table.shape[0] if isinstance(page_table, torch.Tensor) and page_table.dim() else 0
         _refuse_tables(what, page_table, seq_lens, None, dict(
             new_rows=(new_rows, B), free_pages=(free_pages, None), free_count=(free_count, 1),

@@ -397,11 +397,14 @@ class SabrePagedKVCache(Cache):
                          ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
         """Makes room for ``new_rows`` (int32 ``[B]``, on the device) more rows of each
         sequence, num_rows or fewer in all, from the pages lent: ``(q_start, slots,
-        positions)`` as :func:`kernels.paged_extend` gives them. May be captured."""
+        positions)`` as :func:`kernels.paged_extend` gives them. May be captured. A
+        sequence has no room past max_seq_len rows."""
         if self._lent is None:
             raise ValueError("SabrePagedKVCache: lend() pages to the device first")
+        # Where whole pages make up max_seq_len the table's width is the limit.
+        limit = dict(max_seq_len=self.max_seq_len) if self.max_seq_len % self.page_size else {}
         return K.paged_extend(new_rows, self.page_table, self.seq_lens, self.free_pages, self.free_count,
-                              page_size=self.page_size, num_pages=self.num_pages, num_rows=num_rows)
+                              page_size=self.page_size, num_pages=self.num_pages, num_rows=num_rows, **limit)
 
     def store_rows(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor, q_start: torch.Tensor,
                    slots: torch.Tensor) -> None:
@@ -429,7 +432,7 @@ class SabrePagedKVCache(Cache):
         lengths, rows = self.seq_lens.tolist(), self.page_table.tolist()
         taken = {}
         for b, n in enumerate(lengths):
-            if n < self.lengths[b] or n > self.max_pages * ps:
+            if n < self.lengths[b] or n > self.max_seq_len:
                 raise ValueError(f"SabrePagedKVCache: sequence {b} went from {self.lengths[b]} rows to {n} on the device")
             for col in range(len(self.tables[b]), -(-n // ps)):
                 taken[rows[b][col]] = taken.get(rows[b][col], 0) + 1

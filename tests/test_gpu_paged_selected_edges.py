@@ -97,3 +97,45 @@ def test_settling_waits_for_steps_on_other_streams(K):
                                      num_pages=c.num_pages, num_rows=21)
     side.synchronize()
     assert (slots == -1).all() and c.seq_lens.tolist() == c.lengths and K.device_status(clear=True) == 8
+
+
+@pytest.mark.parametrize("extra_rows", [0, 3000])
+@pytest.mark.parametrize("new,fits", [([10, 2, 0, 700], True), ([10, 3, 0, 700], False), ([0, 0, 1, 0], False),
+                                      ([0, 0, 0, 0], True)])
+def test_extend_within_a_greatest_length(K, new, fits, extra_rows):
+    """1000 rows at most on pages of 16; one sequence is there already."""
+    old, ps, pool = [5, 998, 1000, 300], 16, 300
+    table = [[63 * b + p if p * ps < n else -1 for p in range(63)] for b, n in enumerate(old)]
+    free, rows = list(range(260, 300)) + list(range(10, 62)), sum(new) + 2 + extra_rows
+    want = PO.extend(new, table, old, free, len(free), ps, pool, rows, 1000)
+    assert want[0] == fits
+    t, lens, count = i32(table), i32(old), i32([len(free)])
+    starts, slots, positions = K.paged_extend(i32(new), t, lens, i32(free), count, page_size=ps, num_pages=pool,
+                                              num_rows=rows, max_seq_len=1000)
+    for got, w in zip((t, lens, count, starts, slots, positions), (*want[1:3], [want[3]], *want[4:])):
+        assert got.tolist() == w
+    assert K.device_status(clear=True) == (0 if fits else 8)
+
+
+def test_captured_steps_keep_max_seq_len(K):
+    """A replayed step stands still at max_seq_len, as the host's would raise."""
+    from sabrecoder_b200.paged_cache import SabrePagedKVCache
+    c = SabrePagedKVCache(batch_size=2, max_seq_len=40, page_size=16, num_layers=1, num_kv_heads=1, head_dim=D)
+    one, k = i32([1, 1]), torch.ones(2, 1, D, device="cuda", dtype=BF)
+    c.extend([30, 30])
+    c.truncate(1, 20)
+    c.lend()
+    c.extend_on_device(one, 2)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        starts, slots, _ = c.extend_on_device(one, 2)
+        c.store_rows(0, k, k, starts, slots)
+    for _ in range(9):
+        graph.replay()
+    assert K.device_status(clear=True) == 0
+    graph.replay()
+    assert slots.tolist() == [-1, -1] and K.device_status(clear=True) == 8
+    c.settle()
+    assert c.lengths == [40, 30]
+    c.extend([0, 10])
+    assert c.lengths == c.seq_lens.tolist() == [40, 40]
