@@ -19,7 +19,7 @@ follows them) are what the kernels read.
   ``topk_pages`` others whose mean key suits them best. All pages are kept.
 * :meth:`lend` hands free pages to the device, where :meth:`extend_on_device`
   makes room for rows, also inside a capture, until :meth:`settle` brings the host
-  up to date.
+  up to date (``lengths`` and ``tables`` stand still meanwhile).
 
 As a transformers ``Cache`` it takes the same number of new rows for every
 sequence of the batch; the patched attention writes its rows through
@@ -90,7 +90,7 @@ class SabrePagedCacheLayer(CacheLayerMixin):
 
     def get_seq_length(self) -> int:
         c = self._cache
-        return max(c.lengths, default=0) - (c.step_rows if self.step < c.step else 0)
+        return max(c._lengths_now(), default=0) - (c.step_rows if self.step < c.step else 0)
 
     def get_mask_sizes(self, query_length) -> Tuple[int, int]:
         n = query_length if isinstance(query_length, int) else query_length.shape[0]
@@ -208,9 +208,22 @@ class SabrePagedKVCache(Cache):
         if _capturing(self.pool):
             raise ValueError("SabrePagedKVCache: sequences do not change inside a capture (extend, and the like, go "
                              "between replays; a captured step stores with paged_store)")
+        self._not_lent()
+
+    def _not_lent(self) -> None:
+        """For what needs the sequences' lengths on the host."""
         if self._lent is not None:
             raise ValueError("SabrePagedKVCache: pages are lent to the device, which changes the sequences; settle() "
                              "comes first")
+
+    def _lengths_now(self) -> List[int]:
+        """The sequences' lengths; while pages are lent those on the device, behind what
+        the current stream does."""
+        if self._lent is None:
+            return self.lengths
+        if _capturing(self.pool):
+            raise ValueError("SabrePagedKVCache: pages are lent to the device, whose lengths a capture cannot read")
+        return self.seq_lens.tolist()
 
     def _seq(self, seq: int) -> int:
         """A sequence's index (from the end when negative)."""
@@ -593,7 +606,7 @@ class SabrePagedKVCache(Cache):
     def gather(self, layer_idx: int) -> Tuple[torch.Tensor, torch.Tensor]:
         """All rows of a layer as ``[B, Hkv, T, D]`` (T the longest length; rows a
         sequence does not have are zero)."""
-        T = max(self.lengths)
+        T = max(self._lengths_now())
         pages = self.page_table[:, :-(-T // self.page_size)].long()
         have = torch.arange(T, device=pages.device)[None] < self.seq_lens[:, None]
         out = []

@@ -139,3 +139,24 @@ def test_captured_steps_keep_max_seq_len(K):
     assert c.lengths == [40, 30]
     c.extend([0, 10])
     assert c.lengths == c.seq_lens.tolist() == [40, 40]
+
+
+def test_reading_rows_while_pages_are_lent(K):
+    """gather() and the length that a model asks for follow the steps on the device."""
+    from sabrecoder_b200.paged_cache import SabrePagedKVCache
+    c = SabrePagedKVCache(batch_size=2, max_seq_len=64, page_size=16, num_layers=1, num_kv_heads=2, head_dim=D)
+    rows = torch.randn(40, 2, D, device="cuda").to(BF)
+    c.append(0, rows[None, :10].repeat(2, 1, 1, 1), -rows[None, :10].repeat(2, 1, 1, 1))
+    c.lend()
+    starts, slots, _ = c.extend_on_device(i32([30, 1]), 31)
+    c.store_rows(0, torch.cat([rows[10:], rows[10:11]]), -torch.cat([rows[10:], rows[10:11]]), starts, slots)
+    assert c.get_seq_length() == 40 and c.get_mask_sizes(1, 0) == (41, 0)
+    k, v = c.gather(0)
+    assert torch.equal(k[0], rows.transpose(0, 1)) and torch.equal(v, -k)
+    assert torch.equal(k[1, :, :11], rows[:11].transpose(0, 1)) and (k[1, :, 11:] == 0).all()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(ValueError, match="capture"), torch.cuda.graph(graph):
+        c.gather(0)
+    torch.cuda.synchronize()
+    c.settle()
+    assert torch.equal(c.gather(0)[0], k) and c.get_seq_length() == 40

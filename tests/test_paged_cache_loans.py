@@ -1,5 +1,5 @@
-"""Pages lent to the device, on the CPU: sequences whose greatest length is no
-multiple of the page."""
+"""Pages lent to the device, on the CPU: what reads the sequences meanwhile, and
+sequences whose greatest length is no multiple of the page."""
 
 import pytest
 import torch
@@ -71,3 +71,36 @@ def test_greatest_length_refusals(monkeypatch):
         got, msg = status("sabre_paged_extend_within", [*b, 9 if changed else -1, 2, None])
         assert got == code and match in msg and b"extend_within" in msg
     assert b"sabre_paged_extend:" in c_extend(page_size=24)[1]
+
+
+def test_rows_and_lengths_follow_the_device_while_pages_are_lent():
+    """What the device added is gathered, and is in the length that a model asks for."""
+    gen = torch.Generator().manual_seed(8)
+    c = cache()
+    add(c, [38, 38, 10], gen)
+    c.lend()
+    starts, slots, _ = c.extend_on_device(i32([5, 0, 2]), 7)
+    rows = torch.randn(7, 2, 8, generator=gen)
+    for i in range(2):
+        c.store_rows(i, rows, -rows, starts, slots)
+    for _ in range(2):  # during the loan and after it
+        k, v = c.gather(0)
+        assert k.shape == (3, 2, 43, 8)
+        assert torch.equal(k[0, :, 38:], rows[:5].transpose(0, 1)) and torch.equal(v[0, :, 38:], -k[0, :, 38:])
+        assert torch.equal(k[2, :, 10:12], rows[5:].transpose(0, 1)) and (k[2, :, 12:] == 0).all()
+        assert c.get_seq_length() == 43 and c.get_mask_sizes(1, 0) == (44, 0)
+        c.settle()
+    assert c.lengths == [43, 38, 12]
+
+
+def test_a_capture_cannot_read_lengths_that_are_the_devices(monkeypatch):
+    c = cache()
+    add(c, [20, 20, 20], torch.Generator().manual_seed(10))
+    monkeypatch.setattr(PC, "_capturing", lambda pool: True)
+    assert c.get_seq_length() == 20 and c.gather(0)[0].shape[2] == 20
+    monkeypatch.setattr(PC, "_capturing", lambda pool: False)
+    c.lend()
+    monkeypatch.setattr(PC, "_capturing", lambda pool: True)
+    for call in (c.get_seq_length, lambda: c.gather(0)):
+        with pytest.raises(ValueError, match="capture"):
+            call()
