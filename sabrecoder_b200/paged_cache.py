@@ -82,6 +82,7 @@ class SabrePagedCacheLayer(CacheLayerMixin):
             raise ValueError("SabrePagedKVCache with a window serves the patched attention only (pages are dropped)")
         if c.topk_pages is not None:
             raise ValueError("SabrePagedKVCache with topk_pages serves the patched attention only")
+        c._not_lent()
         if len(set(c.lengths)) > 1:
             raise ValueError(f"SabrePagedKVCache: sequences of different lengths ({c.lengths}) serve the patched "
                              f"attention only (its mask knows one length)")
@@ -474,6 +475,7 @@ class SabrePagedKVCache(Cache):
         additive, boolean, or one flag a key) may not say more than the cache does:
         it must show the keys that each query sees here and none of its future. Both
         are read from the device, once a step."""
+        self._not_lent()
         if self.layers[layer_idx].step != self.step:
             return
         if len(set(self.lengths)) > 1:
@@ -514,6 +516,7 @@ class SabrePagedKVCache(Cache):
         B, n = k.shape[:2]
         if B != self.batch_size:
             raise ValueError(f"SabrePagedKVCache holds {self.batch_size} sequences (got rows of {B})")
+        self._not_lent()  # a step that was begun before the loan does not go on in it
         if layer.step == self.step:
             pool = self.pool
             for x in (k, v):  # before room is made for them

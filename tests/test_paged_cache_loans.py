@@ -93,6 +93,24 @@ def test_rows_and_lengths_follow_the_device_while_pages_are_lent():
     assert c.lengths == [43, 38, 12]
 
 
+@pytest.mark.parametrize("call", [lambda c: c.append(1, torch.zeros(3, 1, 2, 8), torch.zeros(3, 1, 2, 8)),
+                                  lambda c: c.check_step(0, 1, None), lambda c: c.check_step(1, 1, None),
+                                  lambda c: c.layers[0].update(torch.zeros(3, 2, 1, 8), torch.zeros(3, 2, 1, 8))])
+def test_steps_of_the_host_wait_for_the_end_of_the_loan(call):
+    """Also those whose first layer was stored before it."""
+    c = cache()
+    add(c, [20, 20, 20], torch.Generator().manual_seed(9))
+    c.append(0, torch.ones(3, 1, 2, 8), torch.ones(3, 1, 2, 8))
+    c.lend()
+    pool = c.pool.clone()
+    with pytest.raises(ValueError, match="settle"):
+        call(c)
+    assert torch.equal(pool.nan_to_num(7.0), c.pool.nan_to_num(7.0)) and c.lengths == [21] * 3
+    c.settle()
+    c.append(1, torch.ones(3, 1, 2, 8), torch.ones(3, 1, 2, 8))
+    consistent(c)
+
+
 def test_a_capture_cannot_read_lengths_that_are_the_devices(monkeypatch):
     c = cache()
     add(c, [20, 20, 20], torch.Generator().manual_seed(10))
