@@ -160,3 +160,40 @@ def test_reading_rows_while_pages_are_lent(K):
     torch.cuda.synchronize()
     c.settle()
     assert torch.equal(c.gather(0)[0], k) and c.get_seq_length() == 40
+
+
+def test_new_outputs_go_through_torch(K):
+    """Outputs of the listed calls are filled in deterministic mode and seen by dispatch
+    modes, as those of the other calls."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Seen(TorchDispatchMode):
+        count = 0
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.count += "empty" in str(func)
+            return func(*args, **(kwargs or {}))
+
+    args = make(407, [100, 60], [40, 30], 2, 2, 16, BF)
+    q, kp, vp, table, sl, starts = args
+    lists, counts = i32([[[0, 1], [0, 2]]] * 2), i32([[2, 2], [2, 1]])
+    pad = torch.cat([q, q[:5]])
+    more = K.lib().sabre_paged_query_blocks(75, 2, 64) - 2
+    lists, counts = (torch.cat([t, t[:1].repeat(more, *[1] * (t.dim() - 1))]) for t in (lists, counts))
+
+    def call():
+        return K.paged_prefill_listed(pad, kp, vp, table, sl, starts, lists, counts, query_block=64)
+
+    want = call()
+    before = torch.are_deterministic_algorithms_enabled(), torch.utils.deterministic.fill_uninitialized_memory
+    try:
+        torch.use_deterministic_algorithms(True)
+        torch.utils.deterministic.fill_uninitialized_memory = True
+        out = call()
+    finally:
+        torch.use_deterministic_algorithms(before[0])
+        torch.utils.deterministic.fill_uninitialized_memory = before[1]
+    assert torch.equal(out[:70], want[:70]) and out[70:].isnan().all()
+    with Seen() as seen:
+        out = call()
+    assert seen.count >= 1 and torch.equal(out[:70], want[:70])
