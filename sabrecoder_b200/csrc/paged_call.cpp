@@ -401,9 +401,10 @@ PyObject* attend_listed(PyObject*, PyObject* const* a, Py_ssize_t n) {
                                       orr, ls, cs, p.table->stride(0), scale, p.dtype, wp, wb, stream);
   if (st != SABRE_OK) return PyLong_FromLong(st);
   // As in attend: prompts whose pairs are cut into parts ask for a workspace; decodes of
-  // more than one key tile are joined by a second kernel, unless they run in clusters.
+  // more than one key tile are joined by a second kernel, unless they run in clusters:
+  // up to 28 pairs of up to 32 tiles.
   const int64_t tiles = (int64_t{entries} * p.page_size + 63) / 64, pairs = int64_t{p.batch} * p.heads;
-  const bool joined = p.starts ? need > 0 : tiles * pairs > 1 && !(pairs * 8 <= 296 && tiles > 1 && tiles <= 32);
+  const bool joined = p.starts ? need > 0 : tiles * pairs > 1 && !(pairs <= 28 && tiles > 1 && tiles <= 32);
   return result(out, joined ? 2 : 1);
   END_HANDLE_TH_ERRORS
 }

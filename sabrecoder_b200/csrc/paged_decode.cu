@@ -337,9 +337,19 @@ __device__ __forceinline__ void cluster_sync() {
 // Short lists of few pairs run in clusters: kCluster CTAs take a pair's tiles in equal
 // runs and the first joins them over the cluster's shared memory, which spares the
 // joining kernel (one sequence of 14 pages at 16/16 heads 8.0 -> 6.8 us). A CTA then has
-// at most kClusterTiles tiles.
+// at most kClusterTiles tiles. Clusters find fewer places than CTAs alone do: 30 run at
+// once here, and a 32nd waits for another's end, so kClusterPairs stays below that.
+// Device us in clusters and in shares with the joining kernel, one head a group:
+//   tiles a pair      2            8            16           32           33
+//   1 pair        5.1 / 7.0    5.2 / 7.2    5.7 / 7.4    6.8 / 7.7    7.3 / 8.2
+//   16 pairs      6.0 / 7.6    6.3 / 7.8    6.9 / 8.3    8.1 / 8.9    8.5 / 9.0
+//   28 pairs      6.2 / 7.6    6.5 / 7.8    7.2 / 9.6    8.4 / 10.4
+//   32 pairs      9.4 / 7.7    9.8 / 8.1   11.0 / 9.7   13.2 / 10.4
+// (64 tiles: 8.9 / 8.7 for one pair; seven heads a group: 5.7 / 7.4 for one pair of two
+// tiles, 9.4 / 12.0 for 28 of 32.)
 constexpr int kCluster = 8;
 constexpr int kClusterTiles = 4;
+constexpr int kClusterPairs = 28;
 
 // kMode: over all rows, or the window's; over the pages of p.lists; the same in clusters.
 enum DecodeMode { kDense, kOverPages, kInClusters };
@@ -901,9 +911,9 @@ static int decode_call(const char* fn, const void* q, const void* k_pages, const
     return st;
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   cudaError_t e;
-  // Clusters for pairs whose CTAs all have a place at once (tiles: of all pairs).
+  // tiles: of all pairs.
   const long long pairs = static_cast<long long>(batch) * heads_kv;
-  if (lists && pairs * kCluster <= kDecCtas && tiles > pairs && tiles <= pairs * kCluster * kClusterTiles)
+  if (lists && pairs <= kClusterPairs && tiles > pairs && tiles <= pairs * kCluster * kClusterTiles)
     e = dtype == SABRE_BF16 ? launch_paged_decode<__nv_bfloat16, kInClusters>(mk, mv, p, s)
                             : launch_paged_decode<__half, kInClusters>(mk, mv, p, s);
   else if (lists)

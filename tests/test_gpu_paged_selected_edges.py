@@ -197,3 +197,19 @@ def test_new_outputs_go_through_torch(K):
     with Seen() as seen:
         out = call()
     assert seen.count >= 1 and torch.equal(out[:70], want[:70])
+
+
+@pytest.mark.parametrize("tiles", [1, 2, 32, 33])
+@pytest.mark.parametrize("pairs", [27, 28, 29, 30])
+def test_decode_listed_where_clusters_end(K, pairs, tiles):
+    """Clusters of up to 28 pairs of two to 32 key tiles, and shares with a joining kernel
+    past them: results, and the kernels that are counted."""
+    args = make(500 + pairs, [tiles * 64 + 10 - b for b in range(pairs)], [1] * pairs, 3, 1, 64, BF)
+    q, kp, vp, table, sl, _ = args
+    lists = torch.arange(tiles, dtype=torch.int32, device="cuda").expand(pairs, 1, tiles)
+    counts = torch.full((pairs, 1), tiles, dtype=torch.int32, device="cuda")
+    before = K.LAUNCHES[0]
+    out = K.paged_decode_listed(q, kp, vp, table, sl, lists, counts)
+    assert K.LAUNCHES[0] - before == (1 if pairs <= 28 and 2 <= tiles <= 32 else 2)
+    check(out, args, lists, counts)
+    assert K.device_status(clear=True) == 0
