@@ -121,6 +121,7 @@ namespace sel {
 
 constexpr int kMaxPages = 32768;  // of a sequence: their keys are kept in shared memory
 constexpr int kMaxCtas = 8;       // of a cluster: the portable size
+constexpr int kSms = 148;         // a B200's
 constexpr int kGroupBlocks = 4;   // query blocks that share the means they read
 constexpr int kGroupPages = 2048; // columns up to which they do (32 KB of keys)
 
@@ -429,9 +430,11 @@ __device__ __forceinline__ void write_list(const Params& p, const Cut& cut, cons
 // nearer (one list in a thousand), those near it are computed in 64 bits. A bound that
 // is not finite sends every page that way. 64 bits throughout cost 79 us for the
 // 12288-row prompt at 16/16 heads; so it takes 25.5 (28.5 with inputs from HBM), of
-// which half is the sum of the queries. Groups of two and of eight take 29 and 39, a CTA
-// a block 49. One row on 12288 takes 5.8 us, 32 rows on up to 16383 (56/8 heads, 16-row
-// pages) 25 to 32.
+// which half is the sum of the queries (128 registers, of which a few spill: 24 bytes of
+// stack). Groups of two and of eight took 29 and 39 where four took 27. One row on 12288
+// takes 5.8 us, 32 rows on up to 16383 (56/8 heads, 16-row pages) 25 to 32, 16
+// continuations of up to 200 rows (32/32 heads, 16-row pages) 34 to 39, a chunk of 512 rows
+// on 15872 (56/8 heads) 14 over 128-row pages and 35 over 16-row ones.
 template <typename T, int kGroup, int kWarps>
 __global__ void __launch_bounds__(kWarps * 32, kGroup == 1 ? 5 : 16 / kGroup) paged_select_kernel(const Params p) {
   constexpr int kThreads = kWarps * 32;
@@ -844,13 +847,23 @@ int sabre_paged_select(const void* q, const float* key_means, const int32_t* pag
   const long long blocks = row_slots(rows, batch, query_block);
   // Blocks that fill the card in groups run in groups; else clusters of as many CTAs
   // as leave each warp eight pages, while the card has places.
+  // Device us in groups and without them, 16 heads, a table of 192 columns:
+  //   groups * heads       128          160          192          256          320
+  //   blocks of 128    17.0 / 14.5  18.2 / 15.4  17.8 / 15.7  20.8 / 20.4  23.4 / 25.1
+  //   blocks of 16      6.9 / 12.1   7.9 / 9.3    8.3 / 11.7   9.7 / 14.0  10.8 / 16.9
+  // (the 12288-row prompt in blocks of 128: 24.9 / 30.3), and by the table's width, whose
+  // keys take 4 KB a 256 columns: 24.9 / 30.4 for 2049 columns, 25.4 / 30.7 for 4096, 43 /
+  // 31 for 8192. Past 8192 columns a block's own keys leave few CTAs an SM: 38 us for
+  // 16384 columns, 80 for 32768.
   const long long groups = q_start ? row_slots(rows, batch, query_block * sel::kGroupBlocks) : 0;
-  const bool grouped = groups * heads_kv >= 148 && max_pages <= sel::kGroupPages;
+  const bool grouped = groups * heads_kv >= sel::kSms && max_pages <= sel::kGroupPages;
   p.ctas = 1;
   // Each CTA of a cluster sums the block's queries, so blocks of many rows run in
   // clusters over long tables only (32 blocks of 112 rows on 124 pages, 8 heads: 19 us
   // in pairs of CTAs, 13 alone; on 1000 pages 30 and 47).
-  auto places = [&](int ctas) { return query_block * p.group <= 16 || max_pages > 256 * ctas ? 4 * 148 : 148; };
+  auto places = [&](int ctas) {
+    return query_block * p.group <= 16 || max_pages > 256 * ctas ? 4 * sel::kSms : sel::kSms;
+  };
   while (!grouped && p.ctas < sel::kMaxCtas && max_pages >= 32 * p.ctas && blocks * heads_kv * p.ctas <= places(p.ctas))
     p.ctas *= 2;
   if (blocks * p.ctas > INT_MAX) return sabre_fail(SABRE_ERR_UNSUPPORTED, "%s: too many query blocks", fn);

@@ -46,8 +46,8 @@ def test_select_with_row_starts_that_do_not_ascend(K, starts, rows, block):
     lists = torch.full((2 * blocks + B * rows, H, width), -7, dtype=torch.int32, device="cuda")
     counts = torch.full((2 * blocks + B * rows, H), -7, dtype=torch.int32, device="cuda")
     st = L.sabre_paged_select(q.data_ptr(), means.data_ptr(), table.data_ptr(), lens.data_ptr(), start.data_ptr(),
-                              lists[blocks:].data_ptr(), counts[blocks:].data_ptr(), rows, B, H, H, D, cols, ps, cols, 3,
-                              block, 0, 0, _lib.i64([H * D, D]), _lib.i64([H * D, D]), cols, 0,
+                              lists[blocks:].data_ptr(), counts[blocks:].data_ptr(), rows, B, H, H, D, cols, ps, cols,
+                              3, block, 0, 0, _lib.i64([H * D, D]), _lib.i64([H * D, D]), cols, 0,
                               torch.cuda.current_stream().cuda_stream)
     assert st == 0
     for t in (lists, counts):
@@ -213,3 +213,58 @@ def test_decode_listed_where_clusters_end(K, pairs, tiles):
     assert K.LAUNCHES[0] - before == (1 if pairs <= 28 and 2 <= tiles <= 32 else 2)
     check(out, args, lists, counts)
     assert K.device_status(clear=True) == 0
+
+
+@pytest.mark.parametrize("Hq,Hkv,max_len", [(4, 2, 300), (7, 1, 1000)])
+def test_a_ragged_prompt_on_the_device(K, Hq, Hkv, max_len):
+    """Prompts and turns of different lengths in one step on the device: room, rows,
+    means, selection and attention, captured and replayed, against the oracle."""
+    from sabrecoder_b200.paged_cache import SabrePagedKVCache
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    c = SabrePagedKVCache(batch_size=3, max_seq_len=max_len, num_pages=3 * 1008 // 16, page_size=16, num_layers=2,
+                          num_kv_heads=Hkv, head_dim=D, topk_pages=2, window_size=20, num_prefix_tokens=5)
+    c.pool.fill_(float("nan"))
+    c.key_means.fill_(float("nan"))
+    n = 160
+    new = i32([0, 0, 0])
+    q = torch.empty(2, n, Hq, D, dtype=BF, device="cuda")
+    k, v = (torch.empty(2, n, Hkv, D, dtype=BF, device="cuda") for _ in range(2))
+    outs = [torch.full((n, Hq, D), 7.0, dtype=BF, device="cuda") for _ in range(2)]
+
+    def step():
+        q_start, slots, _ = c.extend_on_device(new, n)
+        lists, counts = [], []
+        for i, layer in enumerate(c.layers):
+            c.store_rows(i, k[i], v[i], q_start, slots)
+            li, co = c.select(i, q[i], q_start)
+            K.paged_prefill_listed(q[i], layer.k_pages, layer.v_pages, c.page_table, c.seq_lens, q_start, li, co,
+                                   query_block=c.block_rows(Hq), out=outs[i])
+            lists.append(li)
+            counts.append(co)
+        return q_start, lists, counts
+
+    c.lend()
+    step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        q_start, lists, counts = step()
+    before = [0, 0, 0]
+    for rows in ([130, 1, 29], [0, 0, 0], [3, 150, 0], [17, 1, 142]):
+        new.copy_(i32(rows))
+        for t in (q, k, v):
+            t.copy_(torch.randn(t.shape, generator=gen, device="cuda"))
+        for o in outs:
+            o.fill_(7.0)
+        graph.replay()
+        before = [a + b for a, b in zip(before, rows)]
+        assert c.seq_lens.tolist() == before and q_start.tolist()[-1] == sum(rows)
+        for i, layer in enumerate(c.layers):
+            args = (q[i, :sum(rows)], layer.k_pages, layer.v_pages, c.page_table, c.seq_lens, q_start)
+            block = c.block_rows(Hq)
+            check_lists(lists[i], counts[i], PO.select(q[i], layer.key_means, c.page_table, c.seq_lens, q_start,
+                                                       page_size=16, topk=2, block=block, window=20, prefix=5))
+            if sum(rows):
+                check(outs[i][:sum(rows)], args, lists[i], counts[i], q_start, block)
+            assert (outs[i][sum(rows):] == 7.0).all()
+    c.settle()
+    assert c.lengths == before and K.device_status(clear=True) == 0

@@ -14,8 +14,8 @@ from test_paged_listed_refusals import args, c_extend, extend, status
 @pytest.fixture(autouse=True)
 def extend_within(plain_kernels, monkeypatch):  # noqa: F811
     def fn(new, table, lens, free, count, *, page_size, num_pages, num_rows, max_seq_len=None):
-        _, t, n, c, starts, slots, pos = PO.extend(new.tolist(), table.tolist(), lens.tolist(), free.tolist(), int(count),
-                                                   page_size, num_pages, num_rows, max_seq_len)
+        _, t, n, c, starts, slots, pos = PO.extend(new.tolist(), table.tolist(), lens.tolist(), free.tolist(),
+                                                   int(count), page_size, num_pages, num_rows, max_seq_len)
         table.copy_(torch.tensor(t))
         lens.copy_(torch.tensor(n))
         count.fill_(c)
